@@ -44,7 +44,19 @@ typedef enum {
 /* OM_C32 / OM_C64: complex numbers as interleaved (re, im) pairs of
  * f32 / f64 (the layout of num_complex::Complex and of the reference's
  * CudaComplex, src/backend/cuda/mod.rs:56-208); Standard algebra only. */
-typedef enum { OM_F32 = 0, OM_F64 = 1, OM_U32 = 2, OM_C32 = 3, OM_C64 = 4 } om_dtype;
+typedef enum {
+  OM_F32 = 0,
+  OM_F64 = 1,
+  OM_U32 = 2,
+  OM_C32 = 3,
+  OM_C64 = 4,
+  /* taken by the sequence-model operators only (end of this header) */
+  OM_BF16 = 5,
+  OM_F16 = 6,
+  OM_I8 = 7,
+  OM_I32 = 8,
+  OM_I64 = 9
+} om_dtype;
 
 enum {
   OM_OK = 0,
@@ -70,6 +82,14 @@ int om_b200_last_error(char* buf, size_t len);
  * (src/backend/cuda/mod.rs:258-265): a bad ordinal is an error, not a panic. */
 int om_b200_create(int device, om_backend** out);
 int om_b200_destroy(om_backend* be);
+
+/* A backend whose work is ordered on the caller's stream (a cudaStream_t of
+ * `device`; NULL = the legacy default stream) instead of one of its own, for
+ * hosts that keep their tensors on a stream already.  The stream is borrowed:
+ * it must outlive the backend and om_b200_destroy leaves it open.  No
+ * counterpart in the reference.  Recording (om_b200_graph_begin) needs a
+ * stream that can be captured, so not the legacy default stream. */
+int om_b200_create_on_stream(int device, void* stream, om_backend** out);
 
 /* The backend's stream (a cudaStream_t), for callers that interoperate. */
 int om_b200_stream(om_backend* be, void** stream_out);
@@ -323,6 +343,103 @@ int om_b200_graph_branch(om_backend* be, int branch);
 int om_b200_tropical_matmul_argmax_noalloc(void* stream, om_algebra alg, int64_t m, int64_t n,
                                            int64_t k, const float* a, int64_t lda, const float* b,
                                            int64_t ldb, float* c, int64_t ldc, uint32_t* argmax);
+
+/* ---- sequence-model operators ---------------------------------------------
+ * Contractions with a step that the pairwise engine has no form for (no
+ * counterpart in the reference).  Like every other call they are ordered on
+ * the backend's stream, take device pointers and strides in elements, and may
+ * be recorded; scratch memory comes from the backend.  They leave the
+ * caller's current device as it was.  Outputs must not overlap inputs unless
+ * said otherwise.  Input strides may be zero (broadcast) or negative. */
+
+/* Gated linear recurrence along time, a chain of contractions per channel:
+ *     h_t = a_t h_{t-1} + b_t,   t = 1 .. T
+ *   OM_GATE_LINEAR:   a = gate,           b = x
+ *   OM_GATE_SIGMOID:  a = sigmoid(gate),  b = (1 - a) x
+ * gate, x and h are [D, T, B] (channels, time, batch) with shape[3] and their
+ * own strides; dtype is OM_F32, OM_F64, OM_BF16 or OM_F16.  The state is kept
+ * in f32 (f64 for OM_F64): h0 and h_last are contiguous [D, B] in that type;
+ * h0 == NULL starts from zero, h_last (may be NULL, may be h0 itself) gets the
+ * state after the last step, and h the state after every step, rounded once.
+ * lengths (device, B int32, may be NULL): sequence b has
+ * min(max(lengths[b], 0), T) steps; what lies behind them is not read, h is
+ * zero there, and h_last is the state after the last real step.  T == 1 is the
+ * form for decoding one token. */
+typedef enum { OM_GATE_LINEAR = 0, OM_GATE_SIGMOID = 1 } om_gate;
+int om_b200_gated_scan(om_backend* be, om_gate kind, om_dtype dtype, const int64_t* shape,
+                       const void* gate, const int64_t* strides_gate, const void* x,
+                       const int64_t* strides_x, const void* h0, const int32_t* lengths, void* h,
+                       const int64_t* strides_h, void* h_last);
+
+/* Its backward pass.  h is the forward's output, dh the gradient reaching it
+ * and dh_last (contiguous [D, B] in the state's type, may be NULL) the one
+ * reaching h_last.  With G_t = dh_t + a_{t+1} G_{t+1}:
+ *   OM_GATE_LINEAR:   dx = G,          dgate = G h_{t-1}          (x may be NULL)
+ *   OM_GATE_SIGMOID:  dx = (1 - a) G,  dgate = G (h_{t-1} - x) a (1 - a)
+ * and dh0 = a_1 G_1 (contiguous [D, B], may be NULL).  dgate and dx are zero
+ * behind the last step of a sequence. */
+int om_b200_gated_scan_backward(om_backend* be, om_gate kind, om_dtype dtype, const int64_t* shape,
+                                const void* gate, const int64_t* strides_gate, const void* x,
+                                const int64_t* strides_x, const void* h, const int64_t* strides_h,
+                                const void* h0, const int32_t* lengths, const void* dh,
+                                const int64_t* strides_dh, const void* dh_last, void* dgate,
+                                const int64_t* strides_dgate, void* dx, const int64_t* strides_dx,
+                                void* dh0);
+
+/* Softmax cross entropy of the logits z = x w^T over a vocabulary, in pieces
+ * of the vocabulary and without keeping the logits:
+ *     lse_n  = log sum_v exp(z_nv),   loss_n = lse_n - z_{n, targets[n]}
+ * shape[3] is {D, N, V} (width, tokens, vocabulary); x is [D, N] and w [D, V]
+ * with their own strides, dtype OM_F32, OM_F64, OM_BF16 or OM_F16.  targets
+ * (N contiguous OM_I32 or OM_I64 values, target_dtype) outside [0, V) carry no
+ * loss: loss is 0 there (lse is still written).  loss and lse are N contiguous
+ * f32 values (f64 for OM_F64).  16-bit products accumulate in f32; f32 ones
+ * follow om_b200_set_f32_mode. */
+int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, const int64_t* shape,
+                                 const void* x, const int64_t* strides_x, const void* w,
+                                 const int64_t* strides_w, om_dtype target_dtype,
+                                 const void* targets, void* loss, void* lse);
+
+/* Its gradients, from lse and the gradient dloss of each token's loss (both N
+ * contiguous values): with p = exp(z - lse),
+ *     dz_nv = dloss_n (p_nv - [v == targets[n]]),  dx = dz w,  dw = dz^T x
+ * Tokens without a loss get dx = 0 and reach dw with nothing, whatever their
+ * row of x holds.  In the 16-bit types dz is rounded to dtype before the two
+ * products, whose sums are f32. */
+int om_b200_linear_cross_entropy_backward(om_backend* be, om_dtype dtype, const int64_t* shape,
+                                          const void* x, const int64_t* strides_x, const void* w,
+                                          const int64_t* strides_w, om_dtype target_dtype,
+                                          const void* targets, const void* lse, const void* dloss,
+                                          void* dx, const int64_t* strides_dx, void* dw,
+                                          const int64_t* strides_dw);
+
+/* 8-bit rows: scale_m = max_k |x_km| / 127 (f32) and
+ * q_km = x_km / scale_m rounded to the nearest whole number (ties to even;
+ * zero in a row of zeros).  shape[2] is {K, M}; x is [K, M] in OM_F32, OM_BF16
+ * or OM_F16, q [K, M] in OM_I8, each with its own strides; scale holds M
+ * values.  A row holding a NaN or an infinity gets that as its scale and only
+ * zeros as q. */
+int om_b200_quantize_rows(om_backend* be, om_dtype dtype, const int64_t* shape, const void* x,
+                          const int64_t* strides_x, void* q, const int64_t* strides_q,
+                          float* scale);
+
+/* Matrix product in 8-bit integers with a scale for each row of q (token) and
+ * of w (channel):
+ *     y_nm = (sum_k q_km w_kn) q_scale_m w_scale_n + bias_n
+ * shape[3] is {K, M, N}; q [K, M] and w [K, N] are OM_I8 with their own
+ * strides, q_scale, w_scale and bias (may be NULL) contiguous f32, y [N, M] in
+ * dtype OM_F32, OM_BF16 or OM_F16.  The sum is a 32-bit integer (K at most
+ * 131071), the rest f32, rounded once. */
+int om_b200_matmul_i8(om_backend* be, om_dtype dtype, const int64_t* shape, const void* q,
+                      const int64_t* strides_q, const float* q_scale, const void* w,
+                      const int64_t* strides_w, const float* w_scale, const float* bias, void* y,
+                      const int64_t* strides_y);
+
+/* om_b200_quantize_rows and om_b200_matmul_i8 in one call: x [K, M] and
+ * y [N, M] are both of dtype. */
+int om_b200_linear_i8(om_backend* be, om_dtype dtype, const int64_t* shape, const void* x,
+                      const int64_t* strides_x, const void* w, const int64_t* strides_w,
+                      const float* w_scale, const float* bias, void* y, const int64_t* strides_y);
 
 #ifdef __cplusplus
 }

@@ -27,8 +27,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libomeinsum_b200.so")
 
 ALGEBRAS = {"standard": 0, "maxplus": 1, "minplus": 2, "maxmul": 3}
+# numpy has no bfloat16: a one-field record of its 16 bits
+BF16 = np.dtype([("bf16", np.uint16)])
 DTYPES = {np.dtype(np.float32): 0, np.dtype(np.float64): 1, np.dtype(np.uint32): 2,
-          np.dtype(np.complex64): 3, np.dtype(np.complex128): 4}
+          np.dtype(np.complex64): 3, np.dtype(np.complex128): 4, BF16: 5,
+          np.dtype(np.float16): 6, np.dtype(np.int8): 7, np.dtype(np.int32): 8,
+          np.dtype(np.int64): 9}
 NP_OF = {0: np.float32, 1: np.float64, 2: np.uint32, 3: np.complex64, 4: np.complex128}
 
 # every symbol the header declares (checked by the CPU test suite)
@@ -41,6 +45,9 @@ EXPORTS = [
     "om_b200_tape_free", "om_b200_graph_begin", "om_b200_graph_end", "om_b200_graph_launch",
     "om_b200_graph_free", "om_b200_tape_release", "om_b200_einsum_backward_linked",
     "om_b200_set_f32_mode", "om_b200_scatter_index", "om_b200_gather_views", "om_b200_einsum_tape_values", "om_b200_optimize_tree", "om_b200_graph_branch", "om_b200_download_async",
+    "om_b200_create_on_stream", "om_b200_gated_scan", "om_b200_gated_scan_backward",
+    "om_b200_linear_cross_entropy", "om_b200_linear_cross_entropy_backward",
+    "om_b200_quantize_rows", "om_b200_matmul_i8", "om_b200_linear_i8",
 ]
 
 
@@ -72,6 +79,7 @@ def lib():
         L.om_b200_name.restype = ctypes.c_char_p
         L.om_b200_last_error.argtypes = [ctypes.c_char_p, SZ]
         L.om_b200_create.argtypes = [I, ctypes.POINTER(P)]
+        L.om_b200_create_on_stream.argtypes = [I, P, ctypes.POINTER(P)]
         L.om_b200_destroy.argtypes = [P]
         L.om_b200_stream.argtypes = [P, ctypes.POINTER(P)]
         L.om_b200_sync.argtypes = [P]
@@ -208,13 +216,21 @@ class View(Storage):
 
 
 class B200:
-    """The B200 backend: `impl Backend for B200` in the reference's terms."""
+    """The B200 backend: `impl Backend for B200` in the reference's terms.
 
-    def __init__(self, device: int = 0):
+    stream: a cudaStream_t (as an integer, 0 = the legacy default stream) to
+    order the backend's work on, instead of a stream of its own."""
+
+    def __init__(self, device: int = 0, stream: int | None = None):
         h = ctypes.c_void_p()
-        _check(lib().om_b200_create(device, ctypes.byref(h)))
+        if stream is None:
+            _check(lib().om_b200_create(device, ctypes.byref(h)))
+        else:
+            _check(lib().om_b200_create_on_stream(device, stream, ctypes.byref(h)))
         self.h = h.value
         self.device = device
+        self.recording = False  # between graph_begin and graph_end
+        self.home_stream = self.stream()
 
     @staticmethod
     def name() -> str:
@@ -242,6 +258,7 @@ class B200:
     def graph_begin(self):
         """Start recording the work issued on this backend's stream."""
         _check(lib().om_b200_graph_begin(self.h))
+        self.recording = True
 
     def graph_branch(self, branch: int):
         """While recording: issue the following work on concurrent branch
@@ -251,6 +268,7 @@ class B200:
     def graph_end(self) -> "Graph":
         """Stop recording; the recorded work as a replayable graph."""
         g = ctypes.c_void_p()
+        self.recording = False
         _check(lib().om_b200_graph_end(self.h, ctypes.byref(g)))
         return Graph(self, g.value)
 

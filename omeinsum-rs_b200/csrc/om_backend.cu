@@ -226,7 +226,7 @@ int64_t om_b200_launch_count(void) {
   return n;
 }
 
-int om_b200_create(int device, om_backend** out) {
+static int create_backend(int device, om_backend** out, bool borrow, cudaStream_t stream) {
   if (!out) return set_error(OM_ERR_INVALID, "om_b200_create: out is null");
   *out = nullptr;
   int count = 0;
@@ -243,7 +243,9 @@ int om_b200_create(int device, om_backend** out) {
   auto* be = new om_backend();
   be->device = device;
   be->num_sms = prop.multiProcessorCount;
-  cudaError_t e = cudaStreamCreateWithFlags(&be->stream, cudaStreamNonBlocking);
+  be->borrowed_stream = borrow;
+  be->stream = stream;
+  cudaError_t e = borrow ? cudaSuccess : cudaStreamCreateWithFlags(&be->stream, cudaStreamNonBlocking);
   if (e != cudaSuccess) {
     delete be;
     return check_cuda(e, "cudaStreamCreateWithFlags");
@@ -256,7 +258,7 @@ int om_b200_create(int device, om_backend** out) {
   e = cudaMalloc(&be->d_flags, 64);
   if (e == cudaSuccess) e = cudaMemset(be->d_flags, 0, 64);
   if (e != cudaSuccess) {
-    cudaStreamDestroy(be->stream);
+    if (!borrow) cudaStreamDestroy(be->stream);
     delete be;
     return check_cuda(e, "cudaMalloc(flags)");
   }
@@ -264,6 +266,15 @@ int om_b200_create(int device, om_backend** out) {
   backend_live(be, true);
   *out = be;
   return OM_OK;
+}
+
+int om_b200_create(int device, om_backend** out) {
+  return create_backend(device, out, false, nullptr);
+}
+
+int om_b200_create_on_stream(int device, void* stream, om_backend** out) {
+  om::DeviceGuard guard(device);  // the caller keeps its current device
+  return create_backend(device, out, true, (cudaStream_t)stream);
 }
 
 int om_b200_destroy(om_backend* be) {
@@ -277,7 +288,7 @@ int om_b200_destroy(om_backend* be) {
   be->branch_streams.clear();
   if (be->fork_event) cudaEventDestroy(be->fork_event);
   be->fork_event = nullptr;
-  cudaStreamDestroy(be->stream);
+  if (!be->borrowed_stream) cudaStreamDestroy(be->stream);
   be->stream = nullptr;
   be->pending.clear();
   be->prof_totals.clear();

@@ -537,6 +537,8 @@ extern "C" int om_b200_copy_strided(om_backend* be, om_dtype dtype, const void* 
   using namespace om;
   if (!be || !src || !dst || (ndim > 0 && (!shape || !strides)))
     return set_error(OM_ERR_INVALID, "om_b200_copy_strided: null argument");
+  if (dtype > OM_C64)
+    return set_error(OM_ERR_UNSUPPORTED, "om_b200_copy_strided: dtype must be f32, f64, u32 or complex");
   OM_CUDA(cudaSetDevice(be->device), "cudaSetDevice");
   if (is_complex(dtype)) {  // the two parts as a leading unit-stride axis of extent 2
     if (ndim < 0 || ndim + 1 > OM_MAX_DIMS) return set_error(OM_ERR_INVALID, "gather: bad rank");

@@ -25,6 +25,7 @@ struct om_backend {
   // from this arena (owned by the graph) instead of the stream-ordered pool
   om::Arena* recording = nullptr;
   cudaStream_t stream = nullptr;
+  bool borrowed_stream = false;  // the caller's (om_b200_create_on_stream)
   // branches of a recording (om_b200_graph_branch): while one is selected,
   // `stream` is that branch's stream and `main_stream` the backend's own
   cudaStream_t main_stream = nullptr;
@@ -64,6 +65,25 @@ struct ProfScope {
   om_backend::Pending p{};
   ProfScope(om_backend* b, const char* name);
   ~ProfScope();
+};
+
+// Makes the backend's device current for a scope and puts the caller's back.
+struct DeviceGuard {
+  int prev = -1;
+  cudaError_t status = cudaSuccess;
+  explicit DeviceGuard(int device) {
+    int cur = -1;
+    status = cudaGetDevice(&cur);
+    if (status == cudaSuccess && cur != device) {
+      status = cudaSetDevice(device);
+      if (status == cudaSuccess) prev = cur;
+    }
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  DeviceGuard(const DeviceGuard&) = delete;
+  DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 
 #define OM_TRY(expr)            \
