@@ -6,8 +6,10 @@
 // The vocabulary is walked in pieces; a piece's logits live in scratch memory
 // until the next piece and are computed a second time by the backward pass.
 #include <algorithm>
+#include <cfloat>
 
 #include "om_convert.cuh"
+#include "om_sm100.cuh"
 
 namespace om {
 namespace {
@@ -263,6 +265,396 @@ int loss_backward(om_backend* be, const LossArgs& p, const typename Elem<T>::Sta
   return check_cuda(cudaGetLastError(), "loss backward launch");
 }
 
+// ---- 16-bit types on the tensor cores ----------------------------------------
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Maximum and sum of exponentials of a lane's columns of one row, and the
+// target's logit.
+struct StatsEpi {
+  const void* targets;
+  int t64;
+  float2* part;  // [slot][rows]
+  int64_t rows;
+  float* hit;
+  struct Row {
+    float m, s;
+    int64_t target;
+  };
+  __device__ __forceinline__ Row begin(int m, bool in, int) const {
+    return Row{-INFINITY, 0.f, in ? target_of(targets, t64, m) : -1};
+  }
+  __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
+                                          const uint32_t (&r)[32]) const {
+    if (n0 >= N) return;
+    const int n = N - n0;  // columns that exist
+    float top = __uint_as_float(r[0]);
+    if (n >= 32) {
+#pragma unroll
+      for (int c = 1; c < 32; ++c) top = fmaxf(top, __uint_as_float(r[c]));
+    } else {
+#pragma unroll
+      for (int c = 1; c < 32; ++c)
+        if (c < n) top = fmaxf(top, __uint_as_float(r[c]));
+    }
+    if (top > row.m) {
+      row.s *= exp2_fast((row.m - top) * LOG2E);
+      row.m = top;
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (n >= 32) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - row.m) * LOG2E);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (c < n) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - row.m) * LOG2E);
+    }
+    row.s += (s[0] + s[1]) + (s[2] + s[3]);
+    const int64_t at = row.target - n0;
+    if (at >= 0 && at < 32 && at < n) {
+      float z = 0.f;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (at == c) z = __uint_as_float(r[c]);
+      hit[m] = z;
+    }
+  }
+  __device__ __forceinline__ void end(Row& row, int m, bool in, int slot) const {
+    if (in) part[(int64_t)slot * rows + m] = make_float2(row.m, row.s);
+  }
+};
+
+// Joins the slots of 32 rows per block, each thread every eighth slot.
+__global__ void join_stats(const float2* __restrict__ part, int slots, int64_t rows,
+                           const void* targets, int t64, int64_t vocab, const float* hit,
+                           float* loss, float* lse) {
+  __shared__ float sm[8][33], ss[8][33];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x * (int64_t)32 + tx;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows)
+    for (int i = ty; i < slots; i += 8) {
+      const float2 v = part[(int64_t)i * rows + row];
+      merge(m, s, v.x, v.y);
+    }
+  sm[ty][tx] = m;
+  ss[ty][tx] = s;
+  __syncthreads();
+  if (ty || row >= rows) return;
+  for (int i = 1; i < 8; ++i) merge(m, s, sm[i][tx], ss[i][tx]);
+  const float total = m + logf(s);
+  const int64_t t = target_of(targets, t64, row);
+  lse[row] = total;
+  loss[row] = t >= 0 && t < vocab ? total - hit[row] : 0.f;
+}
+
+// dz is rounded to 16 bits as dz / scale, scale = max |dloss| of the counted
+// tokens over `top`, and the products' f32 sums are multiplied by it: where all
+// tokens weigh the same, the one-hot part is a power of two and rounds to
+// itself, while the rounding of dloss would be the same error in every term
+// (measured on 4096 x 1024 x 50001: the gradients' error against 64 bits falls
+// from 3.4e-3 to 1.7e-3, the f32 result's own rounding). top = 2^14 in f16 holds dz down to 2^-38 of the
+// largest; bf16 needs no room and takes 1.
+__global__ void gradient_scale(const float* __restrict__ dloss, const void* targets, int t64,
+                               int64_t vocab, int64_t n, float top, float* scale) {
+  float m = 0.f;
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t t = target_of(targets, t64, i);
+    if (t >= 0 && t < vocab) m = fmaxf(m, fabsf(dloss[i]));
+  }
+  __shared__ float part[32];
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 1; i < (int)(blockDim.x >> 5); ++i) m = fmaxf(m, part[i]);
+  // a scale below f32's normal numbers would lose bits, none is needed at 0
+  const float f = m / top;
+  *scale = f >= FLT_MIN && f < INFINITY ? f : 1.f;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 values of a row as T, 16 bytes at a time
+template <typename T>
+__device__ __forceinline__ void store_half_row(T* dst, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 8)
+    *reinterpret_cast<uint4*>(dst + c) =
+        make_uint4(pack2(v[c], v[c + 1], T()), pack2(v[c + 2], v[c + 3], T()),
+                   pack2(v[c + 4], v[c + 5], T()), pack2(v[c + 6], v[c + 7], T()));
+}
+
+// dz of a piece, rounded to T; the buffer's rows hold whole tiles
+template <typename T>
+struct GradEpi {
+  const void* targets;
+  int t64;
+  int64_t vocab, v0;
+  const float *lse, *dloss, *scale;
+  T* dz;
+  int64_t ld;
+  struct Row {
+    float lse, g;
+    int64_t target;  // within the piece
+  };
+  __device__ __forceinline__ Row begin(int m, bool in, int) const {
+    Row row{0.f, 0.f, -1};
+    if (in) {
+      const int64_t t = target_of(targets, t64, m);
+      row.lse = lse[m];
+      if (t >= 0 && t < vocab) {
+        row.g = dloss[m] / *scale;
+        row.target = t - v0;
+      } else {  // exp(z - inf) = 0, whatever this row's lse is
+        row.lse = INFINITY;
+      }
+    }
+    return row;
+  }
+  __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
+                                          const uint32_t (&r)[32]) const {
+    if (!in) return;
+    float v[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      v[c] = row.g * exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E);
+    const int64_t at = row.target - n0;
+    if (at >= 0 && at < 32) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
+    }
+    store_half_row(dz + (int64_t)m * ld + n0, v);
+  }
+  __device__ __forceinline__ void end(Row&, int, bool, int) const {}
+};
+
+// Sums in f32 kept for later pieces or splits, or the finished result as T.
+template <typename T>
+struct OutEpi {
+  T* out;
+  int64_t dr, dc;
+  int vec;             // rows of `out` may be written 16 bytes at a time
+  const float* scale;  // gradient_scale's
+  float* acc;          // [split][rows][acc_ld], whole tiles
+  int64_t acc_ld, acc_split;
+  int load, keep;      // add what acc holds; leave the sum there
+  struct Row {
+    float f;
+    float* acc;
+  };
+  __device__ __forceinline__ Row begin(int m, bool in, int split) const {
+    return Row{*scale,
+               acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr};
+  }
+  __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
+                                          const uint32_t (&r)[32]) const {
+    if (!in || n0 >= N) return;
+    float v[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]);
+    if (load) {
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(row.acc + n0 + c);
+        v[c] += a.x, v[c + 1] += a.y, v[c + 2] += a.z, v[c + 3] += a.w;
+      }
+    }
+    if (keep) {
+#pragma unroll
+      for (int c = 0; c < 32; c += 4)
+        *reinterpret_cast<float4*>(row.acc + n0 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < 32; ++c) v[c] *= row.f;
+    T* to = out + (int64_t)m * dr;
+    if (vec && N - n0 >= 32) {
+      store_half_row(to + n0, v);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (n0 + c < N) to[(n0 + c) * dc] = Elem<T>::store(v[c]);
+    }
+  }
+  __device__ __forceinline__ void end(Row&, int, bool, int) const {}
+};
+
+// out = scale * sum of the splits
+template <typename T>
+__global__ void join_splits(const float* __restrict__ acc, int splits, int64_t acc_split,
+                            int64_t acc_ld, int64_t rows, int64_t cols, const float* scale,
+                            T* __restrict__ out, int64_t dr, int64_t dc) {
+  const float f = *scale;
+  const int64_t total = rows * cols;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / cols, c = i - r * cols;
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += acc[k * acc_split + r * acc_ld + c];
+    out[r * dr + c * dc] = Elem<T>::store(s * f);
+  }
+}
+
+// Rows of [rows, cols] as T with 16-byte aligned rows; zero where the target
+// lies outside the vocabulary (targets given), and in the padding
+template <typename T>
+__global__ void pack_rows(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
+                          int64_t sc, T* __restrict__ dst, int64_t ld, const void* targets, int t64,
+                          int64_t vocab) {
+  const int64_t total = rows * ld;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / ld, c = i - r * ld;
+    bool keep = c < cols;
+    if (targets) {
+      const int64_t t = target_of(targets, t64, r);
+      keep = keep && t >= 0 && t < vocab;
+    }
+    dst[i] = keep ? src[r * sr + c * sc] : T(0.f);
+  }
+}
+
+// The operand itself when TMA can read its rows, else a packed copy.
+template <typename T>
+int readable(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
+             Scratch& copy, mma::Matrix* out) {
+  *out = mma::Matrix{src, rows, cols, sr, 2};
+  if ((sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2)) return OM_OK;
+  const int64_t ld = (cols + 7) / 8 * 8;
+  OM_TRY(copy.alloc(be, (size_t)rows * ld * 2));
+  pack_rows<T><<<flat_grid(be, rows * ld), 256, 0, be->stream>>>(src, rows, cols, sr, sc,
+                                                                 (T*)copy.ptr, ld, nullptr, 0, 0);
+  note_launch();
+  *out = mma::Matrix{copy.ptr, rows, cols, ld, 2};
+  return check_cuda(cudaGetLastError(), "loss pack launch");
+}
+
+// Tile columns and whether a pair of CTAs shares a tile, from the result's
+// size: pairs of 256 x 256 when they fill the card, else the widest tile of
+// one CTA that gives three quarters of the SMs one.
+struct Tiling {
+  int bn, pair;
+};
+Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
+  if (M > mma::TM && (M + 255) / 256 * ((N + 255) / 256) >= be->num_sms / 2) return {256, 0};
+  const int64_t tm = (M + mma::TM - 1) / mma::TM;
+  for (int bn = 256; bn > least; bn /= 2)
+    if (tm * ((N + bn - 1) / bn) * 4 >= be->num_sms * 3) return {bn, 0};
+  return {least, 0};
+}
+
+template <bool AMN, bool BMN, class Epi>
+int product16(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
+              bool bf16, Tiling t, int splits, const Epi& epi) {
+  if (t.pair) return mma::launch_product<false, AMN, BMN, 2>(be, name, a, b, bf16, t.bn, splits, epi);
+  return mma::launch_product<false, AMN, BMN, 1>(be, name, a, b, bf16, t.bn, splits, epi);
+}
+
+template <typename T>
+int loss_forward16(om_backend* be, const LossArgs& p, float* loss, float* lse) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  Scratch xc, wc, ws;
+  mma::Matrix x, w;
+  OM_TRY(readable<T>(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
+  OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
+  const Tiling t = tiling(be, p.N, p.V, 64);
+  const int64_t slots = (p.V + t.bn - 1) / t.bn * 2;
+  OM_TRY(ws.alloc(be, (size_t)p.N * (slots * 8 + 4)));
+  float2* part = (float2*)ws.ptr;
+  float* hit = (float*)(part + slots * p.N);
+  const StatsEpi epi{p.targets, p.target64, part, p.N, hit};
+  OM_TRY((product16<false, false>(be, "loss_logits", x, w, bf16, t, 1, epi)));
+  ProfScope prof(be, "loss_join_stats");
+  join_stats<<<(unsigned)((p.N + 31) / 32), 256, 0, be->stream>>>(
+      part, (int)slots, p.N, p.targets, p.target64, p.V, hit, loss, lse);
+  note_launch();
+  return check_cuda(cudaGetLastError(), "loss join launch");
+}
+
+template <typename T>
+int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const float* dloss, T* dx,
+                    int64_t dxd, int64_t dxn, T* dw, int64_t dwd, int64_t dwv) {
+  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  if (p.N == 0) {
+    zero_rows<T><<<flat_grid(be, p.V * p.D), 256, 0, be->stream>>>(dw, p.V, p.D, dwv, dwd);
+    note_launch();
+    return check_cuda(cudaGetLastError(), "loss backward launch");
+  }
+  // a piece's dz takes at most 512 MiB
+  const int64_t fit = ((int64_t)256 << 20) / p.N / 256 * 256;
+  const int64_t P = std::min((p.V + 255) / 256 * 256, std::max<int64_t>(256, fit));
+  const int64_t Dp = (p.D + 7) / 8 * 8;
+  Scratch xs, wc, dzs, accs, scales;
+  OM_TRY(xs.alloc(be, (size_t)p.N * Dp * 2));
+  OM_TRY(dzs.alloc(be, (size_t)p.N * P * 2));
+  T* dz = (T*)dzs.ptr;
+  // rows without a loss are zero here: whatever they hold reaches no gradient
+  pack_rows<T><<<flat_grid(be, p.N * Dp), 256, 0, be->stream>>>(
+      (const T*)p.x, p.N, p.D, p.xn, p.xd, (T*)xs.ptr, Dp, p.targets, p.target64, p.V);
+  note_launch();
+  mma::Matrix w;
+  OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
+  OM_TRY(scales.alloc(be, 4));
+  float* scale = (float*)scales.ptr;
+  gradient_scale<<<1, 1024, 0, be->stream>>>(dloss, p.targets, p.target64, p.V, p.N,
+                                             bf16 ? 1.f : 16384.f, scale);
+  note_launch();
+  // dx sums over the vocabulary: few tokens and a narrow width leave SMs idle
+  // unless the sum is split; each split needs 8 slabs to be worth its f32 sums
+  const Tiling tx = tiling(be, p.N, p.D, 64);
+  const int64_t rows = tx.pair ? 256 : 128;
+  const int64_t txt = (p.N + rows - 1) / rows * ((p.D + tx.bn - 1) / tx.bn);
+  const int64_t slots = tx.pair ? be->num_sms / 2 : be->num_sms;
+  const int64_t least = (std::min(P, p.V) + 63) / 64;
+  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / txt, least / 8, 64}));
+  const int64_t acc_ld = (p.D + tx.bn - 1) / tx.bn * tx.bn;
+  const bool sums = splits > 1 || P < p.V;
+  if (sums) OM_TRY(accs.alloc(be, (size_t)splits * p.N * acc_ld * 4));
+  float* acc = (float*)accs.ptr;
+  const bool vecx = dxd == 1 && dxn % 8 == 0 && ((uintptr_t)dx & 15) == 0;
+  const bool vecw = dwd == 1 && dwv % 8 == 0 && ((uintptr_t)dw & 15) == 0;
+  for (int64_t v0 = 0; v0 < p.V; v0 += P) {
+    const int64_t n = std::min(P, p.V - v0);
+    const bool last = v0 + n == p.V;
+    const T* wp = (const T*)w.ptr + v0 * w.ld;
+    const mma::Matrix x{xs.ptr, p.N, p.D, Dp, 2};
+    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dz, P};
+    OM_TRY((product16<false, false>(be, "loss_dlogits", x, mma::Matrix{wp, n, p.D, w.ld, 2}, bf16,
+                                    tiling(be, p.N, n, 64), 1, ge)));
+    const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
+    const OutEpi<T> xe{dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
+    OM_TRY((product16<false, true>(be, "loss_dx", mma::Matrix{dz, p.N, n, P, 2},
+                                   mma::Matrix{wp, p.D, n, w.ld, 2}, bf16, tx, now, xe)));
+    const OutEpi<T> we{dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
+    OM_TRY((product16<true, true>(be, "loss_dw", mma::Matrix{dz, n, p.N, P, 2},
+                                  mma::Matrix{xs.ptr, p.D, p.N, Dp, 2}, bf16,
+                                  tiling(be, n, p.D, 64), 1, we)));
+  }
+  if (splits > 1) {
+    ProfScope prof(be, "loss_join_splits");
+    join_splits<T><<<flat_grid(be, p.N * p.D), 256, 0, be->stream>>>(
+        acc, splits, p.N * acc_ld, acc_ld, p.N, p.D, scale, dx, dxn, dxd);
+    note_launch();
+  }
+  return check_cuda(cudaGetLastError(), "loss backward launch");
+}
+
 int check_loss(const char* who, om_backend* be, om_dtype dtype, const int64_t* shape,
                om_dtype target_dtype) {
   const std::string w(who);
@@ -297,8 +689,8 @@ extern "C" int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, cons
   const LossArgs p{shape[1], shape[0], shape[2], x, strides_x[0], strides_x[1], w, strides_w[0],
                    strides_w[1], targets, target_dtype == OM_I64};
   if (dtype == OM_F64) return loss_forward<double>(be, p, (double*)loss, (double*)lse);
-  if (dtype == OM_BF16) return loss_forward<__nv_bfloat16>(be, p, (float*)loss, (float*)lse);
-  if (dtype == OM_F16) return loss_forward<__half>(be, p, (float*)loss, (float*)lse);
+  if (dtype == OM_BF16) return loss_forward16<__nv_bfloat16>(be, p, (float*)loss, (float*)lse);
+  if (dtype == OM_F16) return loss_forward16<__half>(be, p, (float*)loss, (float*)lse);
   return loss_forward<float>(be, p, (float*)loss, (float*)lse);
 }
 
@@ -317,12 +709,12 @@ extern "C" int om_b200_linear_cross_entropy_backward(
   if (shape[1] == 0) strides_x = strides_dx = zero;
   const LossArgs p{shape[1], shape[0], shape[2], x, strides_x[0], strides_x[1], w, strides_w[0],
                    strides_w[1], targets, target_dtype == OM_I64};
-#define OM_LOSS_BWD(T, S)                                                                         \
-  loss_backward<T>(be, p, (const S*)lse, (const S*)dloss, (T*)dx, strides_dx[0], strides_dx[1], \
+#define OM_LOSS_BWD(FN, T, S)                                                               \
+  FN<T>(be, p, (const S*)lse, (const S*)dloss, (T*)dx, strides_dx[0], strides_dx[1], \
                    (T*)dw, strides_dw[0], strides_dw[1])
-  if (dtype == OM_F64) return OM_LOSS_BWD(double, double);
-  if (dtype == OM_BF16) return OM_LOSS_BWD(__nv_bfloat16, float);
-  if (dtype == OM_F16) return OM_LOSS_BWD(__half, float);
-  return OM_LOSS_BWD(float, float);
+  if (dtype == OM_F64) return OM_LOSS_BWD(loss_backward, double, double);
+  if (dtype == OM_BF16) return OM_LOSS_BWD(loss_backward16, __nv_bfloat16, float);
+  if (dtype == OM_F16) return OM_LOSS_BWD(loss_backward16, __half, float);
+  return OM_LOSS_BWD(loss_backward, float, float);
 #undef OM_LOSS_BWD
 }

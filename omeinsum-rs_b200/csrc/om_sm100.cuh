@@ -1,0 +1,429 @@
+// Tensor-core product D[m, n] = sum_k A[m, k] B[n, k] of 16-bit or 8-bit
+// operands on sm_100a, with the caller's own epilogue.
+//
+// Persistent: each CTA (CG = 1) or pair of CTAs (CG = 2) takes tiles of
+// 128 CG x BN round robin. 320 threads: warp 0 issues TMA loads of 128-byte
+// deep k slabs into a ring of stages, one thread of warp 1 issues the MMAs
+// (accumulators in tensor memory, two of them, so that one tile's epilogue
+// runs under the next tile's products), warps 2..9 read a finished
+// accumulator and hand it to the epilogue 32 columns at a time: warp w has the
+// rows 32 (w % 4) .. + 31, one per lane, and every second group of columns.
+//
+// With CG = 2 two SMs share a tile: each holds its own 128 rows of A and half
+// of B's rows, so a slab costs each SM 32 KiB of loads instead of 48 for the
+// same 256 columns; the even CTA issues the MMAs of both.
+//
+// An operand is K-major (k contiguous) or MN-major (rows contiguous); both are
+// read by TMA where they lie, with a 128-byte swizzle. TMA fills what lies
+// outside the matrix with zeros, so no size needs padding.
+//
+// Every wait is bounded; on expiry the kernel records an error word that
+// om_b200_sync reports, and leaves after its other bounded waits.
+#pragma once
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "om_internal.h"
+
+namespace om {
+
+// cuTensorMapEncodeTiled, looked up once (null: not available)
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+
+namespace mma {
+
+constexpr int TM = 128;             // rows of a CTA's accumulator
+constexpr int THREADS = 320;        // 2 + 8 warps
+constexpr int MAX_STAGES = 12;
+constexpr int SLAB = 128;           // bytes of k per stage
+constexpr int A_BYTES = TM * SLAB;
+constexpr uint32_t WAIT_LIMIT = 1u << 24;
+
+struct Shape {
+  int M, N;        // rows of A and of B
+  int slabs;       // of 128 bytes along k, all splits together
+  int BN;          // columns of a tile: 32 .. 256
+  int stages;
+  int tiles_m, tiles_n, splits;
+  int group;       // row tiles that are walked before the next column tile
+  uint32_t idesc;  // instruction descriptor
+  uint32_t* err;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+
+__device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                         uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else  // the barrier may lie in the other CTA of the pair
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// 128-byte swizzled operand. K-major: 8-row groups 1024 bytes apart.
+// MN-major: 64 rows x 8 k take 1024 bytes, the next 8 k follow, the next 64
+// rows lie 64 k further (8192 bytes).
+template <bool MN>
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  const uint64_t lead = MN ? 8192 >> 4 : 1, stride = 1024 >> 4;
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (lead << 16) | (stride << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+
+template <bool I8, int CG>
+__device__ __forceinline__ void issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                      uint32_t acc) {
+#define OM_MMA(KIND, GROUP)                                        \
+  asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"         \
+               "tcgen05.mma.cta_group::" GROUP ".kind::" KIND      \
+               " [%0], %1, %2, %3, p;\n}\n" ::"r"(d),              \
+               "l"(a), "l"(b), "r"(idesc), "r"(acc))
+  if constexpr (I8) {
+    if constexpr (CG == 1) OM_MMA("i8", "1");
+    else OM_MMA("i8", "2");
+  } else {
+    if constexpr (CG == 1) OM_MMA("f16", "1");
+    else OM_MMA("f16", "2");
+  }
+#undef OM_MMA
+}
+
+// arrives on the barrier (of both CTAs of a pair) when the MMAs issued so far
+// are done
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+__device__ __forceinline__ void read_columns(uint32_t addr, uint32_t (&x)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]),
+        "=r"(x[7]), "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]),
+        "=r"(x[14]), "=r"(x[15]), "=r"(x[16]), "=r"(x[17]), "=r"(x[18]), "=r"(x[19]), "=r"(x[20]),
+        "=r"(x[21]), "=r"(x[22]), "=r"(x[23]), "=r"(x[24]), "=r"(x[25]), "=r"(x[26]), "=r"(x[27]),
+        "=r"(x[28]), "=r"(x[29]), "=r"(x[30]), "=r"(x[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// the k slabs of split s: [first, last)
+__device__ __forceinline__ int slab_at(const Shape& g, int s) {
+  return (int)((int64_t)g.slabs * s / g.splits);
+}
+
+struct Tile {
+  int m, n, split;
+};
+__device__ __forceinline__ Tile tile_at(const Shape& g, int t) {
+  const int per = g.tiles_m * g.tiles_n;
+  Tile r;
+  r.split = t / per;
+  t -= r.split * per;
+  const int band = g.group * g.tiles_n, b = t / band, first = b * g.group;
+  const int rows = min(g.group, g.tiles_m - first);
+  t -= b * band;
+  r.m = first + t % rows;
+  r.n = t / rows;
+  return r;
+}
+
+// Epi, per lane and tile: Row begin(m, in, split) before the accumulator is
+// read; columns(row, m, in, n0, N, values) for each 32 columns from n0 on; and
+// end(row, m, in, slot) with slot = 2 * column tile + column group. `in`: row m
+// exists; columns from N on do not.
+template <bool I8, bool AMN, bool BMN, int CG, class Epi>
+__global__ void __launch_bounds__(THREADS, 1)
+    product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
+                   const __grid_constant__ Shape g, const __grid_constant__ Epi epi) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  // the same offset in both CTAs of a pair: the dynamic base is the same
+  const uint32_t ring = (smem_addr(smem_raw) + 1023) & ~1023u;
+  __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_base;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t rank = 0;
+  if constexpr (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  const int first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int tiles = g.tiles_m * g.tiles_n * g.splits;
+  const int b_rows = g.BN / CG;  // of B that this CTA loads
+  const uint32_t stage_bytes = A_BYTES + b_rows * SLAB;
+  const int kstep = I8 ? 128 : 64;  // elements of a slab
+
+  if (warp == 1) {
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+          smem_addr(&tmem_base)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+          smem_addr(&tmem_base)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+  }
+  if (tid == 0) {
+    for (int s = 0; s < g.stages; ++s) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&full[s])));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&empty[s])));
+    }
+    for (int b = 0; b < 2; ++b) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(&tfull[b])));
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(&tempty[b])),
+                   "r"(8 * CG));
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = tmem_base;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {  // loads
+      int q = 0, s = 0;
+      uint32_t phase = 1;  // of empty[s]: passes at once on the first round
+      for (int t = first; t < tiles && ok; t += step) {
+        const Tile at = tile_at(g, t);
+        const int m0 = (at.m * CG + (int)rank) * TM;
+        const int n0 = at.n * g.BN + (int)rank * b_rows;
+        const int k1 = slab_at(g, at.split + 1);
+        for (int k = slab_at(g, at.split); k < k1; ++k, ++q) {
+          if (q >= g.stages) ok = wait(smem_addr(&empty[s]), phase);
+          if (!ok) break;
+          uint32_t bar = smem_addr(&full[s]);
+          if (CG == 1 || rank == 0)
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                         "r"(stage_bytes * CG)
+                         : "memory");
+          if constexpr (CG == 2) bar = in_rank(bar, 0);
+          const uint32_t a = ring + s * stage_bytes, b = a + A_BYTES;
+          if constexpr (AMN) {
+            for (int i = 0; i < TM; i += 64) load_box<CG>(a + i * SLAB, &amap, m0 + i, k * kstep, bar);
+          } else {
+            load_box<CG>(a, &amap, k * kstep, m0, bar);
+          }
+          if constexpr (BMN) {
+            for (int i = 0; i < b_rows; i += 64)
+              load_box<CG>(b + i * SLAB, &bmap, n0 + i, k * kstep, bar);
+          } else {
+            load_box<CG>(b, &bmap, k * kstep, n0, bar);
+          }
+          if (++s == g.stages) s = 0, phase ^= 1;
+        }
+      }
+      if (!ok) atomicOr(g.err, 1u);
+      // nothing of the last round is in flight when the block leaves: the
+      // stages' products are done, or (after an expired wait) their copies in
+      for (int j = max(0, q - g.stages); j < q; ++j) {
+        uint64_t* bar = ok ? empty : full;
+        if (ok || rank == 0) wait(smem_addr(&bar[j % g.stages]), (j / g.stages) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {  // products
+      int s = 0, i = 0;
+      uint32_t phase = 0;
+      for (int t = first; t < tiles && ok; t += step, ++i) {
+        const Tile at = tile_at(g, t);
+        const int ab = i & 1;
+        if (i >= 2) ok = wait(smem_addr(&tempty[ab]), ((i >> 1) - 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        const uint32_t d = tmem + ab * 256;
+        const int k0 = slab_at(g, at.split), k1 = slab_at(g, at.split + 1);
+        for (int k = k0; k < k1; ++k) {
+          ok = wait(smem_addr(&full[s]), phase);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;");
+          const uint32_t a = ring + s * stage_bytes, b = a + A_BYTES;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            issue<I8, CG>(d, operand<AMN>(a + j * (AMN ? 2048 : 32)),
+                          operand<BMN>(b + j * (BMN ? 2048 : 32)), g.idesc, k > k0 || j > 0);
+          commit<CG>(smem_addr(&empty[s]));
+          if (++s == g.stages) s = 0, phase ^= 1;
+        }
+        commit<CG>(smem_addr(&tfull[ab]));
+      }
+      if (!ok) atomicOr(g.err, 1u);
+    }
+  } else {  // epilogue
+    const int quad = warp & 3, part = (warp - 2) >> 2;
+    int i = 0;
+    for (int t = first; t < tiles; t += step, ++i) {
+      const Tile at = tile_at(g, t);
+      const int ab = i & 1;
+      const int m = (at.m * CG + (int)rank) * TM + 32 * quad + lane;
+      const bool in = m < g.M;
+      typename Epi::Row row = epi.begin(m, in, at.split);
+      ok = wait(smem_addr(&tfull[ab]), (i >> 1) & 1);
+      if (!ok) break;
+      asm volatile("tcgen05.fence::after_thread_sync;");
+      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16) + ab * 256;
+      for (int c = part * 32; c < g.BN; c += 64) {
+        uint32_t r[32];
+        read_columns(base + c, r);
+        epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;");
+      __syncwarp();
+      if (lane == 0) {
+        uint32_t bar = smem_addr(&tempty[ab]);
+        if constexpr (CG == 2) bar = in_rank(bar, 0);
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                     : "memory");
+      }
+      epi.end(row, m, in, at.n * 2 + part);
+    }
+    if (!ok && lane == 0) atomicOr(g.err, 1u);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  if (warp == 1) {
+    if constexpr (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// ---- host side ---------------------------------------------------------------
+
+// A matrix operand: `rows` x `k` elements of 1 or 2 bytes; K-major: rows `ld`
+// elements apart; MN-major: k steps `ld` apart.
+struct Matrix {
+  const void* ptr;
+  int64_t rows, k, ld;
+  int elem;
+};
+
+inline bool tma_readable(const void* ptr, int64_t ld, int elem) {
+  return ((uintptr_t)ptr & 15) == 0 && ld > 0 && (ld * elem) % 16 == 0 &&
+         ld * elem < ((int64_t)1 << 40);
+}
+
+inline int encode(CUtensorMap* map, const Matrix& x, bool mn, int box_rows) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+  const cuuint64_t dims[2] = {(cuuint64_t)(mn ? x.rows : x.k), (cuuint64_t)(mn ? x.k : x.rows)};
+  const cuuint64_t strides[1] = {(cuuint64_t)(x.ld * x.elem)};
+  const cuuint32_t box[2] = {(cuuint32_t)(SLAB / x.elem), (cuuint32_t)(mn ? SLAB / x.elem : box_rows)};
+  const cuuint32_t one[2] = {1, 1};
+  const CUresult r = fn(map, x.elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                        2, (void*)x.ptr, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return OM_OK;
+}
+
+// Instruction descriptor: accumulator format (f32 / s32), operand formats,
+// which operands are MN-major, the tile's columns and rows.
+inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, int cols) {
+  const uint32_t d = i8 ? 2 : 1, fmt = i8 ? 1 : (bf16 ? 1 : 0);
+  return (d << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)amn << 15) | ((uint32_t)bmn << 16) |
+         ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24);
+}
+
+// D = A B^T through `epi`. bn: tile columns (32, 64, 128 or 256; at least 64
+// for an MN-major B); pair: two CTAs per tile (bn 128 or 256). splits > 1
+// cuts k into that many ranges of whole slabs, each handed to the epilogue
+// as its own tile.
+template <bool I8, bool AMN, bool BMN, int CG, class Epi>
+int launch_product(om_backend* be, const char* name, const Matrix& a, const Matrix& b, bool bf16,
+                   int bn, int splits, const Epi& epi) {
+  const int kstep = I8 ? 128 : 64;
+  const int64_t tm = (a.rows + TM * CG - 1) / (TM * CG), tn = (b.rows + bn - 1) / bn;
+  const int64_t slabs = (a.k + kstep - 1) / kstep;
+  if (a.rows > 0x7fffff00 || b.rows > 0x7fffff00 || a.k > 0x7fffff00 || splits < 1 ||
+      splits > slabs || tm * tn * splits > 0x7fffffff)
+    return set_error(OM_ERR_SHAPE, std::string(name) + ": extents out of range");
+  CUtensorMap ma, mb;
+  OM_TRY(encode(&ma, a, AMN, TM));
+  OM_TRY(encode(&mb, b, BMN, bn / CG));
+  Shape g{};
+  g.M = (int)a.rows, g.N = (int)b.rows, g.slabs = (int)slabs, g.BN = bn;
+  g.tiles_m = (int)tm, g.tiles_n = (int)tn, g.splits = splits;
+  // a wave's tiles form a square of rows and columns, so that each slab is
+  // read by many SMs while it is in L2
+  g.group = std::max(1, std::min<int>((int)tm, CG == 2 ? 8 : 16));
+  const int stage = A_BYTES + bn / CG * SLAB;
+  g.stages = std::min(MAX_STAGES, 208 * 1024 / stage);
+  g.idesc = instruction(I8, bf16, AMN, BMN, TM * CG, bn);
+  g.err = be->d_flags + 1;
+  const size_t smem = (size_t)g.stages * stage + 1024;
+  auto kernel = product_kernel<I8, AMN, BMN, CG, Epi>;
+  OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), name);
+  const int64_t work = tm * tn * splits;
+  ProfScope prof(be, name);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(work, be->num_sms / CG)));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = be->stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  OM_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, epi), name);
+  note_launch();
+  return OM_OK;
+}
+
+}  // namespace mma
+}  // namespace om
