@@ -36,6 +36,30 @@ struct Elem<__half> {
   static __device__ __forceinline__ __half store(float v) { return __float2half_rn(v); }
 };
 
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// 32 values of a row as T, 16 bytes at a time
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 8)
+    *reinterpret_cast<uint4*>(dst + c) =
+        make_uint4(pack2(v[c], v[c + 1], T()), pack2(v[c + 2], v[c + 3], T()),
+                   pack2(v[c + 4], v[c + 5], T()), pack2(v[c + 6], v[c + 7], T()));
+}
+__device__ __forceinline__ void store_row(float* dst, const float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 4)
+    *reinterpret_cast<float4*>(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+}
+
 inline bool is_half(om_dtype dt) { return dt == OM_BF16 || dt == OM_F16; }
 
 }  // namespace om

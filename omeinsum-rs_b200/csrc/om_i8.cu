@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "om_convert.cuh"
+#include "om_sm100.cuh"
 
 namespace om {
 namespace {
@@ -56,31 +57,142 @@ struct I8Args {
   int64_t yn, ym;
 };
 
-// 32 x 32 outputs per block of 256 threads, 32 k per step
+__device__ __forceinline__ float scaled(int acc, float q_scale, float w_scale) {
+  return __fmul_rn(__fmul_rn((float)acc, q_scale), w_scale);
+}
+
+// ---- many rows: tensor cores ---------------------------------------------------
+
 template <typename T>
-__global__ void matmul_i8_kernel(I8Args p, int64_t tiles_n) {
-  __shared__ int8_t a[32][33], b[32][33];
-  const int64_t m0 = blockIdx.x / tiles_n * 32, n0 = blockIdx.x % tiles_n * 32;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  int acc[4] = {0, 0, 0, 0};
-  for (int64_t k0 = 0; k0 < p.K; k0 += 32) {
-    for (int i = ty; i < 32; i += 8) {
-      const bool in = k0 + tx < p.K;
-      a[i][tx] = in && m0 + i < p.M ? p.q[(m0 + i) * p.qm + (k0 + tx) * p.qk] : (int8_t)0;
-      b[i][tx] = in && n0 + i < p.N ? p.w[(n0 + i) * p.wn + (k0 + tx) * p.wk] : (int8_t)0;
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
-      for (int i = 0; i < 4; ++i) acc[i] += (int)a[ty + 8 * i][k] * (int)b[tx][k];
-    __syncthreads();
+struct ScaleEpi {
+  const float *q_scale, *w_scale, *bias;
+  T* y;
+  int64_t dr, dc;
+  int vec;  // rows of y may be written, and w_scale and bias read, 16 bytes at a time
+  struct Row {
+    float s;
+  };
+  __device__ __forceinline__ Row begin(int m, bool in, int) const {
+    return Row{in ? q_scale[m] : 0.f};
   }
-  const int64_t n = n0 + tx;
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + ty + 8 * i;
-    if (m >= p.M || n >= p.N) continue;
-    float v = __fmul_rn(__fmul_rn((float)acc[i], p.q_scale[m]), p.w_scale[n]);
-    if (p.bias) v = __fadd_rn(v, p.bias[n]);
-    ((T*)p.y)[m * p.ym + n * p.yn] = Elem<T>::store(v);
+  __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
+                                          const uint32_t (&r)[32]) const {
+    if (!in || n0 >= N) return;
+    T* to = y + (int64_t)m * dr;
+    if (vec && N - n0 >= 32) {
+      float v[32];
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) {
+        const float4 w = __ldg(reinterpret_cast<const float4*>(w_scale + n0 + c));
+        v[c] = scaled((int)r[c], row.s, w.x);
+        v[c + 1] = scaled((int)r[c + 1], row.s, w.y);
+        v[c + 2] = scaled((int)r[c + 2], row.s, w.z);
+        v[c + 3] = scaled((int)r[c + 3], row.s, w.w);
+        if (bias) {
+          const float4 b = __ldg(reinterpret_cast<const float4*>(bias + n0 + c));
+          v[c] = __fadd_rn(v[c], b.x), v[c + 1] = __fadd_rn(v[c + 1], b.y);
+          v[c + 2] = __fadd_rn(v[c + 2], b.z), v[c + 3] = __fadd_rn(v[c + 3], b.w);
+        }
+      }
+      store_row(to + n0, v);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (n0 + c < N) {
+          float v = scaled((int)r[c], row.s, w_scale[n0 + c]);
+          if (bias) v = __fadd_rn(v, bias[n0 + c]);
+          to[(n0 + c) * dc] = Elem<T>::store(v);
+        }
+    }
+  }
+  __device__ __forceinline__ void end(Row&, int, bool, int) const {}
+};
+
+// Rows of 8-bit numbers at 16-byte aligned places, zero behind their end
+__global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int64_t K, int64_t sr,
+                        int64_t sk, int8_t* __restrict__ dst, int64_t ld) {
+  const int64_t total = rows * ld;
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / ld, c = i - r * ld;
+    dst[i] = c < K ? src[r * sr + c * sk] : (int8_t)0;
+  }
+}
+
+// ---- few rows: the weights stream through the CUDA cores --------------------------
+
+constexpr int TOKEN_ROWS = 8;
+constexpr int TOKEN_SMEM = 160 * 1024;
+
+// A block keeps the M <= MM rows of q in shared memory and walks its share of
+// the channels, a warp per channel: 16 weights per lane and step, four
+// products per instruction, one shuffle reduction per row. T: the type of y,
+// and of x where the rows are quantised here (q == null).
+template <typename T, int MM>
+__global__ void __launch_bounds__(256) token_i8_kernel(I8Args p, const T* __restrict__ x,
+                                                       int64_t xk, int64_t xm, int64_t Kp) {
+  extern __shared__ __align__(16) int8_t qs[];  // [MM][Kp]
+  __shared__ float scale[MM];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int M = (int)p.M;
+  for (int m = 0; m < M; ++m) {
+    if (p.q) {
+      for (int64_t k = tid; k < Kp; k += 256)
+        qs[m * Kp + k] = k < p.K ? p.q[m * p.qm + k * p.qk] : (int8_t)0;
+      if (tid == 0) scale[m] = p.q_scale[m];
+    } else {
+      const T* xr = x + m * xm;
+      float top = 0.f;
+      for (int64_t k = tid; k < p.K; k += 256) top = max_abs(top, Elem<T>::load(xr[k * xk]));
+      top = block_max_abs(top);
+      const float s = __fdiv_rn(top, 127.f);
+      for (int64_t k = tid; k < Kp; k += 256)
+        qs[m * Kp + k] =
+            k < p.K && s > 0.f ? quantized(Elem<T>::load(xr[k * xk]), s) : (int8_t)0;
+      if (tid == 0) scale[m] = s;
+      __syncthreads();  // block_max_abs's scratch is used again
+    }
+  }
+  __syncthreads();
+  const int64_t n0 = p.N * blockIdx.x / gridDim.x, n1 = p.N * (blockIdx.x + 1) / gridDim.x;
+  for (int64_t n = n0 + warp; n < n1; n += 8) {
+    const int8_t* wr = p.w + n * p.wn;
+    int acc[MM];
+#pragma unroll
+    for (int m = 0; m < MM; ++m) acc[m] = 0;
+#pragma unroll 4
+    for (int64_t k = lane * 16; k < Kp; k += 512) {
+      int4 w = make_int4(0, 0, 0, 0);
+      if (k + 16 <= p.K) {
+        w = __ldcs(reinterpret_cast<const int4*>(wr + k));
+      } else {  // the row's end: nothing behind it is read
+        __align__(16) int8_t tail[16] = {};
+#pragma unroll
+        for (int i = 0; i < 15; ++i)
+          if (k + i < p.K) tail[i] = wr[k + i];
+        w = *reinterpret_cast<const int4*>(tail);
+      }
+#pragma unroll
+      for (int m = 0; m < MM; ++m) {
+        if (m >= M) break;
+        const int4 q = *reinterpret_cast<const int4*>(qs + m * Kp + k);
+        acc[m] = __dp4a(w.x, q.x, acc[m]);
+        acc[m] = __dp4a(w.y, q.y, acc[m]);
+        acc[m] = __dp4a(w.z, q.z, acc[m]);
+        acc[m] = __dp4a(w.w, q.w, acc[m]);
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MM; ++m) {
+      if (m >= M) break;
+      int a = acc[m];
+      for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (lane == m) {
+        float v = scaled(a, scale[m], p.w_scale[n]);
+        if (p.bias) v = __fadd_rn(v, p.bias[n]);
+        ((T*)p.y)[m * p.ym + n * p.yn] = Elem<T>::store(v);
+      }
+    }
   }
 }
 
@@ -101,17 +213,86 @@ int quantize(om_backend* be, om_dtype dtype, int64_t K, int64_t M, const void* x
   return launch_quantize<float>(be, K, M, x, sx, q, qk, qm, scale);
 }
 
-template <typename T>
-int launch_matmul(om_backend* be, const I8Args& p) {
-  const int64_t tm = (p.M + 31) / 32, tn = (p.N + 31) / 32;
-  if (tm * tn > 0x7fffffff) return set_error(OM_ERR_SHAPE, "matmul_i8: too many tiles");
-  ProfScope prof(be, "matmul_i8");
-  matmul_i8_kernel<T><<<(unsigned)(tm * tn), 256, 0, be->stream>>>(p, tn);
+// Whether the weights can be read in place 16 bytes at a time; else they are
+// packed for the call.
+int readable_i8(om_backend* be, const int8_t* src, int64_t rows, int64_t K, int64_t sr, int64_t sk,
+                Scratch& copy, mma::Matrix* out) {
+  *out = mma::Matrix{src, rows, K, sr, 1};
+  if ((sk == 1 || K == 1) && sr >= K && mma::tma_readable(src, sr, 1)) return OM_OK;
+  const int64_t ld = (K + 15) / 16 * 16;
+  OM_TRY(copy.alloc(be, (size_t)rows * ld));
+  const int64_t n = rows * ld;
+  pack_i8<<<(unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)be->num_sms * 32), 256, 0,
+            be->stream>>>(src, rows, K, sr, sk, (int8_t*)copy.ptr, ld);
+  note_launch();
+  *out = mma::Matrix{copy.ptr, rows, K, ld, 1};
+  return check_cuda(cudaGetLastError(), "matmul_i8 pack launch");
+}
+
+template <typename T, int MM>
+int launch_token_rows(om_backend* be, const I8Args& p, const T* x, int64_t xk, int64_t xm,
+                      int64_t Kp) {
+  const size_t smem = (size_t)p.M * Kp;
+  if (smem > 48 * 1024)
+    OM_CUDA(cudaFuncSetAttribute(token_i8_kernel<T, MM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 TOKEN_SMEM),
+            "matmul_i8");
+  const int64_t blocks = std::min<int64_t>((p.N + 7) / 8, (int64_t)be->num_sms * 2);
+  ProfScope prof(be, "matmul_i8_token");
+  token_i8_kernel<T, MM><<<(unsigned)blocks, 256, smem, be->stream>>>(p, x, xk, xm, Kp);
   note_launch();
   return check_cuda(cudaGetLastError(), "matmul_i8 launch");
 }
 
+bool few_rows(int64_t M, int64_t K) {
+  return M <= TOKEN_ROWS && M * ((K + 15) / 16 * 16) <= TOKEN_SMEM;
+}
+
+// p.q == null: the rows are x's, quantised within the kernel
+template <typename T>
+int launch_tokens(om_backend* be, I8Args p, const T* x, int64_t xk, int64_t xm) {
+  Scratch copy;
+  mma::Matrix w;
+  OM_TRY(readable_i8(be, p.w, p.N, p.K, p.wn, p.wk, copy, &w));
+  p.w = (const int8_t*)w.ptr;
+  p.wn = w.ld;
+  const int64_t Kp = (p.K + 15) / 16 * 16;
+  if (p.M == 1) return launch_token_rows<T, 1>(be, p, x, xk, xm, Kp);
+  if (p.M <= 4) return launch_token_rows<T, 4>(be, p, x, xk, xm, Kp);
+  return launch_token_rows<T, 8>(be, p, x, xk, xm, Kp);
+}
+
+template <typename T>
+int launch_matmul(om_backend* be, const I8Args& p) {
+  if (few_rows(p.M, p.K)) return launch_tokens<T>(be, p, nullptr, 0, 0);
+  Scratch qc, wc;
+  mma::Matrix q, w;
+  OM_TRY(readable_i8(be, p.q, p.M, p.K, p.qm, p.qk, qc, &q));
+  OM_TRY(readable_i8(be, p.w, p.N, p.K, p.wn, p.wk, wc, &w));
+  const int vec = p.yn == 1 && (p.ym * (int64_t)sizeof(T)) % 16 == 0 && !((uintptr_t)p.y & 15) &&
+                  !((uintptr_t)p.w_scale & 15) && !((uintptr_t)p.bias & 15);
+  const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn, vec};
+  const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
+  if (t.pair) return mma::launch_product<true, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
+  return mma::launch_product<true, false, false, 1>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
+}
+
 int matmul(om_backend* be, om_dtype dtype, const I8Args& p) {
+  if (p.K == 0) {  // nothing is summed: the token kernel's loop is empty
+    I8Args one = p;
+    for (int64_t m = 0; m < p.M; m += TOKEN_ROWS) {
+      one.M = std::min<int64_t>(TOKEN_ROWS, p.M - m);
+      one.q_scale = p.q_scale + m;
+      one.q = (const int8_t*)p.q_scale;  // not read
+      one.w = (const int8_t*)p.w_scale;
+      one.wn = 16, one.wk = 1;
+      one.y = (char*)p.y + m * p.ym * (dtype == OM_F32 ? 4 : 2);
+      if (dtype == OM_BF16) OM_TRY((launch_token_rows<__nv_bfloat16, 8>(be, one, nullptr, 0, 0, 0)));
+      else if (dtype == OM_F16) OM_TRY((launch_token_rows<__half, 8>(be, one, nullptr, 0, 0, 0)));
+      else OM_TRY((launch_token_rows<float, 8>(be, one, nullptr, 0, 0, 0)));
+    }
+    return OM_OK;
+  }
   if (dtype == OM_BF16) return launch_matmul<__nv_bfloat16>(be, p);
   if (dtype == OM_F16) return launch_matmul<__half>(be, p);
   return launch_matmul<float>(be, p);
@@ -182,6 +363,14 @@ extern "C" int om_b200_linear_i8(om_backend* be, om_dtype dtype, const int64_t* 
   OM_CUDA(guard.status, "linear_i8: device");
   const int64_t none[2] = {0, 0};
   if (!K) strides_x = strides_w = none;
+  if (K && few_rows(M, K)) {
+    const I8Args p{M, N, K, nullptr, 0, 0, (const int8_t*)w, strides_w[0], strides_w[1], nullptr,
+                   w_scale, bias, y, strides_y[0], strides_y[1]};
+    if (dtype == OM_BF16)
+      return launch_tokens(be, p, (const __nv_bfloat16*)x, strides_x[0], strides_x[1]);
+    if (dtype == OM_F16) return launch_tokens(be, p, (const __half*)x, strides_x[0], strides_x[1]);
+    return launch_tokens(be, p, (const float*)x, strides_x[0], strides_x[1]);
+  }
   const int64_t Kp = (K + 15) / 16 * 16;
   Scratch ws;
   OM_TRY(ws.alloc(be, (size_t)M * (Kp + 4) + 16));

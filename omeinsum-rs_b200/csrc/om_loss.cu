@@ -380,25 +380,6 @@ __global__ void gradient_scale(const float* __restrict__ dloss, const void* targ
   *scale = f >= FLT_MIN && f < INFINITY ? f : 1.f;
 }
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// 32 values of a row as T, 16 bytes at a time
-template <typename T>
-__device__ __forceinline__ void store_half_row(T* dst, const float (&v)[32]) {
-#pragma unroll
-  for (int c = 0; c < 32; c += 8)
-    *reinterpret_cast<uint4*>(dst + c) =
-        make_uint4(pack2(v[c], v[c + 1], T()), pack2(v[c + 2], v[c + 3], T()),
-                   pack2(v[c + 4], v[c + 5], T()), pack2(v[c + 6], v[c + 7], T()));
-}
-
 // dz of a piece, rounded to T; the buffer's rows hold whole tiles
 template <typename T>
 struct GradEpi {
@@ -439,7 +420,7 @@ struct GradEpi {
       for (int c = 0; c < 32; ++c)
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
     }
-    store_half_row(dz + (int64_t)m * ld + n0, v);
+    store_row(dz + (int64_t)m * ld + n0, v);
   }
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
@@ -485,7 +466,7 @@ struct OutEpi {
     for (int c = 0; c < 32; ++c) v[c] *= row.f;
     T* to = out + (int64_t)m * dr;
     if (vec && N - n0 >= 32) {
-      store_half_row(to + n0, v);
+      store_row(to + n0, v);
     } else {
 #pragma unroll
       for (int c = 0; c < 32; ++c)
@@ -545,23 +526,9 @@ int readable(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t s
   return check_cuda(cudaGetLastError(), "loss pack launch");
 }
 
-// Tile columns and whether a pair of CTAs shares a tile, from the result's
-// size: pairs of 256 x 256 when they fill the card, else the widest tile of
-// one CTA that gives three quarters of the SMs one.
-struct Tiling {
-  int bn, pair;
-};
-Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
-  if (M > mma::TM && (M + 255) / 256 * ((N + 255) / 256) >= be->num_sms / 2) return {256, 0};
-  const int64_t tm = (M + mma::TM - 1) / mma::TM;
-  for (int bn = 256; bn > least; bn /= 2)
-    if (tm * ((N + bn - 1) / bn) * 4 >= be->num_sms * 3) return {bn, 0};
-  return {least, 0};
-}
-
 template <bool AMN, bool BMN, class Epi>
 int product16(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
-              bool bf16, Tiling t, int splits, const Epi& epi) {
+              bool bf16, mma::Tiling t, int splits, const Epi& epi) {
   if (t.pair) return mma::launch_product<false, AMN, BMN, 2>(be, name, a, b, bf16, t.bn, splits, epi);
   return mma::launch_product<false, AMN, BMN, 1>(be, name, a, b, bf16, t.bn, splits, epi);
 }
@@ -573,7 +540,7 @@ int loss_forward16(om_backend* be, const LossArgs& p, float* loss, float* lse) {
   mma::Matrix x, w;
   OM_TRY(readable<T>(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
   OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
-  const Tiling t = tiling(be, p.N, p.V, 64);
+  const mma::Tiling t = mma::tiling(be, p.N, p.V, 64);
   const int64_t slots = (p.V + t.bn - 1) / t.bn * 2;
   OM_TRY(ws.alloc(be, (size_t)p.N * (slots * 8 + 4)));
   float2* part = (float2*)ws.ptr;
@@ -617,7 +584,7 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
   note_launch();
   // dx sums over the vocabulary: few tokens and a narrow width leave SMs idle
   // unless the sum is split; each split needs 8 slabs to be worth its f32 sums
-  const Tiling tx = tiling(be, p.N, p.D, 64);
+  const mma::Tiling tx = mma::tiling(be, p.N, p.D, 64);
   const int64_t rows = tx.pair ? 256 : 128;
   const int64_t txt = (p.N + rows - 1) / rows * ((p.D + tx.bn - 1) / tx.bn);
   const int64_t slots = tx.pair ? be->num_sms / 2 : be->num_sms;
@@ -636,7 +603,7 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
     const mma::Matrix x{xs.ptr, p.N, p.D, Dp, 2};
     const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dz, P};
     OM_TRY((product16<false, false>(be, "loss_dlogits", x, mma::Matrix{wp, n, p.D, w.ld, 2}, bf16,
-                                    tiling(be, p.N, n, 64), 1, ge)));
+                                    mma::tiling(be, p.N, n, 64), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
     const OutEpi<T> xe{dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
     OM_TRY((product16<false, true>(be, "loss_dx", mma::Matrix{dz, p.N, n, P, 2},
@@ -644,7 +611,7 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
     const OutEpi<T> we{dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
     OM_TRY((product16<true, true>(be, "loss_dw", mma::Matrix{dz, n, p.N, P, 2},
                                   mma::Matrix{xs.ptr, p.D, p.N, Dp, 2}, bf16,
-                                  tiling(be, n, p.D, 64), 1, we)));
+                                  mma::tiling(be, n, p.D, 64), 1, we)));
   }
   if (splits > 1) {
     ProfScope prof(be, "loss_join_splits");

@@ -379,6 +379,20 @@ inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, in
          ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24);
 }
 
+// Tile columns and whether a pair of CTAs shares a tile, from the result's
+// size: pairs of 256 x 256 when they fill the card, else the widest tile of
+// one CTA that gives three quarters of the SMs one.
+struct Tiling {
+  int bn, pair;
+};
+inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
+  if (M > TM && (M + 255) / 256 * ((N + 255) / 256) >= be->num_sms / 2) return {256, 1};
+  const int64_t tm = (M + TM - 1) / TM;
+  for (int bn = 256; bn > least; bn /= 2)
+    if (tm * ((N + bn - 1) / bn) * 4 >= be->num_sms * 3) return {bn, 0};
+  return {least, 0};
+}
+
 // D = A B^T through `epi`. bn: tile columns (32, 64, 128 or 256; at least 64
 // for an MN-major B); pair: two CTAs per tile (bn 128 or 256). splits > 1
 // cuts k into that many ranges of whole slabs, each handed to the epilogue

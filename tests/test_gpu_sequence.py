@@ -238,6 +238,15 @@ def test_loss(be, seq, shape, dtype):
     check_loss(be, seq, up(x), up(w), seq.upload(be, targets, "i64"), seq.upload(be, g), x, w, targets, g, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("shape", [(600, 72, 6500), (2300, 2100, 2305), (130, 264, 9700)], ids=str)
+def test_loss_in_pairs_of_sms(be, seq, shape, dtype):
+    """Results large enough for two SMs to share a tile, with ragged ends."""
+    x, w, targets, g = loss_inputs(sum(shape), *shape, dtype)
+    up = lambda v: seq.upload(be, v, dtype)  # noqa: E731
+    check_loss(be, seq, up(x), up(w), seq.upload(be, targets, "i64"), seq.upload(be, g), x, w, targets, g, dtype)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("layout", ["transposed", "offset", "wide_rows"])
 def test_loss_strides(be, seq, layout, dtype):
