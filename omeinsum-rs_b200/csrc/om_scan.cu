@@ -1,4 +1,23 @@
-// Gated linear recurrence h_t = a_t h_{t-1} + b_t and its backward pass.
+// Gated linear recurrence h_t = a_t h_{t-1} + b_t and its backward pass
+//     S_t = a_t (dh_t + S_{t+1}),   G_t = dh_t + S_{t+1},
+// in one pass over the data: each element is read once and written once.
+//
+// A step is the map s -> P s + Q with (P, Q) = (a, b) (backward: (a, a dh)), and
+// maps compose, so time can be cut. A tile is 256 bytes of channels (32 lanes
+// of 8 bytes) by up to 64 steps, four warps of 16 steps each; it is copied to
+// shared memory asynchronously and lives there until its results have taken
+// its place. Each warp first composes its 16 steps (from shared memory), the
+// block its four warps, and, where a sequence has more than one tile, tiles
+// find the state that enters them by looking back: 32 consecutive tiles of one
+// column form a group; a tile composes the maps of its predecessors in the
+// group with the state that left the group before, and the group's last tile
+// passes the state on. So the serial chain has one link per 2048 steps, and
+// every sum is formed in one order whatever the timing. Tiles are handed out by
+// a counter, first tiles first, so whatever a tile waits for has started.
+//
+// Bound by HBM: 3 arrays (forward) or 5 to 6 (backward) per element; the two
+// passes over shared memory cost instructions, not traffic, and leave six
+// tiles (32 KiB each) per SM in flight, which hides the look-back.
 #include <algorithm>
 
 #include "om_convert.cuh"
@@ -28,99 +47,556 @@ struct ScanArgs {
   void* dh0;
 };
 
-// a = sigmoid(g) and 1 - a without cancellation on either side
+constexpr int ROW = 256;       // bytes of channels in a tile
+constexpr int STEPS = 16;      // of a warp
+constexpr int WARPS = 4;       // of a block
+constexpr int GROUP = 32;      // tiles that look back at one another
+constexpr uint32_t POLL_LIMIT = 1u << 22;
+
+struct TileArgs {
+  int64_t channels;  // B * D
+  int grain;         // bytes of a row that one copy moves
+  int warps_t;       // warps along time: 4, or 1 (then the block has four columns)
+  int rows;          // steps of a tile
+  int columns;       // of 256 bytes
+  int tiles;         // along time
+  // looking back; null when a sequence is one tile
+  uint32_t* ticket;
+  uint32_t* flags;   // [tile][column]: the tile's map is in `maps`
+  uint64_t* state;   // [group][channel][words]: 32 bits of the state and a set mark
+  void* maps;        // [tile][channel] pairs (P, Q)
+  uint32_t* err;
+};
+
+// a = sigmoid(g) and 1 - a without cancellation. f32: an exponential formed as
+// a power of two and an approximate reciprocal, together below 24 half steps
+// for |g| <= 16 (most of it the rounding of the exponent).
 template <typename S>
 __device__ __forceinline__ void sigmoid_pair(S g, S* a, S* keep) {
-  const S e = exp(-fabs(g));
-  const S r = S(1) / (S(1) + e);
-  *a = g >= 0 ? r : e * r;
-  *keep = g >= 0 ? e * r : r;
-  if (g != g) *a = *keep = g;
+  if constexpr (sizeof(S) == 4) {
+    float e, r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    *a = r;
+    *keep = e > 1.f ? 1.f - r : e * r;  // e may be infinite, r is then 0
+  } else {
+    const S e = exp(-fabs(g));
+    const S r = S(1) / (S(1) + e);
+    *a = g >= 0 ? r : e * r;
+    *keep = g >= 0 ? e * r : r;
+    if (g != g) *a = *keep = g;
+  }
 }
 
-// One thread per channel, step by step.
-template <typename T, bool SIG>
-__global__ void scan_forward(ScanArgs p) {
-  using S = typename Elem<T>::State;
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= p.D * p.B) return;
-  const int64_t d = i % p.D, b = i / p.D;
-  int64_t len = p.T;
-  if (p.lengths) len = min(max((int64_t)p.lengths[b], (int64_t)0), p.T);
-  const T* g = (const T*)p.gate + d * p.gd + b * p.gb;
-  const T* x = (const T*)p.x + d * p.xd + b * p.xb;
-  T* h = (T*)p.h + d * p.hd + b * p.hb;
-  S s = p.h0 ? ((const S*)p.h0)[i] : S(0);
-  for (int64_t t = 0; t < len; ++t) {
-    S a = Elem<T>::load(g[t * p.gt]), v = Elem<T>::load(x[t * p.xt]);
-    if constexpr (SIG) {
-      S keep;
-      sigmoid_pair(a, &a, &keep);
-      v *= keep;
+// ---- data of a tile --------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t shared_at(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(shared_at(dst)), "l"(src), "n"(N)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at(dst)), "l"(src)
+               : "memory");
+}
+
+// One array's view in bytes; `shift`: row r of the tile is step t0 + r + shift
+struct View {
+  const char* ptr;
+  int64_t d, t, b;
+};
+
+// Calls f(shared place, global place) for each piece of `grain` bytes of rows
+// [r0, r1) of column `col` that lies inside the array, threads tt of tn.
+template <typename F>
+__device__ __forceinline__ void each_piece(const TileArgs& a, int64_t D, int elem, const View& v,
+                                           char* tile, int col, int64_t t0, int r0, int r1,
+                                           int64_t first, int64_t last, int tt, int tn, F f) {
+  const int per_row = ROW / a.grain, lanes = min(per_row, tn);
+  for (int p = tt % lanes; p < per_row; p += lanes) {
+    const int64_t c = ((int64_t)col * per_row + p) * a.grain / elem;
+    if (c >= a.channels) break;
+    const int64_t b = (uint64_t)c / (uint64_t)D, d = c - b * D;
+    const char* g = v.ptr + b * v.b + d * v.d + t0 * v.t;
+    for (int r = r0 + tt / lanes; r < r1; r += tn / lanes) {
+      const int64_t t = t0 + r;
+      if (t >= first && t < last) f(tile + r * ROW + p * a.grain, g + (int64_t)r * v.t);
     }
-    s = a * s + v;
-    h[t * p.ht] = Elem<T>::store(s);
   }
-  for (int64_t t = len; t < p.T; ++t) h[t * p.ht] = Elem<T>::store(S(0));
-  if (p.h_last) ((S*)p.h_last)[i] = s;
 }
 
-template <typename T, bool SIG>
-__global__ void scan_backward(ScanArgs p) {
-  using S = typename Elem<T>::State;
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-  if (i >= p.D * p.B) return;
-  const int64_t d = i % p.D, b = i / p.D;
-  int64_t len = p.T;
-  if (p.lengths) len = min(max((int64_t)p.lengths[b], (int64_t)0), p.T);
-  const T* g = (const T*)p.gate + d * p.gd + b * p.gb;
-  const T* x = (const T*)p.x + d * p.xd + b * p.xb;
-  const T* h = (const T*)p.h + d * p.hd + b * p.hb;
-  const T* e = (const T*)p.dh + d * p.ed + b * p.eb;
-  T* dg = (T*)p.dgate + d * p.pd + b * p.pb;
-  T* dx = (T*)p.dx + d * p.qd + b * p.qb;
-  const S start = p.h0 ? ((const S*)p.h0)[i] : S(0);
-  S carry = p.dh_last ? ((const S*)p.dh_last)[i] : S(0);  // a_{t+1} G_{t+1}
-  for (int64_t t = p.T - 1; t >= len; --t) {
-    dg[t * p.pt] = Elem<T>::store(S(0));
-    dx[t * p.qt] = Elem<T>::store(S(0));
-  }
-  for (int64_t t = len - 1; t >= 0; --t) {
-    S a = Elem<T>::load(g[t * p.gt]);
-    const S total = Elem<T>::load(e[t * p.et]) + carry;
-    const S before = t ? (S)Elem<T>::load(h[(t - 1) * p.ht]) : start;
-    S sx = total, sg = total * before;
-    if constexpr (SIG) {
-      S keep;
-      sigmoid_pair(a, &a, &keep);
-      sx = total * keep;
-      sg = total * (before - Elem<T>::load(x[t * p.xt])) * (a * keep);
-    }
-    dx[t * p.qt] = Elem<T>::store(sx);
-    dg[t * p.pt] = Elem<T>::store(sg);
-    carry = a * total;
-  }
-  if (p.dh0) ((S*)p.dh0)[i] = carry;
-}
-
-template <typename T, bool SIG>
-int launch_scan(om_backend* be, const ScanArgs& p, bool backward) {
-  const int64_t n = p.D * p.B;
-  const int64_t blocks = (n + 127) / 128;
-  if (blocks > 0x7fffffff) return set_error(OM_ERR_INVALID, "gated_scan: too many channels");
-  ProfScope prof(be, backward ? "gated_scan_backward" : "gated_scan");
-  if (backward)
-    scan_backward<T, SIG><<<(unsigned)blocks, 128, 0, be->stream>>>(p);
+__device__ __forceinline__ void load_rows(const TileArgs& a, int64_t D, int elem, const View& v,
+                                          char* tile, int col, int64_t t0, int64_t first,
+                                          int64_t last, int tt, int tn) {
+  if (a.grain == 16)
+    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+               [](char* s, const char* g) { copy_async16(s, g); });
+  else if (a.grain == 8)
+    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+               [](char* s, const char* g) { copy_async<8>(s, g); });
+  else if (a.grain == 4)
+    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+               [](char* s, const char* g) { copy_async<4>(s, g); });
   else
-    scan_forward<T, SIG><<<(unsigned)blocks, 128, 0, be->stream>>>(p);
+    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+               [](char* s, const char* g) { *(uint16_t*)s = *(const uint16_t*)g; });
+}
+
+__device__ __forceinline__ void store_rows_of(const TileArgs& a, int64_t D, int elem, const View& v,
+                                              char* tile, int col, int64_t t0, int r0, int r1,
+                                              int64_t last, int lane) {
+  if (a.grain == 16)
+    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+               [](char* s, const char* g) { *(uint4*)g = *(const uint4*)s; });
+  else if (a.grain == 8)
+    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+               [](char* s, const char* g) { *(uint2*)g = *(const uint2*)s; });
+  else if (a.grain == 4)
+    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+               [](char* s, const char* g) { *(uint32_t*)g = *(const uint32_t*)s; });
+  else
+    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+               [](char* s, const char* g) { *(uint16_t*)g = *(const uint16_t*)s; });
+}
+
+template <typename T>
+struct Lane8 {  // 8 bytes of a row
+  static constexpr int N = 8 / sizeof(T);
+  T v[N];
+};
+template <typename T>
+__device__ __forceinline__ Lane8<T> lane_load(const char* row, int lane) {
+  Lane8<T> r;
+  const uint2 u = *reinterpret_cast<const uint2*>(row + lane * 8);
+  memcpy(&r, &u, 8);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void lane_store(char* row, int lane, const Lane8<T>& r) {
+  uint2 u;
+  memcpy(&u, &r, 8);
+  *reinterpret_cast<uint2*>(row + lane * 8) = u;
+}
+
+// ---- looking back ------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t load_flag(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint64_t load_word(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_word(uint64_t* p, uint64_t v) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+
+// Polls until `ready`; gives up when the limit or another block's error says so
+template <typename F>
+__device__ __forceinline__ void poll(uint32_t* err, F ready) {
+  for (uint32_t i = 0; i < POLL_LIMIT; ++i) {
+    if (ready()) return;
+    if ((i & 255) == 255 && load_flag(err)) return;
+  }
+  atomicOr(err, 1u);
+}
+
+template <typename S>
+struct Pair {
+  S p, q;
+};
+
+// The state that entered from the group before, one word per 32 bits
+template <typename S>
+__device__ __forceinline__ S read_state(const uint64_t* w, uint32_t* err) {
+  constexpr int NW = sizeof(S) / 4;
+  uint64_t v[NW];
+  poll(err, [&] {
+    bool all = true;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      v[i] = load_word(w + i);
+      all = all && (v[i] >> 32);
+    }
+    return all;
+  });
+  uint32_t bits[NW];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) bits[i] = (uint32_t)v[i];
+  S s;
+  memcpy(&s, bits, sizeof(S));
+  return s;
+}
+template <typename S>
+__device__ __forceinline__ void write_state(uint64_t* w, S s) {
+  constexpr int NW = sizeof(S) / 4;
+  uint32_t bits[NW];
+  memcpy(bits, &s, sizeof(S));
+#pragma unroll
+  for (int i = 0; i < NW; ++i) store_word(w + i, (1ull << 32) | bits[i]);
+}
+
+// ---- the kernel --------------------------------------------------------------------
+
+template <typename T, bool SIG, bool BWD>
+__global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant__ ScanArgs p,
+                                                          const __grid_constant__ TileArgs a) {
+  using S = typename Elem<T>::State;
+  constexpr int N = Lane8<T>::N;                           // channels of a lane
+  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;          // gate, x or dh, h, x
+  extern __shared__ __align__(16) char smem[];
+  __shared__ Pair<S> part[WARPS][32 * N];
+  __shared__ uint32_t ticket;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wt = a.warps_t, team = warp / wt, tw = warp % wt;  // teams of warps per column
+  int64_t index = blockIdx.x;
+  if (a.ticket) {
+    if (threadIdx.x == 0) ticket = atomicAdd(a.ticket, 1u);
+    __syncthreads();
+    index = ticket;
+  }
+  // (tile along time, column); backward starts at the end of time
+  int tile, col;
+  if (a.ticket) {
+    tile = (int)(index / a.columns);
+    col = (int)(index % a.columns);
+  } else {
+    tile = 0;
+    col = (int)(index * (WARPS / wt)) + team;
+  }
+  const int order = tile;  // place in the chain
+  if (BWD) tile = a.tiles - 1 - tile;
+  const bool live = col < a.columns;
+  const int64_t t0 = (int64_t)tile * a.rows;
+  char* gate = smem + (size_t)team * ARRAYS * a.rows * ROW;
+  char* second = gate + a.rows * ROW;        // x, or dh
+  char* before = second + a.rows * ROW;      // h, a step late (backward)
+  char* xrow = before + a.rows * ROW;        // x (backward, sigmoid)
+  constexpr int E = sizeof(T);
+
+  if (live) {
+    const int tt = threadIdx.x - team * wt * 32, tn = wt * 32;
+    load_rows(a, p.D, E, View{(const char*)p.gate, p.gd * E, p.gt * E, p.gb * E}, gate, col, t0, 0,
+              p.T, tt, tn);
+    if constexpr (!BWD) {
+      load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, second, col, t0, 0,
+                p.T, tt, tn);
+    } else {
+      load_rows(a, p.D, E, View{(const char*)p.dh, p.ed * E, p.et * E, p.eb * E}, second, col, t0, 0,
+                p.T, tt, tn);
+      load_rows(a, p.D, E, View{(const char*)p.h - p.ht * E, p.hd * E, p.ht * E, p.hb * E}, before,
+                col, t0, 1, p.T, tt, tn);
+      if constexpr (SIG)
+        load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, xrow, col, t0, 0,
+                  p.T, tt, tn);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+
+  // this lane's channels and where their sequences end, relative to t0
+  const int64_t c0 = ((int64_t)col * 32 + lane) * N;
+  int end[N];
+  bool full = true;  // every step of this warp's rows exists in every lane
+  const int r0 = tw * STEPS, r1 = min(r0 + STEPS, a.rows);
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    int64_t len = 0;
+    if (live && c0 + v < a.channels) {
+      len = p.T;
+      if (p.lengths) {
+        const int64_t n = p.lengths[(c0 + v) / p.D];
+        len = n < 0 ? 0 : (n < p.T ? n : p.T);
+      }
+    }
+    end[v] = (int)max((int64_t)-1, min(len - t0, (int64_t)a.rows));
+    full = full && end[v] >= r1;
+  }
+  full = __all_sync(0xffffffffu, full);
+
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+
+  // the map of this warp's steps
+  S P[N], Q[N];
+#pragma unroll
+  for (int v = 0; v < N; ++v) P[v] = 1, Q[v] = 0;
+  const bool chain = a.tiles > 1 || wt > 1;
+  if (chain) {
+    auto compose = [&](int r, bool masked) {
+      const Lane8<T> g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        S f = Elem<T>::load(g.v[v]), b = Elem<T>::load(x.v[v]);
+        if constexpr (SIG) {
+          S keep;
+          sigmoid_pair(f, &f, &keep);
+          if constexpr (!BWD) b *= keep;
+        }
+        S q = BWD ? f * (b + Q[v]) : f * Q[v] + b;
+        S pp = f * P[v];
+        if (masked && r >= end[v]) q = Q[v], pp = P[v];
+        Q[v] = q;
+        P[v] = pp;
+      }
+    };
+    if (full) {
+#pragma unroll 4
+      for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, false);
+    } else {
+      for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, true);
+    }
+  }
+
+  // The state that enters the tile; the first group starts from the caller's.
+  // It is read before this tile's map is published: the last tile, which may
+  // overwrite it (h_last == h0), comes after every map of its group.
+  S s[N];
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    const S* from = (const S*)(BWD ? p.dh_last : p.h0);
+    s[v] = order < GROUP && from && live && c0 + v < a.channels ? from[c0 + v] : S(0);
+  }
+  if (wt > 1) {
+#pragma unroll
+    for (int v = 0; v < N; ++v) part[warp][lane * N + v] = Pair<S>{P[v], Q[v]};
+    __syncthreads();
+    // steps run forward from the first warp, backward from the last
+    auto nth = [&](int i) { return BWD ? wt - 1 - i : i; };
+    const int place = BWD ? wt - 1 - tw : tw;
+    if (a.ticket) {
+      Pair<S>* maps = (Pair<S>*)a.maps;
+      S BP[N], BQ[N];  // the whole tile's map
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        BP[v] = 1, BQ[v] = 0;
+        for (int i = 0; i < WARPS; ++i) {
+          const Pair<S> m = part[nth(i)][lane * N + v];
+          BQ[v] = m.p * BQ[v] + m.q;
+          BP[v] = m.p * BP[v];
+        }
+      }
+      const int group = order / GROUP, in_group = order % GROUP;
+      if (warp == 0 && in_group < GROUP - 1 && order < a.tiles - 1) {
+#pragma unroll
+        for (int v = 0; v < N; ++v)
+          if (c0 + v < a.channels) maps[(int64_t)order * a.channels + c0 + v] = Pair<S>{BP[v], BQ[v]};
+        __threadfence();
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(a.flags + (int64_t)order * a.columns + col)
+                       : "memory");
+      }
+      // predecessors in the group, a quarter of them per warp
+      S LP[N], LQ[N];
+#pragma unroll
+      for (int v = 0; v < N; ++v) LP[v] = 1, LQ[v] = 0;
+      const int i0 = warp * (GROUP / WARPS), i1 = min(i0 + GROUP / WARPS, in_group);
+      if (i0 < i1) {
+        if (lane < i1 - i0) {
+          const uint32_t* f = a.flags + (int64_t)(group * GROUP + i0 + lane) * a.columns + col;
+          poll(a.err, [&] { return load_flag(f) != 0; });
+        }
+        __syncwarp();
+        __threadfence();
+        for (int i = i0; i < i1; ++i) {
+          const Pair<S>* m = maps + (int64_t)(group * GROUP + i) * a.channels + c0;
+#pragma unroll
+          for (int v = 0; v < N; ++v) {
+            if (c0 + v >= a.channels) break;
+            const Pair<S> w = Pair<S>{__ldcg(&m[v].p), __ldcg(&m[v].q)};
+            LQ[v] = w.p * LQ[v] + w.q;
+            LP[v] = w.p * LP[v];
+          }
+        }
+      }
+      __shared__ Pair<S> back[WARPS][32 * N];
+#pragma unroll
+      for (int v = 0; v < N; ++v) back[warp][lane * N + v] = Pair<S>{LP[v], LQ[v]};
+      __syncthreads();
+      constexpr int NW = sizeof(S) / 4;
+      if (group > 0) {
+        const uint64_t* w = a.state + ((int64_t)(group - 1) * a.channels + c0) * NW;
+#pragma unroll
+        for (int v = 0; v < N; ++v)
+          if (c0 + v < a.channels) s[v] = read_state<S>(w + v * NW, a.err);
+      }
+#pragma unroll
+      for (int v = 0; v < N; ++v)
+        for (int i = 0; i < WARPS; ++i) {
+          const Pair<S> m = back[i][lane * N + v];
+          s[v] = m.p * s[v] + m.q;
+        }
+      if (warp == 0 && in_group == GROUP - 1 && order < a.tiles - 1) {
+        uint64_t* w = a.state + ((int64_t)group * a.channels + c0) * NW;
+#pragma unroll
+        for (int v = 0; v < N; ++v)
+          if (c0 + v < a.channels) write_state<S>(w + v * NW, BP[v] * s[v] + BQ[v]);
+      }
+    }
+    // and the warps of the tile before this one
+    for (int i = 0; i < place; ++i)
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        const Pair<S> m = part[team * wt + nth(i)][lane * N + v];
+        s[v] = m.p * s[v] + m.q;
+      }
+  }
+  if (!live) return;
+
+  // the steps themselves; results take the place of what they came from
+  auto step = [&](int r, bool masked) {
+    const Lane8<T> g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
+    if constexpr (!BWD) {
+      Lane8<T> out;
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        S f = Elem<T>::load(g.v[v]), b = Elem<T>::load(x.v[v]);
+        if constexpr (SIG) {
+          S keep;
+          sigmoid_pair(f, &f, &keep);
+          b *= keep;
+        }
+        const S n = f * s[v] + b;
+        const bool on = !masked || r < end[v];
+        if (on) s[v] = n;
+        out.v[v] = Elem<T>::store(on ? n : S(0));
+      }
+      lane_store(second + r * ROW, lane, out);
+    } else {
+      Lane8<T> was = lane_load<T>(before + r * ROW, lane), xv{}, dg, dx;
+      if constexpr (SIG) xv = lane_load<T>(xrow + r * ROW, lane);
+      const bool start = t0 + r == 0;
+#pragma unroll
+      for (int v = 0; v < N; ++v) {
+        S f = Elem<T>::load(g.v[v]);
+        const S total = Elem<T>::load(x.v[v]) + s[v];
+        S prev = Elem<T>::load(was.v[v]);
+        if (start) prev = p.h0 && c0 + v < a.channels ? ((const S*)p.h0)[c0 + v] : S(0);
+        S sx = total, sg = total * prev;
+        if constexpr (SIG) {
+          S keep;
+          sigmoid_pair(f, &f, &keep);
+          sx = total * keep;
+          sg = (prev - Elem<T>::load(xv.v[v])) * f * sx;
+        }
+        const bool on = !masked || r < end[v];
+        if (on) s[v] = f * total;
+        dx.v[v] = Elem<T>::store(on ? sx : S(0));
+        dg.v[v] = Elem<T>::store(on ? sg : S(0));
+      }
+      lane_store(gate + r * ROW, lane, dg);
+      lane_store(second + r * ROW, lane, dx);
+    }
+  };
+  if (full) {
+#pragma unroll 4
+    for (int i = 0; i < r1 - r0; ++i) step(BWD ? r1 - 1 - i : r0 + i, false);
+  } else {
+    for (int i = 0; i < r1 - r0; ++i) step(BWD ? r1 - 1 - i : r0 + i, true);
+  }
+  __syncwarp();
+  if (r0 < r1) {
+    if constexpr (!BWD) {
+      store_rows_of(a, p.D, E, View{(const char*)p.h, p.hd * E, p.ht * E, p.hb * E}, second, col, t0,
+                    r0, r1, p.T, lane);
+    } else {
+      store_rows_of(a, p.D, E, View{(const char*)p.dgate, p.pd * E, p.pt * E, p.pb * E}, gate, col,
+                    t0, r0, r1, p.T, lane);
+      store_rows_of(a, p.D, E, View{(const char*)p.dx, p.qd * E, p.qt * E, p.qb * E}, second, col, t0,
+                    r0, r1, p.T, lane);
+    }
+  }
+  // the state that leaves the last tile
+  S* last = (S*)(BWD ? p.dh0 : p.h_last);
+  if (last && order == a.tiles - 1 && tw == (BWD ? 0 : wt - 1)) {
+#pragma unroll
+    for (int v = 0; v < N; ++v)
+      if (c0 + v < a.channels) last[c0 + v] = s[v];
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------
+
+// The bytes that one copy may move: the widest of 16, 8, 4 (2 for 16-bit
+// types) that divides the rows and every address and stride
+int grain_of(const ScanArgs& p, int elem, bool backward, bool need_x) {
+  struct A {
+    const void* ptr;
+    int64_t d, t, b;
+  };
+  A arrays[6] = {{p.gate, p.gd, p.gt, p.gb}, {p.h, p.hd, p.ht, p.hb}};
+  int n = 2;
+  if (need_x) arrays[n++] = {p.x, p.xd, p.xt, p.xb};
+  if (backward) {
+    arrays[n++] = {p.dh, p.ed, p.et, p.eb};
+    arrays[n++] = {p.dgate, p.pd, p.pt, p.pb};
+    arrays[n++] = {p.dx, p.qd, p.qt, p.qb};
+  }
+  for (int g = 16; g > elem; g /= 2) {
+    bool fits = p.D * elem % g == 0;
+    for (int i = 0; i < n && fits; ++i)
+      fits = (arrays[i].d == 1 || p.D == 1) && (uintptr_t)arrays[i].ptr % g == 0 &&
+             arrays[i].t * elem % g == 0 && arrays[i].b * elem % g == 0;
+    if (fits) return g;
+  }
+  return elem;
+}
+
+template <typename T, bool SIG, bool BWD>
+int launch_scan(om_backend* be, const ScanArgs& p) {
+  using S = typename Elem<T>::State;
+  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;
+  TileArgs a{};
+  a.channels = p.D * p.B;
+  a.grain = grain_of(p, sizeof(T), BWD, SIG || !BWD);
+  const int64_t columns = (a.channels * (int64_t)sizeof(T) + ROW - 1) / ROW;
+  // up to 16 steps are one warp's work, four columns then share a block
+  a.warps_t = p.T > STEPS ? WARPS : 1;
+  a.rows = (int)std::min<int64_t>(p.T, STEPS * a.warps_t);
+  const int64_t tiles = p.T == 0 ? 1 : (p.T + a.rows - 1) / a.rows;
+  const int64_t blocks = tiles > 1 ? tiles * columns : (columns + WARPS / a.warps_t - 1) / (WARPS / a.warps_t);
+  if (blocks > 0x7fffffff || columns > 0x7ffffff0)
+    return set_error(OM_ERR_SHAPE, "gated_scan: too many channels and steps");
+  a.columns = (int)columns;
+  a.tiles = (int)tiles;
+  a.err = be->d_flags + 1;
+  Scratch ws;
+  if (tiles > 1) {
+    const int64_t groups = (tiles + GROUP - 1) / GROUP;
+    const size_t state = (size_t)groups * a.channels * (sizeof(S) / 4) * 8;
+    const size_t flags = ((size_t)blocks * 4 + 15) / 16 * 16;
+    OM_TRY(ws.alloc(be, 16 + flags + state + (size_t)tiles * a.channels * sizeof(Pair<S>)));
+    char* at = (char*)ws.ptr;
+    OM_CUDA(cudaMemsetAsync(at, 0, 16 + flags + state, be->stream), "gated_scan marks");
+    a.ticket = (uint32_t*)at;
+    a.flags = (uint32_t*)(at + 16);
+    a.state = (uint64_t*)(at + 16 + flags);
+    a.maps = at + 16 + flags + state;
+  }
+  const size_t smem = (size_t)(WARPS / a.warps_t) * ARRAYS * a.rows * ROW;
+  auto kernel = scan_kernel<T, SIG, BWD>;
+  if (smem > 48 * 1024 - 8 * 1024)
+    OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+            "gated_scan");
+  ProfScope prof(be, BWD ? "gated_scan_backward" : "gated_scan");
+  kernel<<<(unsigned)blocks, WARPS * 32, smem, be->stream>>>(p, a);
   note_launch();
   return check_cuda(cudaGetLastError(), "gated_scan launch");
 }
 
 template <typename T>
 int launch_scan_kind(om_backend* be, om_gate kind, const ScanArgs& p, bool backward) {
-  return kind == OM_GATE_SIGMOID ? launch_scan<T, true>(be, p, backward)
-                                 : launch_scan<T, false>(be, p, backward);
+  if (kind == OM_GATE_SIGMOID)
+    return backward ? launch_scan<T, true, true>(be, p) : launch_scan<T, true, false>(be, p);
+  return backward ? launch_scan<T, false, true>(be, p) : launch_scan<T, false, false>(be, p);
 }
 
 int dispatch_scan(om_backend* be, om_gate kind, om_dtype dtype, const ScanArgs& p, bool backward) {

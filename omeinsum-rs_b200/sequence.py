@@ -30,13 +30,18 @@ F32, F64, OM_BF16, F16, I8, I32, I64 = 0, 1, 5, 6, 7, 8, 9
 _NP = {v: k for k, v in DTYPES.items()}
 _NAMES = {"f32": F32, "f64": F64, "bf16": OM_BF16, "f16": F16, "i8": I8, "i32": I32, "i64": I64}
 _KINDS = {"linear": 0, "sigmoid": 1}
-_torch_codes = {}  # torch dtype -> code, filled on the first torch tensor
+_torch = None  # the module, from the first torch tensor on
+_torch_codes = {}  # torch dtype -> code
 _torch_types = {}
 
 
+_bound = None
+
+
 def _bind():
-    L = lib()
-    if not getattr(L, "_sequence_bound", False):
+    global _bound
+    if _bound is None:
+        L = lib()
         P, I = ctypes.c_void_p, ctypes.c_int
         L.om_b200_gated_scan.argtypes = [P, I, I] + [P] * 10
         L.om_b200_gated_scan_backward.argtypes = [P, I, I] + [P] * 17
@@ -45,8 +50,8 @@ def _bind():
         L.om_b200_quantize_rows.argtypes = [P, I] + [P] * 6
         L.om_b200_matmul_i8.argtypes = [P, I] + [P] * 10
         L.om_b200_linear_i8.argtypes = [P, I] + [P] * 9
-        L._sequence_bound = True
-    return L
+        _bound = L
+    return _bound
 
 
 def _invalid(msg):
@@ -104,32 +109,10 @@ def upload(be, array, dtype: str | None = None) -> Strided:
     return Strided(be.from_slice(data), shape)
 
 
-class _Operand:
-    """Device pointer, dtype code, shape and strides of one argument."""
-    __slots__ = ("ptr", "code", "shape", "strides", "keep")
-
-    def __init__(self, be, t, name):
-        if isinstance(t, Strided):
-            if t.storage.backend.device != be.device:
-                raise _invalid(f"{name}: on device {t.storage.backend.device}, the backend on {be.device}")
-            self.code = DTYPES[t.storage.dtype]
-            self.ptr = (t.storage.ptr or 0) + t.offset * t.storage.dtype.itemsize
-            self.shape, self.strides = t.shape, t.strides
-        elif hasattr(t, "data_ptr"):
-            if not t.is_cuda or t.device.index != be.device:
-                raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
-            code = _torch_codes.get(t.dtype)
-            if code is None:
-                code = _learn_torch(t.dtype, name)
-            self.code, self.ptr = code, t.data_ptr()
-            self.shape, self.strides = tuple(t.shape), t.stride()
-        else:
-            raise _invalid(f"{name}: a Strided view or a torch CUDA tensor is needed, not {type(t).__name__}")
-        self.keep = t
-
-
 def _learn_torch(dtype, name):
+    global _torch
     import torch
+    _torch = torch
     for tt, code in ((torch.float32, F32), (torch.float64, F64), (torch.bfloat16, OM_BF16),
                      (torch.float16, F16), (torch.int8, I8), (torch.int32, I32),
                      (torch.int64, I64)):
@@ -140,85 +123,114 @@ def _learn_torch(dtype, name):
     return _torch_codes[dtype]
 
 
-class _Call:
-    """One call's outputs and its order with torch's current stream."""
-
-    def __init__(self, be, like, *others):
-        self.be = be
-        self.torch = self.cur = None
-        own = isinstance(like, Strided)
-        for t in others:
-            if t is not None and isinstance(t, Strided) != own:
-                raise _invalid("Strided views and torch tensors cannot be mixed in one call")
-        if not own:
-            import torch
-            self.torch = torch
-            self.device = like.device
-            if not be.recording:
-                cur = torch.cuda.current_stream(like.device)
-                if cur.cuda_stream != be.home_stream:
-                    self.cur = cur
-                    self.mine = torch.cuda.ExternalStream(be.home_stream, device=like.device)
-                    self.mine.wait_stream(cur)
-
-    def empty(self, code, *shape):
-        if self.torch is not None:
-            return self.torch.empty(shape, dtype=_torch_types[code], device=self.device)
-        n = 1
-        for s in shape:
-            n *= s
-        return Strided(self.be.alloc(n, _NP[code]), shape)
-
-    def done(self, rc):
-        if self.cur is not None:
-            self.cur.wait_stream(self.mine)
-        _check(rc)
+def _operand(be, t, name):
+    """(device pointer, type code, shape, strides) of one argument."""
+    if isinstance(t, Strided):
+        s = t.storage
+        if s.backend.device != be.device:
+            raise _invalid(f"{name}: on device {s.backend.device}, the backend on {be.device}")
+        return (s.ptr or 0) + t.offset * s.dtype.itemsize, DTYPES[s.dtype], t.shape, t.strides
+    if not hasattr(t, "data_ptr"):
+        raise _invalid(f"{name}: a Strided view or a torch CUDA tensor is needed, not {type(t).__name__}")
+    if t.get_device() != be.device:  # -1: not on a device at all
+        raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
+    code = _torch_codes.get(t.dtype)
+    if code is None:
+        code = _learn_torch(t.dtype, name)
+    return t.data_ptr(), code, t.shape, t.stride()
 
 
-_A3 = ctypes.c_int64 * 3
+def _typed(be, t, name, ndim, codes):
+    o = _operand(be, t, name)
+    if len(o[2]) != ndim:
+        raise _invalid(f"{name}: must have {ndim} axes")
+    if o[1] not in codes:
+        raise _invalid(f"{name}: type {_NP[o[1]]} not accepted here")
+    return o
 
 
-def _dtb(o: _Operand):
-    """Strides of a [batch, time, channel] operand in the ABI's order."""
-    s = o.strides
-    return _A3(s[2], s[1], s[0])
-
-
-def _want(o: _Operand, name, shape, *codes):
-    if o.shape != tuple(shape):
-        raise _invalid(f"{name}: shape {list(o.shape)}, expected {list(shape)}")
-    if o.code not in codes:
-        raise _invalid(f"{name}: type {_NP[o.code]} not accepted here")
+def _like(be, t, name, shape, code):
+    o = _operand(be, t, name)
+    if o[2] != shape:
+        raise _invalid(f"{name}: shape {list(o[2])}, expected {list(shape)}")
+    if o[1] != code:
+        raise _invalid(f"{name}: type {_NP[o[1]]}, expected {_NP[code]}")
+    return o
 
 
 def _vector(be, t, name, shape, code):
     """Pointer of an optional contiguous operand (None: a null pointer)."""
     if t is None:
         return None
-    o = _Operand(be, t, name)
-    _want(o, name, shape, code)
+    ptr, _, shape, strides = _like(be, t, name, shape, code)
+    if len(shape) == 1 and (strides[0] == 1 or shape[0] == 1):
+        return ptr
     s = 1
-    for n, st in zip(reversed(o.shape), reversed(o.strides)):
+    for n, st in zip(reversed(shape), reversed(strides)):
         if n != 1 and st != s:
             raise _invalid(f"{name}: must be contiguous")
         s *= n
-    return o.ptr
+    return ptr
 
 
-def _scan_args(be, gate, x, kind, who):
-    g = _Operand(be, gate, "gate")
-    if kind not in _KINDS:
+class _Call:
+    """One call's outputs and its order with torch's current stream."""
+    __slots__ = ("be", "device", "cur", "mine")
+
+    def __init__(self, be, like, *others):
+        self.be = be
+        self.cur = None
+        own = isinstance(like, Strided)
+        for t in others:
+            if t is not None and isinstance(t, Strided) != own:
+                raise _invalid("Strided views and torch tensors cannot be mixed in one call")
+        if own:
+            self.device = None
+            return
+        self.device = like.device
+        if not be.recording and _torch._C._cuda_getCurrentRawStream(be.device) != be.home_stream:
+            self.cur = _torch.cuda.current_stream(self.device)
+            self.mine = _torch.cuda.ExternalStream(be.home_stream, device=self.device)
+            self.mine.wait_stream(self.cur)
+
+    def empty(self, code, *shape):
+        """(a new row-major tensor, its pointer)"""
+        if self.device is not None:
+            t = _torch.empty(shape, dtype=_torch_types[code], device=self.device)
+            return t, t.data_ptr()
+        n = 1
+        for s in shape:
+            n *= s
+        t = Strided(self.be.alloc(n, _NP[code]), shape)
+        return t, t.storage.ptr
+
+    def done(self, rc):
+        if self.cur is not None:
+            self.cur.wait_stream(self.mine)
+        if rc:
+            _check(rc)
+
+
+_A2 = ctypes.c_int64 * 2
+_A3 = ctypes.c_int64 * 3
+_REALS = (F32, F64, OM_BF16, F16)
+
+
+def _dtb(strides):
+    """Strides of a [batch, time, channel] operand in the ABI's order."""
+    return _A3(strides[2], strides[1], strides[0])
+
+
+def _cr(strides):
+    """Strides of a [row, column] operand in the ABI's order."""
+    return _A2(strides[1], strides[0])
+
+
+def _kind(kind, who):
+    k = _KINDS.get(kind)
+    if k is None:
         raise _invalid(f"{who}: kind must be 'linear' or 'sigmoid', not {kind!r}")
-    if len(g.shape) != 3:
-        raise _invalid(f"{who}: gate must be [batch, time, channels]")
-    if g.code not in (F32, F64, OM_BF16, F16):
-        raise _invalid(f"{who}: gate must be f32, f64, bf16 or f16")
-    v = None
-    if x is not None:
-        v = _Operand(be, x, "x")
-        _want(v, "x", g.shape, g.code)
-    b, t, d = g.shape
-    return g, v, _A3(d, t, b), (b, d), F64 if g.code == F64 else F32
+    return k
 
 
 def gated_scan(be, gate, x, h0=None, lengths=None, kind="linear", h_last=None):
@@ -230,19 +242,23 @@ def gated_scan(be, gate, x, h0=None, lengths=None, kind="linear", h_last=None):
     h_last, when given, receives the last state and may be h0 itself (a decoding
     step updates its state in place)."""
     L = _bind()
-    g, v, shape, bd, st = _scan_args(be, gate, x, kind, "gated_scan")
-    if v is None:
+    k = _kind(kind, "gated_scan")
+    gp, code, shape, gs = _typed(be, gate, "gate", 3, _REALS)
+    if x is None:
         raise _invalid("gated_scan: x is needed")
-    h0p = _vector(be, h0, "h0", bd, st)
-    lp = _vector(be, lengths, "lengths", bd[:1], I32)
+    xp, _, _, xs = _like(be, x, "x", shape, code)
+    b, t, d = shape
+    st = F64 if code == F64 else F32
+    h0p = _vector(be, h0, "h0", (b, d), st)
+    lp = _vector(be, lengths, "lengths", (b,), I32)
     call = _Call(be, gate, x, h0, lengths, h_last)
-    h = call.empty(g.code, *g.shape)
+    h, hp = call.empty(code, b, t, d)
     if h_last is None:
-        h_last = call.empty(st, *bd)
-    lastp = _vector(be, h_last, "h_last", bd, st)
-    o = _Operand(be, h, "h")
-    call.done(L.om_b200_gated_scan(be.h, _KINDS[kind], g.code, shape, g.ptr, _dtb(g), v.ptr, _dtb(v),
-                                   h0p, lp, o.ptr, _dtb(o), lastp))
+        h_last, lastp = call.empty(st, b, d)
+    else:
+        lastp = _vector(be, h_last, "h_last", (b, d), st)
+    call.done(L.om_b200_gated_scan(be.h, k, code, _A3(d, t, b), gp, _dtb(gs), xp, _dtb(xs), h0p, lp, hp,
+                                   _A3(1, d, t * d), lastp))
     return h, h_last
 
 
@@ -250,54 +266,37 @@ def gated_scan_backward(be, gate, x, h, dh, h0=None, dh_last=None, lengths=None,
     """Gradients (dgate, dx, dh0) of gated_scan, given its output h and the
     gradients reaching h and (optionally) h_last.  x may be None for "linear"."""
     L = _bind()
-    g, v, shape, bd, st = _scan_args(be, gate, x, kind, "gated_scan_backward")
-    if v is None and kind != "linear":
+    k = _kind(kind, "gated_scan_backward")
+    gp, code, shape, gs = _typed(be, gate, "gate", 3, _REALS)
+    xp = xs = None
+    if x is not None:
+        xp, _, _, xs = _like(be, x, "x", shape, code)
+        xs = _dtb(xs)
+    elif kind != "linear":
         raise _invalid("gated_scan_backward: x is needed")
-    ho, eo = _Operand(be, h, "h"), _Operand(be, dh, "dh")
-    _want(ho, "h", g.shape, g.code)
-    _want(eo, "dh", g.shape, g.code)
-    h0p = _vector(be, h0, "h0", bd, st)
-    lp = _vector(be, lengths, "lengths", bd[:1], I32)
-    ep = _vector(be, dh_last, "dh_last", bd, st)
+    hp, _, _, hs = _like(be, h, "h", shape, code)
+    ep, _, _, es = _like(be, dh, "dh", shape, code)
+    b, t, d = shape
+    st = F64 if code == F64 else F32
+    h0p = _vector(be, h0, "h0", (b, d), st)
+    lp = _vector(be, lengths, "lengths", (b,), I32)
+    elp = _vector(be, dh_last, "dh_last", (b, d), st)
     call = _Call(be, gate, x, h, dh, h0, dh_last, lengths)
-    dgate, dx = call.empty(g.code, *g.shape), call.empty(g.code, *g.shape)
-    dh0 = call.empty(st, *bd)
-    po, qo = _Operand(be, dgate, "dgate"), _Operand(be, dx, "dx")
-    call.done(L.om_b200_gated_scan_backward(
-        be.h, _KINDS[kind], g.code, shape, g.ptr, _dtb(g), v.ptr if v else None,
-        _dtb(v) if v else None, ho.ptr, _dtb(ho), h0p, lp, eo.ptr, _dtb(eo), ep, po.ptr, _dtb(po),
-        qo.ptr, _dtb(qo), _vector(be, dh0, "dh0", bd, st)))
+    (dgate, pp), (dx, qp), (dh0, d0p) = call.empty(code, b, t, d), call.empty(code, b, t, d), call.empty(st, b, d)
+    rows = _A3(1, d, t * d)
+    call.done(L.om_b200_gated_scan_backward(be.h, k, code, _A3(d, t, b), gp, _dtb(gs), xp, xs, hp, _dtb(hs), h0p, lp,
+                                            ep, _dtb(es), elp, pp, rows, qp, rows, d0p))
     return dgate, dx, dh0
 
 
-_A2 = ctypes.c_int64 * 2
-
-
-def _matrix(be, t, name, *codes):
-    o = _Operand(be, t, name)
-    if len(o.shape) != 2:
-        raise _invalid(f"{name}: must have two axes")
-    if codes and o.code not in codes:
-        raise _invalid(f"{name}: type {_NP[o.code]} not accepted here")
-    return o
-
-
-def _cr(o: _Operand):
-    """Strides of a [row, column] operand in the ABI's order."""
-    return _A2(o.strides[1], o.strides[0])
-
-
 def _loss_args(be, x, w, targets, who):
-    xo = _matrix(be, x, "x", F32, F64, OM_BF16, F16)
-    wo = _matrix(be, w, "w", xo.code)
-    to = _Operand(be, targets, "targets")
-    n, d = xo.shape
-    if wo.shape[1] != d:
-        raise _invalid(f"{who}: x has width {d}, w {wo.shape[1]}")
-    if to.code not in (I32, I64):
-        raise _invalid(f"{who}: targets must be i32 or i64")
-    tp = _vector(be, targets, "targets", (n,), to.code)
-    return xo, wo, to.code, tp, _A3(d, n, wo.shape[0]), F64 if xo.code == F64 else F32
+    xp, code, (n, d), xs = _typed(be, x, "x", 2, _REALS)
+    wp, _, (v, wd), ws = _typed(be, w, "w", 2, (code,))
+    if wd != d:
+        raise _invalid(f"{who}: x has width {d}, w {wd}")
+    tc = _typed(be, targets, "targets", 1, (I32, I64))[1]
+    tp = _vector(be, targets, "targets", (n,), tc)
+    return code, n, d, v, (_A3(d, n, v), xp, _cr(xs), wp, _cr(ws), tc, tp), F64 if code == F64 else F32
 
 
 def linear_cross_entropy(be, x, w, targets):
@@ -306,12 +305,10 @@ def linear_cross_entropy(be, x, w, targets):
     x [tokens, width], w [vocabulary, width], targets [tokens] (i32 or i64;
     one outside the vocabulary carries no loss).  The logits are never kept."""
     L = _bind()
-    xo, wo, tc, tp, shape, st = _loss_args(be, x, w, targets, "linear_cross_entropy")
-    n = xo.shape[0]
+    code, n, _, _, args, st = _loss_args(be, x, w, targets, "linear_cross_entropy")
     call = _Call(be, x, w, targets)
-    loss, lse = call.empty(st, n), call.empty(st, n)
-    call.done(L.om_b200_linear_cross_entropy(be.h, xo.code, shape, xo.ptr, _cr(xo), wo.ptr, _cr(wo), tc, tp,
-                                             _vector(be, loss, "loss", (n,), st), _vector(be, lse, "lse", (n,), st)))
+    (loss, lp), (lse, sp) = call.empty(st, n), call.empty(st, n)
+    call.done(L.om_b200_linear_cross_entropy(be.h, code, *args, lp, sp))
     return loss, lse
 
 
@@ -319,39 +316,44 @@ def linear_cross_entropy_backward(be, x, w, targets, lse, dloss):
     """Gradients (dx, dw) of linear_cross_entropy, given its lse and the
     gradient dloss [tokens] of each token's loss."""
     L = _bind()
-    xo, wo, tc, tp, shape, st = _loss_args(be, x, w, targets, "linear_cross_entropy_backward")
-    n = xo.shape[0]
-    lp, gp = _vector(be, lse, "lse", (n,), st), _vector(be, dloss, "dloss", (n,), st)
+    code, n, d, v, args, st = _loss_args(be, x, w, targets, "linear_cross_entropy_backward")
+    sp, gp = _vector(be, lse, "lse", (n,), st), _vector(be, dloss, "dloss", (n,), st)
     call = _Call(be, x, w, targets, lse, dloss)
-    dx, dw = call.empty(xo.code, *xo.shape), call.empty(xo.code, *wo.shape)
-    do, eo = _Operand(be, dx, "dx"), _Operand(be, dw, "dw")
-    call.done(L.om_b200_linear_cross_entropy_backward(
-        be.h, xo.code, shape, xo.ptr, _cr(xo), wo.ptr, _cr(wo), tc, tp, lp, gp, do.ptr, _cr(do),
-        eo.ptr, _cr(eo)))
+    (dx, dp), (dw, ep) = call.empty(code, n, d), call.empty(code, v, d)
+    rows = _A2(1, d)
+    call.done(L.om_b200_linear_cross_entropy_backward(be.h, code, *args, sp, gp, dp, rows, ep, rows))
     return dx, dw
+
+
+_QUANTISED = (F32, OM_BF16, F16)
 
 
 def quantize_rows(be, x):
     """(q, scale) of a matrix in 8 bits: scale = max |row| / 127 and
     q = row / scale, rounded (om_b200_quantize_rows).  x is f32, bf16 or f16."""
     L = _bind()
-    xo = _matrix(be, x, "x", F32, OM_BF16, F16)
-    m, k = xo.shape
+    xp, code, (m, k), xs = _typed(be, x, "x", 2, _QUANTISED)
     call = _Call(be, x)
-    q, scale = call.empty(I8, m, k), call.empty(F32, m)
-    qo = _Operand(be, q, "q")
-    call.done(L.om_b200_quantize_rows(be.h, xo.code, _A2(k, m), xo.ptr, _cr(xo), qo.ptr, _cr(qo),
-                                      _vector(be, scale, "scale", (m,), F32)))
+    (q, qp), (scale, sp) = call.empty(I8, m, k), call.empty(F32, m)
+    call.done(L.om_b200_quantize_rows(be.h, code, _A2(k, m), xp, _cr(xs), qp, _A2(1, k), sp))
     return q, scale
 
 
 def _code_of(dtype):
-    if isinstance(dtype, str) and dtype in _NAMES:
-        return _NAMES[dtype]
-    code = _torch_codes.get(dtype)
-    if code is None:
-        raise _invalid(f"no device type for {dtype!r}")
+    code = _NAMES.get(dtype) if isinstance(dtype, str) else _torch_codes.get(dtype)
+    if code not in _QUANTISED:
+        raise _invalid(f"a result type of f32, bf16 or f16 is needed, not {dtype!r}")
     return code
+
+
+def _weights(be, w, w_scale, bias, k):
+    wp, _, (n, wk), ws = _typed(be, w, "w", 2, (I8,))
+    if wk != k:
+        raise _invalid(f"w has {wk} columns, the other matrix {k}")
+    tp = _vector(be, w_scale, "w_scale", (n,), F32)
+    if tp is None:
+        raise _invalid("w_scale is needed")
+    return n, wp, _cr(ws), tp, _vector(be, bias, "bias", (n,), F32)
 
 
 def matmul_i8(be, q, q_scale, w, w_scale, bias=None, dtype="f32"):
@@ -360,22 +362,15 @@ def matmul_i8(be, q, q_scale, w, w_scale, bias=None, dtype="f32"):
 
     q [rows, inner], w [columns, inner], one scale per row of each."""
     L = _bind()
-    qo, wo = _matrix(be, q, "q", I8), _matrix(be, w, "w", I8)
-    (m, k), n = qo.shape, wo.shape[0]
-    if wo.shape[1] != k:
-        raise _invalid(f"matmul_i8: q has {k} columns, w {wo.shape[1]}")
-    sp, tp = _vector(be, q_scale, "q_scale", (m,), F32), _vector(be, w_scale, "w_scale", (n,), F32)
-    bp = _vector(be, bias, "bias", (n,), F32)
-    if sp is None or tp is None:
-        raise _invalid("matmul_i8: both scales are needed")
+    qp, _, (m, k), qs = _typed(be, q, "q", 2, (I8,))
+    n, wp, ws, tp, bp = _weights(be, w, w_scale, bias, k)
+    sp = _vector(be, q_scale, "q_scale", (m,), F32)
+    if sp is None:
+        raise _invalid("q_scale is needed")
     code = _code_of(dtype)
-    if code not in (F32, OM_BF16, F16):
-        raise _invalid("matmul_i8: dtype must be f32, bf16 or f16")
     call = _Call(be, q, q_scale, w, w_scale, bias)
-    y = call.empty(code, m, n)
-    yo = _Operand(be, y, "y")
-    call.done(L.om_b200_matmul_i8(be.h, code, _A3(k, m, n), qo.ptr, _cr(qo), sp, wo.ptr, _cr(wo), tp, bp,
-                                  yo.ptr, _cr(yo)))
+    y, yp = call.empty(code, m, n)
+    call.done(L.om_b200_matmul_i8(be.h, code, _A3(k, m, n), qp, _cr(qs), sp, wp, ws, tp, bp, yp, _A2(1, n)))
     return y
 
 
@@ -383,16 +378,9 @@ def linear_i8(be, x, w, w_scale, bias=None):
     """matmul_i8 of x's rows, quantised by quantize_rows within the call; the
     result has x's type."""
     L = _bind()
-    xo, wo = _matrix(be, x, "x", F32, OM_BF16, F16), _matrix(be, w, "w", I8)
-    (m, k), n = xo.shape, wo.shape[0]
-    if wo.shape[1] != k:
-        raise _invalid(f"linear_i8: x has {k} columns, w {wo.shape[1]}")
-    tp, bp = _vector(be, w_scale, "w_scale", (n,), F32), _vector(be, bias, "bias", (n,), F32)
-    if tp is None:
-        raise _invalid("linear_i8: w_scale is needed")
+    xp, code, (m, k), xs = _typed(be, x, "x", 2, _QUANTISED)
+    n, wp, ws, tp, bp = _weights(be, w, w_scale, bias, k)
     call = _Call(be, x, w, w_scale, bias)
-    y = call.empty(xo.code, m, n)
-    yo = _Operand(be, y, "y")
-    call.done(L.om_b200_linear_i8(be.h, xo.code, _A3(k, m, n), xo.ptr, _cr(xo), wo.ptr, _cr(wo), tp, bp,
-                                  yo.ptr, _cr(yo)))
+    y, yp = call.empty(code, m, n)
+    call.done(L.om_b200_linear_i8(be.h, code, _A3(k, m, n), xp, _cr(xs), wp, ws, tp, bp, yp, _A2(1, n)))
     return y
