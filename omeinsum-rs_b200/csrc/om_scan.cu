@@ -68,24 +68,134 @@ struct TileArgs {
   uint32_t* err;
 };
 
+// ---- arithmetic on the channels of a lane ------------------------------------------
+// Two f32 channels share one instruction (the f32x2 forms of sm_100); an f64
+// channel stands alone.
+
+template <typename S>
+struct Pack;
+template <>
+struct Pack<float> {
+  static constexpr int N = 2;
+  float2 v;
+  __device__ __forceinline__ float get(int i) const { return i ? v.y : v.x; }
+  __device__ __forceinline__ void set(int i, float s) { (i ? v.y : v.x) = s; }
+};
+template <>
+struct Pack<double> {
+  static constexpr int N = 1;
+  double v;
+  __device__ __forceinline__ double get(int) const { return v; }
+  __device__ __forceinline__ void set(int, double s) { v = s; }
+};
+
+__device__ __forceinline__ uint64_t bits_of(float2 v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
+  return r;
+}
+__device__ __forceinline__ Pack<float> of_bits(uint64_t r) {
+  Pack<float> p;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(p.v.x), "=f"(p.v.y) : "l"(r));
+  return p;
+}
+__device__ __forceinline__ Pack<float> fill(float s) { return Pack<float>{make_float2(s, s)}; }
+__device__ __forceinline__ Pack<double> fill(double s) { return Pack<double>{s}; }
+__device__ __forceinline__ Pack<float> operator*(Pack<float> a, Pack<float> b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a.v)), "l"(bits_of(b.v)));
+  return of_bits(r);
+}
+__device__ __forceinline__ Pack<float> operator+(Pack<float> a, Pack<float> b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a.v)), "l"(bits_of(b.v)));
+  return of_bits(r);
+}
+__device__ __forceinline__ Pack<float> mad(Pack<float> a, Pack<float> b, Pack<float> c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(bits_of(a.v)), "l"(bits_of(b.v)), "l"(bits_of(c.v)));
+  return of_bits(r);
+}
+__device__ __forceinline__ Pack<double> operator*(Pack<double> a, Pack<double> b) {
+  return Pack<double>{a.v * b.v};
+}
+__device__ __forceinline__ Pack<double> operator+(Pack<double> a, Pack<double> b) {
+  return Pack<double>{a.v + b.v};
+}
+__device__ __forceinline__ Pack<double> mad(Pack<double> a, Pack<double> b, Pack<double> c) {
+  return Pack<double>{fma(a.v, b.v, c.v)};
+}
+
 // a = sigmoid(g) and 1 - a without cancellation. f32: an exponential formed as
 // a power of two and an approximate reciprocal, together below 24 half steps
-// for |g| <= 16 (most of it the rounding of the exponent).
-template <typename S>
-__device__ __forceinline__ void sigmoid_pair(S g, S* a, S* keep) {
-  if constexpr (sizeof(S) == 4) {
-    float e, r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    *a = r;
-    *keep = e > 1.f ? 1.f - r : e * r;  // e may be infinite, r is then 0
-  } else {
-    const S e = exp(-fabs(g));
-    const S r = S(1) / (S(1) + e);
-    *a = g >= 0 ? r : e * r;
-    *keep = g >= 0 ? e * r : r;
-    if (g != g) *a = *keep = g;
-  }
+// for |g| <= 16 (most of it the rounding of the exponent); values below f32's
+// normal numbers become zero.
+__device__ __forceinline__ void sigmoid_pair(Pack<float> g, Pack<float>* a, Pack<float>* keep) {
+  const Pack<float> t = g * fill(-1.4426950408889634f);
+  Pack<float> e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v.x) : "f"(t.v.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v.y) : "f"(t.v.y));
+  const Pack<float> d = e + fill(1.f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v.x) : "f"(d.v.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v.y) : "f"(d.v.y));
+  const Pack<float> small = e * r, large = mad(r, fill(-1.f), fill(1.f));
+  keep->v.x = e.v.x > 1.f ? large.v.x : small.v.x;  // e may be infinite, r is then 0
+  keep->v.y = e.v.y > 1.f ? large.v.y : small.v.y;
+  *a = r;
+}
+__device__ __forceinline__ void sigmoid_pair(Pack<double> g, Pack<double>* a, Pack<double>* keep) {
+  const double e = exp(-fabs(g.v)), r = 1 / (1 + e);
+  a->v = g.v >= 0 ? r : e * r;
+  keep->v = g.v >= 0 ? e * r : r;
+  if (g.v != g.v) a->v = keep->v = g.v;
+}
+
+// 8 bytes of a row as packs, and back
+template <typename T>
+struct Lane {
+  static constexpr int CHANNELS = 8 / sizeof(T);
+  using P = Pack<typename Elem<T>::State>;
+  static constexpr int PACKS = CHANNELS / P::N;
+  P v[PACKS];
+};
+__device__ __forceinline__ void unpack(uint2 u, Lane<__nv_bfloat16>& l) {
+  l.v[0].v = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
+  l.v[1].v = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void unpack(uint2 u, Lane<__half>& l) {
+  l.v[0].v = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  l.v[1].v = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+}
+__device__ __forceinline__ void unpack(uint2 u, Lane<float>& l) {
+  l.v[0].v = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
+}
+__device__ __forceinline__ void unpack(uint2 u, Lane<double>& l) {
+  l.v[0].v = __hiloint2double((int)u.y, (int)u.x);
+}
+__device__ __forceinline__ uint2 repack(const Lane<__nv_bfloat16>& l) {
+  return make_uint2(pack2(l.v[0].v.x, l.v[0].v.y, __nv_bfloat16()),
+                    pack2(l.v[1].v.x, l.v[1].v.y, __nv_bfloat16()));
+}
+__device__ __forceinline__ uint2 repack(const Lane<__half>& l) {
+  return make_uint2(pack2(l.v[0].v.x, l.v[0].v.y, __half()), pack2(l.v[1].v.x, l.v[1].v.y, __half()));
+}
+__device__ __forceinline__ uint2 repack(const Lane<float>& l) {
+  return make_uint2(__float_as_uint(l.v[0].v.x), __float_as_uint(l.v[0].v.y));
+}
+__device__ __forceinline__ uint2 repack(const Lane<double>& l) {
+  return make_uint2((uint32_t)__double2loint(l.v[0].v), (uint32_t)__double2hiint(l.v[0].v));
+}
+template <typename T>
+__device__ __forceinline__ Lane<T> lane_load(const char* row, int lane) {
+  Lane<T> r;
+  unpack(*reinterpret_cast<const uint2*>(row + lane * 8), r);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void lane_store(char* row, int lane, const Lane<T>& r) {
+  *reinterpret_cast<uint2*>(row + lane * 8) = repack(r);
 }
 
 // ---- data of a tile --------------------------------------------------------------
@@ -163,25 +273,6 @@ __device__ __forceinline__ void store_rows_of(const TileArgs& a, int64_t D, int 
                [](char* s, const char* g) { *(uint16_t*)g = *(const uint16_t*)s; });
 }
 
-template <typename T>
-struct Lane8 {  // 8 bytes of a row
-  static constexpr int N = 8 / sizeof(T);
-  T v[N];
-};
-template <typename T>
-__device__ __forceinline__ Lane8<T> lane_load(const char* row, int lane) {
-  Lane8<T> r;
-  const uint2 u = *reinterpret_cast<const uint2*>(row + lane * 8);
-  memcpy(&r, &u, 8);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void lane_store(char* row, int lane, const Lane8<T>& r) {
-  uint2 u;
-  memcpy(&u, &r, 8);
-  *reinterpret_cast<uint2*>(row + lane * 8) = u;
-}
-
 // ---- looking back ------------------------------------------------------------------
 
 __device__ __forceinline__ uint32_t load_flag(const uint32_t* p) {
@@ -249,38 +340,35 @@ template <typename T, bool SIG, bool BWD>
 __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant__ ScanArgs p,
                                                           const __grid_constant__ TileArgs a) {
   using S = typename Elem<T>::State;
-  constexpr int N = Lane8<T>::N;                           // channels of a lane
-  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;          // gate, x or dh, h, x
+  using L = Lane<T>;
+  using K = Pack<S>;
+  constexpr int N = L::CHANNELS, NP = L::PACKS, W = K::N;
+  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;  // gate, x or dh, h, x
+  constexpr int E = sizeof(T);
   extern __shared__ __align__(16) char smem[];
-  __shared__ Pair<S> part[WARPS][32 * N];
+  __shared__ Pair<K> part[WARPS][32 * NP];
   __shared__ uint32_t ticket;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wt = a.warps_t, team = warp / wt, tw = warp % wt;  // teams of warps per column
-  int64_t index = blockIdx.x;
+  // (tile along time, column); backward starts at the end of time
+  int tile = 0, col;
   if (a.ticket) {
     if (threadIdx.x == 0) ticket = atomicAdd(a.ticket, 1u);
     __syncthreads();
-    index = ticket;
-  }
-  // (tile along time, column); backward starts at the end of time
-  int tile, col;
-  if (a.ticket) {
-    tile = (int)(index / a.columns);
-    col = (int)(index % a.columns);
+    tile = (int)(ticket / (uint32_t)a.columns);
+    col = (int)(ticket - (uint32_t)tile * (uint32_t)a.columns);
   } else {
-    tile = 0;
-    col = (int)(index * (WARPS / wt)) + team;
+    col = (int)blockIdx.x * (WARPS / wt) + team;
   }
   const int order = tile;  // place in the chain
   if (BWD) tile = a.tiles - 1 - tile;
   const bool live = col < a.columns;
   const int64_t t0 = (int64_t)tile * a.rows;
   char* gate = smem + (size_t)team * ARRAYS * a.rows * ROW;
-  char* second = gate + a.rows * ROW;        // x, or dh
-  char* before = second + a.rows * ROW;      // h, a step late (backward)
-  char* xrow = before + a.rows * ROW;        // x (backward, sigmoid)
-  constexpr int E = sizeof(T);
+  char* second = gate + a.rows * ROW;    // x, or dh
+  char* before = second + a.rows * ROW;  // h, a step late (backward)
+  char* xrow = before + a.rows * ROW;    // x (backward, sigmoid)
 
   if (live) {
     const int tt = threadIdx.x - team * wt * 32, tn = wt * 32;
@@ -321,30 +409,46 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   }
   full = __all_sync(0xffffffffu, full);
 
+  // The state that enters the tile; the first group starts from the caller's.
+  // It is read before this tile's map is published: the last tile, which may
+  // overwrite it (h_last == h0), comes after every map of its group.
+  K s[NP];
+#pragma unroll
+  for (int v = 0; v < N; ++v) {
+    const S* from = (const S*)(BWD ? p.dh_last : p.h0);
+    s[v / W].set(v % W, order < GROUP && from && live && c0 + v < a.channels ? from[c0 + v] : S(0));
+  }
+
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
 
-  // the map of this warp's steps
-  S P[N], Q[N];
+  if (wt > 1) {
+    // the map of this warp's steps
+    K P[NP], Q[NP];
 #pragma unroll
-  for (int v = 0; v < N; ++v) P[v] = 1, Q[v] = 0;
-  const bool chain = a.tiles > 1 || wt > 1;
-  if (chain) {
+    for (int v = 0; v < NP; ++v) P[v] = fill(S(1)), Q[v] = fill(S(0));
     auto compose = [&](int r, bool masked) {
-      const Lane8<T> g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
+      const L g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
 #pragma unroll
-      for (int v = 0; v < N; ++v) {
-        S f = Elem<T>::load(g.v[v]), b = Elem<T>::load(x.v[v]);
+      for (int v = 0; v < NP; ++v) {
+        K f = g.v[v], b = x.v[v];
         if constexpr (SIG) {
-          S keep;
+          K keep;
           sigmoid_pair(f, &f, &keep);
-          if constexpr (!BWD) b *= keep;
+          if constexpr (!BWD) b = b * keep;
         }
-        S q = BWD ? f * (b + Q[v]) : f * Q[v] + b;
-        S pp = f * P[v];
-        if (masked && r >= end[v]) q = Q[v], pp = P[v];
-        Q[v] = q;
-        P[v] = pp;
+        const K q = BWD ? f * (b + Q[v]) : mad(f, Q[v], b), pp = f * P[v];
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (r < end[v * W + w]) {
+              Q[v].set(w, q.get(w));
+              P[v].set(w, pp.get(w));
+            }
+        } else {
+          Q[v] = q;
+          P[v] = pp;
+        }
       }
     };
     if (full) {
@@ -353,41 +457,33 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
     } else {
       for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, true);
     }
-  }
-
-  // The state that enters the tile; the first group starts from the caller's.
-  // It is read before this tile's map is published: the last tile, which may
-  // overwrite it (h_last == h0), comes after every map of its group.
-  S s[N];
 #pragma unroll
-  for (int v = 0; v < N; ++v) {
-    const S* from = (const S*)(BWD ? p.dh_last : p.h0);
-    s[v] = order < GROUP && from && live && c0 + v < a.channels ? from[c0 + v] : S(0);
-  }
-  if (wt > 1) {
-#pragma unroll
-    for (int v = 0; v < N; ++v) part[warp][lane * N + v] = Pair<S>{P[v], Q[v]};
+    for (int v = 0; v < NP; ++v) part[warp][lane * NP + v] = Pair<K>{P[v], Q[v]};
     __syncthreads();
-    // steps run forward from the first warp, backward from the last
-    auto nth = [&](int i) { return BWD ? wt - 1 - i : i; };
+    // the map of the tile, and of its steps before this warp's (which run
+    // forward from the first warp, backward from the last)
+    K BP[NP], BQ[NP];
     const int place = BWD ? wt - 1 - tw : tw;
+#pragma unroll
+    for (int v = 0; v < NP; ++v) {
+      BP[v] = P[v] = fill(S(1)), BQ[v] = Q[v] = fill(S(0));
+#pragma unroll
+      for (int i = 0; i < WARPS; ++i) {
+        const Pair<K> m = part[BWD ? WARPS - 1 - i : i][lane * NP + v];
+        if (i == place) P[v] = BP[v], Q[v] = BQ[v];
+        BQ[v] = mad(m.p, BQ[v], m.q);
+        BP[v] = m.p * BP[v];
+      }
+    }
     if (a.ticket) {
       Pair<S>* maps = (Pair<S>*)a.maps;
-      S BP[N], BQ[N];  // the whole tile's map
-#pragma unroll
-      for (int v = 0; v < N; ++v) {
-        BP[v] = 1, BQ[v] = 0;
-        for (int i = 0; i < WARPS; ++i) {
-          const Pair<S> m = part[nth(i)][lane * N + v];
-          BQ[v] = m.p * BQ[v] + m.q;
-          BP[v] = m.p * BP[v];
-        }
-      }
       const int group = order / GROUP, in_group = order % GROUP;
       if (warp == 0 && in_group < GROUP - 1 && order < a.tiles - 1) {
 #pragma unroll
         for (int v = 0; v < N; ++v)
-          if (c0 + v < a.channels) maps[(int64_t)order * a.channels + c0 + v] = Pair<S>{BP[v], BQ[v]};
+          if (c0 + v < a.channels)
+            maps[(int64_t)order * a.channels + c0 + v] =
+                Pair<S>{BP[v / W].get(v % W), BQ[v / W].get(v % W)};
         __threadfence();
         __syncwarp();
         if (lane == 0)
@@ -395,9 +491,9 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
                        : "memory");
       }
       // predecessors in the group, a quarter of them per warp
-      S LP[N], LQ[N];
+      K LP[NP], LQ[NP];
 #pragma unroll
-      for (int v = 0; v < N; ++v) LP[v] = 1, LQ[v] = 0;
+      for (int v = 0; v < NP; ++v) LP[v] = fill(S(1)), LQ[v] = fill(S(0));
       const int i0 = warp * (GROUP / WARPS), i1 = min(i0 + GROUP / WARPS, in_group);
       if (i0 < i1) {
         if (lane < i1 - i0) {
@@ -405,95 +501,116 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
           poll(a.err, [&] { return load_flag(f) != 0; });
         }
         __syncwarp();
-        __threadfence();
+#pragma unroll 4
         for (int i = i0; i < i1; ++i) {
           const Pair<S>* m = maps + (int64_t)(group * GROUP + i) * a.channels + c0;
+          K mp[NP], mq[NP];
 #pragma unroll
           for (int v = 0; v < N; ++v) {
-            if (c0 + v >= a.channels) break;
-            const Pair<S> w = Pair<S>{__ldcg(&m[v].p), __ldcg(&m[v].q)};
-            LQ[v] = w.p * LQ[v] + w.q;
-            LP[v] = w.p * LP[v];
+            const bool in = c0 + v < a.channels;
+            mp[v / W].set(v % W, in ? __ldcg(&m[v].p) : S(0));
+            mq[v / W].set(v % W, in ? __ldcg(&m[v].q) : S(0));
+          }
+#pragma unroll
+          for (int v = 0; v < NP; ++v) {
+            LQ[v] = mad(mp[v], LQ[v], mq[v]);
+            LP[v] = mp[v] * LP[v];
           }
         }
       }
-      __shared__ Pair<S> back[WARPS][32 * N];
+      __syncthreads();  // part has been read
 #pragma unroll
-      for (int v = 0; v < N; ++v) back[warp][lane * N + v] = Pair<S>{LP[v], LQ[v]};
+      for (int v = 0; v < NP; ++v) part[warp][lane * NP + v] = Pair<K>{LP[v], LQ[v]};
       __syncthreads();
       constexpr int NW = sizeof(S) / 4;
       if (group > 0) {
         const uint64_t* w = a.state + ((int64_t)(group - 1) * a.channels + c0) * NW;
 #pragma unroll
         for (int v = 0; v < N; ++v)
-          if (c0 + v < a.channels) s[v] = read_state<S>(w + v * NW, a.err);
+          if (c0 + v < a.channels) s[v / W].set(v % W, read_state<S>(w + v * NW, a.err));
       }
 #pragma unroll
-      for (int v = 0; v < N; ++v)
+      for (int v = 0; v < NP; ++v)
+#pragma unroll
         for (int i = 0; i < WARPS; ++i) {
-          const Pair<S> m = back[i][lane * N + v];
-          s[v] = m.p * s[v] + m.q;
+          const Pair<K> m = part[i][lane * NP + v];
+          s[v] = mad(m.p, s[v], m.q);
         }
       if (warp == 0 && in_group == GROUP - 1 && order < a.tiles - 1) {
         uint64_t* w = a.state + ((int64_t)group * a.channels + c0) * NW;
 #pragma unroll
-        for (int v = 0; v < N; ++v)
-          if (c0 + v < a.channels) write_state<S>(w + v * NW, BP[v] * s[v] + BQ[v]);
+        for (int v = 0; v < NP; ++v) {
+          const K out = mad(BP[v], s[v], BQ[v]);
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+            if (c0 + v * W + i < a.channels) write_state<S>(w + (v * W + i) * NW, out.get(i));
+        }
       }
     }
-    // and the warps of the tile before this one
-    for (int i = 0; i < place; ++i)
 #pragma unroll
-      for (int v = 0; v < N; ++v) {
-        const Pair<S> m = part[team * wt + nth(i)][lane * N + v];
-        s[v] = m.p * s[v] + m.q;
-      }
+    for (int v = 0; v < NP; ++v) s[v] = mad(P[v], s[v], Q[v]);
   }
   if (!live) return;
 
   // the steps themselves; results take the place of what they came from
   auto step = [&](int r, bool masked) {
-    const Lane8<T> g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
+    const L g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
+    auto settle = [&](int v, K next, K& out) {  // behind the end: the state stays, results are 0
+      if (!masked) {
+        s[v] = next;
+        return;
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (r < end[v * W + w]) s[v].set(w, next.get(w));
+        else out.set(w, S(0));
+      }
+    };
     if constexpr (!BWD) {
-      Lane8<T> out;
+      L out;
 #pragma unroll
-      for (int v = 0; v < N; ++v) {
-        S f = Elem<T>::load(g.v[v]), b = Elem<T>::load(x.v[v]);
+      for (int v = 0; v < NP; ++v) {
+        K f = g.v[v], b = x.v[v];
         if constexpr (SIG) {
-          S keep;
+          K keep;
           sigmoid_pair(f, &f, &keep);
-          b *= keep;
+          b = b * keep;
         }
-        const S n = f * s[v] + b;
-        const bool on = !masked || r < end[v];
-        if (on) s[v] = n;
-        out.v[v] = Elem<T>::store(on ? n : S(0));
+        out.v[v] = mad(f, s[v], b);
+        settle(v, out.v[v], out.v[v]);
       }
-      lane_store(second + r * ROW, lane, out);
+      lane_store<T>(second + r * ROW, lane, out);
     } else {
-      Lane8<T> was = lane_load<T>(before + r * ROW, lane), xv{}, dg, dx;
+      L was = lane_load<T>(before + r * ROW, lane), xv{}, dg, dx;
       if constexpr (SIG) xv = lane_load<T>(xrow + r * ROW, lane);
-      const bool start = t0 + r == 0;
+      if (t0 + r == 0) {
 #pragma unroll
-      for (int v = 0; v < N; ++v) {
-        S f = Elem<T>::load(g.v[v]);
-        const S total = Elem<T>::load(x.v[v]) + s[v];
-        S prev = Elem<T>::load(was.v[v]);
-        if (start) prev = p.h0 && c0 + v < a.channels ? ((const S*)p.h0)[c0 + v] : S(0);
-        S sx = total, sg = total * prev;
-        if constexpr (SIG) {
-          S keep;
-          sigmoid_pair(f, &f, &keep);
-          sx = total * keep;
-          sg = (prev - Elem<T>::load(xv.v[v])) * f * sx;
-        }
-        const bool on = !masked || r < end[v];
-        if (on) s[v] = f * total;
-        dx.v[v] = Elem<T>::store(on ? sx : S(0));
-        dg.v[v] = Elem<T>::store(on ? sg : S(0));
+        for (int v = 0; v < N; ++v)
+          was.v[v / W].set(v % W, p.h0 && c0 + v < a.channels ? ((const S*)p.h0)[c0 + v] : S(0));
       }
-      lane_store(gate + r * ROW, lane, dg);
-      lane_store(second + r * ROW, lane, dx);
+#pragma unroll
+      for (int v = 0; v < NP; ++v) {
+        K f = g.v[v];
+        const K total = x.v[v] + s[v];
+        if constexpr (SIG) {
+          K keep;
+          sigmoid_pair(f, &f, &keep);
+          dx.v[v] = total * keep;
+          dg.v[v] = mad(xv.v[v], fill(S(-1)), was.v[v]) * f * dx.v[v];
+        } else {
+          dx.v[v] = total;
+          dg.v[v] = total * was.v[v];
+        }
+        const K next = f * total;
+        settle(v, next, dx.v[v]);
+        if (masked) {
+#pragma unroll
+          for (int w = 0; w < W; ++w)
+            if (r >= end[v * W + w]) dg.v[v].set(w, S(0));
+        }
+      }
+      lane_store<T>(gate + r * ROW, lane, dg);
+      lane_store<T>(second + r * ROW, lane, dx);
     }
   };
   if (full) {
@@ -519,7 +636,7 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   if (last && order == a.tiles - 1 && tw == (BWD ? 0 : wt - 1)) {
 #pragma unroll
     for (int v = 0; v < N; ++v)
-      if (c0 + v < a.channels) last[c0 + v] = s[v];
+      if (c0 + v < a.channels) last[c0 + v] = s[v / W].get(v % W);
   }
 }
 
@@ -583,7 +700,7 @@ int launch_scan(om_backend* be, const ScanArgs& p) {
   }
   const size_t smem = (size_t)(WARPS / a.warps_t) * ARRAYS * a.rows * ROW;
   auto kernel = scan_kernel<T, SIG, BWD>;
-  if (smem > 48 * 1024 - 8 * 1024)
+  if (smem > 40 * 1024)
     OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
             "gated_scan");
   ProfScope prof(be, BWD ? "gated_scan_backward" : "gated_scan");
