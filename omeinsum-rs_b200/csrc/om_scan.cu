@@ -4,14 +4,14 @@
 //
 // A step is the map s -> P s + Q with (P, Q) = (a, b) (backward: (a, a dh)), and
 // maps compose, so time can be cut. A tile is 256 bytes of channels (32 lanes
-// of 8 bytes) by up to 64 steps, four warps of 16 steps each; it is copied to
+// of 8 bytes) by up to 128 steps, eight warps of 16 (backward: 8) each; it is copied to
 // shared memory asynchronously and lives there until its results have taken
 // its place. Each warp first composes its 16 steps (from shared memory), the
-// block its four warps, and, where a sequence has more than one tile, tiles
+// block its eight warps, and, where a sequence has more than one tile, tiles
 // find the state that enters them by looking back: 32 consecutive tiles of one
 // column form a group; a tile composes the maps of its predecessors in the
 // group with the state that left the group before, and the group's last tile
-// passes the state on. So the serial chain has one link per 2048 steps, and
+// passes the state on. So the serial chain has one link per 4096 (2048) steps, and
 // every sum is formed in one order whatever the timing. Tiles are handed out by
 // a counter, first tiles first, so whatever a tile waits for has started.
 //
@@ -48,23 +48,25 @@ struct ScanArgs {
 };
 
 constexpr int ROW = 256;       // bytes of channels in a tile
-constexpr int STEPS = 16;      // of a warp
-constexpr int WARPS = 4;       // of a block
+constexpr int WARPS = 8;       // of a block
+constexpr int MAX_STEPS = 16;  // of a warp
 constexpr int GROUP = 32;      // tiles that look back at one another
 constexpr uint32_t POLL_LIMIT = 1u << 22;
 
 struct TileArgs {
   int64_t channels;  // B * D
   int grain;         // bytes of a row that one copy moves
-  int warps_t;       // warps along time: 4, or 1 (then the block has four columns)
+  int warps_t;       // warps along time; the block has 8 / warps_t columns
+  int steps;         // of a warp
   int rows;          // steps of a tile
+  int narrow;        // channel numbers fit 32 bits
   int columns;       // of 256 bytes
   int tiles;         // along time
   // looking back; null when a sequence is one tile
   uint32_t* ticket;
-  uint32_t* flags;   // [tile][column]: the tile's map is in `maps`
-  uint64_t* state;   // [group][channel][words]: 32 bits of the state and a set mark
-  void* maps;        // [tile][channel] pairs (P, Q)
+  uint32_t* flags;   // [tile][column]: warps that have put their part of the map into `maps`
+  uint64_t* state;   // [group][channel of all columns][words]: 32 bits of the state and a set mark
+  void* maps;        // [tile][channel of all columns] pairs (P, Q)
   uint32_t* err;
 };
 
@@ -214,62 +216,88 @@ __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
                : "memory");
 }
 
-// One array's view in bytes; `shift`: row r of the tile is step t0 + r + shift
+// One array's view: byte strides
 struct View {
   const char* ptr;
   int64_t d, t, b;
 };
 
-// Calls f(shared place, global place) for each piece of `grain` bytes of rows
-// [r0, r1) of column `col` that lies inside the array, threads tt of tn.
+// Where piece p (of `grain` bytes) of a row of column `col` lies
+struct Piece {
+  int64_t b, d;
+  bool in;
+};
+__device__ __forceinline__ Piece piece_at(const TileArgs& a, int64_t D, int elem, int col, int p) {
+  const int64_t c = ((int64_t)col * (ROW / a.grain) + p) * (a.grain / elem);
+  Piece r;
+  r.in = c < a.channels;
+  r.b = a.narrow ? (int64_t)((uint32_t)c / (uint32_t)D) : c / D;
+  r.d = c - r.b * D;
+  return r;
+}
+
+// f(shared place, global place) for rows r0, r0 + step, ... < r1 of a piece
+template <typename F>
+__device__ __forceinline__ void each_row(const View& v, const Piece& at, char* to, int64_t t0,
+                                         int r0, int r1, int step, F f) {
+  const char* g = v.ptr + at.b * v.b + at.d * v.d + (t0 + r0) * v.t;
+  char* s = to + r0 * ROW;
+  const int64_t skip = step * v.t;
+#pragma unroll 4
+  for (int r = r0; r < r1; r += step, g += skip, s += step * ROW) f(s, g);
+}
+
+// Rows [r0, r1) of a tile, the pieces of a row shared out over `tn` threads.
+// `once`: this thread's only piece, where a row has at most 32 of them.
 template <typename F>
 __device__ __forceinline__ void each_piece(const TileArgs& a, int64_t D, int elem, const View& v,
-                                           char* tile, int col, int64_t t0, int r0, int r1,
-                                           int64_t first, int64_t last, int tt, int tn, F f) {
-  const int per_row = ROW / a.grain, lanes = min(per_row, tn);
+                                           const Piece& once, char* tile, int col, int64_t t0,
+                                           int r0, int r1, int tt, int tn, F f) {
+  const int per_row = ROW / a.grain;
+  if (per_row <= 32) {
+    const int p = tt & (per_row - 1);
+    if (once.in) each_row(v, once, tile + p * a.grain, t0, r0 + tt / per_row, r1, tn / per_row, f);
+    return;
+  }
+  const int lanes = min(per_row, tn);
   for (int p = tt % lanes; p < per_row; p += lanes) {
-    const int64_t c = ((int64_t)col * per_row + p) * a.grain / elem;
-    if (c >= a.channels) break;
-    const int64_t b = (uint64_t)c / (uint64_t)D, d = c - b * D;
-    const char* g = v.ptr + b * v.b + d * v.d + t0 * v.t;
-    for (int r = r0 + tt / lanes; r < r1; r += tn / lanes) {
-      const int64_t t = t0 + r;
-      if (t >= first && t < last) f(tile + r * ROW + p * a.grain, g + (int64_t)r * v.t);
-    }
+    const Piece at = piece_at(a, D, elem, col, p);
+    if (!at.in) break;
+    each_row(v, at, tile + p * a.grain, t0, r0 + tt / lanes, r1, tn / lanes, f);
   }
 }
 
 __device__ __forceinline__ void load_rows(const TileArgs& a, int64_t D, int elem, const View& v,
-                                          char* tile, int col, int64_t t0, int64_t first,
-                                          int64_t last, int tt, int tn) {
+                                          const Piece& once, char* tile, int col, int64_t t0,
+                                          int r0, int r1, int tt, int tn) {
   if (a.grain == 16)
-    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
                [](char* s, const char* g) { copy_async16(s, g); });
   else if (a.grain == 8)
-    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
                [](char* s, const char* g) { copy_async<8>(s, g); });
   else if (a.grain == 4)
-    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
                [](char* s, const char* g) { copy_async<4>(s, g); });
   else
-    each_piece(a, D, elem, v, tile, col, t0, 0, a.rows, first, last, tt, tn,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
                [](char* s, const char* g) { *(uint16_t*)s = *(const uint16_t*)g; });
 }
 
 __device__ __forceinline__ void store_rows_of(const TileArgs& a, int64_t D, int elem, const View& v,
-                                              char* tile, int col, int64_t t0, int r0, int r1,
-                                              int64_t last, int lane) {
+                                              const Piece& once, char* tile, int col, int64_t t0,
+                                              int r0, int r1, int lane) {
   if (a.grain == 16)
-    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
                [](char* s, const char* g) { *(uint4*)g = *(const uint4*)s; });
   else if (a.grain == 8)
-    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
                [](char* s, const char* g) { *(uint2*)g = *(const uint2*)s; });
   else if (a.grain == 4)
-    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
                [](char* s, const char* g) { *(uint32_t*)g = *(const uint32_t*)s; });
   else
-    each_piece(a, D, elem, v, tile, col, t0, r0, r1, 0, last, lane, 32,
+    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
                [](char* s, const char* g) { *(uint16_t*)g = *(const uint16_t*)s; });
 }
 
@@ -300,9 +328,17 @@ __device__ __forceinline__ void poll(uint32_t* err, F ready) {
 }
 
 template <typename S>
-struct Pair {
+struct alignas(2 * sizeof(S)) Pair {
   S p, q;
 };
+__device__ __forceinline__ Pair<float> load_pair(const Pair<float>* m) {
+  const float2 v = __ldcg(reinterpret_cast<const float2*>(m));
+  return Pair<float>{v.x, v.y};
+}
+__device__ __forceinline__ Pair<double> load_pair(const Pair<double>* m) {
+  const double2 v = __ldcg(reinterpret_cast<const double2*>(m));
+  return Pair<double>{v.x, v.y};
+}
 
 // The state that entered from the group before, one word per 32 bits
 template <typename S>
@@ -346,7 +382,11 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;  // gate, x or dh, h, x
   constexpr int E = sizeof(T);
   extern __shared__ __align__(16) char smem[];
-  __shared__ Pair<K> part[WARPS][32 * NP];
+  constexpr int C = 32 * N;                    // channels of a column
+  constexpr int SLICES = WARPS * 32 / C;       // threads per channel
+  __shared__ __align__(16) S part_p[WARPS][C];
+  __shared__ __align__(16) S part_q[WARPS][C];
+  __shared__ Pair<S> back[SLICES][C];
   __shared__ uint32_t ticket;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -370,41 +410,43 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   char* before = second + a.rows * ROW;  // h, a step late (backward)
   char* xrow = before + a.rows * ROW;    // x (backward, sigmoid)
 
+  const int have = (int)min((int64_t)a.rows, p.T - t0);  // steps of the tile that exist
+  const Piece once = piece_at(a, p.D, E, col, lane & min(31, ROW / a.grain - 1));
   if (live) {
     const int tt = threadIdx.x - team * wt * 32, tn = wt * 32;
-    load_rows(a, p.D, E, View{(const char*)p.gate, p.gd * E, p.gt * E, p.gb * E}, gate, col, t0, 0,
-              p.T, tt, tn);
+    load_rows(a, p.D, E, View{(const char*)p.gate, p.gd * E, p.gt * E, p.gb * E}, once, gate, col,
+              t0, 0, have, tt, tn);
     if constexpr (!BWD) {
-      load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, second, col, t0, 0,
-                p.T, tt, tn);
+      load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, once, second, col,
+                t0, 0, have, tt, tn);
     } else {
-      load_rows(a, p.D, E, View{(const char*)p.dh, p.ed * E, p.et * E, p.eb * E}, second, col, t0, 0,
-                p.T, tt, tn);
-      load_rows(a, p.D, E, View{(const char*)p.h - p.ht * E, p.hd * E, p.ht * E, p.hb * E}, before,
-                col, t0, 1, p.T, tt, tn);
+      load_rows(a, p.D, E, View{(const char*)p.dh, p.ed * E, p.et * E, p.eb * E}, once, second, col,
+                t0, 0, have, tt, tn);
+      // step 0 has no h before it
+      load_rows(a, p.D, E, View{(const char*)p.h - p.ht * E, p.hd * E, p.ht * E, p.hb * E}, once,
+                before, col, t0, t0 == 0, have, tt, tn);
       if constexpr (SIG)
-        load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, xrow, col, t0, 0,
-                  p.T, tt, tn);
+        load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, once, xrow, col,
+                  t0, 0, have, tt, tn);
     }
   }
   asm volatile("cp.async.commit_group;" ::: "memory");
 
-  // this lane's channels and where their sequences end, relative to t0
+  // this lane's channels and where their sequences end in the tile
   const int64_t c0 = ((int64_t)col * 32 + lane) * N;
   int end[N];
   bool full = true;  // every step of this warp's rows exists in every lane
-  const int r0 = tw * STEPS, r1 = min(r0 + STEPS, a.rows);
+  const int r0 = min(tw * a.steps, a.rows), r1 = min(r0 + a.steps, a.rows);
 #pragma unroll
   for (int v = 0; v < N; ++v) {
-    int64_t len = 0;
+    end[v] = 0;
     if (live && c0 + v < a.channels) {
-      len = p.T;
+      end[v] = have;
       if (p.lengths) {
-        const int64_t n = p.lengths[(c0 + v) / p.D];
-        len = n < 0 ? 0 : (n < p.T ? n : p.T);
+        const int64_t n = p.lengths[a.narrow ? (int64_t)((uint32_t)(c0 + v) / (uint32_t)p.D) : (c0 + v) / p.D];
+        end[v] = (int)max((int64_t)0, min(n - t0, (int64_t)have));
       }
     }
-    end[v] = (int)max((int64_t)-1, min(len - t0, (int64_t)a.rows));
     full = full && end[v] >= r1;
   }
   full = __all_sync(0xffffffffu, full);
@@ -412,17 +454,22 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   // The state that enters the tile; the first group starts from the caller's.
   // It is read before this tile's map is published: the last tile, which may
   // overwrite it (h_last == h0), comes after every map of its group.
+  const S* from = (const S*)(BWD ? p.dh_last : p.h0);
   K s[NP];
+  S start = 0;
+  if (!a.ticket) {
 #pragma unroll
-  for (int v = 0; v < N; ++v) {
-    const S* from = (const S*)(BWD ? p.dh_last : p.h0);
-    s[v / W].set(v % W, order < GROUP && from && live && c0 + v < a.channels ? from[c0 + v] : S(0));
+    for (int v = 0; v < N; ++v)
+      s[v / W].set(v % W, from && live && c0 + v < a.channels ? from[c0 + v] : S(0));
+  } else if (order < GROUP && from && threadIdx.x < C) {
+    const int64_t c = (int64_t)col * C + threadIdx.x;
+    if (c < a.channels) start = from[c];
   }
 
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
 
-  if (wt > 1) {
+  if (wt > 1) {  // (all the warps of the block, where tiles look back)
     // the map of this warp's steps
     K P[NP], Q[NP];
 #pragma unroll
@@ -458,97 +505,79 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
       for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, true);
     }
 #pragma unroll
-    for (int v = 0; v < NP; ++v) part[warp][lane * NP + v] = Pair<K>{P[v], Q[v]};
-    __syncthreads();
-    // the map of the tile, and of its steps before this warp's (which run
-    // forward from the first warp, backward from the last)
-    K BP[NP], BQ[NP];
-    const int place = BWD ? wt - 1 - tw : tw;
-#pragma unroll
     for (int v = 0; v < NP; ++v) {
-      BP[v] = P[v] = fill(S(1)), BQ[v] = Q[v] = fill(S(0));
-#pragma unroll
-      for (int i = 0; i < WARPS; ++i) {
-        const Pair<K> m = part[BWD ? WARPS - 1 - i : i][lane * NP + v];
-        if (i == place) P[v] = BP[v], Q[v] = BQ[v];
-        BQ[v] = mad(m.p, BQ[v], m.q);
-        BP[v] = m.p * BP[v];
+      *reinterpret_cast<K*>(&part_p[warp][lane * N + v * W]) = P[v];
+      *reinterpret_cast<K*>(&part_q[warp][lane * N + v * W]) = Q[v];
+    }
+    __syncthreads();
+    // From here a thread has one channel. Those of the first slice replace each
+    // warp's map by that of the steps before it (which run forward from the
+    // first warp, backward from the last) and keep the whole tile's.
+    const int ch = threadIdx.x % C, slice = threadIdx.x / C;
+    S TP = 1, TQ = 0;
+    if (slice < WARPS / wt) {
+      for (int i = 0; i < wt; ++i) {
+        const int w = slice * wt + (BWD ? wt - 1 - i : i);
+        const S mp = part_p[w][ch], mq = part_q[w][ch];
+        part_p[w][ch] = TP;
+        part_q[w][ch] = TQ;
+        TQ = mp * TQ + mq;
+        TP = mp * TP;
       }
     }
     if (a.ticket) {
-      Pair<S>* maps = (Pair<S>*)a.maps;
+      Pair<S>* maps = (Pair<S>*)a.maps + (int64_t)col * C + ch;
       const int group = order / GROUP, in_group = order % GROUP;
-      if (warp == 0 && in_group < GROUP - 1 && order < a.tiles - 1) {
-#pragma unroll
-        for (int v = 0; v < N; ++v)
-          if (c0 + v < a.channels)
-            maps[(int64_t)order * a.channels + c0 + v] =
-                Pair<S>{BP[v / W].get(v % W), BQ[v / W].get(v % W)};
+      const int64_t pitch = (int64_t)a.columns * C;
+      if (slice == 0 && in_group < GROUP - 1 && order < a.tiles - 1) {
+        maps[(int64_t)order * pitch] = Pair<S>{TP, TQ};
         __threadfence();
+        // one mark per warp that wrote a part of the map
         __syncwarp();
         if (lane == 0)
-          asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(a.flags + (int64_t)order * a.columns + col)
+          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(
+                           a.flags + (int64_t)order * a.columns + col)
                        : "memory");
       }
-      // predecessors in the group, a quarter of them per warp
-      K LP[NP], LQ[NP];
-#pragma unroll
-      for (int v = 0; v < NP; ++v) LP[v] = fill(S(1)), LQ[v] = fill(S(0));
-      const int i0 = warp * (GROUP / WARPS), i1 = min(i0 + GROUP / WARPS, in_group);
+      // predecessors in the group, shared out over the slices
+      const int i0 = slice * (GROUP / SLICES), i1 = min(i0 + GROUP / SLICES, in_group);
+      S LP = 1, LQ = 0;
       if (i0 < i1) {
         if (lane < i1 - i0) {
           const uint32_t* f = a.flags + (int64_t)(group * GROUP + i0 + lane) * a.columns + col;
-          poll(a.err, [&] { return load_flag(f) != 0; });
+          poll(a.err, [&] { return load_flag(f) == C / 32; });
         }
         __syncwarp();
-#pragma unroll 4
+        const Pair<S>* m = maps + (int64_t)(group * GROUP) * pitch;
+#pragma unroll 8
         for (int i = i0; i < i1; ++i) {
-          const Pair<S>* m = maps + (int64_t)(group * GROUP + i) * a.channels + c0;
-          K mp[NP], mq[NP];
-#pragma unroll
-          for (int v = 0; v < N; ++v) {
-            const bool in = c0 + v < a.channels;
-            mp[v / W].set(v % W, in ? __ldcg(&m[v].p) : S(0));
-            mq[v / W].set(v % W, in ? __ldcg(&m[v].q) : S(0));
-          }
-#pragma unroll
-          for (int v = 0; v < NP; ++v) {
-            LQ[v] = mad(mp[v], LQ[v], mq[v]);
-            LP[v] = mp[v] * LP[v];
-          }
+          const Pair<S> w = load_pair(m + i * pitch);
+          LQ = w.p * LQ + w.q;
+          LP = w.p * LP;
         }
       }
-      __syncthreads();  // part has been read
-#pragma unroll
-      for (int v = 0; v < NP; ++v) part[warp][lane * NP + v] = Pair<K>{LP[v], LQ[v]};
+      back[slice][ch] = Pair<S>{LP, LQ};
       __syncthreads();
-      constexpr int NW = sizeof(S) / 4;
-      if (group > 0) {
-        const uint64_t* w = a.state + ((int64_t)(group - 1) * a.channels + c0) * NW;
+      if (slice == 0) {
+        constexpr int NW = sizeof(S) / 4;
+        const int64_t c = (int64_t)col * C + ch;
+        uint64_t* w = a.state + ((int64_t)group * pitch + c) * NW;
+        S in = group > 0 ? read_state<S>(w - pitch * NW, a.err) : start;
 #pragma unroll
-        for (int v = 0; v < N; ++v)
-          if (c0 + v < a.channels) s[v / W].set(v % W, read_state<S>(w + v * NW, a.err));
+        for (int i = 0; i < SLICES; ++i) in = back[i][ch].p * in + back[i][ch].q;
+        if (in_group == GROUP - 1 && order < a.tiles - 1) write_state<S>(w, TP * in + TQ);
+        back[0][ch].p = in;
       }
+      __syncthreads();
 #pragma unroll
-      for (int v = 0; v < NP; ++v)
-#pragma unroll
-        for (int i = 0; i < WARPS; ++i) {
-          const Pair<K> m = part[i][lane * NP + v];
-          s[v] = mad(m.p, s[v], m.q);
-        }
-      if (warp == 0 && in_group == GROUP - 1 && order < a.tiles - 1) {
-        uint64_t* w = a.state + ((int64_t)group * a.channels + c0) * NW;
-#pragma unroll
-        for (int v = 0; v < NP; ++v) {
-          const K out = mad(BP[v], s[v], BQ[v]);
-#pragma unroll
-          for (int i = 0; i < W; ++i)
-            if (c0 + v * W + i < a.channels) write_state<S>(w + (v * W + i) * NW, out.get(i));
-        }
-      }
+      for (int v = 0; v < N; ++v) s[v / W].set(v % W, back[0][lane * N + v].p);
+    } else {
+      __syncthreads();
     }
 #pragma unroll
-    for (int v = 0; v < NP; ++v) s[v] = mad(P[v], s[v], Q[v]);
+    for (int v = 0; v < NP; ++v)
+      s[v] = mad(*reinterpret_cast<const K*>(&part_p[warp][lane * N + v * W]), s[v],
+                 *reinterpret_cast<const K*>(&part_q[warp][lane * N + v * W]));
   }
   if (!live) return;
 
@@ -621,14 +650,15 @@ __global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant_
   }
   __syncwarp();
   if (r0 < r1) {
+    const int stop = min(r1, have);
     if constexpr (!BWD) {
-      store_rows_of(a, p.D, E, View{(const char*)p.h, p.hd * E, p.ht * E, p.hb * E}, second, col, t0,
-                    r0, r1, p.T, lane);
+      store_rows_of(a, p.D, E, View{(const char*)p.h, p.hd * E, p.ht * E, p.hb * E}, once, second,
+                    col, t0, r0, stop, lane);
     } else {
-      store_rows_of(a, p.D, E, View{(const char*)p.dgate, p.pd * E, p.pt * E, p.pb * E}, gate, col,
-                    t0, r0, r1, p.T, lane);
-      store_rows_of(a, p.D, E, View{(const char*)p.dx, p.qd * E, p.qt * E, p.qb * E}, second, col, t0,
-                    r0, r1, p.T, lane);
+      store_rows_of(a, p.D, E, View{(const char*)p.dgate, p.pd * E, p.pt * E, p.pb * E}, once, gate,
+                    col, t0, r0, stop, lane);
+      store_rows_of(a, p.D, E, View{(const char*)p.dx, p.qd * E, p.qt * E, p.qb * E}, once, second,
+                    col, t0, r0, stop, lane);
     }
   }
   // the state that leaves the last tile
@@ -675,9 +705,13 @@ int launch_scan(om_backend* be, const ScanArgs& p) {
   a.channels = p.D * p.B;
   a.grain = grain_of(p, sizeof(T), BWD, SIG || !BWD);
   const int64_t columns = (a.channels * (int64_t)sizeof(T) + ROW - 1) / ROW;
-  // up to 16 steps are one warp's work, four columns then share a block
-  a.warps_t = p.T > STEPS ? WARPS : 1;
-  a.rows = (int)std::min<int64_t>(p.T, STEPS * a.warps_t);
+  a.narrow = a.channels < ((int64_t)1 << 32) && p.D < ((int64_t)1 << 32);
+  // Up to 16 steps are one warp's work and eight columns share a block; longer
+  // sequences take all eight warps, the backward pass with half the steps
+  // each: its three or four arrays then leave three blocks on an SM.
+  a.warps_t = p.T > MAX_STEPS ? WARPS : 1;
+  a.steps = a.warps_t > 1 && BWD ? MAX_STEPS / 2 : MAX_STEPS;
+  a.rows = (int)std::min<int64_t>(p.T, a.steps * a.warps_t);
   const int64_t tiles = p.T == 0 ? 1 : (p.T + a.rows - 1) / a.rows;
   const int64_t blocks = tiles > 1 ? tiles * columns : (columns + WARPS / a.warps_t - 1) / (WARPS / a.warps_t);
   if (blocks > 0x7fffffff || columns > 0x7ffffff0)
@@ -688,9 +722,10 @@ int launch_scan(om_backend* be, const ScanArgs& p) {
   Scratch ws;
   if (tiles > 1) {
     const int64_t groups = (tiles + GROUP - 1) / GROUP;
-    const size_t state = (size_t)groups * a.channels * (sizeof(S) / 4) * 8;
+    const size_t pitch = (size_t)columns * (ROW / sizeof(T));
+    const size_t state = (size_t)groups * pitch * (sizeof(S) / 4) * 8;
     const size_t flags = ((size_t)blocks * 4 + 15) / 16 * 16;
-    OM_TRY(ws.alloc(be, 16 + flags + state + (size_t)tiles * a.channels * sizeof(Pair<S>)));
+    OM_TRY(ws.alloc(be, 16 + flags + state + (size_t)tiles * pitch * sizeof(Pair<S>)));
     char* at = (char*)ws.ptr;
     OM_CUDA(cudaMemsetAsync(at, 0, 16 + flags + state, be->stream), "gated_scan marks");
     a.ticket = (uint32_t*)at;
