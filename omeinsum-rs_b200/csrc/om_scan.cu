@@ -1,23 +1,21 @@
 // Gated linear recurrence h_t = a_t h_{t-1} + b_t and its backward pass
-//     S_t = a_t (dh_t + S_{t+1}),   G_t = dh_t + S_{t+1},
-// in one pass over the data: each element is read once and written once.
+//     S_t = a_t (dh_t + S_{t+1}),   G_t = dh_t + S_{t+1}.
 //
 // A step is the map s -> P s + Q with (P, Q) = (a, b) (backward: (a, a dh)), and
-// maps compose, so time can be cut. A tile is 256 bytes of channels (32 lanes
-// of 8 bytes) by up to 128 steps, eight warps of 16 (backward: 8) each; it is copied to
-// shared memory asynchronously and lives there until its results have taken
-// its place. Each warp first composes its 16 steps (from shared memory), the
-// block its eight warps, and, where a sequence has more than one tile, tiles
-// find the state that enters them by looking back: 32 consecutive tiles of one
-// column form a group; a tile composes the maps of its predecessors in the
-// group with the state that left the group before, and the group's last tile
-// passes the state on. So the serial chain has one link per 4096 (2048) steps, and
-// every sum is formed in one order whatever the timing. Tiles are handed out by
-// a counter, first tiles first, so whatever a tile waits for has started.
+// maps compose, so time can be cut into chunks that run side by side:
+//   map_kernel    composes the steps of each chunk, and of eight consecutive
+//                 chunks (a block's) together;
+//   step_kernel   joins the maps before its chunk to the state that enters it
+//                 and takes the chunk's steps one by one, writing the results.
+// A warp has 32 lanes of 8 bytes of channels (fewer where rows are not 8-byte
+// aligned or channels are not contiguous) and a chunk's steps; it loads several steps at once and holds the state in
+// registers, so nothing but the maps passes through shared memory. Sums are
+// formed in one order whatever the timing. Where the channels alone fill the
+// card, a sequence is one chunk and map_kernel does not run.
 //
-// Bound by HBM: 3 arrays (forward) or 5 to 6 (backward) per element; the two
-// passes over shared memory cost instructions, not traffic, and leave six
-// tiles (32 KiB each) per SM in flight, which hides the look-back.
+// Bound by HBM: step_kernel moves 3 arrays (forward) or 5 to 6 (backward) per
+// element, map_kernel 2 more. step_kernel starts at the chunks that map_kernel
+// read last, which are still in L2.
 #include <algorithm>
 
 #include "om_convert.cuh"
@@ -47,634 +45,502 @@ struct ScanArgs {
   void* dh0;
 };
 
-constexpr int ROW = 256;       // bytes of channels in a tile
-constexpr int WARPS = 8;       // of a block
-constexpr int MAX_STEPS = 16;  // of a warp
-constexpr int GROUP = 32;      // tiles that look back at one another
-constexpr uint32_t POLL_LIMIT = 1u << 22;
+constexpr int WARPS = 8;  // of a block
 
-struct TileArgs {
-  int64_t channels;  // B * D
-  int grain;         // bytes of a row that one copy moves
-  int warps_t;       // warps along time; the block has 8 / warps_t columns
-  int steps;         // of a warp
-  int rows;          // steps of a tile
-  int narrow;        // channel numbers fit 32 bits
-  int columns;       // of 256 bytes
-  int tiles;         // along time
-  // looking back; null when a sequence is one tile
-  uint32_t* ticket;
-  uint32_t* flags;   // [tile][column]: warps that have put their part of the map into `maps`
-  uint64_t* state;   // [group][channel of all columns][words]: 32 bits of the state and a set mark
-  void* maps;        // [tile][channel of all columns] pairs (P, Q)
-  uint32_t* err;
+struct ChunkArgs {
+  int64_t groups;   // of VEC channels, a lane's
+  int64_t pitch;    // channels of all columns of 32 lanes
+  int columns;
+  int warps_t;      // warps of a block that take consecutive chunks of one column
+  int chunks;       // of a sequence
+  int64_t steps;    // of a chunk
+  int narrow;       // channel numbers fit 32 bits
+  void* maps;       // [chunk][channel] pairs (P, Q)
+  void* joined;     // [block of chunks][channel]
+  void* start;      // [channel] the caller's state, which h_last may overwrite
 };
 
 // ---- arithmetic on the channels of a lane ------------------------------------------
-// Two f32 channels share one instruction (the f32x2 forms of sm_100); an f64
-// channel stands alone.
+// Two f32 channels share one instruction (the f32x2 forms of sm_100); one alone
+// and f64 take the plain ones.
 
-template <typename S>
+template <typename S, int N>
 struct Pack;
 template <>
-struct Pack<float> {
-  static constexpr int N = 2;
+struct Pack<float, 2> {
   float2 v;
   __device__ __forceinline__ float get(int i) const { return i ? v.y : v.x; }
   __device__ __forceinline__ void set(int i, float s) { (i ? v.y : v.x) = s; }
+  static __device__ __forceinline__ Pack all(float s) { return Pack{make_float2(s, s)}; }
 };
-template <>
-struct Pack<double> {
-  static constexpr int N = 1;
-  double v;
-  __device__ __forceinline__ double get(int) const { return v; }
-  __device__ __forceinline__ void set(int, double s) { v = s; }
+template <typename S>
+struct Pack<S, 1> {
+  S v;
+  __device__ __forceinline__ S get(int) const { return v; }
+  __device__ __forceinline__ void set(int, S s) { v = s; }
+  static __device__ __forceinline__ Pack all(S s) { return Pack{s}; }
 };
+using Two = Pack<float, 2>;
 
 __device__ __forceinline__ uint64_t bits_of(float2 v) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.x), "f"(v.y));
   return r;
 }
-__device__ __forceinline__ Pack<float> of_bits(uint64_t r) {
-  Pack<float> p;
+__device__ __forceinline__ Two of_bits(uint64_t r) {
+  Two p;
   asm("mov.b64 {%0, %1}, %2;" : "=f"(p.v.x), "=f"(p.v.y) : "l"(r));
   return p;
 }
-__device__ __forceinline__ Pack<float> fill(float s) { return Pack<float>{make_float2(s, s)}; }
-__device__ __forceinline__ Pack<double> fill(double s) { return Pack<double>{s}; }
-__device__ __forceinline__ Pack<float> operator*(Pack<float> a, Pack<float> b) {
+__device__ __forceinline__ Two operator*(Two a, Two b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a.v)), "l"(bits_of(b.v)));
   return of_bits(r);
 }
-__device__ __forceinline__ Pack<float> operator+(Pack<float> a, Pack<float> b) {
+__device__ __forceinline__ Two operator+(Two a, Two b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits_of(a.v)), "l"(bits_of(b.v)));
   return of_bits(r);
 }
-__device__ __forceinline__ Pack<float> mad(Pack<float> a, Pack<float> b, Pack<float> c) {
+__device__ __forceinline__ Two mad(Two a, Two b, Two c) {
   uint64_t r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;"
       : "=l"(r)
       : "l"(bits_of(a.v)), "l"(bits_of(b.v)), "l"(bits_of(c.v)));
   return of_bits(r);
 }
-__device__ __forceinline__ Pack<double> operator*(Pack<double> a, Pack<double> b) {
-  return Pack<double>{a.v * b.v};
+template <typename S>
+__device__ __forceinline__ Pack<S, 1> operator*(Pack<S, 1> a, Pack<S, 1> b) {
+  return Pack<S, 1>{a.v * b.v};
 }
-__device__ __forceinline__ Pack<double> operator+(Pack<double> a, Pack<double> b) {
-  return Pack<double>{a.v + b.v};
+template <typename S>
+__device__ __forceinline__ Pack<S, 1> operator+(Pack<S, 1> a, Pack<S, 1> b) {
+  return Pack<S, 1>{a.v + b.v};
 }
-__device__ __forceinline__ Pack<double> mad(Pack<double> a, Pack<double> b, Pack<double> c) {
-  return Pack<double>{fma(a.v, b.v, c.v)};
+template <typename S>
+__device__ __forceinline__ Pack<S, 1> mad(Pack<S, 1> a, Pack<S, 1> b, Pack<S, 1> c) {
+  return Pack<S, 1>{fma(a.v, b.v, c.v)};
 }
 
 // a = sigmoid(g) and 1 - a without cancellation. f32: an exponential formed as
 // a power of two and an approximate reciprocal, together below 24 half steps
 // for |g| <= 16 (most of it the rounding of the exponent); values below f32's
 // normal numbers become zero.
-__device__ __forceinline__ void sigmoid_pair(Pack<float> g, Pack<float>* a, Pack<float>* keep) {
-  const Pack<float> t = g * fill(-1.4426950408889634f);
-  Pack<float> e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v.x) : "f"(t.v.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.v.y) : "f"(t.v.y));
-  const Pack<float> d = e + fill(1.f);
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v.x) : "f"(d.v.x));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v.y) : "f"(d.v.y));
-  const Pack<float> small = e * r, large = mad(r, fill(-1.f), fill(1.f));
+__device__ __forceinline__ float power_of_two(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void sigmoid_pair(Two g, Two* a, Two* keep) {
+  const Two t = g * Two::all(-1.4426950408889634f);
+  const Two e{make_float2(power_of_two(t.v.x), power_of_two(t.v.y))};
+  const Two d = e + Two::all(1.f);
+  const Two r{make_float2(inverse(d.v.x), inverse(d.v.y))};
+  const Two small = e * r, large = mad(r, Two::all(-1.f), Two::all(1.f));
   keep->v.x = e.v.x > 1.f ? large.v.x : small.v.x;  // e may be infinite, r is then 0
   keep->v.y = e.v.y > 1.f ? large.v.y : small.v.y;
   *a = r;
 }
-__device__ __forceinline__ void sigmoid_pair(Pack<double> g, Pack<double>* a, Pack<double>* keep) {
+__device__ __forceinline__ void sigmoid_pair(Pack<float, 1> g, Pack<float, 1>* a,
+                                             Pack<float, 1>* keep) {
+  const float e = power_of_two(g.v * -1.4426950408889634f), r = inverse(e + 1.f);
+  keep->v = e > 1.f ? 1.f - r : e * r;
+  a->v = r;
+}
+__device__ __forceinline__ void sigmoid_pair(Pack<double, 1> g, Pack<double, 1>* a,
+                                             Pack<double, 1>* keep) {
   const double e = exp(-fabs(g.v)), r = 1 / (1 + e);
   a->v = g.v >= 0 ? r : e * r;
   keep->v = g.v >= 0 ? e * r : r;
   if (g.v != g.v) a->v = keep->v = g.v;
 }
 
-// 8 bytes of a row as packs, and back
-template <typename T>
+// ---- a lane's channels of one step ----------------------------------------------------
+
+// V channels as they lie in memory
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<2> {
+  using Type = uint16_t;
+};
+template <>
+struct Raw<4> {
+  using Type = uint32_t;
+};
+template <>
+struct Raw<8> {
+  using Type = uint2;
+};
+
+template <typename T, int V>
 struct Lane {
-  static constexpr int CHANNELS = 8 / sizeof(T);
-  using P = Pack<typename Elem<T>::State>;
-  static constexpr int PACKS = CHANNELS / P::N;
-  P v[PACKS];
-};
-__device__ __forceinline__ void unpack(uint2 u, Lane<__nv_bfloat16>& l) {
-  l.v[0].v = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
-  l.v[1].v = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
-}
-__device__ __forceinline__ void unpack(uint2 u, Lane<__half>& l) {
-  l.v[0].v = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
-  l.v[1].v = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
-}
-__device__ __forceinline__ void unpack(uint2 u, Lane<float>& l) {
-  l.v[0].v = make_float2(__uint_as_float(u.x), __uint_as_float(u.y));
-}
-__device__ __forceinline__ void unpack(uint2 u, Lane<double>& l) {
-  l.v[0].v = __hiloint2double((int)u.y, (int)u.x);
-}
-__device__ __forceinline__ uint2 repack(const Lane<__nv_bfloat16>& l) {
-  return make_uint2(pack2(l.v[0].v.x, l.v[0].v.y, __nv_bfloat16()),
-                    pack2(l.v[1].v.x, l.v[1].v.y, __nv_bfloat16()));
-}
-__device__ __forceinline__ uint2 repack(const Lane<__half>& l) {
-  return make_uint2(pack2(l.v[0].v.x, l.v[0].v.y, __half()), pack2(l.v[1].v.x, l.v[1].v.y, __half()));
-}
-__device__ __forceinline__ uint2 repack(const Lane<float>& l) {
-  return make_uint2(__float_as_uint(l.v[0].v.x), __float_as_uint(l.v[0].v.y));
-}
-__device__ __forceinline__ uint2 repack(const Lane<double>& l) {
-  return make_uint2((uint32_t)__double2loint(l.v[0].v), (uint32_t)__double2hiint(l.v[0].v));
-}
-template <typename T>
-__device__ __forceinline__ Lane<T> lane_load(const char* row, int lane) {
-  Lane<T> r;
-  unpack(*reinterpret_cast<const uint2*>(row + lane * 8), r);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void lane_store(char* row, int lane, const Lane<T>& r) {
-  *reinterpret_cast<uint2*>(row + lane * 8) = repack(r);
-}
-
-// ---- data of a tile --------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t shared_at(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
-
-template <int N>
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(shared_at(dst)), "l"(src), "n"(N)
-               : "memory");
-}
-__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at(dst)), "l"(src)
-               : "memory");
-}
-
-// One array's view: byte strides
-struct View {
-  const char* ptr;
-  int64_t d, t, b;
-};
-
-// Where piece p (of `grain` bytes) of a row of column `col` lies
-struct Piece {
-  int64_t b, d;
-  bool in;
-};
-__device__ __forceinline__ Piece piece_at(const TileArgs& a, int64_t D, int elem, int col, int p) {
-  const int64_t c = ((int64_t)col * (ROW / a.grain) + p) * (a.grain / elem);
-  Piece r;
-  r.in = c < a.channels;
-  r.b = a.narrow ? (int64_t)((uint32_t)c / (uint32_t)D) : c / D;
-  r.d = c - r.b * D;
-  return r;
-}
-
-// f(shared place, global place) for rows r0, r0 + step, ... < r1 of a piece
-template <typename F>
-__device__ __forceinline__ void each_row(const View& v, const Piece& at, char* to, int64_t t0,
-                                         int r0, int r1, int step, F f) {
-  const char* g = v.ptr + at.b * v.b + at.d * v.d + (t0 + r0) * v.t;
-  char* s = to + r0 * ROW;
-  const int64_t skip = step * v.t;
-#pragma unroll 4
-  for (int r = r0; r < r1; r += step, g += skip, s += step * ROW) f(s, g);
-}
-
-// Rows [r0, r1) of a tile, the pieces of a row shared out over `tn` threads.
-// `once`: this thread's only piece, where a row has at most 32 of them.
-template <typename F>
-__device__ __forceinline__ void each_piece(const TileArgs& a, int64_t D, int elem, const View& v,
-                                           const Piece& once, char* tile, int col, int64_t t0,
-                                           int r0, int r1, int tt, int tn, F f) {
-  const int per_row = ROW / a.grain;
-  if (per_row <= 32) {
-    const int p = tt & (per_row - 1);
-    if (once.in) each_row(v, once, tile + p * a.grain, t0, r0 + tt / per_row, r1, tn / per_row, f);
-    return;
+  using S = typename Elem<T>::State;
+  static constexpr int W = sizeof(S) == 4 && V % 2 == 0 ? 2 : 1;  // channels of a pack
+  static constexpr int N = V / W;
+  using K = Pack<S, W>;
+  using R = typename Raw<sizeof(T) * V>::Type;
+  K v[N];
+  static __device__ __forceinline__ Lane of(R r) {
+    Lane l;
+    if constexpr (V == 1) {
+      T t;
+      memcpy(&t, &r, sizeof(T));
+      l.v[0].v = Elem<T>::load(t);
+    } else if constexpr (sizeof(T) == 4) {
+      l.v[0].v = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+    } else {
+      l.v[0] = two(r.x);
+      l.v[1] = two(r.y);
+    }
+    return l;
   }
-  const int lanes = min(per_row, tn);
-  for (int p = tt % lanes; p < per_row; p += lanes) {
-    const Piece at = piece_at(a, D, elem, col, p);
-    if (!at.in) break;
-    each_row(v, at, tile + p * a.grain, t0, r0 + tt / lanes, r1, tn / lanes, f);
+  __device__ __forceinline__ R raw() const {
+    R r;
+    if constexpr (V == 1) {
+      const T t = Elem<T>::store(v[0].v);
+      memcpy(&r, &t, sizeof(T));
+    } else if constexpr (sizeof(T) == 4) {
+      r = make_uint2(__float_as_uint(v[0].v.x), __float_as_uint(v[0].v.y));
+    } else {
+      r = make_uint2(pack2(v[0].v.x, v[0].v.y, T()), pack2(v[1].v.x, v[1].v.y, T()));
+    }
+    return r;
   }
-}
-
-__device__ __forceinline__ void load_rows(const TileArgs& a, int64_t D, int elem, const View& v,
-                                          const Piece& once, char* tile, int col, int64_t t0,
-                                          int r0, int r1, int tt, int tn) {
-  if (a.grain == 16)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
-               [](char* s, const char* g) { copy_async16(s, g); });
-  else if (a.grain == 8)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
-               [](char* s, const char* g) { copy_async<8>(s, g); });
-  else if (a.grain == 4)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
-               [](char* s, const char* g) { copy_async<4>(s, g); });
-  else
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, tt, tn,
-               [](char* s, const char* g) { *(uint16_t*)s = *(const uint16_t*)g; });
-}
-
-__device__ __forceinline__ void store_rows_of(const TileArgs& a, int64_t D, int elem, const View& v,
-                                              const Piece& once, char* tile, int col, int64_t t0,
-                                              int r0, int r1, int lane) {
-  if (a.grain == 16)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
-               [](char* s, const char* g) { *(uint4*)g = *(const uint4*)s; });
-  else if (a.grain == 8)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
-               [](char* s, const char* g) { *(uint2*)g = *(const uint2*)s; });
-  else if (a.grain == 4)
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
-               [](char* s, const char* g) { *(uint32_t*)g = *(const uint32_t*)s; });
-  else
-    each_piece(a, D, elem, v, once, tile, col, t0, r0, r1, lane, 32,
-               [](char* s, const char* g) { *(uint16_t*)g = *(const uint16_t*)s; });
-}
-
-// ---- looking back ------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t load_flag(const uint32_t* p) {
-  uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint64_t load_word(const uint64_t* p) {
-  uint64_t v;
-  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
-}
-__device__ __forceinline__ void store_word(uint64_t* p, uint64_t v) {
-  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-
-// Polls until `ready`; gives up when the limit or another block's error says so
-template <typename F>
-__device__ __forceinline__ void poll(uint32_t* err, F ready) {
-  for (uint32_t i = 0; i < POLL_LIMIT; ++i) {
-    if (ready()) return;
-    if ((i & 255) == 255 && load_flag(err)) return;
+  static __device__ __forceinline__ Two two(uint32_t u) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      return Two{make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u))};
+    } else {
+      __half2 h;
+      memcpy(&h, &u, 4);
+      return Two{__half22float2(h)};
+    }
   }
-  atomicOr(err, 1u);
-}
+  __device__ __forceinline__ S get(int i) const { return v[i / W].get(i % W); }
+  __device__ __forceinline__ void set(int i, S s) { v[i / W].set(i % W, s); }
+};
 
 template <typename S>
 struct alignas(2 * sizeof(S)) Pair {
   S p, q;
 };
-__device__ __forceinline__ Pair<float> load_pair(const Pair<float>* m) {
-  const float2 v = __ldcg(reinterpret_cast<const float2*>(m));
-  return Pair<float>{v.x, v.y};
-}
-__device__ __forceinline__ Pair<double> load_pair(const Pair<double>* m) {
-  const double2 v = __ldcg(reinterpret_cast<const double2*>(m));
-  return Pair<double>{v.x, v.y};
-}
 
-// The state that entered from the group before, one word per 32 bits
-template <typename S>
-__device__ __forceinline__ S read_state(const uint64_t* w, uint32_t* err) {
-  constexpr int NW = sizeof(S) / 4;
-  uint64_t v[NW];
-  poll(err, [&] {
-    bool all = true;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      v[i] = load_word(w + i);
-      all = all && (v[i] >> 32);
-    }
-    return all;
-  });
-  uint32_t bits[NW];
-#pragma unroll
-  for (int i = 0; i < NW; ++i) bits[i] = (uint32_t)v[i];
-  S s;
-  memcpy(&s, bits, sizeof(S));
-  return s;
-}
-template <typename S>
-__device__ __forceinline__ void write_state(uint64_t* w, S s) {
-  constexpr int NW = sizeof(S) / 4;
-  uint32_t bits[NW];
-  memcpy(bits, &s, sizeof(S));
-#pragma unroll
-  for (int i = 0; i < NW; ++i) store_word(w + i, (1ull << 32) | bits[i]);
-}
-
-// ---- the kernel --------------------------------------------------------------------
-
-template <typename T, bool SIG, bool BWD>
-__global__ void __launch_bounds__(WARPS * 32) scan_kernel(const __grid_constant__ ScanArgs p,
-                                                          const __grid_constant__ TileArgs a) {
+// The map of V channels
+template <typename T, int V>
+struct Map {
   using S = typename Elem<T>::State;
-  using L = Lane<T>;
-  using K = Pack<S>;
-  constexpr int N = L::CHANNELS, NP = L::PACKS, W = K::N;
-  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;  // gate, x or dh, h, x
-  constexpr int E = sizeof(T);
-  extern __shared__ __align__(16) char smem[];
-  constexpr int C = 32 * N;                    // channels of a column
-  constexpr int SLICES = WARPS * 32 / C;       // threads per channel
-  __shared__ __align__(16) S part_p[WARPS][C];
-  __shared__ __align__(16) S part_q[WARPS][C];
-  __shared__ Pair<S> back[SLICES][C];
-  __shared__ uint32_t ticket;
+  using L = Lane<T, V>;
+  L p, q;
+  static __device__ __forceinline__ Map identity() {
+    Map m;
+#pragma unroll
+    for (int i = 0; i < L::N; ++i) m.p.v[i] = L::K::all(S(1)), m.q.v[i] = L::K::all(S(0));
+    return m;
+  }
+  __device__ __forceinline__ void then(const Map& m) {
+#pragma unroll
+    for (int i = 0; i < L::N; ++i) {
+      q.v[i] = mad(m.p.v[i], q.v[i], m.q.v[i]);
+      p.v[i] = m.p.v[i] * p.v[i];
+    }
+  }
+  __device__ __forceinline__ L at(const L& s) const {
+    L r;
+#pragma unroll
+    for (int i = 0; i < L::N; ++i) r.v[i] = mad(p.v[i], s.v[i], q.v[i]);
+    return r;
+  }
+  __device__ __forceinline__ void put(Pair<S>* to) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[i] = Pair<S>{p.get(i), q.get(i)};
+  }
+  static __device__ __forceinline__ Map take(const Pair<S>* from) {
+    Map m;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const Pair<S> w = from[i];
+      m.p.set(i, w.p);
+      m.q.set(i, w.q);
+    }
+    return m;
+  }
+};
 
+// Where a lane's channels are, and which steps of its chunk exist
+struct Place {
+  int64_t c0, b, d;   // first channel, its batch and place in the row
+  int64_t t0, t1;     // the chunk
+  int64_t end;        // steps before it exist (t1 at most, t0 at least)
+  bool live;          // the lane has channels, and the chunk is one
+  int order;          // chunk in the order in which states pass
+  int col;
+};
+template <typename T, int V, bool BWD>
+__device__ __forceinline__ Place place_of(const ScanArgs& p, const ChunkArgs& a, int col, int order) {
+  Place r;
+  const int lane = threadIdx.x & 31;
+  r.col = col;
+  r.order = order;
+  const int64_t g = (int64_t)col * 32 + lane;
+  r.c0 = g * V;
+  r.live = col < a.columns && g < a.groups && order < a.chunks;
+  const int64_t c = r.live ? r.c0 : 0;
+  r.b = a.narrow ? (int64_t)((uint32_t)c / (uint32_t)p.D) : c / p.D;
+  r.d = c - r.b * p.D;
+  const int64_t k = BWD ? a.chunks - 1 - order : order;
+  r.t0 = k * a.steps;
+  r.t1 = min(r.t0 + a.steps, p.T);
+  r.end = r.t1;
+  if (p.lengths && r.live) r.end = max(r.t0, min((int64_t)p.lengths[r.b], r.t1));
+  return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ typename Lane<T, V>::R fetch(const T* p) {
+  using R = typename Lane<T, V>::R;
+  return __ldg(reinterpret_cast<const R*>(p));
+}
+template <typename T, int V>
+__device__ __forceinline__ void keep(T* p, const Lane<T, V>& l) {
+  *reinterpret_cast<typename Lane<T, V>::R*>(p) = l.raw();
+}
+
+// ---- the maps of the chunks -------------------------------------------------------------
+
+template <typename T, int V, bool SIG, bool BWD>
+__device__ __forceinline__ void compose(Map<T, V>& m, Lane<T, V> g, Lane<T, V> x) {
+  using L = Lane<T, V>;
+#pragma unroll
+  for (int i = 0; i < L::N; ++i) {
+    typename L::K f = g.v[i], b = x.v[i];
+    if constexpr (SIG) {
+      typename L::K keep;
+      sigmoid_pair(f, &f, &keep);
+      if constexpr (!BWD) b = b * keep;
+    }
+    m.q.v[i] = BWD ? f * (b + m.q.v[i]) : mad(f, m.q.v[i], b);
+    m.p.v[i] = f * m.p.v[i];
+  }
+}
+
+template <typename T, int V, bool SIG, bool BWD>
+__global__ void __launch_bounds__(WARPS * 32, 4) map_kernel(const __grid_constant__ ScanArgs p,
+                                                            const __grid_constant__ ChunkArgs a) {
+  using S = typename Elem<T>::State;
+  using L = Lane<T, V>;
+  constexpr int U = 8;
+  __shared__ Pair<S> part[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int wt = a.warps_t, team = warp / wt, tw = warp % wt;  // teams of warps per column
-  // (tile along time, column); backward starts at the end of time
-  int tile = 0, col;
-  if (a.ticket) {
-    if (threadIdx.x == 0) ticket = atomicAdd(a.ticket, 1u);
-    __syncthreads();
-    tile = (int)(ticket / (uint32_t)a.columns);
-    col = (int)(ticket - (uint32_t)tile * (uint32_t)a.columns);
-  } else {
-    col = (int)blockIdx.x * (WARPS / wt) + team;
-  }
-  const int order = tile;  // place in the chain
-  if (BWD) tile = a.tiles - 1 - tile;
-  const bool live = col < a.columns;
-  const int64_t t0 = (int64_t)tile * a.rows;
-  char* gate = smem + (size_t)team * ARRAYS * a.rows * ROW;
-  char* second = gate + a.rows * ROW;    // x, or dh
-  char* before = second + a.rows * ROW;  // h, a step late (backward)
-  char* xrow = before + a.rows * ROW;    // x (backward, sigmoid)
-
-  const int have = (int)min((int64_t)a.rows, p.T - t0);  // steps of the tile that exist
-  const Piece once = piece_at(a, p.D, E, col, lane & min(31, ROW / a.grain - 1));
-  if (live) {
-    const int tt = threadIdx.x - team * wt * 32, tn = wt * 32;
-    load_rows(a, p.D, E, View{(const char*)p.gate, p.gd * E, p.gt * E, p.gb * E}, once, gate, col,
-              t0, 0, have, tt, tn);
-    if constexpr (!BWD) {
-      load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, once, second, col,
-                t0, 0, have, tt, tn);
-    } else {
-      load_rows(a, p.D, E, View{(const char*)p.dh, p.ed * E, p.et * E, p.eb * E}, once, second, col,
-                t0, 0, have, tt, tn);
-      // step 0 has no h before it
-      load_rows(a, p.D, E, View{(const char*)p.h - p.ht * E, p.hd * E, p.ht * E, p.hb * E}, once,
-                before, col, t0, t0 == 0, have, tt, tn);
-      if constexpr (SIG)
-        load_rows(a, p.D, E, View{(const char*)p.x, p.xd * E, p.xt * E, p.xb * E}, once, xrow, col,
-                  t0, 0, have, tt, tn);
+  const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
+  const int col = (int)(blockIdx.x % (unsigned)((a.columns + WARPS / wt - 1) / (WARPS / wt))) * (WARPS / wt) + team;
+  const int block = (int)(blockIdx.x / (unsigned)((a.columns + WARPS / wt - 1) / (WARPS / wt)));
+  const Place at = place_of<T, V, BWD>(p, a, col, block * wt + tw);
+  Map<T, V> m = Map<T, V>::identity();
+  // the last chunk's map is not needed
+  if (at.live && at.order < a.chunks - 1) {
+    const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
+    const T* x = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed : (const T*)p.x + at.b * p.xb + at.d * p.xd;
+    const int64_t gs = BWD ? -p.gt : p.gt, xs = BWD ? -p.et : p.xt;
+    int64_t n = at.end - at.t0;
+    const int64_t first = BWD ? at.end - 1 : at.t0;
+    g += first * p.gt;
+    x += first * (BWD ? p.et : p.xt);
+    for (; n >= U; n -= U) {
+      typename L::R rg[U], rx[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) rg[u] = fetch<T, V>(g + u * gs), rx[u] = fetch<T, V>(x + u * xs);
+#pragma unroll
+      for (int u = 0; u < U; ++u) compose<T, V, SIG, BWD>(m, L::of(rg[u]), L::of(rx[u]));
+      g += U * gs;
+      x += U * xs;
+    }
+    for (; n > 0; --n, g += gs, x += xs)
+      compose<T, V, SIG, BWD>(m, L::of(fetch<T, V>(g)), L::of(fetch<T, V>(x)));
+    m.put((Pair<S>*)a.maps + (int64_t)at.order * a.pitch + at.c0);
+    const S* from = (const S*)(BWD ? p.dh_last : p.h0);
+    if (at.order == 0) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) ((S*)a.start)[at.c0 + i] = from ? from[at.c0 + i] : S(0);
     }
   }
-  asm volatile("cp.async.commit_group;" ::: "memory");
-
-  // this lane's channels and where their sequences end in the tile
-  const int64_t c0 = ((int64_t)col * 32 + lane) * N;
-  int end[N];
-  bool full = true;  // every step of this warp's rows exists in every lane
-  const int r0 = min(tw * a.steps, a.rows), r1 = min(r0 + a.steps, a.rows);
-#pragma unroll
-  for (int v = 0; v < N; ++v) {
-    end[v] = 0;
-    if (live && c0 + v < a.channels) {
-      end[v] = have;
-      if (p.lengths) {
-        const int64_t n = p.lengths[a.narrow ? (int64_t)((uint32_t)(c0 + v) / (uint32_t)p.D) : (c0 + v) / p.D];
-        end[v] = (int)max((int64_t)0, min(n - t0, (int64_t)have));
-      }
-    }
-    full = full && end[v] >= r1;
-  }
-  full = __all_sync(0xffffffffu, full);
-
-  // The state that enters the tile; the first group starts from the caller's.
-  // It is read before this tile's map is published: the last tile, which may
-  // overwrite it (h_last == h0), comes after every map of its group.
-  const S* from = (const S*)(BWD ? p.dh_last : p.h0);
-  K s[NP];
-  S start = 0;
-  if (!a.ticket) {
-#pragma unroll
-    for (int v = 0; v < N; ++v)
-      s[v / W].set(v % W, from && live && c0 + v < a.channels ? from[c0 + v] : S(0));
-  } else if (order < GROUP && from && threadIdx.x < C) {
-    const int64_t c = (int64_t)col * C + threadIdx.x;
-    if (c < a.channels) start = from[c];
-  }
-
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  if (wt < WARPS) return;  // a block has no more chunks than the sequence
+  m.put(&part[warp][lane * V]);
   __syncthreads();
-
-  if (wt > 1) {  // (all the warps of the block, where tiles look back)
-    // the map of this warp's steps
-    K P[NP], Q[NP];
+  for (int c = threadIdx.x; c < 32 * V; c += WARPS * 32) {
+    S P = 1, Q = 0;
 #pragma unroll
-    for (int v = 0; v < NP; ++v) P[v] = fill(S(1)), Q[v] = fill(S(0));
-    auto compose = [&](int r, bool masked) {
-      const L g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
-#pragma unroll
-      for (int v = 0; v < NP; ++v) {
-        K f = g.v[v], b = x.v[v];
-        if constexpr (SIG) {
-          K keep;
-          sigmoid_pair(f, &f, &keep);
-          if constexpr (!BWD) b = b * keep;
-        }
-        const K q = BWD ? f * (b + Q[v]) : mad(f, Q[v], b), pp = f * P[v];
-        if (masked) {
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (r < end[v * W + w]) {
-              Q[v].set(w, q.get(w));
-              P[v].set(w, pp.get(w));
-            }
-        } else {
-          Q[v] = q;
-          P[v] = pp;
-        }
-      }
-    };
-    if (full) {
-#pragma unroll 4
-      for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, false);
-    } else {
-      for (int i = 0; i < r1 - r0; ++i) compose(BWD ? r1 - 1 - i : r0 + i, true);
+    for (int w = 0; w < WARPS; ++w) {
+      const Pair<S> k = part[w][c];
+      Q = k.p * Q + k.q;
+      P = k.p * P;
     }
-#pragma unroll
-    for (int v = 0; v < NP; ++v) {
-      *reinterpret_cast<K*>(&part_p[warp][lane * N + v * W]) = P[v];
-      *reinterpret_cast<K*>(&part_q[warp][lane * N + v * W]) = Q[v];
-    }
-    __syncthreads();
-    // From here a thread has one channel. Those of the first slice replace each
-    // warp's map by that of the steps before it (which run forward from the
-    // first warp, backward from the last) and keep the whole tile's.
-    const int ch = threadIdx.x % C, slice = threadIdx.x / C;
-    S TP = 1, TQ = 0;
-    if (slice < WARPS / wt) {
-      for (int i = 0; i < wt; ++i) {
-        const int w = slice * wt + (BWD ? wt - 1 - i : i);
-        const S mp = part_p[w][ch], mq = part_q[w][ch];
-        part_p[w][ch] = TP;
-        part_q[w][ch] = TQ;
-        TQ = mp * TQ + mq;
-        TP = mp * TP;
-      }
-    }
-    if (a.ticket) {
-      Pair<S>* maps = (Pair<S>*)a.maps + (int64_t)col * C + ch;
-      const int group = order / GROUP, in_group = order % GROUP;
-      const int64_t pitch = (int64_t)a.columns * C;
-      if (slice == 0 && in_group < GROUP - 1 && order < a.tiles - 1) {
-        maps[(int64_t)order * pitch] = Pair<S>{TP, TQ};
-        __threadfence();
-        // one mark per warp that wrote a part of the map
-        __syncwarp();
-        if (lane == 0)
-          asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(
-                           a.flags + (int64_t)order * a.columns + col)
-                       : "memory");
-      }
-      // predecessors in the group, shared out over the slices
-      const int i0 = slice * (GROUP / SLICES), i1 = min(i0 + GROUP / SLICES, in_group);
-      S LP = 1, LQ = 0;
-      if (i0 < i1) {
-        if (lane < i1 - i0) {
-          const uint32_t* f = a.flags + (int64_t)(group * GROUP + i0 + lane) * a.columns + col;
-          poll(a.err, [&] { return load_flag(f) == C / 32; });
-        }
-        __syncwarp();
-        const Pair<S>* m = maps + (int64_t)(group * GROUP) * pitch;
-#pragma unroll 8
-        for (int i = i0; i < i1; ++i) {
-          const Pair<S> w = load_pair(m + i * pitch);
-          LQ = w.p * LQ + w.q;
-          LP = w.p * LP;
-        }
-      }
-      back[slice][ch] = Pair<S>{LP, LQ};
-      __syncthreads();
-      if (slice == 0) {
-        constexpr int NW = sizeof(S) / 4;
-        const int64_t c = (int64_t)col * C + ch;
-        uint64_t* w = a.state + ((int64_t)group * pitch + c) * NW;
-        S in = group > 0 ? read_state<S>(w - pitch * NW, a.err) : start;
-#pragma unroll
-        for (int i = 0; i < SLICES; ++i) in = back[i][ch].p * in + back[i][ch].q;
-        if (in_group == GROUP - 1 && order < a.tiles - 1) write_state<S>(w, TP * in + TQ);
-        back[0][ch].p = in;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int v = 0; v < N; ++v) s[v / W].set(v % W, back[0][lane * N + v].p);
-    } else {
-      __syncthreads();
-    }
-#pragma unroll
-    for (int v = 0; v < NP; ++v)
-      s[v] = mad(*reinterpret_cast<const K*>(&part_p[warp][lane * N + v * W]), s[v],
-                 *reinterpret_cast<const K*>(&part_q[warp][lane * N + v * W]));
+    ((Pair<S>*)a.joined)[(int64_t)block * a.pitch + (int64_t)col * 32 * V + c] = Pair<S>{P, Q};
   }
-  if (!live) return;
+}
 
-  // the steps themselves; results take the place of what they came from
-  auto step = [&](int r, bool masked) {
-    const L g = lane_load<T>(gate + r * ROW, lane), x = lane_load<T>(second + r * ROW, lane);
-    auto settle = [&](int v, K next, K& out) {  // behind the end: the state stays, results are 0
-      if (!masked) {
-        s[v] = next;
-        return;
-      }
+// ---- the steps ------------------------------------------------------------------------
+
+template <typename T, int V, bool SIG, bool BWD>
+__global__ void __launch_bounds__(WARPS * 32, 4) step_kernel(const __grid_constant__ ScanArgs p,
+                                                             const __grid_constant__ ChunkArgs a) {
+  using S = typename Elem<T>::State;
+  using L = Lane<T, V>;
+  using K = typename L::K;
+  using R = typename L::R;
+  __shared__ Pair<S> part[WARPS][32 * V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
+  const unsigned per = (unsigned)((a.columns + WARPS / wt - 1) / (WARPS / wt));
+  const int blocks = (a.chunks + wt - 1) / wt;
+  const int col = (int)(blockIdx.x % per) * (WARPS / wt) + team;
+  const int block = blocks - 1 - (int)(blockIdx.x / per);  // the last chunks first
+  const Place at = place_of<T, V, BWD>(p, a, col, block * wt + tw);
+
+  // the state that enters: the caller's, through the maps of the blocks of
+  // chunks before this one (shared out over the warps) and of the chunks
+  // before this warp's
+  const S* from = (const S*)(a.chunks > 1 ? a.start : BWD ? p.dh_last : p.h0);
+  L s;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        if (r < end[v * W + w]) s[v].set(w, next.get(w));
-        else out.set(w, S(0));
-      }
-    };
-    if constexpr (!BWD) {
-      L out;
-#pragma unroll
-      for (int v = 0; v < NP; ++v) {
-        K f = g.v[v], b = x.v[v];
-        if constexpr (SIG) {
-          K keep;
-          sigmoid_pair(f, &f, &keep);
-          b = b * keep;
-        }
-        out.v[v] = mad(f, s[v], b);
-        settle(v, out.v[v], out.v[v]);
-      }
-      lane_store<T>(second + r * ROW, lane, out);
-    } else {
-      L was = lane_load<T>(before + r * ROW, lane), xv{}, dg, dx;
-      if constexpr (SIG) xv = lane_load<T>(xrow + r * ROW, lane);
-      if (t0 + r == 0) {
-#pragma unroll
-        for (int v = 0; v < N; ++v)
-          was.v[v / W].set(v % W, p.h0 && c0 + v < a.channels ? ((const S*)p.h0)[c0 + v] : S(0));
-      }
-#pragma unroll
-      for (int v = 0; v < NP; ++v) {
-        K f = g.v[v];
-        const K total = x.v[v] + s[v];
-        if constexpr (SIG) {
-          K keep;
-          sigmoid_pair(f, &f, &keep);
-          dx.v[v] = total * keep;
-          dg.v[v] = mad(xv.v[v], fill(S(-1)), was.v[v]) * f * dx.v[v];
-        } else {
-          dx.v[v] = total;
-          dg.v[v] = total * was.v[v];
-        }
-        const K next = f * total;
-        settle(v, next, dx.v[v]);
-        if (masked) {
-#pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (r >= end[v * W + w]) dg.v[v].set(w, S(0));
-        }
-      }
-      lane_store<T>(gate + r * ROW, lane, dg);
-      lane_store<T>(second + r * ROW, lane, dx);
-    }
-  };
-  if (full) {
+  for (int i = 0; i < V; ++i) s.set(i, from && at.live ? from[at.c0 + i] : S(0));
+  if (a.chunks > 1) {
+    if (wt == WARPS && block > 0) {
+      Map<T, V> m = Map<T, V>::identity();
+      const Pair<S>* j = (const Pair<S>*)a.joined + ((int64_t)col * 32 + lane) * V;
+      const int k1 = (int)((int64_t)block * (warp + 1) / WARPS);
 #pragma unroll 4
-    for (int i = 0; i < r1 - r0; ++i) step(BWD ? r1 - 1 - i : r0 + i, false);
+      for (int k = (int)((int64_t)block * warp / WARPS); k < k1; ++k)
+        m.then(Map<T, V>::take(j + k * a.pitch));
+      m.put(&part[warp][lane * V]);
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) s = Map<T, V>::take(&part[w][lane * V]).at(s);
+    }
+    if (at.live) {
+      const Pair<S>* m = (const Pair<S>*)a.maps + at.c0;
+#pragma unroll 4
+      for (int k = block * wt; k < at.order; ++k) s = Map<T, V>::take(m + k * a.pitch).at(s);
+    }
+  }
+  if (!at.live) return;
+
+  const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
+  if constexpr (!BWD) {
+    constexpr int U = 8;
+    const T* x = (const T*)p.x + at.b * p.xb + at.d * p.xd;
+    T* h = (T*)p.h + at.b * p.hb + at.d * p.hd;
+    auto step = [&](R rg, R rx, T* to) {
+      const L f = L::of(rg), b = L::of(rx);
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) {
+        K fi = f.v[i], bi = b.v[i];
+        if constexpr (SIG) {
+          K rest;
+          sigmoid_pair(fi, &fi, &rest);
+          bi = bi * rest;
+        }
+        s.v[i] = mad(fi, s.v[i], bi);
+      }
+      keep<T, V>(to, s);
+    };
+    int64_t t = at.t0;
+    g += t * p.gt, x += t * p.xt, h += t * p.ht;
+    for (; t + U <= at.end; t += U) {
+      R rg[U], rx[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) rg[u] = fetch<T, V>(g + u * p.gt), rx[u] = fetch<T, V>(x + u * p.xt);
+#pragma unroll
+      for (int u = 0; u < U; ++u) step(rg[u], rx[u], h + u * p.ht);
+      g += U * p.gt, x += U * p.xt, h += U * p.ht;
+    }
+    for (; t < at.end; ++t, g += p.gt, x += p.xt, h += p.ht) step(fetch<T, V>(g), fetch<T, V>(x), h);
+    if (t < at.t1) {
+      L zero;
+#pragma unroll
+      for (int i = 0; i < V; ++i) zero.set(i, S(0));
+      for (; t < at.t1; ++t, h += p.ht) keep<T, V>(h, zero);
+    }
   } else {
-    for (int i = 0; i < r1 - r0; ++i) step(BWD ? r1 - 1 - i : r0 + i, true);
-  }
-  __syncwarp();
-  if (r0 < r1) {
-    const int stop = min(r1, have);
-    if constexpr (!BWD) {
-      store_rows_of(a, p.D, E, View{(const char*)p.h, p.hd * E, p.ht * E, p.hb * E}, once, second,
-                    col, t0, r0, stop, lane);
-    } else {
-      store_rows_of(a, p.D, E, View{(const char*)p.dgate, p.pd * E, p.pt * E, p.pb * E}, once, gate,
-                    col, t0, r0, stop, lane);
-      store_rows_of(a, p.D, E, View{(const char*)p.dx, p.qd * E, p.qt * E, p.qb * E}, once, second,
-                    col, t0, r0, stop, lane);
+    constexpr int U = 4;
+    const T* e = (const T*)p.dh + at.b * p.eb + at.d * p.ed;
+    const T* h = (const T*)p.h + at.b * p.hb + at.d * p.hd;
+    const T* x = SIG ? (const T*)p.x + at.b * p.xb + at.d * p.xd : nullptr;
+    T* dg = (T*)p.dgate + at.b * p.pb + at.d * p.pd;
+    T* dx = (T*)p.dx + at.b * p.qb + at.d * p.qd;
+    auto step = [&](R rg, R re, L before, R rx, T* to_g, T* to_x) {
+      const L f = L::of(rg), d = L::of(re), v = L::of(rx);
+      L og, ox;
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) {
+        K fi = f.v[i];
+        const K total = d.v[i] + s.v[i];
+        if constexpr (SIG) {
+          K rest;
+          sigmoid_pair(fi, &fi, &rest);
+          ox.v[i] = total * rest;
+          og.v[i] = mad(v.v[i], K::all(S(-1)), before.v[i]) * fi * ox.v[i];
+        } else {
+          ox.v[i] = total;
+          og.v[i] = total * before.v[i];
+        }
+        s.v[i] = fi * total;
+      }
+      keep<T, V>(to_g, og);
+      keep<T, V>(to_x, ox);
+    };
+    int64_t t = at.t1 - 1;
+    if (t >= at.end) {
+      L zero;
+#pragma unroll
+      for (int i = 0; i < V; ++i) zero.set(i, S(0));
+      for (; t >= at.end; --t) keep<T, V>(dg + t * p.pt, zero), keep<T, V>(dx + t * p.qt, zero);
+    }
+    g += t * p.gt, e += t * p.et, h += (t - 1) * p.ht, dg += t * p.pt, dx += t * p.qt;
+    if constexpr (SIG) x += t * p.xt;
+    for (; t - U >= at.t0; t -= U) {  // (step 0, which has no h before it, is left to the loop below)
+      R rg[U], re[U], rh[U], rx[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        rg[u] = fetch<T, V>(g - u * p.gt), re[u] = fetch<T, V>(e - u * p.et);
+        rh[u] = fetch<T, V>(h - u * p.ht);
+        rx[u] = SIG ? fetch<T, V>(x - u * p.xt) : rg[u];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) step(rg[u], re[u], L::of(rh[u]), rx[u], dg - u * p.pt, dx - u * p.qt);
+      g -= U * p.gt, e -= U * p.et, h -= U * p.ht, dg -= U * p.pt, dx -= U * p.qt;
+      if constexpr (SIG) x -= U * p.xt;
+    }
+    for (; t >= at.t0; --t) {
+      L before;
+      if (t > 0) {
+        before = L::of(fetch<T, V>(h));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) before.set(i, p.h0 ? ((const S*)p.h0)[at.c0 + i] : S(0));
+      }
+      const R rg = fetch<T, V>(g);
+      step(rg, fetch<T, V>(e), before, SIG ? fetch<T, V>(x) : rg, dg, dx);
+      g -= p.gt, e -= p.et, h -= p.ht, dg -= p.pt, dx -= p.qt;
+      if constexpr (SIG) x -= p.xt;
     }
   }
-  // the state that leaves the last tile
+  // the state that leaves the last chunk
   S* last = (S*)(BWD ? p.dh0 : p.h_last);
-  if (last && order == a.tiles - 1 && tw == (BWD ? 0 : wt - 1)) {
+  if (last && at.order == a.chunks - 1) {
 #pragma unroll
-    for (int v = 0; v < N; ++v)
-      if (c0 + v < a.channels) last[c0 + v] = s[v / W].get(v % W);
+    for (int i = 0; i < V; ++i) last[at.c0 + i] = s.get(i);
   }
 }
 
 // ---- host side ---------------------------------------------------------------------
 
-// The bytes that one copy may move: the widest of 16, 8, 4 (2 for 16-bit
-// types) that divides the rows and every address and stride
-int grain_of(const ScanArgs& p, int elem, bool backward, bool need_x) {
+// Whether every row can be read and written `bytes` at a time
+bool aligned(const ScanArgs& p, int elem, int bytes, bool backward, bool need_x) {
   struct A {
     const void* ptr;
     int64_t d, t, b;
@@ -687,61 +553,58 @@ int grain_of(const ScanArgs& p, int elem, bool backward, bool need_x) {
     arrays[n++] = {p.dgate, p.pd, p.pt, p.pb};
     arrays[n++] = {p.dx, p.qd, p.qt, p.qb};
   }
-  for (int g = 16; g > elem; g /= 2) {
-    bool fits = p.D * elem % g == 0;
-    for (int i = 0; i < n && fits; ++i)
-      fits = (arrays[i].d == 1 || p.D == 1) && (uintptr_t)arrays[i].ptr % g == 0 &&
-             arrays[i].t * elem % g == 0 && arrays[i].b * elem % g == 0;
-    if (fits) return g;
+  if (p.D * elem % bytes) return false;
+  for (int i = 0; i < n; ++i)
+    if (arrays[i].d != 1 || (uintptr_t)arrays[i].ptr % bytes || arrays[i].t * elem % bytes ||
+        arrays[i].b * elem % bytes)
+      return false;
+  return true;
+}
+
+template <typename T, int V, bool SIG, bool BWD>
+int launch_chunks(om_backend* be, const ScanArgs& p) {
+  using S = typename Elem<T>::State;
+  ChunkArgs a{};
+  a.groups = p.B * (p.D / V);
+  const int64_t columns = (a.groups + 31) / 32;
+  a.pitch = columns * 32 * V;
+  a.narrow = a.groups * V < ((int64_t)1 << 32) && p.D < ((int64_t)1 << 32);
+  // Enough chunks for twice the warps that the card holds, of 32 steps at least
+  const int64_t want = ((int64_t)be->num_sms * 64 + columns - 1) / columns;
+  int64_t chunks = std::max<int64_t>(1, std::min(want, p.T / 32));
+  a.steps = std::max<int64_t>(1, (p.T + chunks - 1) / chunks);
+  a.steps = chunks > 1 ? (a.steps + 7) / 8 * 8 : a.steps;
+  chunks = std::max<int64_t>(1, (p.T + a.steps - 1) / a.steps);
+  a.warps_t = 1;
+  while (a.warps_t < WARPS && a.warps_t < chunks) a.warps_t *= 2;
+  const int64_t per = (columns + WARPS / a.warps_t - 1) / (WARPS / a.warps_t);
+  const int64_t rows = (chunks + a.warps_t - 1) / a.warps_t, blocks = per * rows;
+  if (blocks > 0x7fffffff || columns > 0x7fffff00)
+    return set_error(OM_ERR_SHAPE, "gated_scan: too many channels and steps");
+  a.columns = (int)columns;
+  a.chunks = (int)chunks;
+  Scratch ws;
+  if (chunks > 1) {
+    OM_TRY(ws.alloc(be, (size_t)(chunks + rows + 1) * a.pitch * sizeof(Pair<S>)));
+    a.maps = ws.ptr;
+    a.joined = (Pair<S>*)a.maps + chunks * a.pitch;
+    a.start = (Pair<S>*)a.joined + rows * a.pitch;
+    ProfScope prof(be, BWD ? "gated_scan_maps_backward" : "gated_scan_maps");
+    map_kernel<T, V, SIG, BWD><<<(unsigned)blocks, WARPS * 32, 0, be->stream>>>(p, a);
+    note_launch();
   }
-  return elem;
+  ProfScope prof(be, BWD ? "gated_scan_backward" : "gated_scan");
+  step_kernel<T, V, SIG, BWD><<<(unsigned)blocks, WARPS * 32, 0, be->stream>>>(p, a);
+  note_launch();
+  return check_cuda(cudaGetLastError(), "gated_scan launch");
 }
 
 template <typename T, bool SIG, bool BWD>
 int launch_scan(om_backend* be, const ScanArgs& p) {
-  using S = typename Elem<T>::State;
-  constexpr int ARRAYS = BWD ? (SIG ? 4 : 3) : 2;
-  TileArgs a{};
-  a.channels = p.D * p.B;
-  a.grain = grain_of(p, sizeof(T), BWD, SIG || !BWD);
-  const int64_t columns = (a.channels * (int64_t)sizeof(T) + ROW - 1) / ROW;
-  a.narrow = a.channels < ((int64_t)1 << 32) && p.D < ((int64_t)1 << 32);
-  // Up to 16 steps are one warp's work and eight columns share a block; longer
-  // sequences take all eight warps, the backward pass with half the steps
-  // each: its three or four arrays then leave three blocks on an SM.
-  a.warps_t = p.T > MAX_STEPS ? WARPS : 1;
-  a.steps = a.warps_t > 1 && BWD ? MAX_STEPS / 2 : MAX_STEPS;
-  a.rows = (int)std::min<int64_t>(p.T, a.steps * a.warps_t);
-  const int64_t tiles = p.T == 0 ? 1 : (p.T + a.rows - 1) / a.rows;
-  const int64_t blocks = tiles > 1 ? tiles * columns : (columns + WARPS / a.warps_t - 1) / (WARPS / a.warps_t);
-  if (blocks > 0x7fffffff || columns > 0x7ffffff0)
-    return set_error(OM_ERR_SHAPE, "gated_scan: too many channels and steps");
-  a.columns = (int)columns;
-  a.tiles = (int)tiles;
-  a.err = be->d_flags + 1;
-  Scratch ws;
-  if (tiles > 1) {
-    const int64_t groups = (tiles + GROUP - 1) / GROUP;
-    const size_t pitch = (size_t)columns * (ROW / sizeof(T));
-    const size_t state = (size_t)groups * pitch * (sizeof(S) / 4) * 8;
-    const size_t flags = ((size_t)blocks * 4 + 15) / 16 * 16;
-    OM_TRY(ws.alloc(be, 16 + flags + state + (size_t)tiles * pitch * sizeof(Pair<S>)));
-    char* at = (char*)ws.ptr;
-    OM_CUDA(cudaMemsetAsync(at, 0, 16 + flags + state, be->stream), "gated_scan marks");
-    a.ticket = (uint32_t*)at;
-    a.flags = (uint32_t*)(at + 16);
-    a.state = (uint64_t*)(at + 16 + flags);
-    a.maps = at + 16 + flags + state;
-  }
-  const size_t smem = (size_t)(WARPS / a.warps_t) * ARRAYS * a.rows * ROW;
-  auto kernel = scan_kernel<T, SIG, BWD>;
-  if (smem > 40 * 1024)
-    OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-            "gated_scan");
-  ProfScope prof(be, BWD ? "gated_scan_backward" : "gated_scan");
-  kernel<<<(unsigned)blocks, WARPS * 32, smem, be->stream>>>(p, a);
-  note_launch();
-  return check_cuda(cudaGetLastError(), "gated_scan launch");
+  constexpr int V = 8 / sizeof(T);
+  if constexpr (V > 1)
+    if (aligned(p, sizeof(T), 8, BWD, SIG || !BWD)) return launch_chunks<T, V, SIG, BWD>(be, p);
+  return launch_chunks<T, 1, SIG, BWD>(be, p);
 }
 
 template <typename T>

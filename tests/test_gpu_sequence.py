@@ -189,6 +189,16 @@ def test_scan_step_by_step_is_the_scan(be, seq):
     near(state.to_numpy(), last.to_numpy().astype(np.float64), 2 * el)
 
 
+@pytest.mark.parametrize("t", [1, 40, 300, 5000])
+def test_scan_state_in_place(be, seq, t):
+    """h_last may be h0, however the sequence is cut."""
+    gate, x, _, h0, _ = scan_inputs(16, 2, t, 40, "f32", "sigmoid")
+    G, X, state = seq.upload(be, gate, "f32"), seq.upload(be, x, "f32"), seq.upload(be, h0)
+    want, last = seq.gated_scan(be, G, X, h0=seq.upload(be, h0), kind="sigmoid")
+    got, _ = seq.gated_scan(be, G, X, h0=state, kind="sigmoid", h_last=state)
+    assert np.array_equal(got.to_numpy(), want.to_numpy()) and np.array_equal(state.to_numpy(), last.to_numpy())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_scan_repeats_bit_for_bit(be, seq, dtype):
     args = scan_inputs(10, 1, 20000, 64, dtype, "sigmoid")
