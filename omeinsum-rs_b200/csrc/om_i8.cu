@@ -46,6 +46,45 @@ __global__ void quantize_kernel(const T* __restrict__ x, int64_t K, int64_t xk, 
     q[row * qm + k * qk] = s > 0.f ? quantized(Elem<T>::load(xr[k * xk]), s) : (int8_t)0;
 }
 
+// The same where a row is contiguous, 16-byte aligned and short enough for the
+// block's registers: it is read once, 8 elements per thread and turn.
+constexpr int TURNS = 4;
+template <typename T>
+__global__ void __launch_bounds__(256) quantize_vec_kernel(const T* __restrict__ x, int K, int64_t xm,
+                                                           int8_t* __restrict__ q, int64_t qm,
+                                                           float* __restrict__ scale) {
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * xm;
+  __align__(16) T v[TURNS][8];
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
+    if (k >= K) break;
+#pragma unroll
+    for (int b = 0; b < (int)sizeof(T) * 8; b += 16)
+      *reinterpret_cast<uint4*>((char*)v[i] + b) = __ldcs(reinterpret_cast<const uint4*>((const char*)(xr + k) + b));
+  }
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    if ((i * (int)blockDim.x + (int)threadIdx.x) * 8 >= K) break;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) m = max_abs(m, Elem<T>::load(v[i][c]));
+  }
+  m = block_max_abs(m);
+  const float s = __fdiv_rn(m, 127.f);
+  if (threadIdx.x == 0) scale[row] = s;
+#pragma unroll
+  for (int i = 0; i < TURNS; ++i) {
+    const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
+    if (k >= K) break;
+    __align__(8) int8_t o[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) o[c] = s > 0.f ? quantized(Elem<T>::load(v[i][c]), s) : (int8_t)0;
+    *reinterpret_cast<uint2*>(q + row * qm + k) = *reinterpret_cast<const uint2*>(o);
+  }
+}
+
 struct I8Args {
   int64_t M, N, K;
   const int8_t* q;
@@ -200,6 +239,13 @@ template <typename T>
 int launch_quantize(om_backend* be, int64_t K, int64_t M, const void* x, const int64_t* sx, void* q,
                     int64_t qk, int64_t qm, float* scale) {
   ProfScope prof(be, "quantize_rows");
+  if (sx[0] == 1 && qk == 1 && K % 8 == 0 && K <= 256 * 8 * TURNS && !((uintptr_t)x & 15) &&
+      sx[1] * (int64_t)sizeof(T) % 16 == 0 && !((uintptr_t)q & 7) && qm % 8 == 0) {
+    const int threads = (int)std::min<int64_t>(256, (K / 8 + 31) / 32 * 32);
+    quantize_vec_kernel<T><<<(unsigned)M, threads, 0, be->stream>>>((const T*)x, (int)K, sx[1], (int8_t*)q, qm, scale);
+    note_launch();
+    return check_cuda(cudaGetLastError(), "quantize_rows launch");
+  }
   quantize_kernel<T><<<(unsigned)M, 256, 0, be->stream>>>((const T*)x, K, sx[0], sx[1], (int8_t*)q,
                                                           qk, qm, scale);
   note_launch();

@@ -331,28 +331,41 @@ struct StatsEpi {
   }
 };
 
-// Joins the slots of 32 rows per block, each thread every eighth slot.
-__global__ void join_stats(const float2* __restrict__ part, int slots, int64_t rows,
-                           const void* targets, int t64, int64_t vocab, const float* hit,
-                           float* loss, float* lse) {
-  __shared__ float sm[8][33], ss[8][33];
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x * (int64_t)32 + tx;
+// Joins the slots of 8 rows per block, each of 32 threads of a row every 32nd
+// slot; a row's threads are a stride of 8 apart, so that a slot's rows are read
+// together. (32 rows by 8 threads left 4096 rows on 128 blocks of 50 dependent
+// loads each: 36 us against 9.)
+__global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ part, int slots,
+                                                  int64_t rows, const void* targets, int t64,
+                                                  int64_t vocab, const float* hit, float* loss,
+                                                  float* lse) {
+  __shared__ float sm[32][9], ss[32][9];
+  const int r = threadIdx.x & 7, k = threadIdx.x >> 3;
+  const int64_t row = blockIdx.x * (int64_t)8 + r;
   float m = -INFINITY, s = 0.f;
-  if (row < rows)
-    for (int i = ty; i < slots; i += 8) {
+  if (row < rows) {
+#pragma unroll 4
+    for (int i = k; i < slots; i += 32) {
       const float2 v = part[(int64_t)i * rows + row];
       merge(m, s, v.x, v.y);
     }
-  sm[ty][tx] = m;
-  ss[ty][tx] = s;
+  }
+  sm[k][r] = m;
+  ss[k][r] = s;
   __syncthreads();
-  if (ty || row >= rows) return;
-  for (int i = 1; i < 8; ++i) merge(m, s, sm[i][tx], ss[i][tx]);
+  // one warp per row now
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t mine = blockIdx.x * (int64_t)8 + w;
+  m = sm[lane][w];
+  s = ss[lane][w];
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+    merge(m, s, __shfl_down_sync(0xffffffffu, m, o), __shfl_down_sync(0xffffffffu, s, o));
+  if (lane || mine >= rows) return;
   const float total = m + logf(s);
-  const int64_t t = target_of(targets, t64, row);
-  lse[row] = total;
-  loss[row] = t >= 0 && t < vocab ? total - hit[row] : 0.f;
+  const int64_t t = target_of(targets, t64, mine);
+  lse[mine] = total;
+  loss[mine] = t >= 0 && t < vocab ? total - hit[mine] : 0.f;
 }
 
 // dz is rounded to 16 bits as dz / scale, scale = max |dloss| of the counted
@@ -493,22 +506,44 @@ __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t a
 }
 
 // Rows of [rows, cols] as T with 16-byte aligned rows; zero where the target
-// lies outside the vocabulary (targets given), and in the padding
+// lies outside the vocabulary (targets given), and in the padding. A thread
+// makes 8 elements; `vec`: they can be read at once.
 template <typename T>
 __global__ void pack_rows(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
-                          int64_t sc, T* __restrict__ dst, int64_t ld, const void* targets, int t64,
-                          int64_t vocab) {
-  const int64_t total = rows * ld;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ld, c = i - r * ld;
-    bool keep = c < cols;
+                          int64_t sc, int vec, T* __restrict__ dst, int64_t ld,
+                          const void* targets, int t64, int64_t vocab) {
+  const int64_t per = ld / 8;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    bool keep = true;
     if (targets) {
       const int64_t t = target_of(targets, t64, r);
-      keep = keep && t >= 0 && t < vocab;
+      keep = t >= 0 && t < vocab;
     }
-    dst[i] = keep ? src[r * sr + c * sc] : T(0.f);
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < per;
+         i += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t c = i * 8;
+      __align__(16) T v[8];
+      if (vec && keep && c + 8 <= cols) {
+        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + r * sr + c);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          v[k] = keep && c + k < cols ? src[r * sr + (c + k) * sc] : T(0.f);
+      }
+      *reinterpret_cast<uint4*>(dst + r * ld + c) = *reinterpret_cast<const uint4*>(v);
+    }
   }
+}
+template <typename T>
+void launch_pack(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
+                 T* dst, int64_t ld, const void* targets, int t64, int64_t vocab) {
+  const int vec = sc == 1 && sr % 8 == 0 && !((uintptr_t)src & 15);
+  const int threads = (int)std::min<int64_t>(256, (ld / 8 + 31) / 32 * 32);
+  const dim3 grid((unsigned)std::min<int64_t>((ld / 8 + threads - 1) / threads, 65535),
+                  (unsigned)std::min<int64_t>(rows, 65535));
+  ProfScope prof(be, "loss_pack");
+  pack_rows<T><<<grid, threads, 0, be->stream>>>(src, rows, cols, sr, sc, vec, dst, ld, targets, t64, vocab);
+  note_launch();
 }
 
 // The operand itself when TMA can read its rows, else a packed copy.
@@ -519,9 +554,7 @@ int readable(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t s
   if ((sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2)) return OM_OK;
   const int64_t ld = (cols + 7) / 8 * 8;
   OM_TRY(copy.alloc(be, (size_t)rows * ld * 2));
-  pack_rows<T><<<flat_grid(be, rows * ld), 256, 0, be->stream>>>(src, rows, cols, sr, sc,
-                                                                 (T*)copy.ptr, ld, nullptr, 0, 0);
-  note_launch();
+  launch_pack<T>(be, src, rows, cols, sr, sc, (T*)copy.ptr, ld, nullptr, 0, 0);
   *out = mma::Matrix{copy.ptr, rows, cols, ld, 2};
   return check_cuda(cudaGetLastError(), "loss pack launch");
 }
@@ -548,7 +581,7 @@ int loss_forward16(om_backend* be, const LossArgs& p, float* loss, float* lse) {
   const StatsEpi epi{p.targets, p.target64, part, p.N, hit};
   OM_TRY((product16<false, false>(be, "loss_logits", x, w, bf16, t, 1, epi)));
   ProfScope prof(be, "loss_join_stats");
-  join_stats<<<(unsigned)((p.N + 31) / 32), 256, 0, be->stream>>>(
+  join_stats<<<(unsigned)((p.N + 7) / 8), 256, 0, be->stream>>>(
       part, (int)slots, p.N, p.targets, p.target64, p.V, hit, loss, lse);
   note_launch();
   return check_cuda(cudaGetLastError(), "loss join launch");
@@ -572,9 +605,7 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
   OM_TRY(dzs.alloc(be, (size_t)p.N * P * 2));
   T* dz = (T*)dzs.ptr;
   // rows without a loss are zero here: whatever they hold reaches no gradient
-  pack_rows<T><<<flat_grid(be, p.N * Dp), 256, 0, be->stream>>>(
-      (const T*)p.x, p.N, p.D, p.xn, p.xd, (T*)xs.ptr, Dp, p.targets, p.target64, p.V);
-  note_launch();
+  launch_pack<T>(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, (T*)xs.ptr, Dp, p.targets, p.target64, p.V);
   mma::Matrix w;
   OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
   OM_TRY(scales.alloc(be, 4));
