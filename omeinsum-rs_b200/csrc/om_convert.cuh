@@ -45,19 +45,39 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// 32 values of a row as T, 16 bytes at a time
-template <typename T>
-__device__ __forceinline__ void store_row(T* dst, const float (&v)[32]) {
-#pragma unroll
-  for (int c = 0; c < 32; c += 8)
-    *reinterpret_cast<uint4*>(dst + c) =
-        make_uint4(pack2(v[c], v[c + 1], T()), pack2(v[c + 2], v[c + 3], T()),
-                   pack2(v[c + 4], v[c + 5], T()), pack2(v[c + 6], v[c + 7], T()));
+// 32 values of a row as T. `wide`: dst is 32-byte aligned, and each store fills
+// a sector of L2; else 16 bytes at a time.
+__device__ __forceinline__ void store_sector(void* dst, const uint32_t (&u)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(u[0]),
+               "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
 }
-__device__ __forceinline__ void store_row(float* dst, const float (&v)[32]) {
+__device__ __forceinline__ void store_sixteens(void* dst, const uint32_t (&u)[8]) {
+  uint4* d = reinterpret_cast<uint4*>(dst);
+  d[0] = make_uint4(u[0], u[1], u[2], u[3]);
+  d[1] = make_uint4(u[4], u[5], u[6], u[7]);
+}
+template <typename T>
+__device__ __forceinline__ void store_row(T* dst, const float (&v)[32], bool wide) {
+  constexpr int PER = 32 / sizeof(T);  // values of a sector
 #pragma unroll
-  for (int c = 0; c < 32; c += 4)
-    *reinterpret_cast<float4*>(dst + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+  for (int c = 0; c < 32; c += PER) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 4) u[i] = __float_as_uint(v[c + i]);
+      else u[i] = pack2(v[c + 2 * i], v[c + 2 * i + 1], T());
+    }
+    if (wide) store_sector(dst + c, u);
+    else store_sixteens(dst + c, u);
+  }
+}
+
+// How a row-major result may be written: 2 = sectors of 32 bytes, 1 = 16 bytes,
+// 0 = element by element
+inline int row_stores(const void* ptr, int64_t row, int64_t col, int elem) {
+  const uint64_t at = (uint64_t)(uintptr_t)ptr | (uint64_t)(row * elem);
+  return col != 1 || at % 16 ? 0 : at % 32 ? 1 : 2;
 }
 
 inline bool is_half(om_dtype dt) { return dt == OM_BF16 || dt == OM_F16; }

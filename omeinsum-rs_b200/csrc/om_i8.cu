@@ -21,6 +21,57 @@ __device__ __forceinline__ int8_t quantized(float x, float scale) {
   return r != r ? (int8_t)0 : (int8_t)fminf(fmaxf(r, -127.f), 127.f);
 }
 
+// Four values at once, as bytes. x * (1 / s) is off the quotient by less than
+// 3e-5 where |x / s| <= 127, so the nearest whole number is the quotient's
+// unless the product lies within 1e-4 of the middle of two; only then is the
+// division made. Adding 1.5 * 2^23 rounds to a whole number, ties to even, and
+// leaves it in the low byte. (Dividing every element took 71 us for
+// 8192 x 4096 bf16.) `s` is a normal number here.
+__device__ __forceinline__ uint32_t quantized4(const float (&x)[4], float s, float inv) {
+  constexpr float MAGIC = 12582912.f;
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = __fmaf_rn(x[i], inv, MAGIC);
+    const float off = __fmaf_rn(x[i], inv, -__fsub_rn(t, MAGIC));
+    b[i] = __float_as_uint(t);
+    if (fabsf(off) > 0.4999f) b[i] = (uint32_t)(int)quantized(x[i], s);
+  }
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+}
+
+// 8 elements, 16-byte aligned, as f32
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+  __align__(16) T t[8];
+#pragma unroll
+  for (int b = 0; b < (int)sizeof(T) * 8; b += 16)
+    *reinterpret_cast<uint4*>((char*)t + b) = __ldg(reinterpret_cast<const uint4*>((const char*)p + b));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(t[i]);
+}
+
+// the largest magnitude; magnitudes order like their bits, NaN above all
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, const float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+
+// 8 elements quantised; whatever is not a normal scale takes the long way
+__device__ __forceinline__ uint2 quantized8(const float (&v)[8], float s, float inv, bool normal) {
+  if (normal) {
+    const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+    return make_uint2(quantized4(lo, s, inv), quantized4(hi, s, inv));
+  }
+  uint32_t u[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (s > 0.f) u[i / 4] |= (uint32_t)(uint8_t)quantized(v[i], s) << (8 * (i % 4));
+  return make_uint2(u[0], u[1]);
+}
+__device__ __forceinline__ bool normal_scale(float s) { return s > 1e-36f && s < 1e36f; }
+
 __device__ __forceinline__ float block_max_abs(float m) {
   __shared__ float part[32];
   for (int o = 16; o; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -55,33 +106,32 @@ __global__ void __launch_bounds__(256) quantize_vec_kernel(const T* __restrict__
                                                            float* __restrict__ scale) {
   const int64_t row = blockIdx.x;
   const T* xr = x + row * xm;
-  __align__(16) T v[TURNS][8];
-  float m = 0.f;
+  float v[TURNS][8];
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
     if (k >= K) break;
-#pragma unroll
-    for (int b = 0; b < (int)sizeof(T) * 8; b += 16)
-      *reinterpret_cast<uint4*>((char*)v[i] + b) = __ldcs(reinterpret_cast<const uint4*>((const char*)(xr + k) + b));
+    load8(xr + k, v[i]);
   }
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     if ((i * (int)blockDim.x + (int)threadIdx.x) * 8 >= K) break;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) m = max_abs(m, Elem<T>::load(v[i][c]));
+    top = max_bits(top, v[i]);
   }
-  m = block_max_abs(m);
-  const float s = __fdiv_rn(m, 127.f);
+  __shared__ uint32_t part[8];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+  __syncthreads();
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) top = max(top, part[i]);
+  const float s = __fdiv_rn(__uint_as_float(top), 127.f), inv = __fdiv_rn(1.f, s);
+  const bool normal = normal_scale(s);
   if (threadIdx.x == 0) scale[row] = s;
 #pragma unroll
   for (int i = 0; i < TURNS; ++i) {
     const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
     if (k >= K) break;
-    __align__(8) int8_t o[8];
-#pragma unroll
-    for (int c = 0; c < 8; ++c) o[c] = s > 0.f ? quantized(Elem<T>::load(v[i][c]), s) : (int8_t)0;
-    *reinterpret_cast<uint2*>(q + row * qm + k) = *reinterpret_cast<const uint2*>(o);
+    *reinterpret_cast<uint2*>(q + row * qm + k) = quantized8(v[i], s, inv, normal);
   }
 }
 
@@ -107,7 +157,7 @@ struct ScaleEpi {
   const float *q_scale, *w_scale, *bias;
   T* y;
   int64_t dr, dc;
-  int vec;  // rows of y may be written, and w_scale and bias read, 16 bytes at a time
+  int vec;  // row_stores of y, where w_scale and bias can be read 16 bytes at a time
   struct Row {
     float s;
   };
@@ -133,7 +183,7 @@ struct ScaleEpi {
           v[c + 2] = __fadd_rn(v[c + 2], b.z), v[c + 3] = __fadd_rn(v[c + 3], b.w);
         }
       }
-      store_row(to + n0, v);
+      store_row(to + n0, v, vec == 2);
     } else {
 #pragma unroll
       for (int c = 0; c < 32; ++c)
@@ -166,51 +216,94 @@ constexpr int TOKEN_SMEM = 160 * 1024;
 // A block keeps the M <= MM rows of q in shared memory and walks its share of
 // the channels, a warp per channel: 16 weights per lane and step, four
 // products per instruction, one shuffle reduction per row. T: the type of y,
-// and of x where the rows are quantised here (q == null).
+// and of x where the rows are quantised here (q == null): 8 / MM warps a row,
+// while the first weights are already under way.
 template <typename T, int MM>
-__global__ void __launch_bounds__(256) token_i8_kernel(I8Args p, const T* __restrict__ x,
-                                                       int64_t xk, int64_t xm, int64_t Kp) {
+__global__ void __launch_bounds__(256, 2) token_i8_kernel(I8Args p, const T* __restrict__ x, int64_t xk,
+                                                       int64_t xm, int vec, int Kp) {
   extern __shared__ __align__(16) int8_t qs[];  // [MM][Kp]
+  constexpr int AHEAD = 4;
+  constexpr int SHARE = 8 / MM;  // warps per row
   __shared__ float scale[MM];
+  __shared__ uint32_t part[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int M = (int)p.M;
-  for (int m = 0; m < M; ++m) {
-    if (p.q) {
-      for (int64_t k = tid; k < Kp; k += 256)
-        qs[m * Kp + k] = k < p.K ? p.q[m * p.qm + k * p.qk] : (int8_t)0;
-      if (tid == 0) scale[m] = p.q_scale[m];
-    } else {
-      const T* xr = x + m * xm;
-      float top = 0.f;
-      for (int64_t k = tid; k < p.K; k += 256) top = max_abs(top, Elem<T>::load(xr[k * xk]));
-      top = block_max_abs(top);
-      const float s = __fdiv_rn(top, 127.f);
-      for (int64_t k = tid; k < Kp; k += 256)
-        qs[m * Kp + k] =
-            k < p.K && s > 0.f ? quantized(Elem<T>::load(xr[k * xk]), s) : (int8_t)0;
-      if (tid == 0) scale[m] = s;
-      __syncthreads();  // block_max_abs's scratch is used again
+  const int M = (int)p.M, K = (int)p.K;
+  const int64_t n0 = p.N * blockIdx.x / gridDim.x, n1 = p.N * (blockIdx.x + 1) / gridDim.x;
+  auto weights = [&](const int8_t* wr, int k) {
+    int4 w = make_int4(0, 0, 0, 0);
+    if (k + 16 <= K) {
+      w = __ldcs(reinterpret_cast<const int4*>(wr + k));
+    } else if (k < K) {  // the row's end: nothing behind it is read
+      __align__(16) int8_t tail[16] = {};
+#pragma unroll
+      for (int i = 0; i < 15; ++i)
+        if (k + i < K) tail[i] = wr[k + i];
+      w = *reinterpret_cast<const int4*>(tail);
+    }
+    return w;
+  };
+  int64_t n = n0 + warp;
+  int4 ahead[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    ahead[i] = n < n1 ? weights(p.w + n * p.wn, lane * 16 + i * 512) : make_int4(0, 0, 0, 0);
+
+  const int row = warp / SHARE, first = (warp % SHARE) * 32 + lane;  // of the row's threads
+  if (p.q) {
+    if (row < M) {
+      for (int k = first; k < Kp; k += SHARE * 32)
+        qs[row * Kp + k] = k < K ? p.q[row * p.qm + k * p.qk] : (int8_t)0;
+      if (first == 0) scale[row] = p.q_scale[row];
+    }
+  } else {
+    const T* xr = x + row * xm;
+    uint32_t top = 0;
+    if (row < M) {
+      if (vec) {
+#pragma unroll 2
+        for (int k = first * 8; k < K; k += SHARE * 256) {
+          float v[8];
+          load8(xr + k, v);
+          top = max_bits(top, v);
+        }
+      } else {
+        for (int k = first; k < K; k += SHARE * 32)
+          top = max(top, __float_as_uint(Elem<T>::load(xr[k * xk])) & 0x7fffffffu);
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) part[warp] = top;
+    __syncthreads();
+    if (row < M) {
+#pragma unroll
+      for (int i = 0; i < SHARE; ++i) top = max(top, part[row * SHARE + i]);
+      const float s = __fdiv_rn(__uint_as_float(top), 127.f), inv = __fdiv_rn(1.f, s);
+      const bool normal = normal_scale(s);
+      if (first == 0) scale[row] = s;
+      if (vec) {
+        for (int k = first * 8; k < Kp; k += SHARE * 256) {
+          uint2 q = make_uint2(0, 0);
+          if (k < K) {
+            float v[8];
+            load8(xr + k, v);
+            q = quantized8(v, s, inv, normal);
+          }
+          *reinterpret_cast<uint2*>(qs + row * Kp + k) = q;
+        }
+      } else {
+        for (int k = first; k < Kp; k += SHARE * 32)
+          qs[row * Kp + k] = k < K && s > 0.f ? quantized(Elem<T>::load(xr[k * xk]), s) : (int8_t)0;
+      }
     }
   }
   __syncthreads();
-  const int64_t n0 = p.N * blockIdx.x / gridDim.x, n1 = p.N * (blockIdx.x + 1) / gridDim.x;
-  for (int64_t n = n0 + warp; n < n1; n += 8) {
+
+  for (; n < n1; n += 8) {
     const int8_t* wr = p.w + n * p.wn;
     int acc[MM];
 #pragma unroll
     for (int m = 0; m < MM; ++m) acc[m] = 0;
-#pragma unroll 4
-    for (int64_t k = lane * 16; k < Kp; k += 512) {
-      int4 w = make_int4(0, 0, 0, 0);
-      if (k + 16 <= p.K) {
-        w = __ldcs(reinterpret_cast<const int4*>(wr + k));
-      } else {  // the row's end: nothing behind it is read
-        __align__(16) int8_t tail[16] = {};
-#pragma unroll
-        for (int i = 0; i < 15; ++i)
-          if (k + i < p.K) tail[i] = wr[k + i];
-        w = *reinterpret_cast<const int4*>(tail);
-      }
+    auto add = [&](const int4& w, int k) {
 #pragma unroll
       for (int m = 0; m < MM; ++m) {
         if (m >= M) break;
@@ -220,12 +313,30 @@ __global__ void __launch_bounds__(256) token_i8_kernel(I8Args p, const T* __rest
         acc[m] = __dp4a(w.z, q.z, acc[m]);
         acc[m] = __dp4a(w.w, q.w, acc[m]);
       }
+    };
+    // the next AHEAD steps' weights are always under way
+    for (int k0 = lane * 16; k0 < Kp; k0 += AHEAD * 512) {
+      int4 now[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) now[i] = ahead[i];
+      int k1 = k0 + AHEAD * 512;
+      const int8_t* next = wr;
+      if (k1 >= Kp) {
+        next = n + 8 < n1 ? wr + 8 * p.wn : nullptr;
+        k1 = lane * 16;
+      }
+      if (next) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) ahead[i] = weights(next, k1 + i * 512);
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (k0 + i * 512 < Kp) add(now[i], k0 + i * 512);
     }
 #pragma unroll
     for (int m = 0; m < MM; ++m) {
       if (m >= M) break;
-      int a = acc[m];
-      for (int o = 16; o; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      const int a = __reduce_add_sync(0xffffffffu, acc[m]);
       if (lane == m) {
         float v = scaled(a, scale[m], p.w_scale[n]);
         if (p.bias) v = __fadd_rn(v, p.bias[n]);
@@ -285,7 +396,8 @@ int launch_token_rows(om_backend* be, const I8Args& p, const T* x, int64_t xk, i
             "matmul_i8");
   const int64_t blocks = std::min<int64_t>((p.N + 7) / 8, (int64_t)be->num_sms * 2);
   ProfScope prof(be, "matmul_i8_token");
-  token_i8_kernel<T, MM><<<(unsigned)blocks, 256, smem, be->stream>>>(p, x, xk, xm, Kp);
+  const int vec = x && xk == 1 && p.K % 8 == 0 && !((uintptr_t)x & 15) && xm * (int64_t)sizeof(T) % 16 == 0;
+  token_i8_kernel<T, MM><<<(unsigned)blocks, 256, smem, be->stream>>>(p, x, xk, xm, vec, (int)Kp);
   note_launch();
   return check_cuda(cudaGetLastError(), "matmul_i8 launch");
 }
@@ -304,6 +416,7 @@ int launch_tokens(om_backend* be, I8Args p, const T* x, int64_t xk, int64_t xm) 
   p.wn = w.ld;
   const int64_t Kp = (p.K + 15) / 16 * 16;
   if (p.M == 1) return launch_token_rows<T, 1>(be, p, x, xk, xm, Kp);
+  if (p.M == 2) return launch_token_rows<T, 2>(be, p, x, xk, xm, Kp);
   if (p.M <= 4) return launch_token_rows<T, 4>(be, p, x, xk, xm, Kp);
   return launch_token_rows<T, 8>(be, p, x, xk, xm, Kp);
 }
@@ -315,8 +428,7 @@ int launch_matmul(om_backend* be, const I8Args& p) {
   mma::Matrix q, w;
   OM_TRY(readable_i8(be, p.q, p.M, p.K, p.qm, p.qk, qc, &q));
   OM_TRY(readable_i8(be, p.w, p.N, p.K, p.wn, p.wk, wc, &w));
-  const int vec = p.yn == 1 && (p.ym * (int64_t)sizeof(T)) % 16 == 0 && !((uintptr_t)p.y & 15) &&
-                  !((uintptr_t)p.w_scale & 15) && !((uintptr_t)p.bias & 15);
+  const int vec = ((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15 ? 0 : row_stores(p.y, p.ym, p.yn, sizeof(T));
   const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn, vec};
   const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
   if (t.pair) return mma::launch_product<true, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);

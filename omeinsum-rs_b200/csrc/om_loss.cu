@@ -433,7 +433,7 @@ struct GradEpi {
       for (int c = 0; c < 32; ++c)
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
     }
-    store_row(dz + (int64_t)m * ld + n0, v);
+    store_row(dz + (int64_t)m * ld + n0, v, true);
   }
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
@@ -443,7 +443,7 @@ template <typename T>
 struct OutEpi {
   T* out;
   int64_t dr, dc;
-  int vec;             // rows of `out` may be written 16 bytes at a time
+  int vec;             // row_stores of `out`
   const float* scale;  // gradient_scale's
   float* acc;          // [split][rows][acc_ld], whole tiles
   int64_t acc_ld, acc_split;
@@ -470,16 +470,14 @@ struct OutEpi {
       }
     }
     if (keep) {
-#pragma unroll
-      for (int c = 0; c < 32; c += 4)
-        *reinterpret_cast<float4*>(row.acc + n0 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+      store_row(row.acc + n0, v, true);  // (whole tiles: 256-byte rows)
       return;
     }
 #pragma unroll
     for (int c = 0; c < 32; ++c) v[c] *= row.f;
     T* to = out + (int64_t)m * dr;
     if (vec && N - n0 >= 32) {
-      store_row(to + n0, v);
+      store_row(to + n0, v, vec == 2);
     } else {
 #pragma unroll
       for (int c = 0; c < 32; ++c)
@@ -625,8 +623,7 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
   const bool sums = splits > 1 || P < p.V;
   if (sums) OM_TRY(accs.alloc(be, (size_t)splits * p.N * acc_ld * 4));
   float* acc = (float*)accs.ptr;
-  const bool vecx = dxd == 1 && dxn % 8 == 0 && ((uintptr_t)dx & 15) == 0;
-  const bool vecw = dwd == 1 && dwv % 8 == 0 && ((uintptr_t)dw & 15) == 0;
+  const int vecx = row_stores(dx, dxn, dxd, 2), vecw = row_stores(dw, dwv, dwd, 2);
   for (int64_t v0 = 0; v0 < p.V; v0 += P) {
     const int64_t n = std::min(P, p.V - v0);
     const bool last = v0 + n == p.V;

@@ -380,13 +380,13 @@ inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, in
 }
 
 // Tile columns and whether a pair of CTAs shares a tile, from the result's
-// size: pairs of 256 x 256 when they fill the card, else the widest tile of
+// size: pairs of 256 x 256 when they fill four fifths of the card, else the widest tile of
 // one CTA that gives three quarters of the SMs one.
 struct Tiling {
   int bn, pair;
 };
 inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
-  if (M > TM && (M + 255) / 256 * ((N + 255) / 256) >= be->num_sms / 2) return {256, 1};
+  if (M > TM && (M + 255) / 256 * ((N + 255) / 256) * 5 >= be->num_sms * 2) return {256, 1};
   const int64_t tm = (M + TM - 1) / TM;
   for (int bn = 256; bn > least; bn /= 2)
     if (tm * ((N + bn - 1) / bn) * 4 >= be->num_sms * 3) return {bn, 0};

@@ -175,7 +175,7 @@ def _vector(be, t, name, shape, code):
 
 class _Call:
     """One call's outputs and its order with torch's current stream."""
-    __slots__ = ("be", "device", "cur", "mine")
+    __slots__ = ("be", "like", "cur", "mine")
 
     def __init__(self, be, like, *others):
         self.be = be
@@ -185,18 +185,18 @@ class _Call:
             if t is not None and isinstance(t, Strided) != own:
                 raise _invalid("Strided views and torch tensors cannot be mixed in one call")
         if own:
-            self.device = None
+            self.like = None
             return
-        self.device = like.device
+        self.like = like
         if not be.recording and _torch._C._cuda_getCurrentRawStream(be.device) != be.home_stream:
-            self.cur = _torch.cuda.current_stream(self.device)
-            self.mine = _torch.cuda.ExternalStream(be.home_stream, device=self.device)
+            self.cur = _torch.cuda.current_stream(like.device)
+            self.mine = _torch.cuda.ExternalStream(be.home_stream, device=like.device)
             self.mine.wait_stream(self.cur)
 
     def empty(self, code, *shape):
         """(a new row-major tensor, its pointer)"""
-        if self.device is not None:
-            t = _torch.empty(shape, dtype=_torch_types[code], device=self.device)
+        if self.like is not None:
+            t = self.like.new_empty(shape, dtype=_torch_types[code])
             return t, t.data_ptr()
         n = 1
         for s in shape:
@@ -330,12 +330,17 @@ _QUANTISED = (F32, OM_BF16, F16)
 
 def quantize_rows(be, x):
     """(q, scale) of a matrix in 8 bits: scale = max |row| / 127 and
-    q = row / scale, rounded (om_b200_quantize_rows).  x is f32, bf16 or f16."""
+    q = row / scale, rounded (om_b200_quantize_rows).  x is f32, bf16 or f16;
+    q's rows start 16 bytes apart or a multiple of that, which matmul_i8 reads
+    in place."""
     L = _bind()
     xp, code, (m, k), xs = _typed(be, x, "x", 2, _QUANTISED)
     call = _Call(be, x)
-    (q, qp), (scale, sp) = call.empty(I8, m, k), call.empty(F32, m)
-    call.done(L.om_b200_quantize_rows(be.h, code, _A2(k, m), xp, _cr(xs), qp, _A2(1, k), sp))
+    row = (k + 15) // 16 * 16
+    (q, qp), (scale, sp) = call.empty(I8, m, row), call.empty(F32, m)
+    call.done(L.om_b200_quantize_rows(be.h, code, _A2(k, m), xp, _cr(xs), qp, _A2(1, row), sp))
+    if row != k:
+        q = Strided(q.storage, (m, k), (row, 1)) if isinstance(q, Strided) else q[:, :k]
     return q, scale
 
 
