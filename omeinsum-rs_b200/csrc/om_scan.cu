@@ -571,13 +571,19 @@ int launch_chunks(om_backend* be, const ScanArgs& p) {
   a.narrow = a.groups * V < ((int64_t)1 << 32) && p.D < ((int64_t)1 << 32);
   // Six columns per SM run faster uncut, without the maps' second read (1024
   // columns x 512 steps bf16 with the backward pass: 236 us, cut in two 259;
-  // 512 x 1024: 364 and 266). Fewer are cut into as many chunks as make the
-  // 32 warps that an SM holds, of 32 steps at least (half or twice as many
-  // cost 1 to 7 % on 64 x 4096 and 9 x 65537).
-  const int64_t want = columns >= 6 * be->num_sms ? 1 : ((int64_t)be->num_sms * 32 + columns - 1) / columns;
-  int64_t chunks = std::max<int64_t>(1, std::min(want, p.T / 32));
+  // 512 x 1024: 364 and 266). Fewer are cut into as many chunks as one wave of
+  // the 32 warps that an SM holds takes, whole blocks of them (64 x 4096 in 64
+  // chunks: 182 us, in 74, which leave a second wave nearly empty: 207), of
+  // 16 steps at least (96 x 700: 61 us, of 32 steps 67).
+  int64_t chunks = 1;
+  if (columns < 6 * be->num_sms) {
+    chunks = (int64_t)be->num_sms * 32 / columns;
+    if (chunks >= WARPS) chunks = chunks / WARPS * WARPS;
+    else chunks = chunks >= 4 ? 4 : 2;
+    chunks = std::max<int64_t>(1, std::min(chunks, p.T / 16));
+  }
   a.steps = std::max<int64_t>(1, (p.T + chunks - 1) / chunks);
-  a.steps = chunks > 1 ? (a.steps + 7) / 8 * 8 : a.steps;
+  if (chunks > 1) a.steps = (a.steps + 7) / 8 * 8;
   chunks = std::max<int64_t>(1, (p.T + a.steps - 1) / a.steps);
   a.warps_t = 1;
   while (a.warps_t < WARPS && a.warps_t < chunks) a.warps_t *= 2;
