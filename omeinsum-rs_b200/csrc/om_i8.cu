@@ -431,8 +431,8 @@ int launch_matmul(om_backend* be, const I8Args& p) {
   const int vec = ((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15 ? 0 : row_stores(p.y, p.ym, p.yn, sizeof(T));
   const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn, vec};
   const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
-  if (t.pair) return mma::launch_product<true, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
-  return mma::launch_product<true, false, false, 1>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
+  if (t.pair) return mma::launch_product<true, false, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
+  return mma::launch_product<true, false, false, false, 1>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
 }
 
 int matmul(om_backend* be, om_dtype dtype, const I8Args& p) {

@@ -3,8 +3,11 @@
 //     lse_n = log sum_v exp(z_nv),  loss_n = lse_n - z_{n, target_n}
 //     dz_nv = dloss_n (exp(z_nv - lse_n) - [v == target_n]),
 //     dx = dz w,  dw = dz^T x.
-// The vocabulary is walked in pieces; a piece's logits live in scratch memory
-// until the next piece and are computed a second time by the backward pass.
+// The forward keeps a maximum and a sum of exponentials per row and group of
+// columns; the backward computes the logits a second time, a piece of the
+// vocabulary at a time, writes dz of the piece once and multiplies it twice:
+// 8 N D V operations, of which 6 are needed. Bound by the tensor cores, or,
+// for few tokens, by reading w.
 #include <algorithm>
 #include <cfloat>
 
@@ -28,34 +31,29 @@ __device__ __forceinline__ int64_t target_of(const void* t, int t64, int64_t n) 
   return t64 ? ((const int64_t*)t)[n] : (int64_t)((const int32_t*)t)[n];
 }
 
-// the element [r, c] of a strided matrix, into a row-major one of type S;
-// rows whose target lies outside the vocabulary become zero when given
-template <typename T, typename S>
-__global__ void convert_rows(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
-                             int64_t sc, S* __restrict__ dst, const void* targets, int t64,
-                             int64_t vocab) {
+// a strided matrix as a row-major one, zero in rows whose target lies outside
+// the vocabulary
+template <typename S>
+__global__ void masked_rows(const S* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
+                            int64_t sc, S* __restrict__ dst, const void* targets, int t64,
+                            int64_t vocab) {
   const int64_t total = rows * cols;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / cols, c = i - r * cols;
-    bool keep = true;
-    if (targets) {
-      const int64_t t = target_of(targets, t64, r);
-      keep = t >= 0 && t < vocab;
-    }
-    dst[i] = keep ? (S)Elem<T>::load(src[r * sr + c * sc]) : S(0);
+    const int64_t r = i / cols, c = i - r * cols, t = target_of(targets, t64, r);
+    dst[i] = t >= 0 && t < vocab ? src[r * sr + c * sc] : S(0);
   }
 }
 
-// a row-major matrix of type S into a strided one of type T
-template <typename T, typename S>
+// a row-major matrix as a strided one
+template <typename S>
 __global__ void store_rows(const S* __restrict__ src, int64_t rows, int64_t cols,
-                           T* __restrict__ dst, int64_t dr, int64_t dc) {
+                           S* __restrict__ dst, int64_t dr, int64_t dc) {
   const int64_t total = rows * cols;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / cols, c = i - r * cols;
-    dst[r * dr + c * dc] = Elem<T>::store(src[i]);
+    dst[r * dr + c * dc] = src[i];
   }
 }
 
@@ -146,7 +144,7 @@ unsigned flat_grid(om_backend* be, int64_t n) {
 }
 
 template <typename S>
-GemmArgs product(om_dtype dt, int64_t M, int64_t N, int64_t K, const void* a, int64_t am,
+GemmArgs gemm(om_dtype dt, int64_t M, int64_t N, int64_t K, const void* a, int64_t am,
                  int64_t ak, const void* b, int64_t bk, int64_t bn, void* c, int64_t cm) {
   GemmArgs g{};
   g.alg = OM_STANDARD;
@@ -164,40 +162,19 @@ int64_t piece_size(int64_t N, int64_t V, size_t elem) {
   return std::min(V, std::max<int64_t>(128, fit));
 }
 
-// f32 / f64: pieces through the library's own products
-template <typename T>
-int loss_forward(om_backend* be, const LossArgs& p, typename Elem<T>::State* loss,
-                 typename Elem<T>::State* lse) {
-  using S = typename Elem<T>::State;
-  constexpr bool conv = !std::is_same<T, S>::value;
+// f64, and f32 in exact mode: pieces through the library's own products
+template <typename S>
+int loss_forward(om_backend* be, const LossArgs& p, S* loss, S* lse) {
   const om_dtype dt = sizeof(S) == 8 ? OM_F64 : OM_F32;
   const int64_t P = piece_size(p.N, p.V, sizeof(S));
-  Scratch zs, stats, xs, wsc;
+  Scratch zs, stats;
   OM_TRY(zs.alloc(be, (size_t)p.N * P * sizeof(S)));
   OM_TRY(stats.alloc(be, (size_t)p.N * 3 * sizeof(S)));
   S* run = (S*)stats.ptr;
-  const S* x = (const S*)p.x;
-  int64_t xd = p.xd, xn = p.xn;
-  if (conv) {
-    OM_TRY(xs.alloc(be, (size_t)p.N * p.D * sizeof(S)));
-    OM_TRY(wsc.alloc(be, (size_t)P * p.D * sizeof(S)));
-    convert_rows<T, S><<<flat_grid(be, p.N * p.D), 256, 0, be->stream>>>(
-        (const T*)p.x, p.N, p.D, p.xn, p.xd, (S*)xs.ptr, nullptr, 0, 0);
-    note_launch();
-    x = (const S*)xs.ptr, xd = 1, xn = p.D;
-  }
   for (int64_t v0 = 0; v0 < p.V; v0 += P) {
     const int64_t n = std::min(P, p.V - v0);
-    const T* wt = (const T*)p.w + v0 * p.wv;
-    const S* w = (const S*)(const void*)wt;
-    int64_t wd = p.wd, wv = p.wv;
-    if (conv) {
-      convert_rows<T, S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>(
-          wt, n, p.D, p.wv, p.wd, (S*)wsc.ptr, nullptr, 0, 0);
-      note_launch();
-      w = (const S*)wsc.ptr, wd = 1, wv = p.D;
-    }
-    OM_TRY(launch_gemm(be, product<S>(dt, p.N, n, p.D, x, xn, xd, w, wd, wv, zs.ptr, n)));
+    const S* w = (const S*)p.w + v0 * p.wv;
+    OM_TRY(launch_gemm(be, gemm<S>(dt, p.N, n, p.D, p.x, p.xn, p.xd, w, p.wd, p.wv, zs.ptr, n)));
     ProfScope prof(be, "loss_piece_stats");
     piece_stats<S><<<(unsigned)p.N, 256, 0, be->stream>>>(
         (const S*)zs.ptr, n, v0, p.targets, p.target64, p.V, run, run + p.N, run + 2 * p.N, v0 == 0,
@@ -208,64 +185,51 @@ int loss_forward(om_backend* be, const LossArgs& p, typename Elem<T>::State* los
   return OM_OK;
 }
 
-template <typename T>
-int loss_backward(om_backend* be, const LossArgs& p, const typename Elem<T>::State* lse,
-                  const typename Elem<T>::State* dloss, T* dx, int64_t dxd, int64_t dxn, T* dw,
-                  int64_t dwd, int64_t dwv) {
-  using S = typename Elem<T>::State;
-  constexpr bool conv = !std::is_same<T, S>::value;
+template <typename S>
+int loss_backward(om_backend* be, const LossArgs& p, const S* lse, const S* dloss, S* dx,
+                  int64_t dxd, int64_t dxn, S* dw, int64_t dwd, int64_t dwv) {
   const om_dtype dt = sizeof(S) == 8 ? OM_F64 : OM_F32;
   const int64_t P = piece_size(p.N, p.V, sizeof(S));
   const int64_t nx = p.N * p.D;
   if (p.N == 0) {  // no token: the weights' gradient is zero
-    zero_rows<T><<<flat_grid(be, p.V * p.D), 256, 0, be->stream>>>(dw, p.V, p.D, dwv, dwd);
+    zero_rows<S><<<flat_grid(be, p.V * p.D), 256, 0, be->stream>>>(dw, p.V, p.D, dwv, dwd);
     note_launch();
     return check_cuda(cudaGetLastError(), "loss backward launch");
   }
-  Scratch zs, xs, acc, part, wsc, dws;
+  Scratch zs, xs, acc, part, dws;
   OM_TRY(zs.alloc(be, (size_t)p.N * P * sizeof(S)));
   OM_TRY(xs.alloc(be, (size_t)nx * sizeof(S)));
   OM_TRY(acc.alloc(be, (size_t)nx * sizeof(S)));
   if (P < p.V) OM_TRY(part.alloc(be, (size_t)nx * sizeof(S)));
-  if (conv) OM_TRY(wsc.alloc(be, (size_t)P * p.D * sizeof(S)));
   OM_TRY(dws.alloc(be, (size_t)P * p.D * sizeof(S)));
   // rows without a loss are zero here: whatever they hold reaches no gradient
-  convert_rows<T, S><<<flat_grid(be, nx), 256, 0, be->stream>>>(
-      (const T*)p.x, p.N, p.D, p.xn, p.xd, (S*)xs.ptr, p.targets, p.target64, p.V);
+  masked_rows<S><<<flat_grid(be, nx), 256, 0, be->stream>>>(
+      (const S*)p.x, p.N, p.D, p.xn, p.xd, (S*)xs.ptr, p.targets, p.target64, p.V);
   note_launch();
   for (int64_t v0 = 0; v0 < p.V; v0 += P) {
     const int64_t n = std::min(P, p.V - v0);
-    const T* wt = (const T*)p.w + v0 * p.wv;
-    const S* w = (const S*)(const void*)wt;
-    int64_t wd = p.wd, wv = p.wv;
-    if (conv) {
-      convert_rows<T, S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>(
-          wt, n, p.D, p.wv, p.wd, (S*)wsc.ptr, nullptr, 0, 0);
-      note_launch();
-      w = (const S*)wsc.ptr, wd = 1, wv = p.D;
-    }
-    OM_TRY(launch_gemm(be, product<S>(dt, p.N, n, p.D, xs.ptr, p.D, 1, w, wd, wv, zs.ptr, n)));
+    const S* w = (const S*)p.w + v0 * p.wv;
+    OM_TRY(launch_gemm(be, gemm<S>(dt, p.N, n, p.D, xs.ptr, p.D, 1, w, p.wd, p.wv, zs.ptr, n)));
     piece_gradient<S><<<(unsigned)p.N, 256, 0, be->stream>>>((S*)zs.ptr, p.N, n, v0, p.targets,
                                                              p.target64, p.V, lse, dloss);
     note_launch();
     S* to = v0 ? (S*)part.ptr : (S*)acc.ptr;
-    OM_TRY(launch_gemm(be, product<S>(dt, p.N, p.D, n, zs.ptr, n, 1, w, wv, wd, to, p.D)));
+    OM_TRY(launch_gemm(be, gemm<S>(dt, p.N, p.D, n, zs.ptr, n, 1, w, p.wv, p.wd, to, p.D)));
     if (v0) {
       add_into<S><<<flat_grid(be, nx), 256, 0, be->stream>>>((S*)acc.ptr, (const S*)part.ptr, nx);
       note_launch();
     }
-    OM_TRY(launch_gemm(be, product<S>(dt, n, p.D, p.N, zs.ptr, 1, n, xs.ptr, p.D, 1, dws.ptr, p.D)));
-    store_rows<T, S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>(
-        (const S*)dws.ptr, n, p.D, dw + v0 * dwv, dwv, dwd);
+    OM_TRY(launch_gemm(be, gemm<S>(dt, n, p.D, p.N, zs.ptr, 1, n, xs.ptr, p.D, 1, dws.ptr, p.D)));
+    store_rows<S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>((const S*)dws.ptr, n, p.D,
+                                                                 dw + v0 * dwv, dwv, dwd);
     note_launch();
   }
-  store_rows<T, S><<<flat_grid(be, nx), 256, 0, be->stream>>>((const S*)acc.ptr, p.N, p.D, dx, dxn,
-                                                              dxd);
+  store_rows<S><<<flat_grid(be, nx), 256, 0, be->stream>>>((const S*)acc.ptr, p.N, p.D, dx, dxn, dxd);
   note_launch();
   return check_cuda(cudaGetLastError(), "loss backward launch");
 }
 
-// ---- 16-bit types on the tensor cores ----------------------------------------
+// ---- 16-bit types and f32 on the tensor cores ----------------------------------------
 
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -280,6 +244,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 struct StatsEpi {
   const void* targets;
   int t64;
+  int64_t v0;    // vocabulary entry of column 0
   float2* part;  // [slot][rows]
   int64_t rows;
   float* hit;
@@ -288,7 +253,7 @@ struct StatsEpi {
     int64_t target;
   };
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
-    return Row{-INFINITY, 0.f, in ? target_of(targets, t64, m) : -1};
+    return Row{-INFINITY, 0.f, in ? target_of(targets, t64, m) - v0 : -1};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
                                           const uint32_t (&r)[32]) const {
@@ -393,15 +358,16 @@ __global__ void gradient_scale(const float* __restrict__ dloss, const void* targ
   *scale = f >= FLT_MIN && f < INFINITY ? f : 1.f;
 }
 
-// dz of a piece, rounded to T; the buffer's rows hold whole tiles
+// dz of a piece, rounded to T; the buffer's rows hold whole tiles. f32: as the
+// three bf16 planes that the two products take.
 template <typename T>
 struct GradEpi {
   const void* targets;
   int t64;
   int64_t vocab, v0;
   const float *lse, *dloss, *scale;
-  T* dz;
-  int64_t ld;
+  void* dz;
+  int64_t ld, plane;
   struct Row {
     float lse, g;
     int64_t target;  // within the piece
@@ -412,7 +378,7 @@ struct GradEpi {
       const int64_t t = target_of(targets, t64, m);
       row.lse = lse[m];
       if (t >= 0 && t < vocab) {
-        row.g = dloss[m] / *scale;
+        row.g = scale ? dloss[m] / *scale : dloss[m];
         row.target = t - v0;
       } else {  // exp(z - inf) = 0, whatever this row's lse is
         row.lse = INFINITY;
@@ -433,7 +399,17 @@ struct GradEpi {
       for (int c = 0; c < 32; ++c)
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
     }
-    store_row(dz + (int64_t)m * ld + n0, v, true);
+    if constexpr (sizeof(T) == 2) {
+      store_row((T*)dz + (int64_t)m * ld + n0, v, true);
+    } else {
+      __nv_bfloat16* to = (__nv_bfloat16*)dz + (int64_t)m * ld + n0;
+#pragma unroll
+      for (int z = 0; z < 3; ++z) {
+        store_row(to + z * plane, v, true);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] -= __bfloat162float(__float2bfloat16_rn(v[c]));
+      }
+    }
   }
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
@@ -444,7 +420,7 @@ struct OutEpi {
   T* out;
   int64_t dr, dc;
   int vec;             // row_stores of `out`
-  const float* scale;  // gradient_scale's
+  const float* scale;  // null or gradient_scale's
   float* acc;          // [split][rows][acc_ld], whole tiles
   int64_t acc_ld, acc_split;
   int load, keep;      // add what acc holds; leave the sum there
@@ -453,7 +429,7 @@ struct OutEpi {
     float* acc;
   };
   __device__ __forceinline__ Row begin(int m, bool in, int split) const {
-    return Row{*scale,
+    return Row{scale ? *scale : 1.f,
                acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
@@ -492,7 +468,7 @@ template <typename T>
 __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t acc_split,
                             int64_t acc_ld, int64_t rows, int64_t cols, const float* scale,
                             T* __restrict__ out, int64_t dr, int64_t dc) {
-  const float f = *scale;
+  const float f = scale ? *scale : 1.f;
   const int64_t total = rows * cols;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
@@ -544,76 +520,160 @@ void launch_pack(om_backend* be, const T* src, int64_t rows, int64_t cols, int64
   note_launch();
 }
 
+// Rows of f32 as three bf16 planes, x = x0 + x1 + x2 to 24 bits; zero as above.
+// A thread makes 8 elements of each plane.
+__global__ void split_rows(const float* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
+                           int64_t sc, __nv_bfloat16* __restrict__ dst, int64_t ld, int64_t plane,
+                           const void* targets, int t64, int64_t vocab) {
+  const int64_t per = ld / 8;
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    bool keep = true;
+    if (targets) {
+      const int64_t t = target_of(targets, t64, r);
+      keep = t >= 0 && t < vocab;
+    }
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < per;
+         i += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t c = i * 8;
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = keep && c + k < cols ? src[r * sr + (c + k) * sc] : 0.f;
+#pragma unroll
+      for (int z = 0; z < 3; ++z) {
+        __align__(16) __nv_bfloat16 b[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          b[k] = __float2bfloat16_rn(v[k]);
+          v[k] -= __bfloat162float(b[k]);
+        }
+        *reinterpret_cast<uint4*>(dst + z * plane + r * ld + c) = *reinterpret_cast<const uint4*>(b);
+      }
+    }
+  }
+}
+
 // The operand itself when TMA can read its rows, else a packed copy.
+int readable(om_backend* be, const float* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
+             Scratch& copy, mma::Matrix* out, const LossArgs* masked = nullptr) {
+  const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
+  if (!copy.ptr) OM_TRY(copy.alloc(be, (size_t)plane * 6));
+  const int threads = (int)std::min<int64_t>(256, (ld / 8 + 31) / 32 * 32);
+  const dim3 grid((unsigned)std::min<int64_t>((ld / 8 + threads - 1) / threads, 65535),
+                  (unsigned)std::min<int64_t>(rows, 65535));
+  ProfScope prof(be, "loss_split");
+  split_rows<<<grid, threads, 0, be->stream>>>(src, rows, cols, sr, sc, (__nv_bfloat16*)copy.ptr, ld,
+                                               plane, masked ? masked->targets : nullptr,
+                                               masked ? masked->target64 : 0, masked ? masked->V : 0);
+  note_launch();
+  *out = mma::Matrix{copy.ptr, rows, cols, ld, 2, plane};
+  return check_cuda(cudaGetLastError(), "loss split launch");
+}
 template <typename T>
 int readable(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
-             Scratch& copy, mma::Matrix* out) {
+             Scratch& copy, mma::Matrix* out, const LossArgs* masked = nullptr) {
   *out = mma::Matrix{src, rows, cols, sr, 2};
-  if ((sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2)) return OM_OK;
+  if (!masked && (sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2)) return OM_OK;
   const int64_t ld = (cols + 7) / 8 * 8;
-  OM_TRY(copy.alloc(be, (size_t)rows * ld * 2));
-  launch_pack<T>(be, src, rows, cols, sr, sc, (T*)copy.ptr, ld, nullptr, 0, 0);
+  if (!copy.ptr) OM_TRY(copy.alloc(be, (size_t)rows * ld * 2));
+  launch_pack<T>(be, src, rows, cols, sr, sc, (T*)copy.ptr, ld, masked ? masked->targets : nullptr,
+                 masked ? masked->target64 : 0, masked ? masked->V : 0);
   *out = mma::Matrix{copy.ptr, rows, cols, ld, 2};
   return check_cuda(cudaGetLastError(), "loss pack launch");
 }
 
-template <bool AMN, bool BMN, class Epi>
-int product16(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
-              bool bf16, mma::Tiling t, int splits, const Epi& epi) {
-  if (t.pair) return mma::launch_product<false, AMN, BMN, 2>(be, name, a, b, bf16, t.bn, splits, epi);
-  return mma::launch_product<false, AMN, BMN, 1>(be, name, a, b, bf16, t.bn, splits, epi);
+// Rows 16-byte aligned and zero-filled either way: the operand itself when TMA
+// can read it, else a copy (f32: always, as three planes); `masked`: a copy
+// whose rows without a loss are zero.
+template <typename T, bool AMN, bool BMN, class Epi>
+int product(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
+            mma::Tiling t, int splits, const Epi& epi) {
+  constexpr bool P3 = sizeof(T) == 4, BF = !std::is_same<T, __half>::value;
+  if (t.pair) return mma::launch_product<false, P3, AMN, BMN, 2>(be, name, a, b, BF, t.bn, splits, epi);
+  return mma::launch_product<false, P3, AMN, BMN, 1>(be, name, a, b, BF, t.bn, splits, epi);
+}
+template <typename T>
+mma::Tiling tiles(const om_backend* be, int64_t M, int64_t N) {
+  return mma::tiling(be, M, N, 64, sizeof(T) == 4 ? 128 : 256);
+}
+// rows [r0, r0 + n) of a K-major matrix
+mma::Matrix rows_of(const mma::Matrix& m, int64_t r0, int64_t n) {
+  mma::Matrix r = m;
+  r.ptr = (const char*)m.ptr + r0 * m.ld * m.elem;
+  r.rows = n;
+  return r;
+}
+// the same memory with the roles of rows and k exchanged
+mma::Matrix turned(const mma::Matrix& m) {
+  mma::Matrix r = m;
+  r.rows = m.k;
+  r.k = m.rows;
+  return r;
+}
+
+// Vocabulary entries whose f32 weights are split at a time (1 GiB of planes);
+// 16-bit ones are read where they lie, or packed as a whole
+template <typename T>
+int64_t weight_rows(const LossArgs& p) {
+  if (sizeof(T) == 2) return p.V;
+  return std::min(p.V, std::max<int64_t>(256, ((int64_t)1 << 30) / (p.D * 6) / 256 * 256));
 }
 
 template <typename T>
-int loss_forward16(om_backend* be, const LossArgs& p, float* loss, float* lse) {
-  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+int loss_forward_tc(om_backend* be, const LossArgs& p, float* loss, float* lse) {
   Scratch xc, wc, ws;
   mma::Matrix x, w;
-  OM_TRY(readable<T>(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
-  OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
-  const mma::Tiling t = mma::tiling(be, p.N, p.V, 64);
-  const int64_t slots = (p.V + t.bn - 1) / t.bn * 2;
+  OM_TRY(readable(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
+  const int64_t W = weight_rows<T>(p);
+  const mma::Tiling t = tiles<T>(be, p.N, W);
+  const int64_t slots = ((p.V + W - 1) / W) * ((W + t.bn - 1) / t.bn) * 2;
   OM_TRY(ws.alloc(be, (size_t)p.N * (slots * 8 + 4)));
   float2* part = (float2*)ws.ptr;
   float* hit = (float*)(part + slots * p.N);
-  const StatsEpi epi{p.targets, p.target64, part, p.N, hit};
-  OM_TRY((product16<false, false>(be, "loss_logits", x, w, bf16, t, 1, epi)));
+  int64_t used = 0;
+  for (int64_t v0 = 0; v0 < p.V; v0 += W) {
+    const int64_t n = std::min(W, p.V - v0);
+    OM_TRY(readable(be, (const T*)p.w + v0 * p.wv, n, p.D, p.wv, p.wd, wc, &w));
+    const StatsEpi epi{p.targets, p.target64, v0, part + used * p.N, p.N, hit};
+    OM_TRY((product<T, false, false>(be, "loss_logits", x, w, t, 1, epi)));
+    used += (n + t.bn - 1) / t.bn * 2;
+  }
   ProfScope prof(be, "loss_join_stats");
   join_stats<<<(unsigned)((p.N + 7) / 8), 256, 0, be->stream>>>(
-      part, (int)slots, p.N, p.targets, p.target64, p.V, hit, loss, lse);
+      part, (int)used, p.N, p.targets, p.target64, p.V, hit, loss, lse);
   note_launch();
   return check_cuda(cudaGetLastError(), "loss join launch");
 }
 
 template <typename T>
-int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const float* dloss, T* dx,
-                    int64_t dxd, int64_t dxn, T* dw, int64_t dwd, int64_t dwv) {
-  const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const float* dloss, T* dx,
+                     int64_t dxd, int64_t dxn, T* dw, int64_t dwd, int64_t dwv) {
+  constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
   if (p.N == 0) {
     zero_rows<T><<<flat_grid(be, p.V * p.D), 256, 0, be->stream>>>(dw, p.V, p.D, dwv, dwd);
     note_launch();
     return check_cuda(cudaGetLastError(), "loss backward launch");
   }
-  // a piece's dz takes at most 512 MiB
+  // a piece's dz takes at most 512 MiB (f32: 1.5 GiB)
   const int64_t fit = ((int64_t)256 << 20) / p.N / 256 * 256;
-  const int64_t P = std::min((p.V + 255) / 256 * 256, std::max<int64_t>(256, fit));
-  const int64_t Dp = (p.D + 7) / 8 * 8;
+  const int64_t P = std::min({(p.V + 255) / 256 * 256, std::max<int64_t>(256, fit),
+                              (weight_rows<T>(p) + 255) / 256 * 256});
   Scratch xs, wc, dzs, accs, scales;
-  OM_TRY(xs.alloc(be, (size_t)p.N * Dp * 2));
-  OM_TRY(dzs.alloc(be, (size_t)p.N * P * 2));
-  T* dz = (T*)dzs.ptr;
+  OM_TRY(dzs.alloc(be, (size_t)p.N * P * 2 * PLANES));
   // rows without a loss are zero here: whatever they hold reaches no gradient
-  launch_pack<T>(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, (T*)xs.ptr, Dp, p.targets, p.target64, p.V);
-  mma::Matrix w;
-  OM_TRY(readable<T>(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
-  OM_TRY(scales.alloc(be, 4));
-  float* scale = (float*)scales.ptr;
-  gradient_scale<<<1, 1024, 0, be->stream>>>(dloss, p.targets, p.target64, p.V, p.N,
-                                             bf16 ? 1.f : 16384.f, scale);
-  note_launch();
+  mma::Matrix x, w;
+  OM_TRY(readable(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xs, &x, &p));
+  if (PLANES == 1) OM_TRY(readable(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
+  float* scale = nullptr;
+  if (PLANES == 1) {
+    OM_TRY(scales.alloc(be, 4));
+    scale = (float*)scales.ptr;
+    gradient_scale<<<1, 1024, 0, be->stream>>>(dloss, p.targets, p.target64, p.V, p.N,
+                                               std::is_same<T, __half>::value ? 16384.f : 1.f, scale);
+    note_launch();
+  }
   // dx sums over the vocabulary: few tokens and a narrow width leave SMs idle
   // unless the sum is split; each split needs 8 slabs to be worth its f32 sums
-  const mma::Tiling tx = mma::tiling(be, p.N, p.D, 64);
+  const mma::Tiling tx = tiles<T>(be, p.N, p.D);
   const int64_t rows = tx.pair ? 256 : 128;
   const int64_t txt = (p.N + rows - 1) / rows * ((p.D + tx.bn - 1) / tx.bn);
   const int64_t slots = tx.pair ? be->num_sms / 2 : be->num_sms;
@@ -623,23 +683,21 @@ int loss_backward16(om_backend* be, const LossArgs& p, const float* lse, const f
   const bool sums = splits > 1 || P < p.V;
   if (sums) OM_TRY(accs.alloc(be, (size_t)splits * p.N * acc_ld * 4));
   float* acc = (float*)accs.ptr;
-  const int vecx = row_stores(dx, dxn, dxd, 2), vecw = row_stores(dw, dwv, dwd, 2);
+  const int vecx = row_stores(dx, dxn, dxd, sizeof(T)), vecw = row_stores(dw, dwv, dwd, sizeof(T));
   for (int64_t v0 = 0; v0 < p.V; v0 += P) {
     const int64_t n = std::min(P, p.V - v0);
     const bool last = v0 + n == p.V;
-    const T* wp = (const T*)w.ptr + v0 * w.ld;
-    const mma::Matrix x{xs.ptr, p.N, p.D, Dp, 2};
-    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dz, P};
-    OM_TRY((product16<false, false>(be, "loss_dlogits", x, mma::Matrix{wp, n, p.D, w.ld, 2}, bf16,
-                                    mma::tiling(be, p.N, n, 64), 1, ge)));
+    mma::Matrix wp;
+    if (PLANES == 1) wp = rows_of(w, v0, n);
+    else OM_TRY(readable(be, (const T*)p.w + v0 * p.wv, n, p.D, p.wv, p.wd, wc, &wp));
+    const mma::Matrix dz{dzs.ptr, p.N, n, P, 2, PLANES == 3 ? p.N * P : 0};
+    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs.ptr, P, p.N * P};
+    OM_TRY((product<T, false, false>(be, "loss_dlogits", x, wp, tiles<T>(be, p.N, n), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
     const OutEpi<T> xe{dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
-    OM_TRY((product16<false, true>(be, "loss_dx", mma::Matrix{dz, p.N, n, P, 2},
-                                   mma::Matrix{wp, p.D, n, w.ld, 2}, bf16, tx, now, xe)));
+    OM_TRY((product<T, false, true>(be, "loss_dx", dz, turned(wp), tx, now, xe)));
     const OutEpi<T> we{dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
-    OM_TRY((product16<true, true>(be, "loss_dw", mma::Matrix{dz, n, p.N, P, 2},
-                                  mma::Matrix{xs.ptr, p.D, p.N, Dp, 2}, bf16,
-                                  mma::tiling(be, n, p.D, 64), 1, we)));
+    OM_TRY((product<T, true, true>(be, "loss_dw", turned(dz), turned(x), tiles<T>(be, n, p.D), 1, we)));
   }
   if (splits > 1) {
     ProfScope prof(be, "loss_join_splits");
@@ -684,9 +742,10 @@ extern "C" int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, cons
   const LossArgs p{shape[1], shape[0], shape[2], x, strides_x[0], strides_x[1], w, strides_w[0],
                    strides_w[1], targets, target_dtype == OM_I64};
   if (dtype == OM_F64) return loss_forward<double>(be, p, (double*)loss, (double*)lse);
-  if (dtype == OM_BF16) return loss_forward16<__nv_bfloat16>(be, p, (float*)loss, (float*)lse);
-  if (dtype == OM_F16) return loss_forward16<__half>(be, p, (float*)loss, (float*)lse);
-  return loss_forward<float>(be, p, (float*)loss, (float*)lse);
+  if (dtype == OM_BF16) return loss_forward_tc<__nv_bfloat16>(be, p, (float*)loss, (float*)lse);
+  if (dtype == OM_F16) return loss_forward_tc<__half>(be, p, (float*)loss, (float*)lse);
+  if (be->f32_exact) return loss_forward<float>(be, p, (float*)loss, (float*)lse);
+  return loss_forward_tc<float>(be, p, (float*)loss, (float*)lse);
 }
 
 extern "C" int om_b200_linear_cross_entropy_backward(
@@ -708,8 +767,9 @@ extern "C" int om_b200_linear_cross_entropy_backward(
   FN<T>(be, p, (const S*)lse, (const S*)dloss, (T*)dx, strides_dx[0], strides_dx[1], \
                    (T*)dw, strides_dw[0], strides_dw[1])
   if (dtype == OM_F64) return OM_LOSS_BWD(loss_backward, double, double);
-  if (dtype == OM_BF16) return OM_LOSS_BWD(loss_backward16, __nv_bfloat16, float);
-  if (dtype == OM_F16) return OM_LOSS_BWD(loss_backward16, __half, float);
-  return OM_LOSS_BWD(loss_backward, float, float);
+  if (dtype == OM_BF16) return OM_LOSS_BWD(loss_backward_tc, __nv_bfloat16, float);
+  if (dtype == OM_F16) return OM_LOSS_BWD(loss_backward_tc, __half, float);
+  if (be->f32_exact) return OM_LOSS_BWD(loss_backward, float, float);
+  return OM_LOSS_BWD(loss_backward_tc, float, float);
 #undef OM_LOSS_BWD
 }

@@ -17,6 +17,14 @@
 // read by TMA where they lie, with a 128-byte swizzle. TMA fills what lies
 // outside the matrix with zeros, so no size needs padding.
 //
+// P3: operands of three bf16 planes each (x = x0 + x1 + x2 to 24 bits), six
+// products per slab, the smallest first:
+//     A2 B0 + A0 B2 + A1 B1 + A1 B0 + A0 B1 + A0 B0
+// for sums as exact as f32's: what is left out is 2^-24 of a term. The tensor
+// core does not round its running sum to nearest, so every CHUNK slabs are
+// summed from zero and added up in the epilogue warps' registers. The planes
+// of a slab are loaded once for all six.
+//
 // Every wait is bounded; on expiry the kernel records an error word that
 // om_b200_sync reports, and leaves after its other bounded waits.
 #pragma once
@@ -39,6 +47,7 @@ constexpr int TM = 128;             // rows of a CTA's accumulator
 constexpr int THREADS = 320;        // 2 + 8 warps
 constexpr int MAX_STAGES = 12;
 constexpr int SLAB = 128;           // bytes of k per stage
+constexpr int CHUNK = 2;            // slabs of a sum (P3)
 constexpr int A_BYTES = TM * SLAB;
 constexpr uint32_t WAIT_LIMIT = 1u << 24;
 
@@ -80,6 +89,22 @@ __device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void load_box3(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                          int z, uint32_t bar, int cg) {
+  if (cg == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+        "l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 
 template <int CG>
@@ -181,7 +206,7 @@ __device__ __forceinline__ Tile tile_at(const Shape& g, int t) {
 // read; columns(row, m, in, n0, N, values) for each 32 columns from n0 on; and
 // end(row, m, in, slot) with slot = 2 * column tile + column group. `in`: row m
 // exists; columns from N on do not.
-template <bool I8, bool AMN, bool BMN, int CG, class Epi>
+template <bool I8, bool P3, bool AMN, bool BMN, int CG, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
                    const __grid_constant__ Shape g, const __grid_constant__ Epi epi) {
@@ -197,7 +222,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
   const int tiles = g.tiles_m * g.tiles_n * g.splits;
   const int b_rows = g.BN / CG;  // of B that this CTA loads
-  const uint32_t stage_bytes = A_BYTES + b_rows * SLAB;
+  constexpr int PLANES = P3 ? 3 : 1;
+  const uint32_t b_bytes = b_rows * SLAB;
+  const uint32_t stage_bytes = PLANES * (A_BYTES + b_bytes);
   const int kstep = I8 ? 128 : 64;  // elements of a slab
 
   if (warp == 1) {
@@ -248,7 +275,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                          "r"(stage_bytes * CG)
                          : "memory");
           if constexpr (CG == 2) bar = in_rank(bar, 0);
-          const uint32_t a = ring + s * stage_bytes, b = a + A_BYTES;
+          const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
+          if constexpr (P3) {
+            for (int z = 0; z < 3; ++z) {
+              if constexpr (AMN) {
+                for (int i = 0; i < TM; i += 64)
+                  load_box3(a + z * A_BYTES + i * SLAB, &amap, m0 + i, k * kstep, z, bar, CG);
+              } else {
+                load_box3(a + z * A_BYTES, &amap, k * kstep, m0, z, bar, CG);
+              }
+              if constexpr (BMN) {
+                for (int i = 0; i < b_rows; i += 64)
+                  load_box3(b + z * b_bytes + i * SLAB, &bmap, n0 + i, k * kstep, z, bar, CG);
+              } else {
+                load_box3(b + z * b_bytes, &bmap, k * kstep, n0, z, bar, CG);
+              }
+            }
+            if (++s == g.stages) s = 0, phase ^= 1;
+            continue;
+          }
           if constexpr (AMN) {
             for (int i = 0; i < TM; i += 64) load_box<CG>(a + i * SLAB, &amap, m0 + i, k * kstep, bar);
           } else {
@@ -275,48 +320,51 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0 && rank == 0) {  // products
       int s = 0, i = 0;
       uint32_t phase = 0;
-      for (int t = first; t < tiles && ok; t += step, ++i) {
+      for (int t = first; t < tiles && ok; t += step) {
         const Tile at = tile_at(g, t);
-        const int ab = i & 1;
-        if (i >= 2) ok = wait(smem_addr(&tempty[ab]), ((i >> 1) - 1) & 1);
-        if (!ok) break;
-        asm volatile("tcgen05.fence::after_thread_sync;");
-        const uint32_t d = tmem + ab * 256;
         const int k0 = slab_at(g, at.split), k1 = slab_at(g, at.split + 1);
+        uint32_t d = 0;
         for (int k = k0; k < k1; ++k) {
+          const bool fresh = P3 ? (k - k0) % CHUNK == 0 : k == k0;  // an accumulator starts here
+          if (fresh) {
+            if (i >= 2) ok = wait(smem_addr(&tempty[i & 1]), ((i >> 1) - 1) & 1);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;");
+            d = tmem + (i & 1) * 256;
+          }
           ok = wait(smem_addr(&full[s]), phase);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;");
-          const uint32_t a = ring + s * stage_bytes, b = a + A_BYTES;
+          const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
+          if constexpr (P3) {
+            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            issue<I8, CG>(d, operand<AMN>(a + j * (AMN ? 2048 : 32)),
-                          operand<BMN>(b + j * (BMN ? 2048 : 32)), g.idesc, k > k0 || j > 0);
+            for (int p = 0; p < 6; ++p)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                issue<I8, CG>(d, operand<AMN>(a + PA[p] * A_BYTES + j * (AMN ? 2048 : 32)),
+                              operand<BMN>(b + PB[p] * b_bytes + j * (BMN ? 2048 : 32)), g.idesc,
+                              !fresh || p > 0 || j > 0);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              issue<I8, CG>(d, operand<AMN>(a + j * (AMN ? 2048 : 32)),
+                            operand<BMN>(b + j * (BMN ? 2048 : 32)), g.idesc, !fresh || j > 0);
+          }
           commit<CG>(smem_addr(&empty[s]));
           if (++s == g.stages) s = 0, phase ^= 1;
+          if (k + 1 == k1 || (P3 && (k + 1 - k0) % CHUNK == 0)) {
+            commit<CG>(smem_addr(&tfull[i & 1]));
+            ++i;
+          }
         }
-        commit<CG>(smem_addr(&tfull[ab]));
       }
       if (!ok) atomicOr(g.err, 1u);
     }
   } else {  // epilogue
     const int quad = warp & 3, part = (warp - 2) >> 2;
     int i = 0;
-    for (int t = first; t < tiles; t += step, ++i) {
-      const Tile at = tile_at(g, t);
-      const int ab = i & 1;
-      const int m = (at.m * CG + (int)rank) * TM + 32 * quad + lane;
-      const bool in = m < g.M;
-      typename Epi::Row row = epi.begin(m, in, at.split);
-      ok = wait(smem_addr(&tfull[ab]), (i >> 1) & 1);
-      if (!ok) break;
-      asm volatile("tcgen05.fence::after_thread_sync;");
-      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16) + ab * 256;
-      for (int c = part * 32; c < g.BN; c += 64) {
-        uint32_t r[32];
-        read_columns(base + c, r);
-        epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
-      }
+    auto release = [&](int ab) {  // the accumulator has been read
       asm volatile("tcgen05.fence::before_thread_sync;");
       __syncwarp();
       if (lane == 0) {
@@ -324,6 +372,57 @@ __global__ void __launch_bounds__(THREADS, 1)
         if constexpr (CG == 2) bar = in_rank(bar, 0);
         asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                      : "memory");
+      }
+    };
+    for (int t = first; t < tiles && ok; t += step) {
+      const Tile at = tile_at(g, t);
+      const int m = (at.m * CG + (int)rank) * TM + 32 * quad + lane;
+      const bool in = m < g.M;
+      typename Epi::Row row = epi.begin(m, in, at.split);
+      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16);
+      if constexpr (P3) {  // BN <= 128: at most two groups of columns
+        float sum[2][32];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sum[j][c] = 0.f;
+        const int slabs = slab_at(g, at.split + 1) - slab_at(g, at.split);
+        for (int k = 0; k < slabs; k += CHUNK, ++i) {
+          ok = wait(smem_addr(&tfull[i & 1]), (i >> 1) & 1);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int c = part * 32 + j * 64;
+            if (c >= g.BN) break;
+            uint32_t r[32];
+            read_columns(base + (i & 1) * 256 + c, r);
+#pragma unroll
+            for (int q = 0; q < 32; ++q) sum[j][q] += __uint_as_float(r[q]);
+          }
+          release(i & 1);
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int c = part * 32 + j * 64;
+          if (c >= g.BN) break;
+          uint32_t r[32];
+#pragma unroll
+          for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(sum[j][q]);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
+        }
+      } else {
+        ok = wait(smem_addr(&tfull[i & 1]), (i >> 1) & 1);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        for (int c = part * 32; c < g.BN; c += 64) {
+          uint32_t r[32];
+          read_columns(base + (i & 1) * 256 + c, r);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
+        }
+        release(i & 1);
+        ++i;
       }
       epi.end(row, m, in, at.n * 2 + part);
     }
@@ -348,6 +447,7 @@ struct Matrix {
   const void* ptr;
   int64_t rows, k, ld;
   int elem;
+  int64_t plane = 0;  // elements between the three planes of P3
 };
 
 inline bool tma_readable(const void* ptr, int64_t ld, int elem) {
@@ -358,12 +458,12 @@ inline bool tma_readable(const void* ptr, int64_t ld, int elem) {
 inline int encode(CUtensorMap* map, const Matrix& x, bool mn, int box_rows) {
   auto fn = tensor_map_encoder();
   if (!fn) return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
-  const cuuint64_t dims[2] = {(cuuint64_t)(mn ? x.rows : x.k), (cuuint64_t)(mn ? x.k : x.rows)};
-  const cuuint64_t strides[1] = {(cuuint64_t)(x.ld * x.elem)};
-  const cuuint32_t box[2] = {(cuuint32_t)(SLAB / x.elem), (cuuint32_t)(mn ? SLAB / x.elem : box_rows)};
-  const cuuint32_t one[2] = {1, 1};
+  const cuuint64_t dims[3] = {(cuuint64_t)(mn ? x.rows : x.k), (cuuint64_t)(mn ? x.k : x.rows), 3};
+  const cuuint64_t strides[2] = {(cuuint64_t)(x.ld * x.elem), (cuuint64_t)(x.plane * x.elem)};
+  const cuuint32_t box[3] = {(cuuint32_t)(SLAB / x.elem), (cuuint32_t)(mn ? SLAB / x.elem : box_rows), 1};
+  const cuuint32_t one[3] = {1, 1, 1};
   const CUresult r = fn(map, x.elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
-                        2, (void*)x.ptr, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        x.plane ? 3 : 2, (void*)x.ptr, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
@@ -380,15 +480,15 @@ inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, in
 }
 
 // Tile columns and whether a pair of CTAs shares a tile, from the result's
-// size: pairs of 256 x 256 when they fill four fifths of the card, else the widest tile of
+// size: pairs of 256 x `most` when they fill four fifths of the card, else the widest tile of
 // one CTA that gives three quarters of the SMs one.
 struct Tiling {
   int bn, pair;
 };
-inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
-  if (M > TM && (M + 255) / 256 * ((N + 255) / 256) * 5 >= be->num_sms * 2) return {256, 1};
+inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least, int most = 256) {
+  if (M > TM && (M + 255) / 256 * ((N + most - 1) / most) * 5 >= be->num_sms * 2) return {most, 1};
   const int64_t tm = (M + TM - 1) / TM;
-  for (int bn = 256; bn > least; bn /= 2)
+  for (int bn = most; bn > least; bn /= 2)
     if (tm * ((N + bn - 1) / bn) * 4 >= be->num_sms * 3) return {bn, 0};
   return {least, 0};
 }
@@ -396,8 +496,8 @@ inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least) {
 // D = A B^T through `epi`. bn: tile columns (32, 64, 128 or 256; at least 64
 // for an MN-major B); pair: two CTAs per tile (bn 128 or 256). splits > 1
 // cuts k into that many ranges of whole slabs, each handed to the epilogue
-// as its own tile.
-template <bool I8, bool AMN, bool BMN, int CG, class Epi>
+// as its own tile. P3: bf16 planes (Matrix::plane), bn at most 128.
+template <bool I8, bool P3, bool AMN, bool BMN, int CG, class Epi>
 int launch_product(om_backend* be, const char* name, const Matrix& a, const Matrix& b, bool bf16,
                    int bn, int splits, const Epi& epi) {
   const int kstep = I8 ? 128 : 64;
@@ -415,12 +515,12 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
   // a wave's tiles form a square of rows and columns, so that each slab is
   // read by many SMs while it is in L2
   g.group = std::max(1, std::min<int>((int)tm, CG == 2 ? 8 : 16));
-  const int stage = A_BYTES + bn / CG * SLAB;
-  g.stages = std::min(MAX_STAGES, 208 * 1024 / stage);
+  const int stage = (P3 ? 3 : 1) * (A_BYTES + bn / CG * SLAB);
+  g.stages = std::min(MAX_STAGES, 216 * 1024 / stage);
   g.idesc = instruction(I8, bf16, AMN, BMN, TM * CG, bn);
   g.err = be->d_flags + 1;
   const size_t smem = (size_t)g.stages * stage + 1024;
-  auto kernel = product_kernel<I8, AMN, BMN, CG, Epi>;
+  auto kernel = product_kernel<I8, P3, AMN, BMN, CG, Epi>;
   OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), name);
   const int64_t work = tm * tn * splits;
   ProfScope prof(be, name);

@@ -21,6 +21,7 @@ such waits are made: the tensors must be ready, and stay alive with the graph.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import numpy as np
 
@@ -125,14 +126,16 @@ def _learn_torch(dtype, name):
 
 def _operand(be, t, name):
     """(device pointer, type code, shape, strides) of one argument."""
-    if isinstance(t, Strided):
+    if type(t) is Strided:
         s = t.storage
         if s.backend.device != be.device:
             raise _invalid(f"{name}: on device {s.backend.device}, the backend on {be.device}")
         return (s.ptr or 0) + t.offset * s.dtype.itemsize, DTYPES[s.dtype], t.shape, t.strides
-    if not hasattr(t, "data_ptr"):
-        raise _invalid(f"{name}: a Strided view or a torch CUDA tensor is needed, not {type(t).__name__}")
-    if t.get_device() != be.device:  # -1: not on a device at all
+    try:
+        device = t.get_device()
+    except AttributeError:
+        raise _invalid(f"{name}: a Strided view or a torch CUDA tensor is needed, not {type(t).__name__}") from None
+    if device != be.device:  # -1: not on a device at all
         raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
     code = _torch_codes.get(t.dtype)
     if code is None:
@@ -180,9 +183,9 @@ class _Call:
     def __init__(self, be, like, *others):
         self.be = be
         self.cur = None
-        own = isinstance(like, Strided)
+        own = type(like) is Strided
         for t in others:
-            if t is not None and isinstance(t, Strided) != own:
+            if t is not None and (type(t) is Strided) != own:
                 raise _invalid("Strided views and torch tensors cannot be mixed in one call")
         if own:
             self.like = None
@@ -196,7 +199,11 @@ class _Call:
     def empty(self, code, *shape):
         """(a new row-major tensor, its pointer)"""
         if self.like is not None:
-            t = self.like.new_empty(shape, dtype=_torch_types[code])
+            like = self.like
+            if like.dtype is _torch_types[code]:
+                t = like.new_empty(shape)
+            else:
+                t = _torch.empty(shape, dtype=_torch_types[code], device=like.device)
             return t, t.data_ptr()
         n = 1
         for s in shape:
@@ -211,19 +218,23 @@ class _Call:
             _check(rc)
 
 
-_A2 = ctypes.c_int64 * 2
-_A3 = ctypes.c_int64 * 3
+@functools.lru_cache(maxsize=512)
+def _i64s(*values):
+    """An int64 array for the ABI (which only reads it)."""
+    return (ctypes.c_int64 * len(values))(*values)
+
+
 _REALS = (F32, F64, OM_BF16, F16)
 
 
 def _dtb(strides):
     """Strides of a [batch, time, channel] operand in the ABI's order."""
-    return _A3(strides[2], strides[1], strides[0])
+    return _i64s(strides[2], strides[1], strides[0])
 
 
 def _cr(strides):
     """Strides of a [row, column] operand in the ABI's order."""
-    return _A2(strides[1], strides[0])
+    return _i64s(strides[1], strides[0])
 
 
 def _kind(kind, who):
@@ -257,8 +268,8 @@ def gated_scan(be, gate, x, h0=None, lengths=None, kind="linear", h_last=None):
         h_last, lastp = call.empty(st, b, d)
     else:
         lastp = _vector(be, h_last, "h_last", (b, d), st)
-    call.done(L.om_b200_gated_scan(be.h, k, code, _A3(d, t, b), gp, _dtb(gs), xp, _dtb(xs), h0p, lp, hp,
-                                   _A3(1, d, t * d), lastp))
+    call.done(L.om_b200_gated_scan(be.h, k, code, _i64s(d, t, b), gp, _dtb(gs), xp, _dtb(xs), h0p, lp, hp,
+                                   _i64s(1, d, t * d), lastp))
     return h, h_last
 
 
@@ -283,8 +294,8 @@ def gated_scan_backward(be, gate, x, h, dh, h0=None, dh_last=None, lengths=None,
     elp = _vector(be, dh_last, "dh_last", (b, d), st)
     call = _Call(be, gate, x, h, dh, h0, dh_last, lengths)
     (dgate, pp), (dx, qp), (dh0, d0p) = call.empty(code, b, t, d), call.empty(code, b, t, d), call.empty(st, b, d)
-    rows = _A3(1, d, t * d)
-    call.done(L.om_b200_gated_scan_backward(be.h, k, code, _A3(d, t, b), gp, _dtb(gs), xp, xs, hp, _dtb(hs), h0p, lp,
+    rows = _i64s(1, d, t * d)
+    call.done(L.om_b200_gated_scan_backward(be.h, k, code, _i64s(d, t, b), gp, _dtb(gs), xp, xs, hp, _dtb(hs), h0p, lp,
                                             ep, _dtb(es), elp, pp, rows, qp, rows, d0p))
     return dgate, dx, dh0
 
@@ -296,7 +307,7 @@ def _loss_args(be, x, w, targets, who):
         raise _invalid(f"{who}: x has width {d}, w {wd}")
     tc = _typed(be, targets, "targets", 1, (I32, I64))[1]
     tp = _vector(be, targets, "targets", (n,), tc)
-    return code, n, d, v, (_A3(d, n, v), xp, _cr(xs), wp, _cr(ws), tc, tp), F64 if code == F64 else F32
+    return code, n, d, v, (_i64s(d, n, v), xp, _cr(xs), wp, _cr(ws), tc, tp), F64 if code == F64 else F32
 
 
 def linear_cross_entropy(be, x, w, targets):
@@ -320,7 +331,7 @@ def linear_cross_entropy_backward(be, x, w, targets, lse, dloss):
     sp, gp = _vector(be, lse, "lse", (n,), st), _vector(be, dloss, "dloss", (n,), st)
     call = _Call(be, x, w, targets, lse, dloss)
     (dx, dp), (dw, ep) = call.empty(code, n, d), call.empty(code, v, d)
-    rows = _A2(1, d)
+    rows = _i64s(1, d)
     call.done(L.om_b200_linear_cross_entropy_backward(be.h, code, *args, sp, gp, dp, rows, ep, rows))
     return dx, dw
 
@@ -338,7 +349,7 @@ def quantize_rows(be, x):
     call = _Call(be, x)
     row = (k + 15) // 16 * 16
     (q, qp), (scale, sp) = call.empty(I8, m, row), call.empty(F32, m)
-    call.done(L.om_b200_quantize_rows(be.h, code, _A2(k, m), xp, _cr(xs), qp, _A2(1, row), sp))
+    call.done(L.om_b200_quantize_rows(be.h, code, _i64s(k, m), xp, _cr(xs), qp, _i64s(1, row), sp))
     if row != k:
         q = Strided(q.storage, (m, k), (row, 1)) if isinstance(q, Strided) else q[:, :k]
     return q, scale
@@ -375,7 +386,7 @@ def matmul_i8(be, q, q_scale, w, w_scale, bias=None, dtype="f32"):
     code = _code_of(dtype)
     call = _Call(be, q, q_scale, w, w_scale, bias)
     y, yp = call.empty(code, m, n)
-    call.done(L.om_b200_matmul_i8(be.h, code, _A3(k, m, n), qp, _cr(qs), sp, wp, ws, tp, bp, yp, _A2(1, n)))
+    call.done(L.om_b200_matmul_i8(be.h, code, _i64s(k, m, n), qp, _cr(qs), sp, wp, ws, tp, bp, yp, _i64s(1, n)))
     return y
 
 
@@ -387,5 +398,5 @@ def linear_i8(be, x, w, w_scale, bias=None):
     n, wp, ws, tp, bp = _weights(be, w, w_scale, bias, k)
     call = _Call(be, x, w, w_scale, bias)
     y, yp = call.empty(code, m, n)
-    call.done(L.om_b200_linear_i8(be.h, code, _A3(k, m, n), xp, _cr(xs), wp, ws, tp, bp, yp, _A2(1, n)))
+    call.done(L.om_b200_linear_i8(be.h, code, _i64s(k, m, n), xp, _cr(xs), wp, ws, tp, bp, yp, _i64s(1, n)))
     return y

@@ -325,6 +325,17 @@ def test_loss_gradient_of_any_size(be, seq, size):
         near(dw.to_numpy(), aw, ew)
 
 
+def test_loss_exact_f32(seq):
+    """f32 without the tensor cores (the mode of the library's products)."""
+    om = load_pkg()
+    be = om.B200(0)
+    be.set_f32_mode("exact")
+    for shape in [(70, 104, 333), (3, 5, 2), (130, 64, 20000)]:
+        x, w, targets, g = loss_inputs(17, *shape, "f32")
+        check_loss(be, seq, seq.upload(be, x, "f32"), seq.upload(be, w, "f32"), seq.upload(be, targets, "i64"), seq.upload(be, g), x, w, targets, g, "f32")
+    be.close()
+
+
 def test_loss_no_tokens(be, seq):
     for dtype in TYPES:
         st = np.float64 if dtype == "f64" else np.float32
@@ -452,8 +463,8 @@ def test_i8_empty(be, seq):
 def test_refusals_at_the_abi(be, seq):
     """What the front end cannot send: the C entries answer with a status."""
     L = seq._bind()
-    s3, s2 = seq._A3(4, 4, 4), seq._A2(4, 4)
-    neg = seq._A3(4, -1, 4)
+    s3, s2 = seq._i64s(4, 4, 4), seq._i64s(4, 4)
+    neg = seq._i64s(4, -1, 4)
     assert L.om_b200_gated_scan(be.h, 2, 0, s3, *[None] * 9) == 1
     assert L.om_b200_gated_scan(be.h, 0, 3, s3, *[None] * 9) == 2
     assert L.om_b200_gated_scan(be.h, 0, 0, neg, *[None] * 9) == 5
@@ -461,7 +472,7 @@ def test_refusals_at_the_abi(be, seq):
     assert L.om_b200_gated_scan_backward(be.h, 0, 0, s3, *[None] * 16) == 1
     assert L.om_b200_linear_cross_entropy(be.h, 7, s3, *[None] * 4, 9, *[None] * 3) == 2
     assert L.om_b200_linear_cross_entropy(be.h, 0, s3, *[None] * 4, 0, *[None] * 3) == 2
-    assert L.om_b200_linear_cross_entropy(be.h, 0, seq._A3(0, 4, 4), *[None] * 4, 9, *[None] * 3) == 5
+    assert L.om_b200_linear_cross_entropy(be.h, 0, seq._i64s(0, 4, 4), *[None] * 4, 9, *[None] * 3) == 5
     assert L.om_b200_linear_cross_entropy_backward(be.h, 0, s3, *[None] * 4, 9, *[None] * 7) == 1
     assert L.om_b200_quantize_rows(be.h, 1, s2, *[None] * 5) == 2
     assert L.om_b200_quantize_rows(be.h, 0, s2, *[None] * 5) == 1
@@ -469,7 +480,7 @@ def test_refusals_at_the_abi(be, seq):
     assert L.om_b200_matmul_i8(be.h, 0, s3, *[None] * 9) == 1
     assert L.om_b200_linear_i8(be.h, 0, neg, *[None] * 8) == 5
     a = be.alloc(16, np.float32)
-    one = seq._A2(16, 1)
+    one = seq._i64s(16, 1)
     assert L.om_b200_copy_strided(be.h, 5, a.ptr, 1, one, one, 0, a.ptr) == 2  # 16-bit types are not the engine's
 
 
