@@ -73,6 +73,24 @@ __device__ __forceinline__ void store_row(T* dst, const float (&v)[32], bool wid
   }
 }
 
+// A warp's 32 x 32 results, lane by row, where rows cannot be written 16 bytes
+// at a time: turned in shared memory (a word of padding per row), so that each
+// store writes 32 neighbours of one row. rows: how many of the warp's 32 exist.
+template <typename T>
+__device__ __forceinline__ void store_turned(float* turn, const float (&v)[32], T* first, int64_t dr,
+                                             int64_t dc, int rows, int cols) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) turn[lane * 33 + c] = v[c];
+  __syncwarp();
+  if (lane < cols) {
+    T* to = first + lane * dc;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r, to += dr) *to = Elem<T>::store(turn[r * 33 + lane]);
+  }
+  __syncwarp();
+}
+
 // How a row-major result may be written: 2 = sectors of 32 bytes, 1 = 16 bytes,
 // 0 = element by element
 inline int row_stores(const void* ptr, int64_t row, int64_t col, int elem) {

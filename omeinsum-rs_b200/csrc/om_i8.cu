@@ -99,39 +99,52 @@ __global__ void quantize_kernel(const T* __restrict__ x, int64_t K, int64_t xk, 
 
 // The same where a row is contiguous, 16-byte aligned and short enough for the
 // block's registers: it is read once, 8 elements per thread and turn.
-constexpr int TURNS = 4;
+constexpr int TURNS = 8, QUANT_THREADS = 128;
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_vec_kernel(const T* __restrict__ x, int K, int64_t xm,
-                                                           int8_t* __restrict__ q, int64_t qm,
-                                                           float* __restrict__ scale) {
+__device__ __forceinline__ void widen8(const uint4 (&raw)[sizeof(T) / 2], float (&v)[8]) {
+  __align__(16) T t[8];
+  memcpy(t, raw, sizeof(T) * 8);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = Elem<T>::load(t[i]);
+}
+template <typename T, int N>
+__global__ void __launch_bounds__(QUANT_THREADS) quantize_vec_kernel(const T* __restrict__ x, int K,
+                                                                     int64_t xm, int8_t* __restrict__ q,
+                                                                     int64_t qm, float* __restrict__ scale) {
   const int64_t row = blockIdx.x;
   const T* xr = x + row * xm;
-  float v[TURNS][8];
+  constexpr int W = sizeof(T) / 2;
+  uint4 raw[N][W];
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < TURNS; ++i) {
-    const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
-    if (k >= K) break;
-    load8(xr + k, v[i]);
+  for (int i = 0; i < N; ++i) {
+    const int k = (i * QUANT_THREADS + (int)threadIdx.x) * 8;
+#pragma unroll
+    for (int b = 0; b < W; ++b)
+      raw[i][b] = k < K ? __ldcs(reinterpret_cast<const uint4*>(xr + k) + b) : make_uint4(0, 0, 0, 0);
   }
 #pragma unroll
-  for (int i = 0; i < TURNS; ++i) {
-    if ((i * (int)blockDim.x + (int)threadIdx.x) * 8 >= K) break;
-    top = max_bits(top, v[i]);
+  for (int i = 0; i < N; ++i) {
+    float v[8];
+    widen8<T>(raw[i], v);
+    top = max_bits(top, v);
   }
-  __shared__ uint32_t part[8];
+  __shared__ uint32_t part[QUANT_THREADS / 32];
   top = __reduce_max_sync(0xffffffffu, top);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
   __syncthreads();
-  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) top = max(top, part[i]);
+#pragma unroll
+  for (int i = 0; i < QUANT_THREADS / 32; ++i) top = max(top, part[i]);
   const float s = __fdiv_rn(__uint_as_float(top), 127.f), inv = __fdiv_rn(1.f, s);
   const bool normal = normal_scale(s);
   if (threadIdx.x == 0) scale[row] = s;
 #pragma unroll
-  for (int i = 0; i < TURNS; ++i) {
-    const int k = (i * (int)blockDim.x + (int)threadIdx.x) * 8;
+  for (int i = 0; i < N; ++i) {
+    const int k = (i * QUANT_THREADS + (int)threadIdx.x) * 8;
     if (k >= K) break;
-    *reinterpret_cast<uint2*>(q + row * qm + k) = quantized8(v[i], s, inv, normal);
+    float v[8];
+    widen8<T>(raw[i], v);
+    *reinterpret_cast<uint2*>(q + row * qm + k) = quantized8(v, s, inv, normal);
   }
 }
 
@@ -157,19 +170,20 @@ struct ScaleEpi {
   const float *q_scale, *w_scale, *bias;
   T* y;
   int64_t dr, dc;
-  int vec;  // row_stores of y, where w_scale and bias can be read 16 bytes at a time
+  int vec;   // row_stores of y
+  int wide;  // w_scale and bias can be read 16 bytes at a time
   struct Row {
     float s;
   };
+  bool turns() const { return !vec; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     return Row{in ? q_scale[m] : 0.f};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32]) const {
-    if (!in || n0 >= N) return;
-    T* to = y + (int64_t)m * dr;
-    if (vec && N - n0 >= 32) {
-      float v[32];
+                                          const uint32_t (&r)[32], float* turn) const {
+    if (n0 >= N) return;
+    float v[32];
+    if (wide && N - n0 >= 32) {
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 w = __ldg(reinterpret_cast<const float4*>(w_scale + n0 + c));
@@ -177,34 +191,70 @@ struct ScaleEpi {
         v[c + 1] = scaled((int)r[c + 1], row.s, w.y);
         v[c + 2] = scaled((int)r[c + 2], row.s, w.z);
         v[c + 3] = scaled((int)r[c + 3], row.s, w.w);
-        if (bias) {
+      }
+      if (bias) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
           const float4 b = __ldg(reinterpret_cast<const float4*>(bias + n0 + c));
           v[c] = __fadd_rn(v[c], b.x), v[c + 1] = __fadd_rn(v[c + 1], b.y);
           v[c + 2] = __fadd_rn(v[c + 2], b.z), v[c + 3] = __fadd_rn(v[c + 3], b.w);
         }
       }
-      store_row(to + n0, v, vec == 2);
     } else {
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (n0 + c < N) {
-          float v = scaled((int)r[c], row.s, w_scale[n0 + c]);
-          if (bias) v = __fadd_rn(v, bias[n0 + c]);
-          to[(n0 + c) * dc] = Elem<T>::store(v);
-        }
+      for (int c = 0; c < 32; ++c) {
+        if (n0 + c >= N) break;
+        v[c] = scaled((int)r[c], row.s, w_scale[n0 + c]);
+        if (bias) v[c] = __fadd_rn(v[c], bias[n0 + c]);
+      }
+    }
+    const int lane = threadIdx.x & 31;
+    T* to = y + (int64_t)m * dr;
+    if (!vec) {
+      store_turned(turn, v, y + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
+                   __popc(__ballot_sync(0xffffffffu, in)), N - n0);
+    } else if (in) {
+      if (N - n0 >= 32) {
+        store_row(to + n0, v, vec == 2);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c)
+          if (n0 + c < N) to[n0 + c] = Elem<T>::store(v[c]);
+      }
     }
   }
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
 
-// Rows of 8-bit numbers at 16-byte aligned places, zero behind their end
-__global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int64_t K, int64_t sr,
-                        int64_t sk, int8_t* __restrict__ dst, int64_t ld) {
-  const int64_t total = rows * ld;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ld, c = i - r * ld;
-    dst[i] = c < K ? src[r * sr + c * sk] : (int8_t)0;
+// Rows of 8-bit numbers at 16-byte aligned places, zero behind their end. A
+// thread makes 16: contiguous ones from the aligned words that hold them, shifted
+// into place; others one by one.
+__global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int K, int64_t sr, int64_t sk,
+                        int8_t* __restrict__ dst, int64_t ld) {
+  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int c = (blockIdx.x * blockDim.x + threadIdx.x) * 16; c < ld; c += gridDim.x * blockDim.x * 16) {
+      __align__(16) uint32_t o[4] = {0, 0, 0, 0};
+      const int n = min(16, K - c);
+      if (sk == 1) {
+        const uintptr_t at = (uintptr_t)(src + r * sr + c);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+        const int off = (int)(at & 3), shift = off * 8;
+        uint32_t v[5];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) v[i] = i * 4 < n + off ? __ldg(w + i) : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = __funnelshift_r(v[i], v[i + 1], shift);
+          const int keep = n - 4 * i;  // bytes of this word inside the row
+          if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & ((1u << (8 * keep)) - 1u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < n) o[i / 4] |= (uint32_t)(uint8_t)src[r * sr + (int64_t)(c + i) * sk] << (8 * (i % 4));
+      }
+      *reinterpret_cast<uint4*>(dst + r * ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
 }
 
@@ -350,10 +400,13 @@ template <typename T>
 int launch_quantize(om_backend* be, int64_t K, int64_t M, const void* x, const int64_t* sx, void* q,
                     int64_t qk, int64_t qm, float* scale) {
   ProfScope prof(be, "quantize_rows");
-  if (sx[0] == 1 && qk == 1 && K % 8 == 0 && K <= 256 * 8 * TURNS && !((uintptr_t)x & 15) &&
+  if (sx[0] == 1 && qk == 1 && K % 8 == 0 && K <= QUANT_THREADS * 8 * TURNS && !((uintptr_t)x & 15) &&
       sx[1] * (int64_t)sizeof(T) % 16 == 0 && !((uintptr_t)q & 7) && qm % 8 == 0) {
-    const int threads = (int)std::min<int64_t>(256, (K / 8 + 31) / 32 * 32);
-    quantize_vec_kernel<T><<<(unsigned)M, threads, 0, be->stream>>>((const T*)x, (int)K, sx[1], (int8_t*)q, qm, scale);
+    // as many turns as the row needs, so that short rows take few registers
+    auto kernel = K <= QUANT_THREADS * 8 ? quantize_vec_kernel<T, 1>
+                  : K <= QUANT_THREADS * 16 ? quantize_vec_kernel<T, 2>
+                  : K <= QUANT_THREADS * 32 ? quantize_vec_kernel<T, 4> : quantize_vec_kernel<T, TURNS>;
+    kernel<<<(unsigned)M, QUANT_THREADS, 0, be->stream>>>((const T*)x, (int)K, sx[1], (int8_t*)q, qm, scale);
     note_launch();
     return check_cuda(cudaGetLastError(), "quantize_rows launch");
   }
@@ -378,9 +431,10 @@ int readable_i8(om_backend* be, const int8_t* src, int64_t rows, int64_t K, int6
   if ((sk == 1 || K == 1) && sr >= K && mma::tma_readable(src, sr, 1)) return OM_OK;
   const int64_t ld = (K + 15) / 16 * 16;
   OM_TRY(copy.alloc(be, (size_t)rows * ld));
-  const int64_t n = rows * ld;
-  pack_i8<<<(unsigned)std::min<int64_t>((n + 255) / 256, (int64_t)be->num_sms * 32), 256, 0,
-            be->stream>>>(src, rows, K, sr, sk, (int8_t*)copy.ptr, ld);
+  const int threads = (int)std::min<int64_t>(128, (ld / 16 + 31) / 32 * 32);
+  const dim3 grid((unsigned)((ld / 16 + threads - 1) / threads), (unsigned)std::min<int64_t>(rows, 65535));
+  ProfScope prof(be, "pack_i8");
+  pack_i8<<<grid, threads, 0, be->stream>>>(src, rows, (int)K, sr, sk, (int8_t*)copy.ptr, ld);
   note_launch();
   *out = mma::Matrix{copy.ptr, rows, K, ld, 1};
   return check_cuda(cudaGetLastError(), "matmul_i8 pack launch");
@@ -428,8 +482,9 @@ int launch_matmul(om_backend* be, const I8Args& p) {
   mma::Matrix q, w;
   OM_TRY(readable_i8(be, p.q, p.M, p.K, p.qm, p.qk, qc, &q));
   OM_TRY(readable_i8(be, p.w, p.N, p.K, p.wn, p.wk, wc, &w));
-  const int vec = ((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15 ? 0 : row_stores(p.y, p.ym, p.yn, sizeof(T));
-  const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn, vec};
+  const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn,
+                        row_stores(p.y, p.ym, p.yn, sizeof(T)),
+                        !(((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15)};
   const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
   if (t.pair) return mma::launch_product<true, false, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
   return mma::launch_product<true, false, false, false, 1>(be, "matmul_i8", q, w, false, t.bn, 1, epi);

@@ -252,11 +252,12 @@ struct StatsEpi {
     float m, s;
     int64_t target;
   };
+  bool turns() const { return false; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     return Row{-INFINITY, 0.f, in ? target_of(targets, t64, m) - v0 : -1};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32]) const {
+                                          const uint32_t (&r)[32], float* turn) const {
     if (n0 >= N) return;
     const int n = N - n0;  // columns that exist
     float top = __uint_as_float(r[0]);
@@ -309,10 +310,18 @@ __global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ par
   const int64_t row = blockIdx.x * (int64_t)8 + r;
   float m = -INFINITY, s = 0.f;
   if (row < rows) {
-#pragma unroll 4
-    for (int i = k; i < slots; i += 32) {
-      const float2 v = part[(int64_t)i * rows + row];
-      merge(m, s, v.x, v.y);
+    // eight slots at a time: one maximum, then their sums
+    for (int i = k; i < slots; i += 256) {
+      float2 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        v[u] = i + 32 * u < slots ? part[(int64_t)(i + 32 * u) * rows + row] : make_float2(-INFINITY, 0.f);
+      float top = v[0].x, sum = 0.f;
+#pragma unroll
+      for (int u = 1; u < 8; ++u) top = fmaxf(top, v[u].x);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += v[u].y == 0.f ? 0.f : v[u].y * exp2_fast((v[u].x - top) * LOG2E);
+      merge(m, s, top, sum);
     }
   }
   sm[k][r] = m;
@@ -323,9 +332,13 @@ __global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ par
   const int64_t mine = blockIdx.x * (int64_t)8 + w;
   m = sm[lane][w];
   s = ss[lane][w];
+  float top = m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1)
-    merge(m, s, __shfl_down_sync(0xffffffffu, m, o), __shfl_down_sync(0xffffffffu, s, o));
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  s = s == 0.f ? 0.f : s * exp2_fast((m - top) * LOG2E);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  m = top;
   if (lane || mine >= rows) return;
   const float total = m + logf(s);
   const int64_t t = target_of(targets, t64, mine);
@@ -372,6 +385,7 @@ struct GradEpi {
     float lse, g;
     int64_t target;  // within the piece
   };
+  bool turns() const { return false; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     Row row{0.f, 0.f, -1};
     if (in) {
@@ -387,7 +401,7 @@ struct GradEpi {
     return row;
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32]) const {
+                                          const uint32_t (&r)[32], float* turn) const {
     if (!in) return;
     float v[32];
 #pragma unroll
@@ -428,17 +442,18 @@ struct OutEpi {
     float f;
     float* acc;
   };
+  bool turns() const { return !vec && !keep; }
   __device__ __forceinline__ Row begin(int m, bool in, int split) const {
     return Row{scale ? *scale : 1.f,
                acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32]) const {
-    if (!in || n0 >= N) return;
+                                          const uint32_t (&r)[32], float* turn) const {
+    if (n0 >= N) return;
     float v[32];
 #pragma unroll
     for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(r[c]);
-    if (load) {
+    if (load && in) {
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 a = *reinterpret_cast<const float4*>(row.acc + n0 + c);
@@ -446,18 +461,24 @@ struct OutEpi {
       }
     }
     if (keep) {
-      store_row(row.acc + n0, v, true);  // (whole tiles: 256-byte rows)
+      if (in) store_row(row.acc + n0, v, true);  // (whole tiles: 256-byte rows)
       return;
     }
 #pragma unroll
     for (int c = 0; c < 32; ++c) v[c] *= row.f;
+    const int lane = threadIdx.x & 31;
     T* to = out + (int64_t)m * dr;
-    if (vec && N - n0 >= 32) {
-      store_row(to + n0, v, vec == 2);
-    } else {
+    if (!vec) {
+      store_turned(turn, v, out + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
+                   __popc(__ballot_sync(0xffffffffu, in)), N - n0);
+    } else if (in) {
+      if (N - n0 >= 32) {
+        store_row(to + n0, v, vec == 2);
+      } else {
 #pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (n0 + c < N) to[(n0 + c) * dc] = Elem<T>::store(v[c]);
+        for (int c = 0; c < 32; ++c)
+          if (n0 + c < N) to[n0 + c] = Elem<T>::store(v[c]);
+      }
     }
   }
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
@@ -671,14 +692,19 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
                                                std::is_same<T, __half>::value ? 16384.f : 1.f, scale);
     note_launch();
   }
-  // dx sums over the vocabulary: few tokens and a narrow width leave SMs idle
-  // unless the sum is split; each split needs 8 slabs to be worth its f32 sums
-  const mma::Tiling tx = tiles<T>(be, p.N, p.D);
+  // dx sums over the vocabulary. Its tiles are the widest that there are, and
+  // where they leave SMs idle the sum is split, 16 slabs of 64 entries at least
+  // to a split, which is worth its f32 sums (509 x 771 x 8191 f32: 80 us with
+  // narrow tiles in two splits)
+  const int most = PLANES == 3 ? 128 : 256;
+  mma::Tiling tx{(int)std::min<int64_t>(most, std::max<int64_t>(64, (p.D + 63) / 64 * 64)), p.N > 128};
+  while (tx.bn & (tx.bn - 1)) tx.bn += 64;  // 64, 128 or 256
+  if (tx.bn < 128) tx.pair = 0;
   const int64_t rows = tx.pair ? 256 : 128;
   const int64_t txt = (p.N + rows - 1) / rows * ((p.D + tx.bn - 1) / tx.bn);
   const int64_t slots = tx.pair ? be->num_sms / 2 : be->num_sms;
   const int64_t least = (std::min(P, p.V) + 63) / 64;
-  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / txt, least / 8, 64}));
+  const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / txt, least / 16, 64}));
   const int64_t acc_ld = (p.D + tx.bn - 1) / tx.bn * tx.bn;
   const bool sums = splits > 1 || P < p.V;
   if (sums) OM_TRY(accs.alloc(be, (size_t)splits * p.N * acc_ld * 4));

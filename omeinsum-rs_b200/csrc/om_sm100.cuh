@@ -50,12 +50,15 @@ constexpr int SLAB = 128;           // bytes of k per stage
 constexpr int CHUNK = 2;            // slabs of a sum (P3)
 constexpr int A_BYTES = TM * SLAB;
 constexpr uint32_t WAIT_LIMIT = 1u << 24;
+constexpr int TURN_BYTES = 32 * 33 * 4;  // 32 rows of 32 values, a word apart
 
 struct Shape {
   int M, N;        // rows of A and of B
   int slabs;       // of 128 bytes along k, all splits together
   int BN;          // columns of a tile: 32 .. 256
   int stages;
+  int a_rows;      // rows of A's box: 128, or fewer where all of A has fewer
+  int turn;        // bytes of shared memory for turning a warp's results, or 0
   int tiles_m, tiles_n, splits;
   int group;       // row tiles that are walked before the next column tile
   uint32_t idesc;  // instruction descriptor
@@ -70,7 +73,7 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
   for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
     uint32_t done;
     asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         "selp.u32 %0, 1, 0, p;\n}\n"
         : "=r"(done)
         : "r"(bar), "r"(parity)
@@ -203,9 +206,10 @@ __device__ __forceinline__ Tile tile_at(const Shape& g, int t) {
 }
 
 // Epi, per lane and tile: Row begin(m, in, split) before the accumulator is
-// read; columns(row, m, in, n0, N, values) for each 32 columns from n0 on; and
-// end(row, m, in, slot) with slot = 2 * column tile + column group. `in`: row m
-// exists; columns from N on do not.
+// read; columns(row, m, in, n0, N, values, turn) for each 32 columns from n0 on,
+// by whole warps; and end(row, m, in, slot) with slot = 2 * column tile + column
+// group. `in`: row m exists; columns from N on do not. `turn`: shared memory of
+// the warp's own, if turns() asked for it.
 template <bool I8, bool P3, bool AMN, bool BMN, int CG, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
@@ -225,6 +229,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr int PLANES = P3 ? 3 : 1;
   const uint32_t b_bytes = b_rows * SLAB;
   const uint32_t stage_bytes = PLANES * (A_BYTES + b_bytes);
+  const uint32_t loaded = PLANES * ((AMN ? TM : g.a_rows) * SLAB + b_bytes);
   const int kstep = I8 ? 128 : 64;  // elements of a slab
 
   if (warp == 1) {
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint32_t bar = smem_addr(&full[s]);
           if (CG == 1 || rank == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
-                         "r"(stage_bytes * CG)
+                         "r"(loaded * CG)
                          : "memory");
           if constexpr (CG == 2) bar = in_rank(bar, 0);
           const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
@@ -363,6 +368,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else {  // epilogue
     const int quad = warp & 3, part = (warp - 2) >> 2;
+    // this warp's place for turning results (where the launch has one)
+    float* turn = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) +
+                                           (size_t)g.stages * stage_bytes + (warp - 2) * TURN_BYTES);
     int i = 0;
     auto release = [&](int ab) {  // the accumulator has been read
       asm volatile("tcgen05.fence::before_thread_sync;");
@@ -410,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint32_t r[32];
 #pragma unroll
           for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(sum[j][q]);
-          epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, turn);
         }
       } else {
         ok = wait(smem_addr(&tfull[i & 1]), (i >> 1) & 1);
@@ -419,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int c = part * 32; c < g.BN; c += 64) {
           uint32_t r[32];
           read_columns(base + (i & 1) * 256 + c, r);
-          epi.columns(row, m, in, at.n * g.BN + c, g.N, r);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, turn);
         }
         release(i & 1);
         ++i;
@@ -507,7 +515,10 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
       splits > slabs || tm * tn * splits > 0x7fffffff)
     return set_error(OM_ERR_SHAPE, std::string(name) + ": extents out of range");
   CUtensorMap ma, mb;
-  OM_TRY(encode(&ma, a, AMN, TM));
+  // rows that A does not have need no copies of zeros: what an accumulator's
+  // other rows hold is never stored
+  const int a_rows = a.rows < TM && CG == 1 ? (int)((a.rows + 7) / 8 * 8) : TM;
+  OM_TRY(encode(&ma, a, AMN, a_rows));
   OM_TRY(encode(&mb, b, BMN, bn / CG));
   Shape g{};
   g.M = (int)a.rows, g.N = (int)b.rows, g.slabs = (int)slabs, g.BN = bn;
@@ -516,10 +527,12 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
   // read by many SMs while it is in L2
   g.group = std::max(1, std::min<int>((int)tm, CG == 2 ? 8 : 16));
   const int stage = (P3 ? 3 : 1) * (A_BYTES + bn / CG * SLAB);
-  g.stages = std::min(MAX_STAGES, 216 * 1024 / stage);
+  g.a_rows = a_rows;
+  g.turn = epi.turns() ? 8 * TURN_BYTES : 0;
+  g.stages = std::min(MAX_STAGES, (216 * 1024 - g.turn) / stage);
   g.idesc = instruction(I8, bf16, AMN, BMN, TM * CG, bn);
   g.err = be->d_flags + 1;
-  const size_t smem = (size_t)g.stages * stage + 1024;
+  const size_t smem = (size_t)g.stages * stage + g.turn + 1024;
   auto kernel = product_kernel<I8, P3, AMN, BMN, CG, Epi>;
   OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), name);
   const int64_t work = tm * tn * splits;
