@@ -132,15 +132,14 @@ def _operand(be, t, name):
             raise _invalid(f"{name}: on device {s.backend.device}, the backend on {be.device}")
         return (s.ptr or 0) + t.offset * s.dtype.itemsize, DTYPES[s.dtype], t.shape, t.strides
     try:
-        device = t.get_device()
+        if t.get_device() != be.device:  # -1: not on a device at all
+            raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
+        return t.data_ptr(), _torch_codes[t.dtype], t.shape, t.stride()
+    except KeyError:
+        _learn_torch(t.dtype, name)
+        return _operand(be, t, name)
     except AttributeError:
         raise _invalid(f"{name}: a Strided view or a torch CUDA tensor is needed, not {type(t).__name__}") from None
-    if device != be.device:  # -1: not on a device at all
-        raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
-    code = _torch_codes.get(t.dtype)
-    if code is None:
-        code = _learn_torch(t.dtype, name)
-    return t.data_ptr(), code, t.shape, t.stride()
 
 
 def _typed(be, t, name, ndim, codes):
@@ -166,7 +165,9 @@ def _vector(be, t, name, shape, code):
     if t is None:
         return None
     ptr, _, shape, strides = _like(be, t, name, shape, code)
-    if len(shape) == 1 and (strides[0] == 1 or shape[0] == 1):
+    if type(t) is not Strided:
+        if not t.is_contiguous():
+            raise _invalid(f"{name}: must be contiguous")
         return ptr
     s = 1
     for n, st in zip(reversed(shape), reversed(strides)):
@@ -196,12 +197,14 @@ class _Call:
             self.mine = _torch.cuda.ExternalStream(be.home_stream, device=like.device)
             self.mine.wait_stream(self.cur)
 
-    def empty(self, code, *shape):
-        """(a new row-major tensor, its pointer)"""
-        if self.like is not None:
-            like = self.like
-            if like.dtype is _torch_types[code]:
-                t = like.new_empty(shape)
+    def empty(self, code, shape, same=None):
+        """(a new row-major tensor, its pointer); `same`: a tensor of that shape
+        and type, if there is one, whose layout can be taken over when it is
+        row-major too."""
+        like = self.like
+        if like is not None:
+            if same is not None and same.is_contiguous():
+                t = _torch.empty_like(same)
             else:
                 t = _torch.empty(shape, dtype=_torch_types[code], device=like.device)
             return t, t.data_ptr()
@@ -209,6 +212,14 @@ class _Call:
         for s in shape:
             n *= s
         t = Strided(self.be.alloc(n, _NP[code]), shape)
+        return t, t.storage.ptr
+
+    def rows(self, code, m, k, row):
+        """The same of m rows of k elements, `row` apart."""
+        if self.like is not None:
+            t = _torch.empty_strided((m, k), (row, 1), dtype=_torch_types[code], device=self.like.device)
+            return t, t.data_ptr()
+        t = Strided(self.be.alloc(m * row, _NP[code]), (m, k), (row, 1))
         return t, t.storage.ptr
 
     def done(self, rc):
@@ -263,9 +274,9 @@ def gated_scan(be, gate, x, h0=None, lengths=None, kind="linear", h_last=None):
     h0p = _vector(be, h0, "h0", (b, d), st)
     lp = _vector(be, lengths, "lengths", (b,), I32)
     call = _Call(be, gate, x, h0, lengths, h_last)
-    h, hp = call.empty(code, b, t, d)
+    h, hp = call.empty(code, shape, gate)
     if h_last is None:
-        h_last, lastp = call.empty(st, b, d)
+        h_last, lastp = call.empty(st, (b, d), h0)
     else:
         lastp = _vector(be, h_last, "h_last", (b, d), st)
     call.done(L.om_b200_gated_scan(be.h, k, code, _i64s(d, t, b), gp, _dtb(gs), xp, _dtb(xs), h0p, lp, hp,
@@ -293,7 +304,7 @@ def gated_scan_backward(be, gate, x, h, dh, h0=None, dh_last=None, lengths=None,
     lp = _vector(be, lengths, "lengths", (b,), I32)
     elp = _vector(be, dh_last, "dh_last", (b, d), st)
     call = _Call(be, gate, x, h, dh, h0, dh_last, lengths)
-    (dgate, pp), (dx, qp), (dh0, d0p) = call.empty(code, b, t, d), call.empty(code, b, t, d), call.empty(st, b, d)
+    (dgate, pp), (dx, qp), (dh0, d0p) = call.empty(code, shape, gate), call.empty(code, shape, dh), call.empty(st, (b, d), h0)
     rows = _i64s(1, d, t * d)
     call.done(L.om_b200_gated_scan_backward(be.h, k, code, _i64s(d, t, b), gp, _dtb(gs), xp, xs, hp, _dtb(hs), h0p, lp,
                                             ep, _dtb(es), elp, pp, rows, qp, rows, d0p))
@@ -318,7 +329,8 @@ def linear_cross_entropy(be, x, w, targets):
     L = _bind()
     code, n, _, _, args, st = _loss_args(be, x, w, targets, "linear_cross_entropy")
     call = _Call(be, x, w, targets)
-    (loss, lp), (lse, sp) = call.empty(st, n), call.empty(st, n)
+    loss, lp = call.empty(st, (n,))
+    lse, sp = call.empty(st, (n,), loss)
     call.done(L.om_b200_linear_cross_entropy(be.h, code, *args, lp, sp))
     return loss, lse
 
@@ -330,7 +342,7 @@ def linear_cross_entropy_backward(be, x, w, targets, lse, dloss):
     code, n, d, v, args, st = _loss_args(be, x, w, targets, "linear_cross_entropy_backward")
     sp, gp = _vector(be, lse, "lse", (n,), st), _vector(be, dloss, "dloss", (n,), st)
     call = _Call(be, x, w, targets, lse, dloss)
-    (dx, dp), (dw, ep) = call.empty(code, n, d), call.empty(code, v, d)
+    (dx, dp), (dw, ep) = call.empty(code, (n, d), x), call.empty(code, (v, d), w)
     rows = _i64s(1, d)
     call.done(L.om_b200_linear_cross_entropy_backward(be.h, code, *args, sp, gp, dp, rows, ep, rows))
     return dx, dw
@@ -348,10 +360,8 @@ def quantize_rows(be, x):
     xp, code, (m, k), xs = _typed(be, x, "x", 2, _QUANTISED)
     call = _Call(be, x)
     row = (k + 15) // 16 * 16
-    (q, qp), (scale, sp) = call.empty(I8, m, row), call.empty(F32, m)
+    (q, qp), (scale, sp) = call.rows(I8, m, k, row), call.empty(F32, (m,))
     call.done(L.om_b200_quantize_rows(be.h, code, _i64s(k, m), xp, _cr(xs), qp, _i64s(1, row), sp))
-    if row != k:
-        q = Strided(q.storage, (m, k), (row, 1)) if isinstance(q, Strided) else q[:, :k]
     return q, scale
 
 
@@ -385,7 +395,7 @@ def matmul_i8(be, q, q_scale, w, w_scale, bias=None, dtype="f32"):
         raise _invalid("q_scale is needed")
     code = _code_of(dtype)
     call = _Call(be, q, q_scale, w, w_scale, bias)
-    y, yp = call.empty(code, m, n)
+    y, yp = call.empty(code, (m, n))
     call.done(L.om_b200_matmul_i8(be.h, code, _i64s(k, m, n), qp, _cr(qs), sp, wp, ws, tp, bp, yp, _i64s(1, n)))
     return y
 
@@ -397,6 +407,6 @@ def linear_i8(be, x, w, w_scale, bias=None):
     xp, code, (m, k), xs = _typed(be, x, "x", 2, _QUANTISED)
     n, wp, ws, tp, bp = _weights(be, w, w_scale, bias, k)
     call = _Call(be, x, w, w_scale, bias)
-    y, yp = call.empty(code, m, n)
+    y, yp = call.empty(code, (m, n))
     call.done(L.om_b200_linear_i8(be.h, code, _i64s(k, m, n), xp, _cr(xs), wp, ws, tp, bp, yp, _i64s(1, n)))
     return y
