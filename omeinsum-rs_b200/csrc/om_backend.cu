@@ -206,6 +206,17 @@ void be_free(om_backend* be, uint64_t id, void* p) {
   cudaFreeAsync(p, be->stream);
 }
 
+int allow_shared(om_backend* be, const void* kernel, int bytes, const char* what) {
+  static std::mutex& mu = *new std::mutex;
+  static auto& allowed = *new std::map<std::pair<int, const void*>, int>;
+  std::lock_guard<std::mutex> lk(mu);
+  int& had = allowed[{be->device, kernel}];
+  if (bytes <= had) return OM_OK;
+  OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+  had = bytes;
+  return OM_OK;
+}
+
 }  // namespace om
 
 using namespace om;

@@ -445,9 +445,7 @@ int launch_token_rows(om_backend* be, const I8Args& p, const T* x, int64_t xk, i
                       int64_t Kp) {
   const size_t smem = (size_t)p.M * Kp;
   if (smem > 48 * 1024)
-    OM_CUDA(cudaFuncSetAttribute(token_i8_kernel<T, MM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 TOKEN_SMEM),
-            "matmul_i8");
+    OM_TRY(allow_shared(be, (const void*)token_i8_kernel<T, MM>, TOKEN_SMEM, "matmul_i8"));
   const int64_t blocks = std::min<int64_t>((p.N + 7) / 8, (int64_t)be->num_sms * 2);
   ProfScope prof(be, "matmul_i8_token");
   const int vec = x && xk == 1 && p.K % 8 == 0 && !((uintptr_t)x & 15) && xm * (int64_t)sizeof(T) % 16 == 0;
@@ -486,8 +484,7 @@ int launch_matmul(om_backend* be, const I8Args& p) {
                         row_stores(p.y, p.ym, p.yn, sizeof(T)),
                         !(((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15)};
   const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
-  if (t.pair) return mma::launch_product<true, false, false, false, 2>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
-  return mma::launch_product<true, false, false, false, 1>(be, "matmul_i8", q, w, false, t.bn, 1, epi);
+  return mma::launch_product<true, false, false, false>(be, "matmul_i8", q, w, false, t, 1, epi);
 }
 
 int matmul(om_backend* be, om_dtype dtype, const I8Args& p) {

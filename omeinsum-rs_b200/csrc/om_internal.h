@@ -140,6 +140,10 @@ struct Scratch {
   int alloc(om_backend* b, size_t bytes);
 };
 
+// Lets a kernel have `bytes` of dynamic shared memory on the backend's device;
+// asks the driver only when it has not been allowed as much before.
+int allow_shared(om_backend* be, const void* kernel, int bytes, const char* what);
+
 // ---- kernels' host launchers ----------------------------------------------
 // Strided gather of an n-d view into a contiguous column-major buffer.
 // dst axis d has extent shape[d] and source stride strides[d].

@@ -609,8 +609,7 @@ template <typename T, bool AMN, bool BMN, class Epi>
 int product(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
             mma::Tiling t, int splits, const Epi& epi) {
   constexpr bool P3 = sizeof(T) == 4, BF = !std::is_same<T, __half>::value;
-  if (t.pair) return mma::launch_product<false, P3, AMN, BMN, 2>(be, name, a, b, BF, t.bn, splits, epi);
-  return mma::launch_product<false, P3, AMN, BMN, 1>(be, name, a, b, BF, t.bn, splits, epi);
+  return mma::launch_product<false, P3, AMN, BMN>(be, name, a, b, BF, t, splits, epi);
 }
 template <typename T>
 mma::Tiling tiles(const om_backend* be, int64_t M, int64_t N) {
@@ -697,9 +696,8 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
   // to a split, which is worth its f32 sums (509 x 771 x 8191 f32: 80 us with
   // narrow tiles in two splits)
   const int most = PLANES == 3 ? 128 : 256;
-  mma::Tiling tx{(int)std::min<int64_t>(most, std::max<int64_t>(64, (p.D + 63) / 64 * 64)), p.N > 128};
-  while (tx.bn & (tx.bn - 1)) tx.bn += 64;  // 64, 128 or 256
-  if (tx.bn < 128) tx.pair = 0;
+  mma::Tiling tx{p.D > 128 ? most : p.D > 64 ? 128 : 64, 0};
+  tx.pair = p.N > 128 && tx.bn >= 128;
   const int64_t rows = tx.pair ? 256 : 128;
   const int64_t txt = (p.N + rows - 1) / rows * ((p.D + tx.bn - 1) / tx.bn);
   const int64_t slots = tx.pair ? be->num_sms / 2 : be->num_sms;

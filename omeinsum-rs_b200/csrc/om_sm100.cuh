@@ -127,14 +127,32 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// 128-byte swizzled operand. K-major: 8-row groups 1024 bytes apart.
-// MN-major: 64 rows x 8 k take 1024 bytes, the next 8 k follow, the next 64
-// rows lie 64 k further (8192 bytes).
+// 128-byte swizzled operand at a shared-memory address. K-major: 8-row groups
+// 1024 bytes apart, the next MMA's k 32 bytes on. MN-major: 64 rows x 8 k take
+// 1024 bytes, the next 8 k follow, the next 64 rows lie 64 k further (8192
+// bytes); the next MMA's k is 2048 bytes on. Addresses are below 2^18, so moving
+// on is an addition to the low word.
 template <bool MN>
 __device__ __forceinline__ uint64_t operand(uint32_t addr) {
-  const uint64_t lead = MN ? 8192 >> 4 : 1, stride = 1024 >> 4;
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (lead << 16) | (stride << 32) | (1ull << 46) |
-         (2ull << 61);
+  constexpr uint32_t lead = MN ? 8192 >> 4 : 1, high = (1024 >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)high << 32) | ((lead << 16) + (addr >> 4));
+}
+template <bool MN>
+__device__ __forceinline__ uint64_t next_k(uint64_t op, int j) {
+  return op + (uint64_t)(j * (MN ? 2048 >> 4 : 32 >> 4));
+}
+
+// One lane of a converged warp. Loads and MMAs are issued by loops that the
+// whole warp runs, so that their operands are computed once in the uniform
+// registers that the instructions take them from: a loop of one lane's moves
+// them there one by one, 190 cycles per MMA of 128.
+__device__ __forceinline__ bool elected() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait(bar, parity));
 }
 
 template <bool I8, int CG>
@@ -220,7 +238,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   __shared__ __align__(8) uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
   __shared__ uint32_t tmem_base;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   uint32_t rank = 0;
   if constexpr (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
   const int first = blockIdx.x / CG, step = gridDim.x / CG;
@@ -259,28 +278,28 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if constexpr (CG == 2) cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;");
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
   bool ok = true;
 
-  if (warp == 0) {
-    if (lane == 0) {  // loads
-      int q = 0, s = 0;
-      uint32_t phase = 1;  // of empty[s]: passes at once on the first round
-      for (int t = first; t < tiles && ok; t += step) {
-        const Tile at = tile_at(g, t);
-        const int m0 = (at.m * CG + (int)rank) * TM;
-        const int n0 = at.n * g.BN + (int)rank * b_rows;
-        const int k1 = slab_at(g, at.split + 1);
-        for (int k = slab_at(g, at.split); k < k1; ++k, ++q) {
-          if (q >= g.stages) ok = wait(smem_addr(&empty[s]), phase);
-          if (!ok) break;
-          uint32_t bar = smem_addr(&full[s]);
+  if (warp == 0) {  // loads
+    int q = 0, s = 0;
+    uint32_t phase = 1;  // of empty[s]: passes at once on the first round
+    for (int t = first; t < tiles && ok; t += step) {
+      const Tile at = tile_at(g, t);
+      const int m0 = (at.m * CG + (int)rank) * TM;
+      const int n0 = at.n * g.BN + (int)rank * b_rows;
+      const int k1 = slab_at(g, at.split + 1);
+      for (int k = slab_at(g, at.split); k < k1; ++k, ++q) {
+        if (q >= g.stages) ok = wait_all(smem_addr(&empty[s]), phase);
+        if (!ok) break;
+        uint32_t bar = smem_addr(&full[s]);
+        const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
+        if (elected()) {
           if (CG == 1 || rank == 0)
             asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
                          "r"(loaded * CG)
                          : "memory");
           if constexpr (CG == 2) bar = in_rank(bar, 0);
-          const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
           if constexpr (P3) {
             for (int z = 0; z < 3; ++z) {
               if constexpr (AMN) {
@@ -296,76 +315,79 @@ __global__ void __launch_bounds__(THREADS, 1)
                 load_box3(b + z * b_bytes, &bmap, k * kstep, n0, z, bar, CG);
               }
             }
-            if (++s == g.stages) s = 0, phase ^= 1;
-            continue;
-          }
-          if constexpr (AMN) {
-            for (int i = 0; i < TM; i += 64) load_box<CG>(a + i * SLAB, &amap, m0 + i, k * kstep, bar);
           } else {
-            load_box<CG>(a, &amap, k * kstep, m0, bar);
+            if constexpr (AMN) {
+              for (int i = 0; i < TM; i += 64) load_box<CG>(a + i * SLAB, &amap, m0 + i, k * kstep, bar);
+            } else {
+              load_box<CG>(a, &amap, k * kstep, m0, bar);
+            }
+            if constexpr (BMN) {
+              for (int i = 0; i < b_rows; i += 64)
+                load_box<CG>(b + i * SLAB, &bmap, n0 + i, k * kstep, bar);
+            } else {
+              load_box<CG>(b, &bmap, k * kstep, n0, bar);
+            }
           }
-          if constexpr (BMN) {
-            for (int i = 0; i < b_rows; i += 64)
-              load_box<CG>(b + i * SLAB, &bmap, n0 + i, k * kstep, bar);
-          } else {
-            load_box<CG>(b, &bmap, k * kstep, n0, bar);
-          }
-          if (++s == g.stages) s = 0, phase ^= 1;
         }
-      }
-      if (!ok) atomicOr(g.err, 1u);
-      // nothing of the last round is in flight when the block leaves: the
-      // stages' products are done, or (after an expired wait) their copies in
-      for (int j = max(0, q - g.stages); j < q; ++j) {
-        uint64_t* bar = ok ? empty : full;
-        if (ok || rank == 0) wait(smem_addr(&bar[j % g.stages]), (j / g.stages) & 1);
+        __syncwarp();
+        if (++s == g.stages) s = 0, phase ^= 1;
       }
     }
+    if (!ok && lane == 0) atomicOr(g.err, 1u);
+    // nothing of the last round is in flight when the block leaves: the
+    // stages' products are done, or (after an expired wait) their copies in
+    for (int j = max(0, q - g.stages); j < q; ++j) {
+      uint64_t* bar = ok ? empty : full;
+      if (ok || rank == 0) wait(smem_addr(&bar[j % g.stages]), (j / g.stages) & 1);
+    }
+    __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {  // products
+    if (rank == 0) {  // products
       int s = 0, i = 0;
       uint32_t phase = 0;
       for (int t = first; t < tiles && ok; t += step) {
         const Tile at = tile_at(g, t);
         const int k0 = slab_at(g, at.split), k1 = slab_at(g, at.split + 1);
-        uint32_t d = 0;
         for (int k = k0; k < k1; ++k) {
           const bool fresh = P3 ? (k - k0) % CHUNK == 0 : k == k0;  // an accumulator starts here
           if (fresh) {
-            if (i >= 2) ok = wait(smem_addr(&tempty[i & 1]), ((i >> 1) - 1) & 1);
+            if (i >= 2) ok = wait_all(smem_addr(&tempty[i & 1]), ((i >> 1) - 1) & 1);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            d = tmem + (i & 1) * 256;
           }
-          ok = wait(smem_addr(&full[s]), phase);
+          ok = wait_all(smem_addr(&full[s]), phase);
           if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;");
-          const uint32_t a = ring + s * stage_bytes, b = a + PLANES * A_BYTES;
-          if constexpr (P3) {
-            constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
+          const uint32_t d = tmem + (i & 1) * 256, at_a = ring + s * stage_bytes;
+          const bool done = k + 1 == k1 || (P3 && (k + 1 - k0) % CHUNK == 0);
+          if (elected()) {
+            if constexpr (P3) {
+              constexpr int PA[6] = {2, 0, 1, 1, 0, 0}, PB[6] = {0, 2, 1, 0, 1, 0};
 #pragma unroll
-            for (int p = 0; p < 6; ++p)
+              for (int p = 0; p < 6; ++p) {
+                const uint64_t a = operand<AMN>(at_a + PA[p] * A_BYTES);
+                const uint64_t b = operand<BMN>(at_a + 3 * A_BYTES + PB[p] * b_bytes);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  issue<I8, CG>(d, next_k<AMN>(a, j), next_k<BMN>(b, j), g.idesc, !fresh || p > 0 || j > 0);
+              }
+            } else {
+              const uint64_t a = operand<AMN>(at_a), b = operand<BMN>(at_a + A_BYTES);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
-                issue<I8, CG>(d, operand<AMN>(a + PA[p] * A_BYTES + j * (AMN ? 2048 : 32)),
-                              operand<BMN>(b + PB[p] * b_bytes + j * (BMN ? 2048 : 32)), g.idesc,
-                              !fresh || p > 0 || j > 0);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              issue<I8, CG>(d, operand<AMN>(a + j * (AMN ? 2048 : 32)),
-                            operand<BMN>(b + j * (BMN ? 2048 : 32)), g.idesc, !fresh || j > 0);
+                issue<I8, CG>(d, next_k<AMN>(a, j), next_k<BMN>(b, j), g.idesc, !fresh || j > 0);
+            }
+            commit<CG>(smem_addr(&empty[s]));
+            if (done) commit<CG>(smem_addr(&tfull[i & 1]));
           }
-          commit<CG>(smem_addr(&empty[s]));
+          __syncwarp();
+          if (done) ++i;
           if (++s == g.stages) s = 0, phase ^= 1;
-          if (k + 1 == k1 || (P3 && (k + 1 - k0) % CHUNK == 0)) {
-            commit<CG>(smem_addr(&tfull[i & 1]));
-            ++i;
-          }
         }
       }
-      if (!ok) atomicOr(g.err, 1u);
+      if (!ok && lane == 0) atomicOr(g.err, 1u);
     }
+    __syncwarp();
   } else {  // epilogue
     const int quad = warp & 3, part = (warp - 2) >> 2;
     // this warp's place for turning results (where the launch has one)
@@ -384,10 +406,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     for (int t = first; t < tiles && ok; t += step) {
       const Tile at = tile_at(g, t);
+      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16);
       const int m = (at.m * CG + (int)rank) * TM + 32 * quad + lane;
       const bool in = m < g.M;
       typename Epi::Row row = epi.begin(m, in, at.split);
-      const uint32_t base = tmem + ((uint32_t)(32 * quad) << 16);
       if constexpr (P3) {  // BN <= 128: at most two groups of columns
         float sum[2][32];
 #pragma unroll
@@ -487,9 +509,12 @@ inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, in
          ((uint32_t)(cols >> 3) << 17) | ((uint32_t)(rows >> 4) << 24);
 }
 
-// Tile columns and whether a pair of CTAs shares a tile, from the result's
-// size: pairs of 256 x `most` when they fill four fifths of the card, else the widest tile of
-// one CTA that gives three quarters of the SMs one.
+// Tile columns and whether a pair of CTAs shares a tile, from the result's size:
+// pairs of 256 x `most` when they fill four fifths of the card, else the widest
+// tile of one CTA that gives three quarters of the SMs one. (A pair's tile of
+// 512 x 256, its two halves sharing B's slabs, saves a quarter of the loads but
+// fills the tensor memory, so that its epilogue is half exposed: 294 us on 4096
+// x 1024 by 50001 x 1024 with the loss's forward epilogue, this one 262.)
 struct Tiling {
   int bn, pair;
 };
@@ -506,7 +531,7 @@ inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least, int 
 // cuts k into that many ranges of whole slabs, each handed to the epilogue
 // as its own tile. P3: bf16 planes (Matrix::plane), bn at most 128.
 template <bool I8, bool P3, bool AMN, bool BMN, int CG, class Epi>
-int launch_product(om_backend* be, const char* name, const Matrix& a, const Matrix& b, bool bf16,
+int launch_tiles(om_backend* be, const char* name, const Matrix& a, const Matrix& b, bool bf16,
                    int bn, int splits, const Epi& epi) {
   const int kstep = I8 ? 128 : 64;
   const int64_t tm = (a.rows + TM * CG - 1) / (TM * CG), tn = (b.rows + bn - 1) / bn;
@@ -525,7 +550,7 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
   g.tiles_m = (int)tm, g.tiles_n = (int)tn, g.splits = splits;
   // a wave's tiles form a square of rows and columns, so that each slab is
   // read by many SMs while it is in L2
-  g.group = std::max(1, std::min<int>((int)tm, CG == 2 ? 8 : 16));
+  g.group = std::max(1, std::min<int>((int)tm, 2048 / (TM * CG)));
   const int stage = (P3 ? 3 : 1) * (A_BYTES + bn / CG * SLAB);
   g.a_rows = a_rows;
   g.turn = epi.turns() ? 8 * TURN_BYTES : 0;
@@ -534,7 +559,7 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
   g.err = be->d_flags + 1;
   const size_t smem = (size_t)g.stages * stage + g.turn + 1024;
   auto kernel = product_kernel<I8, P3, AMN, BMN, CG, Epi>;
-  OM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), name);
+  OM_TRY(allow_shared(be, (const void*)kernel, (int)smem, name));
   const int64_t work = tm * tn * splits;
   ProfScope prof(be, name);
   cudaLaunchConfig_t cfg{};
@@ -550,6 +575,13 @@ int launch_product(om_backend* be, const char* name, const Matrix& a, const Matr
   OM_CUDA(cudaLaunchKernelEx(&cfg, kernel, ma, mb, g, epi), name);
   note_launch();
   return OM_OK;
+}
+
+template <bool I8, bool P3, bool AMN, bool BMN, class Epi>
+int launch_product(om_backend* be, const char* name, const Matrix& a, const Matrix& b, bool bf16,
+                   const Tiling& t, int splits, const Epi& epi) {
+  if (t.pair) return launch_tiles<I8, P3, AMN, BMN, 2>(be, name, a, b, bf16, t.bn, splits, epi);
+  return launch_tiles<I8, P3, AMN, BMN, 1>(be, name, a, b, bf16, t.bn, splits, epi);
 }
 
 }  // namespace mma

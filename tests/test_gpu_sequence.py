@@ -249,7 +249,7 @@ def test_loss(be, seq, shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-@pytest.mark.parametrize("shape", [(600, 72, 6500), (2300, 2100, 2305), (130, 264, 9700)], ids=str)
+@pytest.mark.parametrize("shape", [(600, 72, 6500), (2300, 2100, 2305), (130, 264, 9700), (1500, 1025, 7000)], ids=str)
 def test_loss_in_pairs_of_sms(be, seq, shape, dtype):
     """Results large enough for two SMs to share a tile, with ragged ends."""
     x, w, targets, g = loss_inputs(sum(shape), *shape, dtype)
@@ -369,7 +369,7 @@ def i8_inputs(seed, m, k, n, dtype):
 
 
 I8_SHAPES = [(1, 64, 64), (1, 4096, 512), (1, 1, 1), (2, 31, 17), (3, 16, 100), (8, 1000, 130), (9, 256, 64), (16, 48, 257), (17, 128, 256), (37, 2048, 520),
-             (64, 515, 129), (127, 96, 33), (128, 128, 128), (129, 160, 300), (300, 1037, 211), (513, 272, 1000), (5, 9000, 40), (260, 64, 2050)]
+             (64, 515, 129), (127, 96, 33), (128, 128, 128), (129, 160, 300), (300, 1037, 211), (513, 272, 1000), (5, 9000, 40), (260, 64, 2050), (2100, 520, 2400), (1300, 2100, 7000)]
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
