@@ -7,15 +7,17 @@
 //                 chunks (a block's) together;
 //   step_kernel   joins the maps before its chunk to the state that enters it
 //                 and takes the chunk's steps one by one, writing the results.
-// A warp has 32 lanes of 8 bytes of channels (fewer where rows are not 8-byte
-// aligned or channels are not contiguous) and a chunk's steps; it loads several steps at once and holds the state in
-// registers, so nothing but the maps passes through shared memory. Sums are
-// formed in one order whatever the timing. Where the channels alone fill the
-// card, a sequence is one chunk and map_kernel does not run.
+// A warp has 32 lanes of 8 bytes of channels (one channel where rows are not
+// 8-byte aligned or channels are not contiguous) and a chunk's steps; the next
+// steps are under way while some are in use, and the state is in registers, so
+// nothing but the maps passes through shared memory. Sums are formed in one
+// order whatever the timing. Where the channels alone fill the card, a sequence
+// is one chunk and map_kernel does not run.
 //
 // Bound by HBM: step_kernel moves 3 arrays (forward) or 5 to 6 (backward) per
-// element, map_kernel 2 more. step_kernel starts at the chunks that map_kernel
-// read last, which are still in L2.
+// element, map_kernel 2 more. (One pass over tiles in shared memory that looked
+// back at one another read everything once, but spent its time on the tiles'
+// bookkeeping: 217 us for 4 x 4096 x 2048 bf16 with the backward pass, this 172.)
 #include <algorithm>
 
 #include "om_convert.cuh"
@@ -46,6 +48,10 @@ struct ScanArgs {
 };
 
 constexpr int WARPS = 8;  // of a block
+// Blocks of an SM: two, whose lanes keep twice eight steps in registers (8-byte
+// rows; four blocks of half as many are up to 20 % slower), three where rows
+// are 4 bytes of a lane.
+constexpr int blocks_of(int lane_bytes) { return lane_bytes == 4 ? 3 : 2; }
 
 struct ChunkArgs {
   int64_t groups;   // of VEC channels, a lane's
@@ -310,6 +316,61 @@ __device__ __forceinline__ void keep(T* p, const Lane<T, V>& l) {
   *reinterpret_cast<typename Lane<T, V>::R*>(p) = l.raw();
 }
 
+// NA arrays' rows of a lane, in order: U rows are in use while the next U are
+// under way. start() asks for the first ones.
+template <typename T, int V, int NA, int U>
+struct Stream {
+  using R = typename Lane<T, V>::R;
+  const T* p[NA];     // the next row
+  int64_t step[NA];   // elements between rows
+  int64_t n;          // rows
+  int64_t asked = 0;
+  R a[U][NA];
+
+  __device__ __forceinline__ void ask(R (&r)[U][NA]) {
+    if (asked + U <= n) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < NA; ++k) r[u][k] = fetch<T, V>(p[k] + u * step[k]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (asked + u < n) {
+#pragma unroll
+          for (int k = 0; k < NA; ++k) r[u][k] = fetch<T, V>(p[k] + u * step[k]);
+        }
+    }
+    asked += U;
+#pragma unroll
+    for (int k = 0; k < NA; ++k) p[k] += U * step[k];
+  }
+  __device__ __forceinline__ void start() { ask(a); }
+  template <typename F>
+  __device__ __forceinline__ void use(const R (&r)[U][NA], int64_t i, F& f) {
+    if (i + U <= n) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) f(r[u]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i + u < n) f(r[u]);
+    }
+  }
+  // f(a row of each array), n times
+  template <typename F>
+  __device__ __forceinline__ void run(F f) {
+    R b[U][NA];
+    for (int64_t i = 0; i < n; i += 2 * U) {
+      ask(b);
+      use(a, i, f);
+      if (i + U >= n) break;
+      ask(a);
+      use(b, i + U, f);
+    }
+  }
+};
+
 // ---- the maps of the chunks -------------------------------------------------------------
 
 template <typename T, int V, bool SIG, bool BWD>
@@ -329,11 +390,10 @@ __device__ __forceinline__ void compose(Map<T, V>& m, Lane<T, V> g, Lane<T, V> x
 }
 
 template <typename T, int V, bool SIG, bool BWD>
-__global__ void __launch_bounds__(WARPS * 32, 4) map_kernel(const __grid_constant__ ScanArgs p,
+__global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) map_kernel(const __grid_constant__ ScanArgs p,
                                                             const __grid_constant__ ChunkArgs a) {
   using S = typename Elem<T>::State;
   using L = Lane<T, V>;
-  constexpr int U = 8;
   __shared__ Pair<S> part[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
@@ -343,24 +403,17 @@ __global__ void __launch_bounds__(WARPS * 32, 4) map_kernel(const __grid_constan
   Map<T, V> m = Map<T, V>::identity();
   // the last chunk's map is not needed
   if (at.live && at.order < a.chunks - 1) {
-    const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
-    const T* x = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed : (const T*)p.x + at.b * p.xb + at.d * p.xd;
-    const int64_t gs = BWD ? -p.gt : p.gt, xs = BWD ? -p.et : p.xt;
-    int64_t n = at.end - at.t0;
     const int64_t first = BWD ? at.end - 1 : at.t0;
-    g += first * p.gt;
-    x += first * (BWD ? p.et : p.xt);
-    for (; n >= U; n -= U) {
-      typename L::R rg[U], rx[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) rg[u] = fetch<T, V>(g + u * gs), rx[u] = fetch<T, V>(x + u * xs);
-#pragma unroll
-      for (int u = 0; u < U; ++u) compose<T, V, SIG, BWD>(m, L::of(rg[u]), L::of(rx[u]));
-      g += U * gs;
-      x += U * xs;
-    }
-    for (; n > 0; --n, g += gs, x += xs)
-      compose<T, V, SIG, BWD>(m, L::of(fetch<T, V>(g)), L::of(fetch<T, V>(x)));
+    const int64_t xt = BWD ? p.et : p.xt;
+    Stream<T, V, 2, 8> rows;
+    rows.n = at.end - at.t0;
+    rows.p[0] = (const T*)p.gate + at.b * p.gb + at.d * p.gd + first * p.gt;
+    rows.p[1] = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed + first * xt
+                    : (const T*)p.x + at.b * p.xb + at.d * p.xd + first * xt;
+    rows.step[0] = BWD ? -p.gt : p.gt;
+    rows.step[1] = BWD ? -xt : xt;
+    rows.start();
+    rows.run([&](const typename L::R (&r)[2]) { compose<T, V, SIG, BWD>(m, L::of(r[0]), L::of(r[1])); });
     m.put((Pair<S>*)a.maps + (int64_t)at.order * a.pitch + at.c0);
     const S* from = (const S*)(BWD ? p.dh_last : p.h0);
     if (at.order == 0) {
@@ -386,13 +439,13 @@ __global__ void __launch_bounds__(WARPS * 32, 4) map_kernel(const __grid_constan
 // ---- the steps ------------------------------------------------------------------------
 
 template <typename T, int V, bool SIG, bool BWD>
-__global__ void __launch_bounds__(WARPS * 32, 4) step_kernel(const __grid_constant__ ScanArgs p,
+__global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) step_kernel(const __grid_constant__ ScanArgs p,
                                                              const __grid_constant__ ChunkArgs a) {
   using S = typename Elem<T>::State;
   using L = Lane<T, V>;
   using K = typename L::K;
   using R = typename L::R;
-  __shared__ Pair<S> part[WARPS][32 * V];
+  __shared__ Pair<S> part[WARPS][32 * V], chunk[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
   const unsigned per = (unsigned)((a.columns + WARPS / wt - 1) / (WARPS / wt));
@@ -404,38 +457,61 @@ __global__ void __launch_bounds__(WARPS * 32, 4) step_kernel(const __grid_consta
   // the state that enters: the caller's, through the maps of the blocks of
   // chunks before this one (shared out over the warps) and of the chunks
   // before this warp's
+  constexpr int NA = BWD ? (SIG ? 4 : 3) : 2;
+  Stream<T, V, NA, NA == 2 ? 8 : NA == 3 ? 4 : 3> rows;
+  // (backward: step 0, which has no h before it, comes after the others)
+  const bool start = BWD && at.t0 == 0 && at.end > 0;
+  const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
+  const T* x = (const T*)p.x + at.b * p.xb + at.d * p.xd;
+  const T* e = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed : nullptr;
+  rows.n = at.live ? at.end - at.t0 - start : 0;
+  if constexpr (!BWD) {
+    rows.p[0] = g + at.t0 * p.gt, rows.step[0] = p.gt;
+    rows.p[1] = x + at.t0 * p.xt, rows.step[1] = p.xt;
+  } else {
+    const int64_t t = at.end - 1;
+    rows.p[0] = g + t * p.gt, rows.step[0] = -p.gt;
+    rows.p[1] = e + t * p.et, rows.step[1] = -p.et;
+    rows.p[2] = (const T*)p.h + at.b * p.hb + at.d * p.hd + (t - 1) * p.ht, rows.step[2] = -p.ht;
+    if constexpr (SIG) rows.p[3] = x + t * p.xt, rows.step[3] = -p.xt;
+  }
   const S* from = (const S*)(a.chunks > 1 ? a.start : BWD ? p.dh_last : p.h0);
   L s;
 #pragma unroll
   for (int i = 0; i < V; ++i) s.set(i, from && at.live ? from[at.c0 + i] : S(0));
   if (a.chunks > 1) {
-    if (wt == WARPS && block > 0) {
-      Map<T, V> m = Map<T, V>::identity();
+    // this warp's own chunk's map goes to shared memory for the warps behind it
+    Map<T, V> own = Map<T, V>::identity();
+    if (at.live && at.order < a.chunks - 1) own = Map<T, V>::take((const Pair<S>*)a.maps + at.order * a.pitch + at.c0);
+    Map<T, V> m = Map<T, V>::identity();
+    if (wt == WARPS) {
       const Pair<S>* j = (const Pair<S>*)a.joined + ((int64_t)col * 32 + lane) * V;
       const int k1 = (int)((int64_t)block * (warp + 1) / WARPS);
 #pragma unroll 4
       for (int k = (int)((int64_t)block * warp / WARPS); k < k1; ++k)
         m.then(Map<T, V>::take(j + k * a.pitch));
-      m.put(&part[warp][lane * V]);
-      __syncthreads();
+    }
+    rows.start();
+    m.put(&part[warp][lane * V]);
+    own.put(&chunk[warp][lane * V]);
+    __syncthreads();
+    if (wt == WARPS && block > 0) {
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) s = Map<T, V>::take(&part[w][lane * V]).at(s);
     }
-    if (at.live) {
-      const Pair<S>* m = (const Pair<S>*)a.maps + at.c0;
-#pragma unroll 4
-      for (int k = block * wt; k < at.order; ++k) s = Map<T, V>::take(m + k * a.pitch).at(s);
-    }
+    for (int w = 0; w < tw; ++w) s = Map<T, V>::take(&chunk[team * wt + w][lane * V]).at(s);
+  } else {
+    rows.start();
   }
   if (!at.live) return;
 
-  const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
+  L zero;
+#pragma unroll
+  for (int i = 0; i < V; ++i) zero.set(i, S(0));
   if constexpr (!BWD) {
-    constexpr int U = 8;
-    const T* x = (const T*)p.x + at.b * p.xb + at.d * p.xd;
-    T* h = (T*)p.h + at.b * p.hb + at.d * p.hd;
-    auto step = [&](R rg, R rx, T* to) {
-      const L f = L::of(rg), b = L::of(rx);
+    T* h = (T*)p.h + at.b * p.hb + at.d * p.hd + at.t0 * p.ht;
+    rows.run([&](const R (&r)[2]) {
+      const L f = L::of(r[0]), b = L::of(r[1]);
 #pragma unroll
       for (int i = 0; i < L::N; ++i) {
         K fi = f.v[i], bi = b.v[i];
@@ -446,33 +522,16 @@ __global__ void __launch_bounds__(WARPS * 32, 4) step_kernel(const __grid_consta
         }
         s.v[i] = mad(fi, s.v[i], bi);
       }
-      keep<T, V>(to, s);
-    };
-    int64_t t = at.t0;
-    g += t * p.gt, x += t * p.xt, h += t * p.ht;
-    for (; t + U <= at.end; t += U) {
-      R rg[U], rx[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) rg[u] = fetch<T, V>(g + u * p.gt), rx[u] = fetch<T, V>(x + u * p.xt);
-#pragma unroll
-      for (int u = 0; u < U; ++u) step(rg[u], rx[u], h + u * p.ht);
-      g += U * p.gt, x += U * p.xt, h += U * p.ht;
-    }
-    for (; t < at.end; ++t, g += p.gt, x += p.xt, h += p.ht) step(fetch<T, V>(g), fetch<T, V>(x), h);
-    if (t < at.t1) {
-      L zero;
-#pragma unroll
-      for (int i = 0; i < V; ++i) zero.set(i, S(0));
-      for (; t < at.t1; ++t, h += p.ht) keep<T, V>(h, zero);
-    }
+      keep<T, V>(h, s);
+      h += p.ht;
+    });
+    for (int64_t t = at.end; t < at.t1; ++t, h += p.ht) keep<T, V>(h, zero);
   } else {
-    constexpr int U = 4;
-    const T* e = (const T*)p.dh + at.b * p.eb + at.d * p.ed;
-    const T* h = (const T*)p.h + at.b * p.hb + at.d * p.hd;
-    const T* x = SIG ? (const T*)p.x + at.b * p.xb + at.d * p.xd : nullptr;
-    T* dg = (T*)p.dgate + at.b * p.pb + at.d * p.pd;
-    T* dx = (T*)p.dx + at.b * p.qb + at.d * p.qd;
-    auto step = [&](R rg, R re, L before, R rx, T* to_g, T* to_x) {
+    T* dg = (T*)p.dgate + at.b * p.pb + at.d * p.pd + (at.t1 - 1) * p.pt;
+    T* dx = (T*)p.dx + at.b * p.qb + at.d * p.qd + (at.t1 - 1) * p.qt;
+    for (int64_t t = at.t1; t > at.end; --t, dg -= p.pt, dx -= p.qt)
+      keep<T, V>(dg, zero), keep<T, V>(dx, zero);
+    auto back = [&](R rg, R re, const L& before, R rx) {
       const L f = L::of(rg), d = L::of(re), v = L::of(rx);
       L og, ox;
 #pragma unroll
@@ -490,43 +549,18 @@ __global__ void __launch_bounds__(WARPS * 32, 4) step_kernel(const __grid_consta
         }
         s.v[i] = fi * total;
       }
-      keep<T, V>(to_g, og);
-      keep<T, V>(to_x, ox);
+      keep<T, V>(dg, og);
+      keep<T, V>(dx, ox);
+      dg -= p.pt;
+      dx -= p.qt;
     };
-    int64_t t = at.t1 - 1;
-    if (t >= at.end) {
-      L zero;
-#pragma unroll
-      for (int i = 0; i < V; ++i) zero.set(i, S(0));
-      for (; t >= at.end; --t) keep<T, V>(dg + t * p.pt, zero), keep<T, V>(dx + t * p.qt, zero);
-    }
-    g += t * p.gt, e += t * p.et, h += (t - 1) * p.ht, dg += t * p.pt, dx += t * p.qt;
-    if constexpr (SIG) x += t * p.xt;
-    for (; t - U >= at.t0; t -= U) {  // (step 0, which has no h before it, is left to the loop below)
-      R rg[U], re[U], rh[U], rx[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        rg[u] = fetch<T, V>(g - u * p.gt), re[u] = fetch<T, V>(e - u * p.et);
-        rh[u] = fetch<T, V>(h - u * p.ht);
-        rx[u] = SIG ? fetch<T, V>(x - u * p.xt) : rg[u];
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) step(rg[u], re[u], L::of(rh[u]), rx[u], dg - u * p.pt, dx - u * p.qt);
-      g -= U * p.gt, e -= U * p.et, h -= U * p.ht, dg -= U * p.pt, dx -= U * p.qt;
-      if constexpr (SIG) x -= U * p.xt;
-    }
-    for (; t >= at.t0; --t) {
+    rows.run([&](const R (&r)[NA]) { back(r[0], r[1], L::of(r[2]), r[NA - 1]); });
+    if (start) {
       L before;
-      if (t > 0) {
-        before = L::of(fetch<T, V>(h));
-      } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) before.set(i, p.h0 ? ((const S*)p.h0)[at.c0 + i] : S(0));
-      }
+      for (int i = 0; i < V; ++i) before.set(i, p.h0 ? ((const S*)p.h0)[at.c0 + i] : S(0));
       const R rg = fetch<T, V>(g);
-      step(rg, fetch<T, V>(e), before, SIG ? fetch<T, V>(x) : rg, dg, dx);
-      g -= p.gt, e -= p.et, h -= p.ht, dg -= p.pt, dx -= p.qt;
-      if constexpr (SIG) x -= p.xt;
+      back(rg, fetch<T, V>(e), before, SIG ? fetch<T, V>(x) : rg);
     }
   }
   // the state that leaves the last chunk
@@ -569,15 +603,16 @@ int launch_chunks(om_backend* be, const ScanArgs& p) {
   const int64_t columns = (a.groups + 31) / 32;
   a.pitch = columns * 32 * V;
   a.narrow = a.groups * V < ((int64_t)1 << 32) && p.D < ((int64_t)1 << 32);
-  // Six columns per SM run faster uncut, without the maps' second read (1024
-  // columns x 512 steps bf16 with the backward pass: 236 us, cut in two 259;
-  // 512 x 1024: 364 and 266). Fewer are cut into as many chunks as one wave of
-  // the 32 warps that an SM holds takes, whole blocks of them (64 x 4096 in 64
-  // chunks: 182 us, in 74, which leave a second wave nearly empty: 207), of
-  // 16 steps at least (96 x 700: 61 us, of 32 steps 67).
+  // Four columns per SM run faster uncut, without the maps' second read (640
+  // columns x 1024 steps bf16 with the backward pass: 305 us, cut 329; 512: cut
+  // 252 us). Fewer are cut into as many chunks as one wave of the 16 warps that
+  // an SM holds takes, whole blocks of them, of 16 steps at least (96 x 700: 50
+  // us, in twice as many chunks 60). Narrow rows keep fewer bytes under way and
+  // take twice the warps.
+  const int64_t warps = (int64_t)be->num_sms * (V == 1 && sizeof(T) < 8 ? 32 : 16);
   int64_t chunks = 1;
-  if (columns < 6 * be->num_sms) {
-    chunks = (int64_t)be->num_sms * 32 / columns;
+  if (columns < 4 * be->num_sms) {
+    chunks = warps / columns;
     if (chunks >= WARPS) chunks = chunks / WARPS * WARPS;
     else chunks = chunks >= 4 ? 4 : 2;
     chunks = std::max<int64_t>(1, std::min(chunks, p.T / 16));
