@@ -364,7 +364,10 @@ int om_b200_tropical_matmul_argmax_noalloc(void* stream, om_algebra alg, int64_t
  * lengths (device, B int32, may be NULL): sequence b has
  * min(max(lengths[b], 0), T) steps; what lies behind them is not read, h is
  * zero there, and h_last is the state after the last real step.  T == 1 is the
- * form for decoding one token. */
+ * form for decoding one token.
+ * Steps may be grouped: gates above one in magnitude whose product over a few
+ * hundred steps leaves the state's type give infinities where the state itself
+ * would not, and an infinite gate gives NaN or infinity from its step on. */
 typedef enum { OM_GATE_LINEAR = 0, OM_GATE_SIGMOID = 1 } om_gate;
 int om_b200_gated_scan(om_backend* be, om_gate kind, om_dtype dtype, const int64_t* shape,
                        const void* gate, const int64_t* strides_gate, const void* x,

@@ -255,6 +255,14 @@ class B200:
         _check(lib().om_b200_stream(self.h, ctypes.byref(s)))
         return s.value or 0
 
+    def torch_stream(self):
+        """The backend's stream as a torch stream (ExternalStream(0) would be
+        a stream of torch's pool, not the legacy default one)."""
+        import torch
+        s = self.stream()
+        return (torch.cuda.ExternalStream(s, device=self.device) if s
+                else torch.cuda.default_stream(self.device))
+
     def graph_begin(self):
         """Start recording the work issued on this backend's stream."""
         _check(lib().om_b200_graph_begin(self.h))

@@ -483,7 +483,7 @@ int launch_matmul(om_backend* be, const I8Args& p) {
   const ScaleEpi<T> epi{p.q_scale, p.w_scale, p.bias, (T*)p.y, p.ym, p.yn,
                         row_stores(p.y, p.ym, p.yn, sizeof(T)),
                         !(((uintptr_t)p.w_scale | (uintptr_t)p.bias) & 15)};
-  const mma::Tiling t = mma::tiling(be, p.M, p.N, 32);
+  const mma::Tiling t = mma::tiling(be, p.M, p.N, 32, 256, true);
   return mma::launch_product<true, false, false, false>(be, "matmul_i8", q, w, false, t, 1, epi);
 }
 

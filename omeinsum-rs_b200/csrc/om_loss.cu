@@ -612,8 +612,8 @@ int product(om_backend* be, const char* name, const mma::Matrix& a, const mma::M
   return mma::launch_product<false, P3, AMN, BMN>(be, name, a, b, BF, t, splits, epi);
 }
 template <typename T>
-mma::Tiling tiles(const om_backend* be, int64_t M, int64_t N) {
-  return mma::tiling(be, M, N, 64, sizeof(T) == 4 ? 128 : 256);
+mma::Tiling tiles(const om_backend* be, int64_t M, int64_t N, bool odd = false) {
+  return mma::tiling(be, M, N, 64, sizeof(T) == 4 ? 128 : 256, odd);
 }
 // rows [r0, r0 + n) of a K-major matrix
 mma::Matrix rows_of(const mma::Matrix& m, int64_t r0, int64_t n) {
@@ -644,7 +644,7 @@ int loss_forward_tc(om_backend* be, const LossArgs& p, float* loss, float* lse) 
   mma::Matrix x, w;
   OM_TRY(readable(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
   const int64_t W = weight_rows<T>(p);
-  const mma::Tiling t = tiles<T>(be, p.N, W);
+  const mma::Tiling t = tiles<T>(be, p.N, W, true);
   const int64_t slots = ((p.V + W - 1) / W) * ((W + t.bn - 1) / t.bn) * 2;
   OM_TRY(ws.alloc(be, (size_t)p.N * (slots * 8 + 4)));
   float2* part = (float2*)ws.ptr;

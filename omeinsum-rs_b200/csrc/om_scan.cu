@@ -249,16 +249,19 @@ struct Map {
     return m;
   }
   __device__ __forceinline__ void then(const Map& m) {
+    q = m.at(q);
 #pragma unroll
-    for (int i = 0; i < L::N; ++i) {
-      q.v[i] = mad(m.p.v[i], q.v[i], m.q.v[i]);
-      p.v[i] = m.p.v[i] * p.v[i];
-    }
+    for (int i = 0; i < L::N; ++i) p.v[i] = m.p.v[i] * p.v[i];
   }
+  // A state of zero leaves q, also where gates above one let p overflow (what
+  // is not a number in a step is in q already).
   __device__ __forceinline__ L at(const L& s) const {
     L r;
 #pragma unroll
     for (int i = 0; i < L::N; ++i) r.v[i] = mad(p.v[i], s.v[i], q.v[i]);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (s.get(i) == S(0)) r.set(i, q.get(i));
     return r;
   }
   __device__ __forceinline__ void put(Pair<S>* to) const {
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) map_kern
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const Pair<S> k = part[w][c];
-      Q = k.p * Q + k.q;
+      Q = Q == S(0) ? k.q : k.p * Q + k.q;  // as Map::at
       P = k.p * P;
     }
     ((Pair<S>*)a.joined)[(int64_t)block * a.pitch + (int64_t)col * 32 * V + c] = Pair<S>{P, Q};

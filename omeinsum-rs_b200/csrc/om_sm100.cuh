@@ -55,7 +55,7 @@ constexpr int TURN_BYTES = 32 * 33 * 4;  // 32 rows of 32 values, a word apart
 struct Shape {
   int M, N;        // rows of A and of B
   int slabs;       // of 128 bytes along k, all splits together
-  int BN;          // columns of a tile: 32 .. 256
+  int BN;          // columns of a tile: 32 .. 256, a multiple of 32
   int stages;
   int a_rows;      // rows of A's box: 128, or fewer where all of A has fewer
   int turn;        // bytes of shared memory for turning a warp's results, or 0
@@ -518,7 +518,16 @@ inline uint32_t instruction(bool i8, bool bf16, bool amn, bool bmn, int rows, in
 struct Tiling {
   int bn, pair;
 };
-inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least, int most = 256) {
+// `odd` (B K-major, an epilogue that writes nothing outside the result): one row
+// of tiles, which waits for B's bytes alone, gets the width in steps of 32 that
+// gives every SM the same share of them (24 x 2048 x 32000 in f16: 143 tiles of
+// 224 columns instead of 125 of 256).
+inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least, int most = 256, bool odd = false) {
+  if (odd && M <= TM) {
+    const int64_t waves = (N + (int64_t)be->num_sms * most - 1) / ((int64_t)be->num_sms * most);
+    const int64_t share = (N + be->num_sms * waves - 1) / (be->num_sms * waves);
+    return {(int)std::max<int64_t>(least, (share + 31) / 32 * 32), 0};
+  }
   if (M > TM && (M + 255) / 256 * ((N + most - 1) / most) * 5 >= be->num_sms * 2) return {most, 1};
   const int64_t tm = (M + TM - 1) / TM;
   for (int bn = most; bn > least; bn /= 2)
@@ -526,7 +535,7 @@ inline Tiling tiling(const om_backend* be, int64_t M, int64_t N, int least, int 
   return {least, 0};
 }
 
-// D = A B^T through `epi`. bn: tile columns (32, 64, 128 or 256; at least 64
+// D = A B^T through `epi`. bn: tile columns (a multiple of 32 up to 256; of 64
 // for an MN-major B); pair: two CTAs per tile (bn 128 or 256). splits > 1
 // cuts k into that many ranges of whole slabs, each handed to the epilogue
 // as its own tile. P3: bf16 planes (Matrix::plane), bn at most 128.

@@ -680,7 +680,7 @@ class DeviceExecutor:
             return [], -1, None
         slots = self._value_slots(assigns[0])
         dev = torch.device(f"cuda:{self.be.device}")
-        stream = torch.cuda.ExternalStream(self.be.stream(), device=dev)
+        stream = self.be.torch_stream()
         tdt = torch.float64 if self.dtype == np.float64 else torch.float32
         n = len(assigns)
         es = np.dtype(self.dtype).itemsize
@@ -1005,7 +1005,7 @@ def run_sliced(executor, alg, ixs, sizes, sliced, rank, world, dist=None, device
     if on_device:
         if device is None:
             device = torch.device(f"cuda:{executor.be.device}")
-        stream = torch.cuda.ExternalStream(executor.be.stream(), device=device)
+        stream = executor.be.torch_stream()
         tdt = torch.float64 if executor.dtype == np.float64 else torch.float32
     import contextlib
     ctx = torch.cuda.stream(stream) if on_device else contextlib.nullcontext()

@@ -7,7 +7,7 @@ om_b200_quantize_rows, om_b200_linear_i8).
 Every function takes the backend first and tensors that are either
 
   - torch CUDA tensors on the backend's device (any strides), or
-  - `Strided` views of a backend's `Storage` (see `upload`),
+  - `Strided` views of this backend's `Storage` (see `upload`),
 
 and returns tensors of the kind it was given, row-major.  Shapes are in the
 order the text names; nothing waits for the device.
@@ -128,8 +128,11 @@ def _operand(be, t, name):
     """(device pointer, type code, shape, strides) of one argument."""
     if type(t) is Strided:
         s = t.storage
-        if s.backend.device != be.device:
-            raise _invalid(f"{name}: on device {s.backend.device}, the backend on {be.device}")
+        if s.backend is not be:
+            if s.backend.device != be.device:
+                raise _invalid(f"{name}: on device {s.backend.device}, the backend on {be.device}")
+            if s.backend.home_stream != be.home_stream:
+                raise _invalid(f"{name}: belongs to a backend on another stream")
         return (s.ptr or 0) + t.offset * s.dtype.itemsize, DTYPES[s.dtype], t.shape, t.strides
     try:
         if t.get_device() != be.device:  # -1: not on a device at all
@@ -194,7 +197,7 @@ class _Call:
         self.like = like
         if not be.recording and _torch._C._cuda_getCurrentRawStream(be.device) != be.home_stream:
             self.cur = _torch.cuda.current_stream(like.device)
-            self.mine = _torch.cuda.ExternalStream(be.home_stream, device=like.device)
+            self.mine = be.torch_stream()
             self.mine.wait_stream(self.cur)
 
     def empty(self, code, shape, same=None):

@@ -51,9 +51,12 @@ def scan(gate, x, h0, lengths, kind, dtype):
 
     The term b_s of h_t passes t - s products and at most as many additions
     (any grouping of the chain included, with 8 more for joining groups), each
-    off by U relative to it; every factor a of kind "sigmoid" by SIGMOID U."""
+    off by U relative to it; every factor a of kind "sigmoid" by SIGMOID U. In
+    f32 a step's result below 2^-126, the smallest normal number, may be lost
+    whole: up to 2^-126 per step, which the later factors carry on."""
     nb, nt, nd = gate.shape
     unit = state_unit(dtype)
+    tiny = 0.0 if dtype == "f64" else 2.0 ** -126 / unit
     per = 2.0 + (SIGMOID if kind == "sigmoid" else 0.0)
     a, b, _ = _factors(gate, x, kind)
     h = np.zeros_like(gate)
@@ -65,7 +68,7 @@ def scan(gate, x, h0, lengths, kind, dtype):
         on = (t < ends)[:, None]
         ra = np.where(on, a[:, t], 1.0)
         rb = np.where(on, b[:, t], 0.0)
-        err = np.where(on, np.abs(ra) * (err + per * mass), err)
+        err = np.where(on, np.abs(ra) * (err + per * mass) + tiny, err)
         s = ra * s + rb
         mass = np.abs(ra) * mass + np.abs(rb)
         h[:, t] = np.where(on, s, 0.0)

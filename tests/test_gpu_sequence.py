@@ -139,6 +139,24 @@ def test_scan_extreme_gates(be, seq, kind):
     assert np.isnan(got[0][0, 300:, 5]).all() and not np.isnan(got[0][0, :300, 5]).any()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f64", "bf16"])
+def test_scan_growing_gates(be, seq, dtype):
+    """Gates above one over a state of zero, long enough for their product to
+    overflow: the state stays zero until something enters it, in both directions."""
+    t = 3000
+    gate, x, dh = np.full((1, t, 24), 8.0), np.zeros((1, t, 24)), np.zeros((1, t, 24))
+    gate[:, 2500:] = 0.5
+    x[:, 2600] = 3.0
+    dh[:, 2700] = 2.0
+    gate[:, :2500, 1], x[:, 1000, 1] = -8.0, 0.0
+    got = run_scan(be, seq, gate, x, dh, None, None, None, "linear", dtype)
+    h = ref.scan(gate[:, 2500:], x[:, 2500:], None, None, "linear", dtype)
+    assert not got[0][:, :2500].any()
+    near(got[0][:, 2500:], h[0], h[2], dtype)
+    near(got[1], h[1], h[3])
+    assert not got[3][:, 2701:].any() and np.isfinite(got[3][:, 2500:]).all()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("layout", ["time_major", "channel_major", "offset", "broadcast", "reversed", "wide_rows"])
 def test_scan_strides(be, seq, layout, dtype):
@@ -551,6 +569,45 @@ def test_other_stream_than_torchs(seq):
         side.synchronize()
         assert all(torch.equal(got[k], want[k]) for k in want)
     be.close()
+
+
+def test_default_stream_backend_called_from_a_side_stream(seq):
+    import torch
+    om = load_pkg()
+    be = om.B200(0, stream=0)
+    want = {k: v.clone() for k, v in layer(seq, be, layer_inputs(2)).items()}
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2_000_000)
+            t = layer_inputs(2)
+            got = {k: v + 0 for k, v in layer(seq, be, t).items()}
+        side.synchronize()
+        assert all(torch.equal(got[k], want[k]) for k in want)
+    be.close()
+
+
+def test_views_of_another_backend_are_refused(be, seq):
+    om = load_pkg()
+    other = om.B200(0)
+    x = seq.upload(other, np.zeros((2, 16), np.float32))
+    with pytest.raises(om.OmError, match="another stream"):
+        seq.quantize_rows(be, x)
+    other.close()
+
+
+def test_current_device_and_profiling_are_left_alone(be, seq):
+    """Kernel classes are timed like the library's others."""
+    be.profile(True)
+    x, w = seq.upload(be, np.ones((4, 64)), "bf16"), seq.upload(be, np.ones((300, 64)), "bf16")
+    T = seq.upload(be, np.zeros(4), "i64")
+    loss, lse = seq.linear_cross_entropy(be, x, w, T)
+    seq.linear_cross_entropy_backward(be, x, w, T, lse, seq.upload(be, np.ones(4, np.float32)))
+    report = be.profile_report()
+    be.profile(False)
+    assert {"loss_logits", "loss_dlogits", "loss_dx", "loss_dw"} <= set(report)
+    # all logits alike: 300 equal parts
+    assert np.allclose(lse.to_numpy(), 64 + np.log(300), rtol=1e-6)
 
 
 def test_calls_without_waiting_between_them(seq):
