@@ -91,6 +91,33 @@ __device__ __forceinline__ void store_turned(float* turn, const float (&v)[32], 
   __syncwarp();
 }
 
+// The `bytes` (16 at most) from `at` on, zero behind them, from the aligned words
+// that hold them, shifted into place
+__device__ __forceinline__ uint4 load_bytes(const void* at, int bytes) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>((uintptr_t)at & ~(uintptr_t)3);
+  const int off = (int)((uintptr_t)at & 3);
+  uint32_t v[5], o[4];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) v[i] = i * 4 < bytes + off ? __ldg(w + i) : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = __funnelshift_r(v[i], v[i + 1], off * 8);
+    const int keep = bytes - 4 * i;
+    if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & ((1u << (8 * keep)) - 1u);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Row and place of item i of rows of `per` items
+struct RowItem {
+  int64_t row;
+  int64_t item;
+};
+__device__ __forceinline__ RowItem row_item(int64_t i, int64_t per, bool narrow) {
+  const int64_t r = narrow ? (int64_t)((uint32_t)i / (uint32_t)per) : i / per;
+  return RowItem{r, i - r * per};
+}
+
 // How a row-major result may be written: 2 = sectors of 32 bytes, 1 = 16 bytes,
 // 0 = element by element
 inline int row_stores(const void* ptr, int64_t row, int64_t col, int elem) {

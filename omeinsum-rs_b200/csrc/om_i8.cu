@@ -226,35 +226,28 @@ struct ScaleEpi {
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
 
-// Rows of 8-bit numbers at 16-byte aligned places, zero behind their end. A
-// thread makes 16: contiguous ones from the aligned words that hold them, shifted
-// into place; others one by one.
+// Rows of 8-bit numbers at 16-byte aligned places, zero behind their end; a
+// thread makes 16
 __global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int K, int64_t sr, int64_t sk,
                         int8_t* __restrict__ dst, int64_t ld) {
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    for (int c = (blockIdx.x * blockDim.x + threadIdx.x) * 16; c < ld; c += gridDim.x * blockDim.x * 16) {
-      __align__(16) uint32_t o[4] = {0, 0, 0, 0};
-      const int n = min(16, K - c);
-      if (sk == 1) {
-        const uintptr_t at = (uintptr_t)(src + r * sr + c);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
-        const int off = (int)(at & 3), shift = off * 8;
-        uint32_t v[5];
+  const int64_t per = ld / 16, total = rows * per;
+  const bool narrow = total < ((int64_t)1 << 32);
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const RowItem at = row_item(i, per, narrow);
+    const int c = (int)at.item * 16, n = min(16, K - c);
+    const int8_t* from = src + at.row * sr + (int64_t)c * sk;
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (sk == 1) {
+      o = load_bytes(from, n);
+    } else {
+      __align__(16) int8_t b[16] = {};
 #pragma unroll
-        for (int i = 0; i < 5; ++i) v[i] = i * 4 < n + off ? __ldg(w + i) : 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[i] = __funnelshift_r(v[i], v[i + 1], shift);
-          const int keep = n - 4 * i;  // bytes of this word inside the row
-          if (keep < 4) o[i] = keep <= 0 ? 0u : o[i] & ((1u << (8 * keep)) - 1u);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (i < n) o[i / 4] |= (uint32_t)(uint8_t)src[r * sr + (int64_t)(c + i) * sk] << (8 * (i % 4));
-      }
-      *reinterpret_cast<uint4*>(dst + r * ld + c) = make_uint4(o[0], o[1], o[2], o[3]);
+      for (int k = 0; k < 16; ++k)
+        if (k < n) b[k] = from[k * sk];
+      o = *reinterpret_cast<const uint4*>(b);
     }
+    *reinterpret_cast<uint4*>(dst + i * 16) = o;
   }
 }
 
@@ -431,10 +424,10 @@ int readable_i8(om_backend* be, const int8_t* src, int64_t rows, int64_t K, int6
   if ((sk == 1 || K == 1) && sr >= K && mma::tma_readable(src, sr, 1)) return OM_OK;
   const int64_t ld = (K + 15) / 16 * 16;
   OM_TRY(copy.alloc(be, (size_t)rows * ld));
-  const int threads = (int)std::min<int64_t>(128, (ld / 16 + 31) / 32 * 32);
-  const dim3 grid((unsigned)((ld / 16 + threads - 1) / threads), (unsigned)std::min<int64_t>(rows, 65535));
+  const int64_t items = rows * (ld / 16);
   ProfScope prof(be, "pack_i8");
-  pack_i8<<<grid, threads, 0, be->stream>>>(src, rows, (int)K, sr, sk, (int8_t*)copy.ptr, ld);
+  pack_i8<<<(unsigned)std::min<int64_t>((items + 255) / 256, (int64_t)be->num_sms * 16), 256, 0, be->stream>>>(
+      src, rows, (int)K, sr, sk, (int8_t*)copy.ptr, ld);
   note_launch();
   *out = mma::Matrix{copy.ptr, rows, K, ld, 1};
   return check_cuda(cudaGetLastError(), "matmul_i8 pack launch");

@@ -491,120 +491,131 @@ __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t a
                             T* __restrict__ out, int64_t dr, int64_t dc) {
   const float f = scale ? *scale : 1.f;
   const int64_t total = rows * cols;
+  const bool narrow = total < ((int64_t)1 << 32);
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / cols, c = i - r * cols;
+    const RowItem at = row_item(i, cols, narrow);
+    const int64_t r = at.row, c = at.item;
+    const float* from = acc + r * acc_ld + c;
     float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += acc[k * acc_split + r * acc_ld + c];
+#pragma unroll 8
+    for (int k = 0; k < splits; ++k) s += __ldcg(from + k * acc_split);
     out[r * dr + c * dc] = Elem<T>::store(s * f);
   }
 }
 
-// Rows of [rows, cols] as T with 16-byte aligned rows; zero where the target
-// lies outside the vocabulary (targets given), and in the padding. A thread
-// makes 8 elements; `vec`: they can be read at once.
+// A 16-bit matrix with rows at 16-byte aligned places, zero behind their end and
+// where the target lies outside the vocabulary (targets given). A thread makes 8
+// elements.
 template <typename T>
 __global__ void pack_rows(const T* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
-                          int64_t sc, int vec, T* __restrict__ dst, int64_t ld,
-                          const void* targets, int t64, int64_t vocab) {
-  const int64_t per = ld / 8;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    bool keep = true;
-    if (targets) {
-      const int64_t t = target_of(targets, t64, r);
-      keep = t >= 0 && t < vocab;
-    }
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < per;
-         i += (int64_t)gridDim.x * blockDim.x) {
-      const int64_t c = i * 8;
-      __align__(16) T v[8];
-      if (vec && keep && c + 8 <= cols) {
-        *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(src + r * sr + c);
+                          int64_t sc, T* __restrict__ dst, int64_t ld, const void* targets, int t64,
+                          int64_t vocab) {
+  const int64_t per = ld / 8, total = rows * per;
+  const bool narrow = total < ((int64_t)1 << 32);
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const RowItem at = row_item(i, per, narrow);
+    const int64_t c = at.item * 8;
+    const int n = (int)min((int64_t)8, cols - c);
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (!targets || (uint64_t)target_of(targets, t64, at.row) < (uint64_t)vocab) {
+      const T* from = src + at.row * sr + c * sc;
+      if (sc == 1 && n == 8 && !((uintptr_t)from & 15)) {
+        o = *reinterpret_cast<const uint4*>(from);
+      } else if (sc == 1) {
+        o = load_bytes(from, n * 2);
       } else {
+        __align__(16) T v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-          v[k] = keep && c + k < cols ? src[r * sr + (c + k) * sc] : T(0.f);
+        for (int k = 0; k < 8; ++k) v[k] = k < n ? from[k * sc] : T(0.f);
+        o = *reinterpret_cast<const uint4*>(v);
       }
-      *reinterpret_cast<uint4*>(dst + r * ld + c) = *reinterpret_cast<const uint4*>(v);
     }
+    *reinterpret_cast<uint4*>(dst + i * 8) = o;
   }
 }
-template <typename T>
-void launch_pack(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
-                 T* dst, int64_t ld, const void* targets, int t64, int64_t vocab) {
-  const int vec = sc == 1 && sr % 8 == 0 && !((uintptr_t)src & 15);
-  const int threads = (int)std::min<int64_t>(256, (ld / 8 + 31) / 32 * 32);
-  const dim3 grid((unsigned)std::min<int64_t>((ld / 8 + threads - 1) / threads, 65535),
-                  (unsigned)std::min<int64_t>(rows, 65535));
-  ProfScope prof(be, "loss_pack");
-  pack_rows<T><<<grid, threads, 0, be->stream>>>(src, rows, cols, sr, sc, vec, dst, ld, targets, t64, vocab);
-  note_launch();
-}
 
-// Rows of f32 as three bf16 planes, x = x0 + x1 + x2 to 24 bits; zero as above.
-// A thread makes 8 elements of each plane.
+// A matrix of f32 as three bf16 planes, x = x0 + x1 + x2 to 24 bits; zero as
+// above. A thread makes 8 elements of each plane.
 __global__ void split_rows(const float* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
                            int64_t sc, __nv_bfloat16* __restrict__ dst, int64_t ld, int64_t plane,
                            const void* targets, int t64, int64_t vocab) {
-  const int64_t per = ld / 8;
-  for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
-    bool keep = true;
-    if (targets) {
-      const int64_t t = target_of(targets, t64, r);
-      keep = t >= 0 && t < vocab;
-    }
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < per;
-         i += (int64_t)gridDim.x * blockDim.x) {
-      const int64_t c = i * 8;
-      float v[8];
+  const int64_t per = ld / 8, total = rows * per;
+  const bool narrow = total < ((int64_t)1 << 32);
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const RowItem at = row_item(i, per, narrow);
+    const int64_t c = at.item * 8;
+    const int n = (int)min((int64_t)8, cols - c);
+    float v[8] = {};
+    if (!targets || (uint64_t)target_of(targets, t64, at.row) < (uint64_t)vocab) {
+      const float* from = src + at.row * sr + c * sc;
+      if (sc == 1 && n == 8 && !((uintptr_t)from & 15)) {
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(from + 4);
+      } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = keep && c + k < cols ? src[r * sr + (c + k) * sc] : 0.f;
-#pragma unroll
-      for (int z = 0; z < 3; ++z) {
-        __align__(16) __nv_bfloat16 b[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          b[k] = __float2bfloat16_rn(v[k]);
-          v[k] -= __bfloat162float(b[k]);
-        }
-        *reinterpret_cast<uint4*>(dst + z * plane + r * ld + c) = *reinterpret_cast<const uint4*>(b);
+        for (int k = 0; k < 8; ++k)
+          if (k < n) v[k] = from[k * sc];
       }
+    }
+#pragma unroll
+    for (int z = 0; z < 3; ++z) {
+      __align__(16) __nv_bfloat16 b[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        b[k] = __float2bfloat16_rn(v[k]);
+        v[k] -= __bfloat162float(b[k]);
+      }
+      *reinterpret_cast<uint4*>(dst + z * plane + i * 8) = *reinterpret_cast<const uint4*>(b);
     }
   }
 }
 
-// The operand itself when TMA can read its rows, else a packed copy.
-int readable(om_backend* be, const float* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
-             Scratch& copy, mma::Matrix* out, const LossArgs* masked = nullptr) {
-  const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld;
-  if (!copy.ptr) OM_TRY(copy.alloc(be, (size_t)plane * 6));
-  const int threads = (int)std::min<int64_t>(256, (ld / 8 + 31) / 32 * 32);
-  const dim3 grid((unsigned)std::min<int64_t>((ld / 8 + threads - 1) / threads, 65535),
-                  (unsigned)std::min<int64_t>(rows, 65535));
-  ProfScope prof(be, "loss_split");
-  split_rows<<<grid, threads, 0, be->stream>>>(src, rows, cols, sr, sc, (__nv_bfloat16*)copy.ptr, ld,
-                                               plane, masked ? masked->targets : nullptr,
-                                               masked ? masked->target64 : 0, masked ? masked->V : 0);
-  note_launch();
-  *out = mma::Matrix{copy.ptr, rows, cols, ld, 2, plane};
-  return check_cuda(cudaGetLastError(), "loss split launch");
-}
+// What a copy of an operand takes: f32 is always split, 16-bit rows are copied
+// where TMA cannot read them or rows without a loss must be zero
 template <typename T>
-int readable(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
-             Scratch& copy, mma::Matrix* out, const LossArgs* masked = nullptr) {
-  *out = mma::Matrix{src, rows, cols, sr, 2};
-  if (!masked && (sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2)) return OM_OK;
+size_t copy_bytes(const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc, bool masked) {
   const int64_t ld = (cols + 7) / 8 * 8;
-  if (!copy.ptr) OM_TRY(copy.alloc(be, (size_t)rows * ld * 2));
-  launch_pack<T>(be, src, rows, cols, sr, sc, (T*)copy.ptr, ld, masked ? masked->targets : nullptr,
-                 masked ? masked->target64 : 0, masked ? masked->V : 0);
-  *out = mma::Matrix{copy.ptr, rows, cols, ld, 2};
-  return check_cuda(cudaGetLastError(), "loss pack launch");
+  if (sizeof(T) == 4) return (size_t)rows * ld * 6;
+  const bool readable = (sc == 1 || cols == 1) && sr >= cols && mma::tma_readable(src, sr, 2);
+  return readable && !masked ? 0 : (size_t)rows * ld * 2;
+}
+// The operand as the products take it, from `copy` (copy_bytes of it) or in place
+template <typename T>
+int operand(om_backend* be, const T* src, int64_t rows, int64_t cols, int64_t sr, int64_t sc,
+            void* copy, mma::Matrix* out, const LossArgs* masked = nullptr) {
+  if (!copy_bytes(src, rows, cols, sr, sc, masked != nullptr)) {
+    *out = mma::Matrix{src, rows, cols, sr, 2};
+    return OM_OK;
+  }
+  const int64_t ld = (cols + 7) / 8 * 8, plane = rows * ld, items = plane / 8;
+  const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, (int64_t)be->num_sms * 16));
+  const void* targets = masked ? masked->targets : nullptr;
+  const int t64 = masked ? masked->target64 : 0;
+  const int64_t vocab = masked ? masked->V : 0;
+  ProfScope prof(be, sizeof(T) == 4 ? "loss_split" : "loss_pack");
+  if constexpr (sizeof(T) == 4)
+    split_rows<<<grid, 256, 0, be->stream>>>(src, rows, cols, sr, sc, (__nv_bfloat16*)copy, ld, plane,
+                                             targets, t64, vocab);
+  else
+    pack_rows<T><<<grid, 256, 0, be->stream>>>(src, rows, cols, sr, sc, (T*)copy, ld, targets, t64, vocab);
+  note_launch();
+  *out = mma::Matrix{copy, rows, cols, ld, 2, sizeof(T) == 4 ? plane : 0};
+  return check_cuda(cudaGetLastError(), "loss operand launch");
 }
 
-// Rows 16-byte aligned and zero-filled either way: the operand itself when TMA
-// can read it, else a copy (f32: always, as three planes); `masked`: a copy
-// whose rows without a loss are zero.
+// One allocation in parts of 256 bytes' alignment
+struct Parts {
+  size_t bytes = 0;
+  size_t add(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+
 template <typename T, bool AMN, bool BMN, class Epi>
 int product(om_backend* be, const char* name, const mma::Matrix& a, const mma::Matrix& b,
             mma::Tiling t, int splits, const Epi& epi) {
@@ -640,19 +651,25 @@ int64_t weight_rows(const LossArgs& p) {
 
 template <typename T>
 int loss_forward_tc(om_backend* be, const LossArgs& p, float* loss, float* lse) {
-  Scratch xc, wc, ws;
-  mma::Matrix x, w;
-  OM_TRY(readable(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xc, &x));
+  const T *px = (const T*)p.x, *pw = (const T*)p.w;
   const int64_t W = weight_rows<T>(p);
   const mma::Tiling t = tiles<T>(be, p.N, W, true);
   const int64_t slots = ((p.V + W - 1) / W) * ((W + t.bn - 1) / t.bn) * 2;
-  OM_TRY(ws.alloc(be, (size_t)p.N * (slots * 8 + 4)));
-  float2* part = (float2*)ws.ptr;
-  float* hit = (float*)(part + slots * p.N);
+  Parts parts;
+  const size_t ax = parts.add(copy_bytes(px, p.N, p.D, p.xn, p.xd, false));
+  const size_t aw = parts.add(copy_bytes(pw, W, p.D, p.wv, p.wd, false));
+  const size_t ap = parts.add((size_t)p.N * slots * 8), ah = parts.add((size_t)p.N * 4);
+  Scratch ws;
+  OM_TRY(ws.alloc(be, parts.bytes));
+  char* at = (char*)ws.ptr;
+  float2* part = (float2*)(at + ap);
+  float* hit = (float*)(at + ah);
+  mma::Matrix x, w;
+  OM_TRY(operand(be, px, p.N, p.D, p.xn, p.xd, at + ax, &x));
   int64_t used = 0;
   for (int64_t v0 = 0; v0 < p.V; v0 += W) {
     const int64_t n = std::min(W, p.V - v0);
-    OM_TRY(readable(be, (const T*)p.w + v0 * p.wv, n, p.D, p.wv, p.wd, wc, &w));
+    OM_TRY(operand(be, pw + v0 * p.wv, n, p.D, p.wv, p.wd, at + aw, &w));
     const StatsEpi epi{p.targets, p.target64, v0, part + used * p.N, p.N, hit};
     OM_TRY((product<T, false, false>(be, "loss_logits", x, w, t, 1, epi)));
     used += (n + t.bn - 1) / t.bn * 2;
@@ -677,20 +694,6 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
   const int64_t fit = ((int64_t)256 << 20) / p.N / 256 * 256;
   const int64_t P = std::min({(p.V + 255) / 256 * 256, std::max<int64_t>(256, fit),
                               (weight_rows<T>(p) + 255) / 256 * 256});
-  Scratch xs, wc, dzs, accs, scales;
-  OM_TRY(dzs.alloc(be, (size_t)p.N * P * 2 * PLANES));
-  // rows without a loss are zero here: whatever they hold reaches no gradient
-  mma::Matrix x, w;
-  OM_TRY(readable(be, (const T*)p.x, p.N, p.D, p.xn, p.xd, xs, &x, &p));
-  if (PLANES == 1) OM_TRY(readable(be, (const T*)p.w, p.V, p.D, p.wv, p.wd, wc, &w));
-  float* scale = nullptr;
-  if (PLANES == 1) {
-    OM_TRY(scales.alloc(be, 4));
-    scale = (float*)scales.ptr;
-    gradient_scale<<<1, 1024, 0, be->stream>>>(dloss, p.targets, p.target64, p.V, p.N,
-                                               std::is_same<T, __half>::value ? 16384.f : 1.f, scale);
-    note_launch();
-  }
   // dx sums over the vocabulary. Its tiles are the widest that there are, and
   // where they leave SMs idle the sum is split, 16 slabs of 64 entries at least
   // to a split, which is worth its f32 sums (509 x 771 x 8191 f32: 80 us with
@@ -704,18 +707,39 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
   const int64_t least = (std::min(P, p.V) + 63) / 64;
   const int splits = (int)std::max<int64_t>(1, std::min<int64_t>({slots / txt, least / 16, 64}));
   const int64_t acc_ld = (p.D + tx.bn - 1) / tx.bn * tx.bn;
-  const bool sums = splits > 1 || P < p.V;
-  if (sums) OM_TRY(accs.alloc(be, (size_t)splits * p.N * acc_ld * 4));
-  float* acc = (float*)accs.ptr;
+  const T *px = (const T*)p.x, *pw = (const T*)p.w;
+  const int64_t W = PLANES == 3 ? std::min(P, p.V) : p.V;
+  Parts parts;
+  const size_t az = parts.add((size_t)p.N * P * 2 * PLANES);
+  const size_t ax = parts.add(copy_bytes(px, p.N, p.D, p.xn, p.xd, true));
+  const size_t aw = parts.add(copy_bytes(pw, W, p.D, p.wv, p.wd, false));
+  const size_t as = parts.add(4);
+  const size_t aa = parts.add(splits > 1 || P < p.V ? (size_t)splits * p.N * acc_ld * 4 : 0);
+  Scratch ws;
+  OM_TRY(ws.alloc(be, parts.bytes));
+  char* at = (char*)ws.ptr;
+  void* dzs = at + az;
+  float* acc = (float*)(at + aa);
+  float* scale = nullptr;
+  // rows without a loss are zero here: whatever they hold reaches no gradient
+  mma::Matrix x, w;
+  OM_TRY(operand(be, px, p.N, p.D, p.xn, p.xd, at + ax, &x, &p));
+  if (PLANES == 1) {
+    OM_TRY(operand(be, pw, p.V, p.D, p.wv, p.wd, at + aw, &w));
+    scale = (float*)(at + as);
+    gradient_scale<<<1, 1024, 0, be->stream>>>(dloss, p.targets, p.target64, p.V, p.N,
+                                               std::is_same<T, __half>::value ? 16384.f : 1.f, scale);
+    note_launch();
+  }
   const int vecx = row_stores(dx, dxn, dxd, sizeof(T)), vecw = row_stores(dw, dwv, dwd, sizeof(T));
   for (int64_t v0 = 0; v0 < p.V; v0 += P) {
     const int64_t n = std::min(P, p.V - v0);
     const bool last = v0 + n == p.V;
     mma::Matrix wp;
     if (PLANES == 1) wp = rows_of(w, v0, n);
-    else OM_TRY(readable(be, (const T*)p.w + v0 * p.wv, n, p.D, p.wv, p.wd, wc, &wp));
-    const mma::Matrix dz{dzs.ptr, p.N, n, P, 2, PLANES == 3 ? p.N * P : 0};
-    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs.ptr, P, p.N * P};
+    else OM_TRY(operand(be, pw + v0 * p.wv, n, p.D, p.wv, p.wd, at + aw, &wp));
+    const mma::Matrix dz{dzs, p.N, n, P, 2, PLANES == 3 ? p.N * P : 0};
+    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs, P, p.N * P};
     OM_TRY((product<T, false, false>(be, "loss_dlogits", x, wp, tiles<T>(be, p.N, n), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
     const OutEpi<T> xe{dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
