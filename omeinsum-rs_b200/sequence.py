@@ -208,6 +208,8 @@ class _Call:
         if like is not None:
             if same is not None and same.is_contiguous():
                 t = _torch.empty_like(same)
+            elif like.dtype is _torch_types[code]:
+                t = like.new_empty(shape)
             else:
                 t = _torch.empty(shape, dtype=_torch_types[code], device=like.device)
             return t, t.data_ptr()
