@@ -3,8 +3,8 @@
 //
 // A step is the map s -> P s + Q with (P, Q) = (a, b) (backward: (a, a dh)), and
 // maps compose, so time can be cut into chunks that run side by side:
-//   map_kernel    composes the steps of each chunk, and of eight consecutive
-//                 chunks (a block's) together;
+//   map_kernel    composes the steps of each chunk, and of the consecutive
+//                 chunks of a block together;
 //   step_kernel   joins the maps before its chunk to the state that enters it
 //                 and takes the chunk's steps one by one, writing the results.
 // A warp has 32 lanes of 8 bytes of channels (one channel where rows are not
@@ -47,11 +47,13 @@ struct ScanArgs {
   void* dh0;
 };
 
-constexpr int WARPS = 8;  // of a block
-// Blocks of an SM: two, whose lanes keep twice eight steps in registers (8-byte
-// rows; four blocks of half as many are up to 20 % slower), three where rows
-// are 4 bytes of a lane.
-constexpr int blocks_of(int lane_bytes) { return lane_bytes == 4 ? 3 : 2; }
+// Warps of a block and blocks of an SM, by the bytes of a row that a lane has.
+// 16 warps of 8-byte rows keep twice eight steps in registers (32 with half as
+// many under way are up to 20 % slower), in blocks of four, which share out
+// evenly; narrower rows do better in blocks of eight (7 x 1531 x 1001 f32 with
+// the backward pass: 106 us, in blocks of four 121).
+constexpr int warps_of(int lane_bytes) { return lane_bytes == 8 ? 4 : 8; }
+constexpr int blocks_of(int lane_bytes) { return lane_bytes == 8 ? 4 : lane_bytes == 4 ? 3 : 2; }
 
 struct ChunkArgs {
   int64_t groups;   // of VEC channels, a lane's
@@ -393,10 +395,11 @@ __device__ __forceinline__ void compose(Map<T, V>& m, Lane<T, V> g, Lane<T, V> x
 }
 
 template <typename T, int V, bool SIG, bool BWD>
-__global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) map_kernel(const __grid_constant__ ScanArgs p,
+__global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof(T) * V)) map_kernel(const __grid_constant__ ScanArgs p,
                                                             const __grid_constant__ ChunkArgs a) {
   using S = typename Elem<T>::State;
   using L = Lane<T, V>;
+  constexpr int WARPS = warps_of(sizeof(T) * V);
   __shared__ Pair<S> part[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
@@ -442,12 +445,13 @@ __global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) map_kern
 // ---- the steps ------------------------------------------------------------------------
 
 template <typename T, int V, bool SIG, bool BWD>
-__global__ void __launch_bounds__(WARPS * 32, blocks_of(sizeof(T) * V)) step_kernel(const __grid_constant__ ScanArgs p,
+__global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof(T) * V)) step_kernel(const __grid_constant__ ScanArgs p,
                                                              const __grid_constant__ ChunkArgs a) {
   using S = typename Elem<T>::State;
   using L = Lane<T, V>;
   using K = typename L::K;
   using R = typename L::R;
+  constexpr int WARPS = warps_of(sizeof(T) * V);
   __shared__ Pair<S> part[WARPS][32 * V], chunk[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int wt = a.warps_t, team = warp / wt, tw = warp % wt;
@@ -601,6 +605,7 @@ bool aligned(const ScanArgs& p, int elem, int bytes, bool backward, bool need_x)
 template <typename T, int V, bool SIG, bool BWD>
 int launch_chunks(om_backend* be, const ScanArgs& p) {
   using S = typename Elem<T>::State;
+  constexpr int WARPS = warps_of(sizeof(T) * V);
   ChunkArgs a{};
   a.groups = p.B * (p.D / V);
   const int64_t columns = (a.groups + 31) / 32;
@@ -617,7 +622,7 @@ int launch_chunks(om_backend* be, const ScanArgs& p) {
   if (columns < 4 * be->num_sms) {
     chunks = warps / columns;
     if (chunks >= WARPS) chunks = chunks / WARPS * WARPS;
-    else chunks = chunks >= 4 ? 4 : 2;
+    else chunks = chunks >= 4 ? 4 : chunks >= 2 ? 2 : 1;
     chunks = std::max<int64_t>(1, std::min(chunks, p.T / 16));
   }
   a.steps = std::max<int64_t>(1, (p.T + chunks - 1) / chunks);
