@@ -1,5 +1,7 @@
 // Matrix product in 8-bit integers with scales for each row and channel, and
-// the quantiser of its rows.
+// the quantiser of its rows. Sums are 32-bit integers; the scales are applied in
+// f32, in one order, and the result is rounded once, so every variant gives the
+// same bits.
 #include <algorithm>
 
 #include "om_convert.cuh"
@@ -256,6 +258,11 @@ __global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int K, int
 constexpr int TOKEN_ROWS = 8;
 constexpr int TOKEN_SMEM = 160 * 1024;
 
+// Up to eight rows: from nine on the tensor cores' product, which wastes most of
+// its rows but none of the weights, is as fast (the dot products of sixteen rows
+// would take longer than the weights). One row of 4096 through 4096 x 4096:
+// 5.6 us with the weights in L2, 9.3 us from memory (floor 2.6 us): latency of
+// the row, its maximum and the first weights.
 // A block keeps the M <= MM rows of q in shared memory and walks its share of
 // the channels, a warp per channel: 16 weights per lane and step, four
 // products per instruction, one shuffle reduction per row. T: the type of y,

@@ -7,7 +7,10 @@
 // columns; the backward computes the logits a second time, a piece of the
 // vocabulary at a time, writes dz of the piece once and multiplies it twice:
 // 8 N D V operations, of which 6 are needed. Bound by the tensor cores, or,
-// for few tokens, by reading w.
+// for few tokens, by reading w. Measured: 8192 x 4096 x 128000 bf16 with
+// gradients 25.3 ms (34.4 TFLOP at 1.36 PFLOP/s, the card's power limit; writing
+// the logits once and reading them three times would save 8.6 TFLOP and cost
+// 4.2 GB held); 24 x 2048 x 32000 f16 forward 34 us, 20 of which w needs.
 #include <algorithm>
 #include <cfloat>
 
@@ -300,7 +303,7 @@ struct StatsEpi {
 // Joins the slots of 8 rows per block, each of 32 threads of a row every 32nd
 // slot; a row's threads are a stride of 8 apart, so that a slot's rows are read
 // together. (32 rows by 8 threads left 4096 rows on 128 blocks of 50 dependent
-// loads each: 36 us against 9.)
+// loads each: 36 us against 8.)
 __global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ part, int slots,
                                                   int64_t rows, const void* targets, int t64,
                                                   int64_t vocab, const float* hit, float* loss,
@@ -484,7 +487,7 @@ struct OutEpi {
   __device__ __forceinline__ void end(Row&, int, bool, int) const {}
 };
 
-// out = scale * sum of the splits
+// out = scale * sum of the splits; bound by reading them
 template <typename T>
 __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t acc_split,
                             int64_t acc_ld, int64_t rows, int64_t cols, const float* scale,

@@ -3,7 +3,7 @@
 //
 // Persistent: each CTA (CG = 1) or pair of CTAs (CG = 2) takes tiles of
 // 128 CG x BN round robin. 320 threads: warp 0 issues TMA loads of 128-byte
-// deep k slabs into a ring of stages, one thread of warp 1 issues the MMAs
+// deep k slabs into a ring of stages, warp 1 issues the MMAs
 // (accumulators in tensor memory, two of them, so that one tile's epilogue
 // runs under the next tile's products), warps 2..9 read a finished
 // accumulator and hand it to the epilogue 32 columns at a time: warp w has the
@@ -24,6 +24,12 @@
 // core does not round its running sum to nearest, so every CHUNK slabs are
 // summed from zero and added up in the epilogue warps' registers. The planes
 // of a slab are loaded once for all six.
+//
+// Bound by the tensor cores: 4096 x 1024 by 50001 x 1024 bf16 with the cross
+// entropy's forward epilogue takes 257 us, 1.63 PFLOP/s with the tensor pipe 93 %
+// active (the library product of the same size 293 us); 8192 x 4096 by 12288 x 4096
+// in 8 bits 239 us, 3.4 POP/s, 92 %. Launches that follow one another for
+// milliseconds run at the card's power limit, 1.36 PFLOP/s.
 //
 // Every wait is bounded; on expiry the kernel records an error word that
 // om_b200_sync reports, and leaves after its other bounded waits.
