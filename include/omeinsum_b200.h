@@ -398,7 +398,8 @@ int om_b200_gated_scan_backward(om_backend* be, om_gate kind, om_dtype dtype, co
  * loss: loss is 0 there (lse is still written).  loss and lse are N contiguous
  * f32 values (f64 for OM_F64).  16-bit products accumulate in f32. f32 runs on
  * the tensor cores as three bf16 parts of each number (six products, error about
- * 2^-22 * sum_d |x||w|), or as f32 FMA in OM_F32_EXACT mode. */
+ * 2^-22 * sum_d |x||w|), or as f32 FMA in OM_F32_EXACT mode and for up to
+ * eight tokens. */
 int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, const int64_t* shape,
                                  const void* x, const int64_t* strides_x, const void* w,
                                  const int64_t* strides_w, om_dtype target_dtype,

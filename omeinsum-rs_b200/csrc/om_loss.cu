@@ -759,6 +759,27 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
   return check_cuda(cudaGetLastError(), "loss backward launch");
 }
 
+#include "om_loss_few.cuh"
+
+int forward_f32(om_backend* be, const LossArgs& p, float* loss, float* lse) {
+  if (few_tokens(p)) {
+    if (p.N == 1) return few_forward<1>(be, few_args(p), p, loss, lse);
+    if (p.N <= 4) return few_forward<4>(be, few_args(p), p, loss, lse);
+    return few_forward<FEW>(be, few_args(p), p, loss, lse);
+  }
+  return be->f32_exact ? loss_forward<float>(be, p, loss, lse) : loss_forward_tc<float>(be, p, loss, lse);
+}
+int backward_f32(om_backend* be, const LossArgs& p, const float* lse, const float* dloss, float* dx,
+                 int64_t dxd, int64_t dxn, float* dw, int64_t dwd, int64_t dwv) {
+  if (p.N > 0 && few_tokens(p)) {
+    if (p.N == 1) return few_backward<1>(be, few_args(p), p, lse, dloss, dx, dxd, dxn, dw, dwd, dwv);
+    if (p.N <= 4) return few_backward<4>(be, few_args(p), p, lse, dloss, dx, dxd, dxn, dw, dwd, dwv);
+    return few_backward<FEW>(be, few_args(p), p, lse, dloss, dx, dxd, dxn, dw, dwd, dwv);
+  }
+  return be->f32_exact ? loss_backward<float>(be, p, lse, dloss, dx, dxd, dxn, dw, dwd, dwv)
+                       : loss_backward_tc<float>(be, p, lse, dloss, dx, dxd, dxn, dw, dwd, dwv);
+}
+
 int check_loss(const char* who, om_backend* be, om_dtype dtype, const int64_t* shape,
                om_dtype target_dtype) {
   const std::string w(who);
@@ -795,8 +816,7 @@ extern "C" int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, cons
   if (dtype == OM_F64) return loss_forward<double>(be, p, (double*)loss, (double*)lse);
   if (dtype == OM_BF16) return loss_forward_tc<__nv_bfloat16>(be, p, (float*)loss, (float*)lse);
   if (dtype == OM_F16) return loss_forward_tc<__half>(be, p, (float*)loss, (float*)lse);
-  if (be->f32_exact) return loss_forward<float>(be, p, (float*)loss, (float*)lse);
-  return loss_forward_tc<float>(be, p, (float*)loss, (float*)lse);
+  return forward_f32(be, p, (float*)loss, (float*)lse);
 }
 
 extern "C" int om_b200_linear_cross_entropy_backward(
@@ -815,12 +835,11 @@ extern "C" int om_b200_linear_cross_entropy_backward(
   const LossArgs p{shape[1], shape[0], shape[2], x, strides_x[0], strides_x[1], w, strides_w[0],
                    strides_w[1], targets, target_dtype == OM_I64};
 #define OM_LOSS_BWD(FN, T, S)                                                               \
-  FN<T>(be, p, (const S*)lse, (const S*)dloss, (T*)dx, strides_dx[0], strides_dx[1], \
+  FN(be, p, (const S*)lse, (const S*)dloss, (T*)dx, strides_dx[0], strides_dx[1], \
                    (T*)dw, strides_dw[0], strides_dw[1])
-  if (dtype == OM_F64) return OM_LOSS_BWD(loss_backward, double, double);
-  if (dtype == OM_BF16) return OM_LOSS_BWD(loss_backward_tc, __nv_bfloat16, float);
-  if (dtype == OM_F16) return OM_LOSS_BWD(loss_backward_tc, __half, float);
-  if (be->f32_exact) return OM_LOSS_BWD(loss_backward, float, float);
-  return OM_LOSS_BWD(loss_backward_tc, float, float);
+  if (dtype == OM_F64) return OM_LOSS_BWD(loss_backward<double>, double, double);
+  if (dtype == OM_BF16) return OM_LOSS_BWD(loss_backward_tc<__nv_bfloat16>, __nv_bfloat16, float);
+  if (dtype == OM_F16) return OM_LOSS_BWD(loss_backward_tc<__half>, __half, float);
+  return OM_LOSS_BWD(backward_f32, float, float);
 #undef OM_LOSS_BWD
 }

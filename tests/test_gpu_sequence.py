@@ -255,7 +255,7 @@ def check_loss(be, seq, X, W, T, G, x, w, targets, g, dtype):
 
 
 LOSS_SHAPES = [(1, 64, 100), (1, 1, 1), (3, 5, 2), (24, 2048, 1000), (7, 33, 129), (128, 64, 256), (129, 65, 257), (130, 136, 1030), (300, 200, 4111),
-               (64, 512, 20000), (513, 96, 777), (257, 1000, 384)]
+               (64, 512, 20000), (513, 96, 777), (257, 1000, 384), (8, 1000, 5003), (5, 2304, 130), (4, 72, 9001), (2, 9001, 40), (2, 16380, 33), (5, 6540, 33), (8, 8000, 70)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
