@@ -122,7 +122,7 @@ __device__ __forceinline__ RowItem row_item(int64_t i, int64_t per, bool narrow)
 // 0 = element by element
 inline int row_stores(const void* ptr, int64_t row, int64_t col, int elem) {
   const uint64_t at = (uint64_t)(uintptr_t)ptr | (uint64_t)(row * elem);
-  return col != 1 || at % 16 ? 0 : at % 32 ? 1 : 2;
+  return col != 1 || row <= 0 || at % 16 ? 0 : at % 32 ? 1 : 2;
 }
 
 inline bool is_half(om_dtype dt) { return dt == OM_BF16 || dt == OM_F16; }

@@ -177,12 +177,12 @@ struct ScaleEpi {
   struct Row {
     float s;
   };
-  bool turns() const { return !vec; }
+  int lent_bytes() const { return vec ? 0 : mma::TURN_BYTES; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     return Row{in ? q_scale[m] : 0.f};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32], float* turn) const {
+                                          const uint32_t (&r)[32], mma::Lent& lent) const {
     if (n0 >= N) return;
     float v[32];
     if (wide && N - n0 >= 32) {
@@ -213,7 +213,7 @@ struct ScaleEpi {
     const int lane = threadIdx.x & 31;
     T* to = y + (int64_t)m * dr;
     if (!vec) {
-      store_turned(turn, v, y + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
+      store_turned(lent.words, v, y + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
                    __popc(__ballot_sync(0xffffffffu, in)), N - n0);
     } else if (in) {
       if (N - n0 >= 32) {

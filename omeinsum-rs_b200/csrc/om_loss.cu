@@ -255,12 +255,12 @@ struct StatsEpi {
     float m, s;
     int64_t target;
   };
-  bool turns() const { return false; }
+  int lent_bytes() const { return 0; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     return Row{-INFINITY, 0.f, in ? target_of(targets, t64, m) - v0 : -1};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32], float* turn) const {
+                                          const uint32_t (&r)[32], mma::Lent& lent) const {
     if (n0 >= N) return;
     const int n = N - n0;  // columns that exist
     float top = __uint_as_float(r[0]);
@@ -374,10 +374,23 @@ __global__ void gradient_scale(const float* __restrict__ dloss, const void* targ
   *scale = f >= FLT_MIN && f < INFINITY ? f : 1.f;
 }
 
+// 32 columns of a warp's rows, rounded to T, through TMA; m: this lane's row. A
+// warp whose first row does not exist has none.
+template <typename T>
+__device__ __forceinline__ void store_half_box(mma::Lent& lent, const CUtensorMap* map,
+                                               const float (&v)[32], int n0, int m, bool in) {
+  if (!__shfl_sync(0xffffffffu, in, 0)) return;
+  uint32_t u[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c) u[c] = pack2(v[2 * c], v[2 * c + 1], T());
+  mma::store_box(lent, map, u, n0, m - (int)(threadIdx.x & 31));
+}
+
 // dz of a piece, rounded to T; the buffer's rows hold whole tiles. f32: as the
 // three bf16 planes that the two products take.
 template <typename T>
 struct GradEpi {
+  CUtensorMap map;  // of the piece of dz (16 bits)
   const void* targets;
   int t64;
   int64_t vocab, v0;
@@ -388,7 +401,7 @@ struct GradEpi {
     float lse, g;
     int64_t target;  // within the piece
   };
-  bool turns() const { return false; }
+  int lent_bytes() const { return sizeof(T) == 2 ? 2 * mma::BOX_BYTES : 0; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     Row row{0.f, 0.f, -1};
     if (in) {
@@ -404,8 +417,8 @@ struct GradEpi {
     return row;
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32], float* turn) const {
-    if (!in) return;
+                                          const uint32_t (&r)[32], mma::Lent& lent) const {
+    if (n0 >= N) return;
     float v[32];
 #pragma unroll
     for (int c = 0; c < 32; ++c)
@@ -417,8 +430,8 @@ struct GradEpi {
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
     }
     if constexpr (sizeof(T) == 2) {
-      store_row((T*)dz + (int64_t)m * ld + n0, v, true);
-    } else {
+      store_half_box<T>(lent, &map, v, n0, m, in);
+    } else if (in) {
       __nv_bfloat16* to = (__nv_bfloat16*)dz + (int64_t)m * ld + n0;
 #pragma unroll
       for (int z = 0; z < 3; ++z) {
@@ -434,6 +447,7 @@ struct GradEpi {
 // Sums in f32 kept for later pieces or splits, or the finished result as T.
 template <typename T>
 struct OutEpi {
+  CUtensorMap map;     // of `out` (16 bits, vec)
   T* out;
   int64_t dr, dc;
   int vec;             // row_stores of `out`
@@ -445,13 +459,15 @@ struct OutEpi {
     float f;
     float* acc;
   };
-  bool turns() const { return !vec && !keep; }
+  int lent_bytes() const {
+    return keep ? 0 : !vec ? mma::TURN_BYTES : sizeof(T) == 2 ? 2 * mma::BOX_BYTES : 0;
+  }
   __device__ __forceinline__ Row begin(int m, bool in, int split) const {
     return Row{scale ? *scale : 1.f,
                acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
-                                          const uint32_t (&r)[32], float* turn) const {
+                                          const uint32_t (&r)[32], mma::Lent& lent) const {
     if (n0 >= N) return;
     float v[32];
 #pragma unroll
@@ -470,11 +486,13 @@ struct OutEpi {
 #pragma unroll
     for (int c = 0; c < 32; ++c) v[c] *= row.f;
     const int lane = threadIdx.x & 31;
-    T* to = out + (int64_t)m * dr;
     if (!vec) {
-      store_turned(turn, v, out + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
+      store_turned(lent.words, v, out + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
                    __popc(__ballot_sync(0xffffffffu, in)), N - n0);
+    } else if constexpr (sizeof(T) == 2) {
+      store_half_box<T>(lent, &map, v, n0, m, in);
     } else if (in) {
+      T* to = out + (int64_t)m * dr;
       if (N - n0 >= 32) {
         store_row(to + n0, v, vec == 2);
       } else {
@@ -742,12 +760,15 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
     if (PLANES == 1) wp = rows_of(w, v0, n);
     else OM_TRY(operand(be, pw + v0 * p.wv, n, p.D, p.wv, p.wd, at + aw, &wp));
     const mma::Matrix dz{dzs, p.N, n, P, 2, PLANES == 3 ? p.N * P : 0};
-    const GradEpi<T> ge{p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs, P, p.N * P};
+    GradEpi<T> ge{{}, p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs, P, p.N * P};
+    if (PLANES == 1) OM_TRY(mma::encode_result(&ge.map, dzs, p.N, n, P));
     OM_TRY((product<T, false, false>(be, "loss_dlogits", x, wp, tiles<T>(be, p.N, n), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
-    const OutEpi<T> xe{dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
+    OutEpi<T> xe{{}, dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
+    if (PLANES == 1 && vecx) OM_TRY(mma::encode_result(&xe.map, dx, p.N, p.D, dxn));
     OM_TRY((product<T, false, true>(be, "loss_dx", dz, turned(wp), tx, now, xe)));
-    const OutEpi<T> we{dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
+    OutEpi<T> we{{}, dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
+    if (PLANES == 1 && vecw) OM_TRY(mma::encode_result(&we.map, dw + v0 * dwv, n, p.D, dwv));
     OM_TRY((product<T, true, true>(be, "loss_dw", turned(dz), turned(x), tiles<T>(be, n, p.D), 1, we)));
   }
   if (splits > 1) {

@@ -56,7 +56,10 @@ constexpr int SLAB = 128;           // bytes of k per stage
 constexpr int CHUNK = 2;            // slabs of a sum (P3)
 constexpr int A_BYTES = TM * SLAB;
 constexpr uint32_t WAIT_LIMIT = 1u << 24;
-constexpr int TURN_BYTES = 32 * 33 * 4;  // 32 rows of 32 values, a word apart
+// Shared memory that an epilogue asks for, per warp: for turning 32 rows of 32
+// values (a word of padding each), or for two boxes of 32 x 32 16-bit results
+// that TMA stores.
+constexpr int TURN_BYTES = 32 * 33 * 4, BOX_BYTES = 32 * 32 * 2;
 
 struct Shape {
   int M, N;        // rows of A and of B
@@ -64,7 +67,7 @@ struct Shape {
   int BN;          // columns of a tile: 32 .. 256, a multiple of 32
   int stages;
   int a_rows;      // rows of A's box: 128, or fewer where all of A has fewer
-  int turn;        // bytes of shared memory for turning a warp's results, or 0
+  int lent;        // bytes of shared memory lent to each epilogue warp
   int tiles_m, tiles_n, splits;
   int group;       // row tiles that are walked before the next column tile
   uint32_t idesc;  // instruction descriptor
@@ -208,6 +211,41 @@ __device__ __forceinline__ void read_columns(uint32_t addr, uint32_t (&x)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// What a warp's epilogue has been lent, and how many boxes it has stored from it
+struct Lent {
+  float* words;
+  int boxes = 0;
+};
+
+// A 32 x 32 box of 16-bit results (row by lane, 64 bytes each) to (x, y) of a
+// map made by encode_result: written to shared memory with the map's 64-byte
+// swizzle, two boxes in turn, and stored by TMA, which leaves out what lies
+// outside the matrix. (Lanes storing their own row touch 32 lines with each
+// instruction, which took longer than the products of a few slabs.)
+__device__ __forceinline__ void store_box(Lent& lent, const CUtensorMap* map, const uint32_t (&u)[16],
+                                          int x, int y) {
+  const int lane = threadIdx.x & 31;
+  char* box = reinterpret_cast<char*>(lent.words) + (lent.boxes & 1) * BOX_BYTES;
+  if (lent.boxes >= 2) {  // the box's last store has read it
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        make_uint4(u[4 * j], u[4 * j + 1], u[4 * j + 2], u[4 * j + 3]);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  if (lane == 0) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                     (uint64_t)map),
+                 "r"(x), "r"(y), "r"(smem_addr(box))
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+  }
+  ++lent.boxes;
+}
+
 // the k slabs of split s: [first, last)
 __device__ __forceinline__ int slab_at(const Shape& g, int s) {
   return (int)((int64_t)g.slabs * s / g.splits);
@@ -230,10 +268,10 @@ __device__ __forceinline__ Tile tile_at(const Shape& g, int t) {
 }
 
 // Epi, per lane and tile: Row begin(m, in, split) before the accumulator is
-// read; columns(row, m, in, n0, N, values, turn) for each 32 columns from n0 on,
+// read; columns(row, m, in, n0, N, values, lent) for each 32 columns from n0 on,
 // by whole warps; and end(row, m, in, slot) with slot = 2 * column tile + column
-// group. `in`: row m exists; columns from N on do not. `turn`: shared memory of
-// the warp's own, if turns() asked for it.
+// group. `in`: row m exists; columns from N on do not. `lent`: shared memory of
+// the warp's own, as much as lent_bytes() says.
 template <bool I8, bool P3, bool AMN, bool BMN, int CG, class Epi>
 __global__ void __launch_bounds__(THREADS, 1)
     product_kernel(const __grid_constant__ CUtensorMap amap, const __grid_constant__ CUtensorMap bmap,
@@ -396,9 +434,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncwarp();
   } else {  // epilogue
     const int quad = warp & 3, part = (warp - 2) >> 2;
-    // this warp's place for turning results (where the launch has one)
-    float* turn = reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) +
-                                           (size_t)g.stages * stage_bytes + (warp - 2) * TURN_BYTES);
+    Lent lent{reinterpret_cast<float*>(smem_raw + (ring - smem_addr(smem_raw)) +
+                                       (size_t)g.stages * stage_bytes + (warp - 2) * g.lent)};
     int i = 0;
     auto release = [&](int ab) {  // the accumulator has been read
       asm volatile("tcgen05.fence::before_thread_sync;");
@@ -446,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint32_t r[32];
 #pragma unroll
           for (int q = 0; q < 32; ++q) r[q] = __float_as_uint(sum[j][q]);
-          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, turn);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, lent);
         }
       } else {
         ok = wait(smem_addr(&tfull[i & 1]), (i >> 1) & 1);
@@ -455,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int c = part * 32; c < g.BN; c += 64) {
           uint32_t r[32];
           read_columns(base + (i & 1) * 256 + c, r);
-          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, turn);
+          epi.columns(row, m, in, at.n * g.BN + c, g.N, r, lent);
         }
         release(i & 1);
         ++i;
@@ -463,6 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       epi.end(row, m, in, at.n * 2 + part);
     }
     if (!ok && lane == 0) atomicOr(g.err, 1u);
+    if (lent.boxes && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
@@ -502,6 +540,20 @@ inline int encode(CUtensorMap* map, const Matrix& x, bool mn, int box_rows) {
                         x.plane ? 3 : 2, (void*)x.ptr, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return OM_OK;
+}
+
+// The map that store_box stores 16-bit results through; rows 16-byte aligned
+inline int encode_result(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int64_t ld) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)(ld * 2)};
+  const cuuint32_t box[2] = {32, 32}, one[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, ptr, dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return set_error(OM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return OM_OK;
@@ -568,11 +620,11 @@ int launch_tiles(om_backend* be, const char* name, const Matrix& a, const Matrix
   g.group = std::max(1, std::min<int>((int)tm, 2048 / (TM * CG)));
   const int stage = (P3 ? 3 : 1) * (A_BYTES + bn / CG * SLAB);
   g.a_rows = a_rows;
-  g.turn = epi.turns() ? 8 * TURN_BYTES : 0;
-  g.stages = std::min(MAX_STAGES, (216 * 1024 - g.turn) / stage);
+  g.lent = epi.lent_bytes();
+  g.stages = std::min(MAX_STAGES, (216 * 1024 - 8 * g.lent) / stage);
   g.idesc = instruction(I8, bf16, AMN, BMN, TM * CG, bn);
   g.err = be->d_flags + 1;
-  const size_t smem = (size_t)g.stages * stage + g.turn + 1024;
+  const size_t smem = (size_t)g.stages * stage + 8 * g.lent + 1024;
   auto kernel = product_kernel<I8, P3, AMN, BMN, CG, Epi>;
   OM_TRY(allow_shared(be, (const void*)kernel, (int)smem, name));
   const int64_t work = tm * tn * splits;
