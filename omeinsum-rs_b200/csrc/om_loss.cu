@@ -386,11 +386,21 @@ __device__ __forceinline__ void store_half_box(mma::Lent& lent, const CUtensorMa
   mma::store_box(lent, map, u, n0, m - (int)(threadIdx.x & 31));
 }
 
+// Whether 16-bit results go through store_box: sums of up to 8 slabs, whose tiles
+// are bound by their stores (dw of 8 x 4096 x 128000 in bf16: 272 to 325 us, lanes
+// storing their own rows 355 to 365). Longer ones hide their stores and need the stages that the boxes
+// take (4096 x 1024 x 50001 with gradients: 1.4 % slower with boxes).
+template <typename T>
+int boxes(int64_t k, int vec) {
+  return sizeof(T) == 2 && vec && k <= 512;
+}
+
 // dz of a piece, rounded to T; the buffer's rows hold whole tiles. f32: as the
 // three bf16 planes that the two products take.
 template <typename T>
 struct GradEpi {
-  CUtensorMap map;  // of the piece of dz (16 bits)
+  CUtensorMap map;  // of the piece of dz, where it is stored in boxes
+  int boxed;
   const void* targets;
   int t64;
   int64_t vocab, v0;
@@ -401,7 +411,7 @@ struct GradEpi {
     float lse, g;
     int64_t target;  // within the piece
   };
-  int lent_bytes() const { return sizeof(T) == 2 ? 2 * mma::BOX_BYTES : 0; }
+  int lent_bytes() const { return boxed ? 2 * mma::BOX_BYTES : 0; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
     Row row{0.f, 0.f, -1};
     if (in) {
@@ -430,7 +440,8 @@ struct GradEpi {
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
     }
     if constexpr (sizeof(T) == 2) {
-      store_half_box<T>(lent, &map, v, n0, m, in);
+      if (boxed) store_half_box<T>(lent, &map, v, n0, m, in);
+      else if (in) store_row((T*)dz + (int64_t)m * ld + n0, v, true);
     } else if (in) {
       __nv_bfloat16* to = (__nv_bfloat16*)dz + (int64_t)m * ld + n0;
 #pragma unroll
@@ -447,7 +458,8 @@ struct GradEpi {
 // Sums in f32 kept for later pieces or splits, or the finished result as T.
 template <typename T>
 struct OutEpi {
-  CUtensorMap map;     // of `out` (16 bits, vec)
+  CUtensorMap map;     // of `out`, where it is stored in boxes
+  int boxed;
   T* out;
   int64_t dr, dc;
   int vec;             // row_stores of `out`
@@ -460,7 +472,7 @@ struct OutEpi {
     float* acc;
   };
   int lent_bytes() const {
-    return keep ? 0 : !vec ? mma::TURN_BYTES : sizeof(T) == 2 ? 2 * mma::BOX_BYTES : 0;
+    return keep ? 0 : !vec ? mma::TURN_BYTES : boxed ? 2 * mma::BOX_BYTES : 0;
   }
   __device__ __forceinline__ Row begin(int m, bool in, int split) const {
     return Row{scale ? *scale : 1.f,
@@ -489,8 +501,8 @@ struct OutEpi {
     if (!vec) {
       store_turned(lent.words, v, out + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
                    __popc(__ballot_sync(0xffffffffu, in)), N - n0);
-    } else if constexpr (sizeof(T) == 2) {
-      store_half_box<T>(lent, &map, v, n0, m, in);
+    } else if (boxed) {
+      if constexpr (sizeof(T) == 2) store_half_box<T>(lent, &map, v, n0, m, in);
     } else if (in) {
       T* to = out + (int64_t)m * dr;
       if (N - n0 >= 32) {
@@ -760,15 +772,14 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
     if (PLANES == 1) wp = rows_of(w, v0, n);
     else OM_TRY(operand(be, pw + v0 * p.wv, n, p.D, p.wv, p.wd, at + aw, &wp));
     const mma::Matrix dz{dzs, p.N, n, P, 2, PLANES == 3 ? p.N * P : 0};
-    GradEpi<T> ge{{}, p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs, P, p.N * P};
-    if (PLANES == 1) OM_TRY(mma::encode_result(&ge.map, dzs, p.N, n, P));
+    GradEpi<T> ge{{}, boxes<T>(p.D, 1), p.targets, p.target64, p.V, v0, lse, dloss, scale, dzs, P, p.N * P};
+    if (ge.boxed) OM_TRY(mma::encode_result(&ge.map, dzs, p.N, n, P));
     OM_TRY((product<T, false, false>(be, "loss_dlogits", x, wp, tiles<T>(be, p.N, n), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
-    OutEpi<T> xe{{}, dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
-    if (PLANES == 1 && vecx) OM_TRY(mma::encode_result(&xe.map, dx, p.N, p.D, dxn));
+    const OutEpi<T> xe{{}, 0, dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
     OM_TRY((product<T, false, true>(be, "loss_dx", dz, turned(wp), tx, now, xe)));
-    OutEpi<T> we{{}, dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
-    if (PLANES == 1 && vecw) OM_TRY(mma::encode_result(&we.map, dw + v0 * dwv, n, p.D, dwv));
+    OutEpi<T> we{{}, boxes<T>(p.N, vecw), dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
+    if (we.boxed) OM_TRY(mma::encode_result(&we.map, dw + v0 * dwv, n, p.D, dwv));
     OM_TRY((product<T, true, true>(be, "loss_dw", turned(dz), turned(x), tiles<T>(be, n, p.D), 1, we)));
   }
   if (splits > 1) {
