@@ -470,9 +470,88 @@ def test_i8_empty(be, seq):
     w, ws, b = seq.upload(be, np.zeros((3, 0), np.int8)), seq.upload(be, np.ones(3, np.float32)), np.array([1, 2, 3], np.float32)
     y = seq.matmul_i8(be, q, s, w, ws, bias=seq.upload(be, b))
     assert np.array_equal(y.to_numpy(), np.stack([b, b]))
+    # more rows than one launch of the few-row kernel takes
+    q, s = seq.upload(be, np.zeros((20, 0), np.int8)), seq.upload(be, np.ones(20, np.float32))
+    assert np.array_equal(seq.matmul_i8(be, q, s, w, ws, bias=seq.upload(be, b)).to_numpy(), np.tile(b, (20, 1)))
+    assert not seq.linear_i8(be, seq.upload(be, np.zeros((20, 0), np.float32)), w, ws).to_numpy().any()
     with pytest.raises(load_pkg().OmError):
         big = seq.Strided(be.alloc(131072, np.int8), (1, 131072))
         seq.matmul_i8(be, big, seq.upload(be, np.ones(1, np.float32)), big, seq.upload(be, np.ones(1, np.float32)))
+
+
+# ---- more than 2^31 elements -----------------------------------------------
+
+
+def torch_backend():
+    import torch
+    return load_pkg().B200(0, stream=torch.cuda.current_stream().cuda_stream)
+
+
+def test_scan_past_32_bits(seq):
+    """2.29e9 elements; a gate of 1/2 and inputs of 1 lead to whole numbers."""
+    import torch
+    be, t, d = torch_backend(), 70000, 32768
+    x = torch.ones(1, t, d, device="cuda", dtype=torch.bfloat16)
+    x[0, -1, -1] = 5
+    gate = torch.full((1, 1, 1), 0.5, device="cuda", dtype=torch.bfloat16).expand(1, t, d)
+    h, last = seq.gated_scan(be, gate, x)
+    assert (h[0, 64::997] == 2)[:, :-1].all() and h[0, -1, -1] == 6 and (h[0, -1, :-1] == 2).all() and last[0, -1] == 6
+    dgate, dx, dh0 = seq.gated_scan_backward(be, gate, x, h, torch.ones(1, 1, 1, device="cuda", dtype=torch.bfloat16).expand(1, t, d))
+    assert (dx[0, -1] == 1).all() and (dx[0, -2] == 1.5).all() and (dx[0, :-64:997] == 2).all()
+    assert (dgate[0, -1] == 2).all() and (dgate[0, 64:-64:997] == 4).all() and (dh0 == 1).all()
+    be.close()
+
+
+def test_loss_past_32_bits(seq):
+    """600000 x 4096 weights, against 64-bit values of the last entries."""
+    import torch
+    be, n, d, v = torch_backend(), 64, 4096, 600000
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(n, d, generator=g, device="cuda").bfloat16()
+    w = torch.empty(v, d, device="cuda", dtype=torch.bfloat16)
+    for i in range(0, v, 100000):
+        w[i:i + 100000] = torch.randn(100000, d, generator=g, device="cuda").mul_(1 / 64)
+    targets = torch.arange(v - n, v, device="cuda")
+    loss, lse = seq.linear_cross_entropy(be, x, w, targets)
+    z = torch.cat([x.double() @ w[i:i + 50000].double().t() for i in range(0, v, 50000)], 1)
+    want = torch.logsumexp(z, 1)
+    hit = z[torch.arange(n), targets]
+    # a logit is off by 2 (D / 8 + 16) half steps of its terms' sum, below 40 here
+    bound = 2 * (d / 8 + 16) * 2.0 ** -24 * 40
+    assert (lse.double() - want).abs().max() < bound and (loss.double() - (want - hit)).abs().max() < 2 * bound
+    dloss = torch.full((n,), 1 / 64, device="cuda")
+    dx, dw = seq.linear_cross_entropy_backward(be, x, w, targets, lse, dloss)
+    tail = 1000
+    dz = torch.exp(z[:, -tail:] - lse.double()[:, None])
+    dz[torch.arange(n), targets - (v - tail)] -= 1
+    dz /= 64
+    ref_dw = dz.t() @ x.double()
+    # dz to half a step of bf16, the result too, and dz's own error from its logit
+    ok = (dw[-tail:].double() - ref_dw).abs() <= (dz.abs().t() @ x.double().abs()) * (2.0 ** -8 + bound) + ref_dw.abs() * 2.0 ** -8 + 2.0 ** -30
+    assert ok.all()
+    p = torch.exp(z - lse.double()[:, None])
+    p[torch.arange(n), targets] -= 1
+    ref_dx, mass = torch.zeros(n, d, device="cuda", dtype=torch.double), torch.zeros(n, d, device="cuda", dtype=torch.double)
+    for i in range(0, v, 50000):
+        part = w[i:i + 50000].double()
+        ref_dx += p[:, i:i + 50000] @ part / 64
+        mass += p[:, i:i + 50000].abs() @ part.abs() / 64
+    assert ((dx.double() - ref_dx).abs() <= mass * (2.0 ** -8 + bound + 2 * (v / 8 + 16) * 2.0 ** -24) + ref_dx.abs() * 2.0 ** -8).all()
+    be.close()
+
+
+def test_i8_past_32_bits(seq):
+    """2.5e9 results, the last rows and columns checked."""
+    import torch
+    be, m, k = torch_backend(), 50000, 64
+    g = torch.Generator("cuda").manual_seed(2)
+    q, w = (torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8) for _ in range(2))
+    one = torch.ones(m, device="cuda")
+    y = seq.matmul_i8(be, q, one, w, one, dtype=torch.bfloat16)
+    for rows, cols in ((slice(m - 300, m), slice(0, m)), (slice(0, m), slice(m - 300, m))):
+        want = (q[rows].double() @ w[cols].double().t()).float().bfloat16()
+        assert torch.equal(y[rows, cols], want)
+    be.close()
 
 
 # ---- together, streams, graphs ---------------------------------------------
