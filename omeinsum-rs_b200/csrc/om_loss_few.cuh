@@ -13,7 +13,7 @@
 // formed in one order. Measured with gradients: 3 x 1344 x 11307 93 us (tensor
 // cores 202), 8 x 2048 x 32000 341 us (nine tokens, on the tensor cores, 617). In
 // 16 bits, where w needs no planes, the tensor cores win even for one token (8 x
-// 2048 x 32000 bf16: 160 us against 418 in this form).
+// 2048 x 32000 bf16: 149 us against 418 in this form).
 #pragma once
 
 constexpr int FEW = 8;                     // tokens
