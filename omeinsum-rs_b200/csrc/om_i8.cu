@@ -444,7 +444,7 @@ template <typename T, int MM>
 int launch_token_rows(om_backend* be, const I8Args& p, const T* x, int64_t xk, int64_t xm,
                       int64_t Kp) {
   const size_t smem = (size_t)p.M * Kp;
-  if (smem > 48 * 1024)
+  if (smem > PLAIN_SHARED)
     OM_TRY(allow_shared(be, (const void*)token_i8_kernel<T, MM>, TOKEN_SMEM, "matmul_i8"));
   const int64_t blocks = std::min<int64_t>((p.N + 7) / 8, (int64_t)be->num_sms * 2);
   ProfScope prof(be, "matmul_i8_token");

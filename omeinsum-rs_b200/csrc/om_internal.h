@@ -141,7 +141,10 @@ struct Scratch {
 };
 
 // Lets a kernel have `bytes` of dynamic shared memory on the backend's device;
-// asks the driver only when it has not been allowed as much before.
+// asks the driver only when it has not been allowed as much before. A launch
+// needs none of this up to PLAIN_SHARED bytes: the 48 KiB that every kernel has
+// hold its static arrays and what the system reserves (1 KiB) as well.
+constexpr int PLAIN_SHARED = 40 * 1024;
 int allow_shared(om_backend* be, const void* kernel, int bytes, const char* what);
 
 // ---- kernels' host launchers ----------------------------------------------

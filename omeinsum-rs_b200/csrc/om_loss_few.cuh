@@ -251,7 +251,7 @@ int launch_few_rows(om_backend* be, const FewArgs& a, int blocks) {
   const bool vec = a.wd == 1 && !((uintptr_t)a.w & 15) && a.wv * 4 % 16 == 0;
   const int smem = (int)(NN * ((a.D + E - 1) / E * E) * 4);
   auto kernel = vec ? few_rows_kernel<NN, true, BWD> : few_rows_kernel<NN, false, BWD>;
-  if (smem > 40 * 1024) OM_TRY(allow_shared(be, (const void*)kernel, smem, "loss"));
+  if (smem > PLAIN_SHARED) OM_TRY(allow_shared(be, (const void*)kernel, smem, "loss"));
   ProfScope prof(be, BWD ? "loss_few_dlogits" : "loss_few_logits");
   kernel<<<blocks, 256, smem, be->stream>>>(a);
   note_launch();

@@ -1,0 +1,43 @@
+"""The sequence-model operators on the device where values leave the ordinary
+range: infinite logits and weights, products of gates that overflow, sizes next
+to a limit of the launch, more than one piece of the vocabulary."""
+import numpy as np
+import pytest
+
+import sequence_ref as ref
+from conftest import load_pkg
+from test_gpu_sequence import be, check_loss, check_scan, i8_inputs, loss_inputs, near, run_scan, seq, torch_backend  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+TYPES = ["f32", "f64", "bf16", "f16"]
+
+
+# ---- sizes next to a limit of the launch ---------------------------------------
+
+# rows x (inner rounded up to 16) up to and from 40 KiB and 48 KiB, the kernels'
+# static shared memory (1 KiB) below 48 KiB among them, and up to 160 KiB, for each
+# number of rows that the few-row kernel is compiled for; smaller ones first
+I8_SHARED = [(8, 5120, 40), (8, 5136, 40), (7, 6880, 40), (8, 6016, 64), (8, 6032, 64), (8, 6144, 64), (8, 6160, 64), (6, 8192, 64), (5, 9820, 33),
+             (7, 7008, 64), (4, 12032, 40), (4, 12288, 64), (3, 16384, 40), (2, 24064, 24), (2, 24576, 24), (1, 40960, 16), (1, 48128, 16),
+             (1, 48144, 16), (1, 49152, 16), (1, 49168, 16), (8, 20480, 24), (5, 32768, 24), (8, 20496, 24)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", I8_SHARED, ids=str)
+def test_i8_rows_next_to_48_kib(be, seq, shape, dtype):
+    x, w, ws, _ = i8_inputs(sum(shape), *shape, dtype)
+    X, W, WS = seq.upload(be, x, dtype), seq.upload(be, w), seq.upload(be, ws)
+    rq, rs = ref.quantize(x)
+    want = ref.matmul_i8(rq, rs, w, ws, None, dtype)
+    assert np.array_equal(seq.linear_i8(be, X, W, WS).to_numpy().astype(np.float64), want)
+    q, scale = seq.quantize_rows(be, X)
+    assert np.array_equal(seq.matmul_i8(be, q, scale, W, WS, dtype=dtype).to_numpy().astype(np.float64), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(8, 6136, 9), (5, 6136, 9), (5, 6137, 9), (4, 12280, 9), (1, 10230, 9), (1, 10232, 40), (8, 1278, 9), (8, 1280, 9)], ids=str)
+def test_loss_rows_next_to_a_limit(be, seq, shape, dtype):
+    """x at the sizes where f32 asks for more shared memory, or for another kernel."""
+    x, w, targets, g = loss_inputs(sum(shape), *shape, dtype)
+    up = lambda v: seq.upload(be, v, dtype)  # noqa: E731
+    check_loss(be, seq, up(x), up(w), seq.upload(be, targets, "i64"), seq.upload(be, g), x, w, targets, g, dtype)
