@@ -242,6 +242,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return r;
 }
 
+// What exponentials are taken relative to: the largest logit, kept finite. -inf
+// then adds exp(-inf) = 0 where every logit so far is -inf (and not the NaN of
+// -inf - -inf), an infinite maximum makes the sum infinite, NaN stays.
+__device__ __forceinline__ float shift_of(float top) { return fminf(fmaxf(top, -FLT_MAX), FLT_MAX); }
+
 // Maximum and sum of exponentials of a lane's columns of one row, and the
 // target's logit.
 struct StatsEpi {
@@ -276,14 +281,15 @@ struct StatsEpi {
       row.s *= exp2_fast((row.m - top) * LOG2E);
       row.m = top;
     }
+    const float base = shift_of(row.m);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (n >= 32) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - row.m) * LOG2E);
+      for (int c = 0; c < 32; ++c) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - base) * LOG2E);
     } else {
 #pragma unroll
       for (int c = 0; c < 32; ++c)
-        if (c < n) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - row.m) * LOG2E);
+        if (c < n) s[c & 3] += exp2_fast((__uint_as_float(r[c]) - base) * LOG2E);
     }
     row.s += (s[0] + s[1]) + (s[2] + s[3]);
     const int64_t at = row.target - n0;
@@ -323,7 +329,8 @@ __global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ par
 #pragma unroll
       for (int u = 1; u < 8; ++u) top = fmaxf(top, v[u].x);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) sum += v[u].y == 0.f ? 0.f : v[u].y * exp2_fast((v[u].x - top) * LOG2E);
+      for (int u = 0; u < 8; ++u)
+        sum += v[u].y == 0.f ? 0.f : v[u].y * exp2_fast((v[u].x - shift_of(top)) * LOG2E);
       merge(m, s, top, sum);
     }
   }
@@ -338,7 +345,7 @@ __global__ void __launch_bounds__(256) join_stats(const float2* __restrict__ par
   float top = m;
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  s = s == 0.f ? 0.f : s * exp2_fast((m - top) * LOG2E);
+  s = s == 0.f ? 0.f : s * exp2_fast((m - shift_of(top)) * LOG2E);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   m = top;

@@ -41,3 +41,88 @@ def test_loss_rows_next_to_a_limit(be, seq, shape, dtype):
     x, w, targets, g = loss_inputs(sum(shape), *shape, dtype)
     up = lambda v: seq.upload(be, v, dtype)  # noqa: E731
     check_loss(be, seq, up(x), up(w), seq.upload(be, targets, "i64"), seq.upload(be, g), x, w, targets, g, dtype)
+
+
+# ---- infinite logits ---------------------------------------------------------
+
+
+def masked_vocabulary(n, v, masked, dtype, seed=21, d=40):
+    """x, w, targets, dloss with a column of ones in x and -inf in w's column for
+    the masked entries; targets are never masked.  `live`: the other entries."""
+    x, w, _, g = loss_inputs(seed, n, d, v, dtype)
+    live = np.setdiff1d(np.arange(v), masked)
+    r = np.random.default_rng(seed)
+    targets = r.choice(live, n)
+    x[:, -1], w[:, -1] = 1, 0
+    w[masked, -1] = -np.inf
+    return x, w, targets, g, live
+
+
+MASKS = {"end": (32128, np.arange(32000, 32128)), "start": (1000, np.arange(300)), "tiles": (2100, np.r_[256:768, 1024:1280, 2000:2100]),
+         "short": (64, np.arange(32, 64))}
+
+
+def check_masked_forward(be, seq, n, mask, dtype):
+    v, masked = MASKS[mask]
+    x, w, targets, _, live = masked_vocabulary(n, v, masked, dtype)
+    loss, lse = seq.linear_cross_entropy(be, seq.upload(be, x, dtype), seq.upload(be, w, dtype), seq.upload(be, targets, "i64"))
+    # masked entries add exactly nothing: the bounds are those of the others
+    rl, rs, _, _, el, es = ref.loss(x, w[live], np.searchsorted(live, targets), dtype)
+    near(loss.to_numpy(), rl, el)
+    near(lse.to_numpy(), rs, es)
+
+
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("n", [1, 8, 9, 200])
+@pytest.mark.parametrize("dtype", ["f64", "bf16", "f16"])
+def test_loss_of_a_masked_vocabulary(be, seq, dtype, n, mask):
+    check_masked_forward(be, seq, n, mask, dtype)
+
+
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("n", [1, 8])
+def test_loss_of_a_masked_vocabulary_few_tokens_f32(be, seq, n, mask):
+    check_masked_forward(be, seq, n, mask, "f32")
+
+
+def check_infinite_logits(be, seq, n, dtype):
+    """lse by its definition: -inf where every logit is, inf where one is, NaN
+    where one is NaN; a masked target's loss is inf."""
+    d, v = 24, 600
+    x, w, _, _ = loss_inputs(22, n, d, v, dtype)
+    x[:, -1], w[:, -1] = 1, 0
+    T = seq.upload(be, np.full(n, 5), "i64")
+
+    def run(w):
+        loss, lse = seq.linear_cross_entropy(be, seq.upload(be, x, dtype), seq.upload(be, w, dtype), T)
+        return loss.to_numpy(), lse.to_numpy()
+
+    gone = w.copy()
+    gone[:, -1] = -np.inf
+    assert (run(gone)[1] == -np.inf).all()
+    one = w.copy()
+    one[300, -1] = np.inf
+    loss, lse = run(one)
+    assert (lse == np.inf).all() and (loss == np.inf).all()
+    both = gone.copy()
+    both[300:302, -1] = np.inf
+    assert (run(both)[1] == np.inf).all()
+    for base in (w, gone, one):
+        bad = base.copy()
+        bad[17, -1] = np.nan
+        assert np.isnan(run(bad)[1]).all()
+    target = w.copy()
+    target[5, -1] = -np.inf
+    loss, lse = run(target)
+    assert (loss == np.inf).all() and np.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("n", [1, 8, 9, 200])
+@pytest.mark.parametrize("dtype", ["f64", "bf16", "f16"])
+def test_loss_of_infinite_logits(be, seq, dtype, n):
+    check_infinite_logits(be, seq, n, dtype)
+
+
+@pytest.mark.parametrize("n", [1, 8])
+def test_loss_of_infinite_logits_few_tokens_f32(be, seq, n):
+    check_infinite_logits(be, seq, n, "f32")
