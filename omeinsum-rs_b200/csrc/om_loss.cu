@@ -34,6 +34,18 @@ __device__ __forceinline__ int64_t target_of(const void* t, int t64, int64_t n) 
   return t64 ? ((const int64_t*)t)[n] : (int64_t)((const int32_t*)t)[n];
 }
 
+// Which tokens carry no loss: those whose target lies outside the vocabulary. Their
+// rows of dx are zero, and not 0 * w, which an infinite weight would make NaN.
+// targets == null: all carry one.
+struct Counted {
+  const void* targets;
+  int t64;
+  int64_t vocab;
+  __device__ __forceinline__ bool out(int64_t row) const {
+    return targets && (uint64_t)target_of(targets, t64, row) >= (uint64_t)vocab;
+  }
+};
+
 // a strided matrix as a row-major one, zero in rows whose target lies outside
 // the vocabulary
 template <typename S>
@@ -50,13 +62,13 @@ __global__ void masked_rows(const S* __restrict__ src, int64_t rows, int64_t col
 
 // a row-major matrix as a strided one
 template <typename S>
-__global__ void store_rows(const S* __restrict__ src, int64_t rows, int64_t cols,
+__global__ void store_rows(const S* __restrict__ src, int64_t rows, int64_t cols, Counted counted,
                            S* __restrict__ dst, int64_t dr, int64_t dc) {
   const int64_t total = rows * cols;
   for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / cols, c = i - r * cols;
-    dst[r * dr + c * dc] = src[i];
+    dst[r * dr + c * dc] = counted.out(r) ? S(0) : src[i];
   }
 }
 
@@ -142,6 +154,8 @@ __global__ void piece_gradient(S* __restrict__ z, int64_t rows, int64_t cols, in
     zr[c] = counts ? g * (exp(zr[c] - l) - (v0 + c == t ? S(1) : S(0))) : S(0);
 }
 
+Counted counted_of(const LossArgs& p) { return Counted{p.targets, p.target64, p.V}; }
+
 unsigned flat_grid(om_backend* be, int64_t n) {
   return (unsigned)std::max<int64_t>(1, std::min<int64_t>((n + 255) / 256, (int64_t)be->num_sms * 16));
 }
@@ -223,11 +237,12 @@ int loss_backward(om_backend* be, const LossArgs& p, const S* lse, const S* dlos
       note_launch();
     }
     OM_TRY(launch_gemm(be, gemm<S>(dt, n, p.D, p.N, zs.ptr, 1, n, xs.ptr, p.D, 1, dws.ptr, p.D)));
-    store_rows<S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>((const S*)dws.ptr, n, p.D,
+    store_rows<S><<<flat_grid(be, n * p.D), 256, 0, be->stream>>>((const S*)dws.ptr, n, p.D, Counted{},
                                                                  dw + v0 * dwv, dwv, dwd);
     note_launch();
   }
-  store_rows<S><<<flat_grid(be, nx), 256, 0, be->stream>>>((const S*)acc.ptr, p.N, p.D, dx, dxn, dxd);
+  store_rows<S><<<flat_grid(be, nx), 256, 0, be->stream>>>((const S*)acc.ptr, p.N, p.D, counted_of(p), dx, dxn,
+                                                            dxd);
   note_launch();
   return check_cuda(cudaGetLastError(), "loss backward launch");
 }
@@ -417,18 +432,18 @@ struct GradEpi {
   struct Row {
     float lse, g;
     int64_t target;  // within the piece
+    bool counts;
   };
   int lent_bytes() const { return boxed ? 2 * mma::BOX_BYTES : 0; }
   __device__ __forceinline__ Row begin(int m, bool in, int) const {
-    Row row{0.f, 0.f, -1};
+    Row row{0.f, 0.f, -1, false};
     if (in) {
       const int64_t t = target_of(targets, t64, m);
-      row.lse = lse[m];
       if (t >= 0 && t < vocab) {
+        row.lse = lse[m];
         row.g = scale ? dloss[m] / *scale : dloss[m];
         row.target = t - v0;
-      } else {  // exp(z - inf) = 0, whatever this row's lse is
-        row.lse = INFINITY;
+        row.counts = true;
       }
     }
     return row;
@@ -445,6 +460,10 @@ struct GradEpi {
 #pragma unroll
       for (int c = 0; c < 32; ++c)
         if (at == c) v[c] = row.g * (exp2_fast((__uint_as_float(r[c]) - row.lse) * LOG2E) - 1.f);
+    }
+    if (!row.counts) {  // zero times an infinite weight made its logits NaN
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = 0.f;
     }
     if constexpr (sizeof(T) == 2) {
       if (boxed) store_half_box<T>(lent, &map, v, n0, m, in);
@@ -474,16 +493,18 @@ struct OutEpi {
   float* acc;          // [split][rows][acc_ld], whole tiles
   int64_t acc_ld, acc_split;
   int load, keep;      // add what acc holds; leave the sum there
+  Counted counted;     // rows that are zero whatever their sums are (dx)
   struct Row {
     float f;
     float* acc;
+    bool zero;
   };
   int lent_bytes() const {
     return keep ? 0 : !vec ? mma::TURN_BYTES : boxed ? 2 * mma::BOX_BYTES : 0;
   }
   __device__ __forceinline__ Row begin(int m, bool in, int split) const {
     return Row{scale ? *scale : 1.f,
-               acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr};
+               acc ? acc + (int64_t)split * acc_split + (int64_t)m * acc_ld : nullptr, in && counted.out(m)};
   }
   __device__ __forceinline__ void columns(Row& row, int m, bool in, int n0, int N,
                                           const uint32_t (&r)[32], mma::Lent& lent) const {
@@ -504,6 +525,10 @@ struct OutEpi {
     }
 #pragma unroll
     for (int c = 0; c < 32; ++c) v[c] *= row.f;
+    if (row.zero) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = 0.f;
+    }
     const int lane = threadIdx.x & 31;
     if (!vec) {
       store_turned(lent.words, v, out + (int64_t)(m - lane) * dr + n0 * dc, dr, dc,
@@ -528,7 +553,7 @@ struct OutEpi {
 template <typename T>
 __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t acc_split,
                             int64_t acc_ld, int64_t rows, int64_t cols, const float* scale,
-                            T* __restrict__ out, int64_t dr, int64_t dc) {
+                            Counted counted, T* __restrict__ out, int64_t dr, int64_t dc) {
   const float f = scale ? *scale : 1.f;
   const int64_t total = rows * cols;
   const bool narrow = total < ((int64_t)1 << 32);
@@ -540,7 +565,7 @@ __global__ void join_splits(const float* __restrict__ acc, int splits, int64_t a
     float s = 0.f;
 #pragma unroll 8
     for (int k = 0; k < splits; ++k) s += __ldcg(from + k * acc_split);
-    out[r * dr + c * dc] = Elem<T>::store(s * f);
+    out[r * dr + c * dc] = Elem<T>::store(counted.out(r) ? 0.f : s * f);
   }
 }
 
@@ -783,16 +808,17 @@ int loss_backward_tc(om_backend* be, const LossArgs& p, const float* lse, const 
     if (ge.boxed) OM_TRY(mma::encode_result(&ge.map, dzs, p.N, n, P));
     OM_TRY((product<T, false, false>(be, "loss_dlogits", x, wp, tiles<T>(be, p.N, n), 1, ge)));
     const int now = (int)std::min<int64_t>(splits, (n + 63) / 64);
-    const OutEpi<T> xe{{}, 0, dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last};
+    const OutEpi<T> xe{{}, 0, dx, dxn, dxd, vecx, scale, acc, acc_ld, p.N * acc_ld, v0 > 0, splits > 1 || !last,
+                       counted_of(p)};
     OM_TRY((product<T, false, true>(be, "loss_dx", dz, turned(wp), tx, now, xe)));
-    OutEpi<T> we{{}, boxes<T>(p.N, vecw), dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0};
+    OutEpi<T> we{{}, boxes<T>(p.N, vecw), dw + v0 * dwv, dwv, dwd, vecw, scale, nullptr, 0, 0, 0, 0, Counted{}};
     if (we.boxed) OM_TRY(mma::encode_result(&we.map, dw + v0 * dwv, n, p.D, dwv));
     OM_TRY((product<T, true, true>(be, "loss_dw", turned(dz), turned(x), tiles<T>(be, n, p.D), 1, we)));
   }
   if (splits > 1) {
     ProfScope prof(be, "loss_join_splits");
     join_splits<T><<<flat_grid(be, p.N * p.D), 256, 0, be->stream>>>(
-        acc, splits, p.N * acc_ld, acc_ld, p.N, p.D, scale, dx, dxn, dxd);
+        acc, splits, p.N * acc_ld, acc_ld, p.N, p.D, scale, counted_of(p), dx, dxn, dxd);
     note_launch();
   }
   return check_cuda(cudaGetLastError(), "loss backward launch");

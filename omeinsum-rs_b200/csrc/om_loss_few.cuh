@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const __grid_constant__ F
   const bool counts = target >= 0 && target < p.V;
   float lse = 0.f, g = 0.f, m = -INFINITY, s = 0.f;
   if (BWD && lane < p.N) {
-    lse = counts ? p.lse[lane] : INFINITY;  // exp(z - inf) = 0 where there is no loss
+    lse = counts ? p.lse[lane] : 0.f;
     g = counts ? p.dloss[lane] : 0.f;
   }
   __syncthreads();
@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(256) few_outer_kernel(const __grid_constant__ 
 
 // dx = sum of the blocks, 32 columns by 8 groups of blocks per block
 __global__ void few_join(const float* __restrict__ acc, int blocks, int64_t total, int64_t D,
-                         float* __restrict__ dx, int64_t dxd, int64_t dxn) {
+                         Counted counted, float* __restrict__ dx, int64_t dxd, int64_t dxn) {
   __shared__ float part[8][32];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t i = blockIdx.x * (int64_t)32 + tx;
@@ -236,7 +236,7 @@ __global__ void few_join(const float* __restrict__ acc, int blocks, int64_t tota
   if (ty || i >= total) return;
 #pragma unroll
   for (int k = 1; k < 8; ++k) s += part[k][tx];
-  dx[i / D * dxn + i % D * dxd] = s;
+  dx[i / D * dxn + i % D * dxd] = counted.out(i / D) ? 0.f : s;
 }
 
 // tokens that the kernels are compiled for
@@ -298,7 +298,7 @@ int few_backward(om_backend* be, FewArgs a, const LossArgs& p, const float* lse,
     note_launch();
   }
   ProfScope prof(be, "loss_join_splits");
-  few_join<<<(unsigned)((nd + 31) / 32), 256, 0, be->stream>>>(a.acc, ranges, nd, p.D, dx, dxd, dxn);
+  few_join<<<(unsigned)((nd + 31) / 32), 256, 0, be->stream>>>(a.acc, ranges, nd, p.D, counted_of(p), dx, dxd, dxn);
   note_launch();
   return check_cuda(cudaGetLastError(), "loss backward launch");
 }

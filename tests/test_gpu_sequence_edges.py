@@ -126,3 +126,39 @@ def test_loss_of_infinite_logits(be, seq, dtype, n):
 @pytest.mark.parametrize("n", [1, 8])
 def test_loss_of_infinite_logits_few_tokens_f32(be, seq, n):
     check_infinite_logits(be, seq, n, "f32")
+
+
+def check_masked_backward(be, seq, n, mask, dtype):
+    """Tokens without a loss get exact zeros and reach nothing, although their
+    logits are NaN (0 * -inf); the masked column of dx is 0 * -inf = NaN for the
+    others, as the formula has it, and nothing else is touched."""
+    v, masked = MASKS[mask]
+    x, w, targets, g, live = masked_vocabulary(n, v, masked, dtype)
+    x[::3], targets[::3] = np.nan, -100
+    if n > 3:
+        targets[3] = v
+    ignored = (targets < 0) | (targets >= v)
+    clean = np.where(ignored[:, None], 0.0, x)
+    where = np.where(ignored, -100, np.searchsorted(live, targets))
+    lse = np.where(ignored, 0.0, ref.loss(clean, w[live], where, dtype)[1]).astype(g.dtype)
+    dx, dw = seq.linear_cross_entropy_backward(be, seq.upload(be, x, dtype), seq.upload(be, w, dtype), seq.upload(be, targets, "i64"),
+                                               seq.upload(be, np.where(ignored, np.nan, lse).astype(g.dtype)), seq.upload(be, g))
+    dx, dw = (np.asarray(a.to_numpy(), np.float64) for a in (dx, dw))
+    ax, aw, ex, ew = ref.loss_backward(clean, w[live], where, lse.astype(np.float64), g, dtype)
+    near(dw[live], aw, ew)
+    assert not dw[masked].any()  # (NaN counts as any)
+    near(dx[:, :-1], ax[:, :-1], ex[:, :-1])
+    assert not dx[ignored].any() and np.isnan(dx[~ignored, -1]).all()
+
+
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("n", [1, 2, 8, 9, 200])
+@pytest.mark.parametrize("dtype", ["f64", "bf16", "f16"])
+def test_loss_gradients_of_a_masked_vocabulary(be, seq, dtype, n, mask):
+    check_masked_backward(be, seq, n, mask, dtype)
+
+
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("n", [1, 2, 8])
+def test_loss_gradients_of_a_masked_vocabulary_few_tokens_f32(be, seq, n, mask):
+    check_masked_backward(be, seq, n, mask, "f32")
