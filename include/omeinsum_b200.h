@@ -396,10 +396,13 @@ int om_b200_gated_scan_backward(om_backend* be, om_gate kind, om_dtype dtype, co
  * with their own strides, dtype OM_F32, OM_F64, OM_BF16 or OM_F16.  targets
  * (N contiguous OM_I32 or OM_I64 values, target_dtype) outside [0, V) carry no
  * loss: loss is 0 there (lse is still written).  loss and lse are N contiguous
- * f32 values (f64 for OM_F64).  16-bit products accumulate in f32. f32 runs on
- * the tensor cores as three bf16 parts of each number (six products, error about
- * 2^-22 * sum_d |x||w|), or as f32 FMA in OM_F32_EXACT mode and for up to
- * eight tokens. */
+ * f32 values (f64 for OM_F64).  Logits may be infinite: one of -inf adds nothing
+ * to lse, so a vocabulary can be masked.  16-bit products accumulate in f32.
+ * f32 is computed as f32 FMA in OM_F32_EXACT mode and for one token of a width up
+ * to 49144, two to four up to 12280 and five to eight up to 6136; else on the tensor
+ * cores as three bf16 parts of each number: six products, error about 2^-22 *
+ * sum_d |x||w|.  There a factor below 2^-109 is held to 2^-134 only, one below
+ * 2^-126 may count as zero, and an infinity times an infinity is NaN. */
 int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, const int64_t* shape,
                                  const void* x, const int64_t* strides_x, const void* w,
                                  const int64_t* strides_w, om_dtype target_dtype,

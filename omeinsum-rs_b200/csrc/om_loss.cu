@@ -417,6 +417,20 @@ int boxes(int64_t k, int vec) {
   return sizeof(T) == 2 && vec && k <= 512;
 }
 
+// The next of the three bf16 parts of an f32 number, as f32; what is left stays in
+// v. x = x0 + x1 + x2 to 24 bits. x0 is cut at bf16's largest number, which f32's
+// largest would round past. Infinity and NaN are the third part of 0, 0, x: in the
+// products it meets the other operand's first part alone (A2 B0, A0 B2), where in
+// the first it would meet zeros among the others' second and third parts.
+__device__ __forceinline__ float next_part(float& v, bool third) {
+  constexpr float LARGEST = 0x1.fep127f;
+  const bool finite = fabsf(v) < INFINITY;
+  if (third) return v;
+  const float part = finite ? __bfloat162float(__float2bfloat16_rn(fminf(fmaxf(v, -LARGEST), LARGEST))) : 0.f;
+  v -= part;
+  return part;
+}
+
 // dz of a piece, rounded to T; the buffer's rows hold whole tiles. f32: as the
 // three bf16 planes that the two products take.
 template <typename T>
@@ -472,9 +486,10 @@ struct GradEpi {
       __nv_bfloat16* to = (__nv_bfloat16*)dz + (int64_t)m * ld + n0;
 #pragma unroll
       for (int z = 0; z < 3; ++z) {
-        store_row(to + z * plane, v, true);
+        float part[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] -= __bfloat162float(__float2bfloat16_rn(v[c]));
+        for (int c = 0; c < 32; ++c) part[c] = next_part(v[c], z == 2);
+        store_row(to + z * plane, part, true);
       }
     }
   }
@@ -601,7 +616,7 @@ __global__ void pack_rows(const T* __restrict__ src, int64_t rows, int64_t cols,
   }
 }
 
-// A matrix of f32 as three bf16 planes, x = x0 + x1 + x2 to 24 bits; zero as
+// A matrix of f32 as three bf16 planes, the parts of next_part; zero as
 // above. A thread makes 8 elements of each plane.
 __global__ void split_rows(const float* __restrict__ src, int64_t rows, int64_t cols, int64_t sr,
                            int64_t sc, __nv_bfloat16* __restrict__ dst, int64_t ld, int64_t plane,
@@ -629,10 +644,7 @@ __global__ void split_rows(const float* __restrict__ src, int64_t rows, int64_t 
     for (int z = 0; z < 3; ++z) {
       __align__(16) __nv_bfloat16 b[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        b[k] = __float2bfloat16_rn(v[k]);
-        v[k] -= __bfloat162float(b[k]);
-      }
+      for (int k = 0; k < 8; ++k) b[k] = __float2bfloat16_rn(next_part(v[k], z == 2));
       *reinterpret_cast<uint4*>(dst + z * plane + i * 8) = *reinterpret_cast<const uint4*>(b);
     }
   }

@@ -1,5 +1,6 @@
-// Cross entropy of up to eight tokens in f32: the weights stream through the
-// CUDA cores. (Part of om_loss.cu.)
+// Cross entropy of up to eight tokens in f32 whose rows of x fit FEW_SHARED bytes
+// (8 x 6136, 4 x 12280, 1 x 49144): the weights stream through the CUDA cores. (Part
+// of om_loss.cu.)
 //
 //   few_rows_kernel  a warp takes four rows of w at a time and their dot products
 //                    with every token (x in shared memory); forward: the running
@@ -18,7 +19,7 @@
 
 constexpr int FEW = 8;                     // tokens
 constexpr int FEW_ROWS = 4;                // of w per warp and turn
-constexpr int FEW_SHARED = 192 * 1024;     // bytes of x
+constexpr int FEW_SHARED = 192 * 1024;     // bytes of x, rows rounded up to few_of
 
 struct FewArgs {
   int N;

@@ -162,3 +162,71 @@ def test_loss_gradients_of_a_masked_vocabulary(be, seq, dtype, n, mask):
 @pytest.mark.parametrize("n", [1, 2, 8])
 def test_loss_gradients_of_a_masked_vocabulary_few_tokens_f32(be, seq, n, mask):
     check_masked_backward(be, seq, n, mask, "f32")
+
+
+@pytest.mark.parametrize("mask", sorted(MASKS))
+@pytest.mark.parametrize("n", [9, 200])
+def test_loss_of_a_masked_vocabulary_f32(be, seq, n, mask):
+    check_masked_forward(be, seq, n, mask, "f32")
+    check_masked_backward(be, seq, n, mask, "f32")
+
+
+@pytest.mark.parametrize("n", [9, 200])
+def test_loss_of_infinite_logits_f32(be, seq, n):
+    check_infinite_logits(be, seq, n, "f32")
+
+
+@pytest.mark.parametrize("n", [8, 9, 200])
+def test_loss_of_an_infinite_activation_f32(be, seq, n):
+    """One token's row holds an infinity: its logits alone are infinite."""
+    x, w, _, g = loss_inputs(23, n, 40, 300, "f32")
+    w[:, 7] = np.abs(w[:, 7]) + 0.5
+    targets = np.random.default_rng(1).integers(0, 300, n)
+    clean = x.copy()
+    x[4, 7] = np.inf
+    loss, lse = seq.linear_cross_entropy(be, seq.upload(be, x, "f32"), seq.upload(be, w, "f32"), seq.upload(be, targets, "i64"))
+    rl, rs, _, _, el, es = ref.loss(clean, w, targets, "f32")
+    others = np.arange(n) != 4
+    near(loss.to_numpy()[others], rl[others], el[others])
+    near(lse.to_numpy()[others], rs[others], es[others])
+    assert lse.to_numpy()[4] == np.inf
+
+
+@pytest.mark.parametrize("n", [8, 9, 200])
+def test_loss_of_the_largest_f32(be, seq, n):
+    """Numbers within half a bf16 step of f32's largest, which round to infinity
+    in bf16, times ones of 2^-100 and 2^-110."""
+    top = float(np.finfo(np.float32).max)
+    for huge, size in (("x", 2.0 ** -100), ("w", 2.0 ** -100), ("w", 2.0 ** -110)):
+        x, w, targets, g = loss_inputs(24, n, 24, 200, "f32")
+        a, b = (x, w) if huge == "x" else (w, x)
+        a[:, 3] = top * np.sign(a[:, 3])
+        a[1, 3] = top * (1 - 2.0 ** -9)
+        b[:, 3] *= size
+        x, w = ref.rounded(x, "f32"), ref.rounded(w, "f32")
+        loss, lse = seq.linear_cross_entropy(be, seq.upload(be, x, "f32"), seq.upload(be, w, "f32"), seq.upload(be, targets, "i64"))
+        rl, rs, _, _, el, es = ref.loss(x, w, targets, "f32")
+        # A number's third bf16 part is rounded to bf16's smallest step, 2^-133, where
+        # the number is below 2^-109: up to 2^-134 of it are lost, times the other
+        # factor, for each term of a logit; a loss has two logits.  (Here: 2^-134 *
+        # 2^128 = 2^-6 for x of 2^-116 beside w of 2^128.)
+        lost = 2.0 ** -134 * (np.abs(x).sum(1) + np.abs(w).sum(1).max())
+        near(loss.to_numpy(), rl, el + 2 * lost)
+        near(lse.to_numpy(), rs, es + lost)
+
+
+@pytest.mark.parametrize("n", [8, 9, 200])
+def test_loss_gradients_of_infinite_dloss_f32(be, seq, n):
+    """A token's dloss of infinity makes its own row of dx infinite or NaN and
+    leaves the other rows alone."""
+    x, w, targets, g = loss_inputs(25, n, 40, 300, "f32")
+    targets = np.abs(targets) % 300
+    g[2] = np.inf
+    X, W, T = seq.upload(be, x, "f32"), seq.upload(be, w, "f32"), seq.upload(be, targets, "i64")
+    _, lse = seq.linear_cross_entropy(be, X, W, T)
+    dx, _ = seq.linear_cross_entropy_backward(be, X, W, T, lse, seq.upload(be, g))
+    g[2] = 0
+    ax, _, ex, _ = ref.loss_backward(x, w, targets, lse.to_numpy().astype(np.float64), g, "f32")
+    others = np.arange(n) != 2
+    near(dx.to_numpy()[others], ax[others], ex[others])
+    assert not np.isfinite(dx.to_numpy()[2]).any()
