@@ -365,9 +365,10 @@ int om_b200_tropical_matmul_argmax_noalloc(void* stream, om_algebra alg, int64_t
  * min(max(lengths[b], 0), T) steps; what lies behind them is not read, h is
  * zero there, and h_last is the state after the last real step.  T == 1 is the
  * form for decoding one token.
- * Steps may be grouped: gates above one in magnitude whose product over a few
- * hundred steps leaves the state's type give infinities where the state itself
- * would not, and an infinite gate gives NaN or infinity from its step on. */
+ * Steps are grouped, but the result is the definition's, also where a product of
+ * gates over a group leaves the state's type or a state is infinite: such a channel
+ * takes its steps one by one, which is slower.  A group's product of gates below
+ * the type's smallest number counts as zero. */
 typedef enum { OM_GATE_LINEAR = 0, OM_GATE_SIGMOID = 1 } om_gate;
 int om_b200_gated_scan(om_backend* be, om_gate kind, om_dtype dtype, const int64_t* shape,
                        const void* gate, const int64_t* strides_gate, const void* x,

@@ -379,6 +379,11 @@ struct Stream {
   }
 };
 
+template <typename S>
+__device__ __forceinline__ bool finite(S s) {
+  return fabs(s) < S(INFINITY);
+}
+
 // ---- the maps of the chunks -------------------------------------------------------------
 
 template <typename T, int V, bool SIG, bool BWD>
@@ -447,13 +452,168 @@ __global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof
 
 // ---- the steps ------------------------------------------------------------------------
 
+// A chunk's steps: open() asks for the first rows, take() goes through them from
+// the state s that enters and writes the results.
+template <typename T, int V, bool SIG, bool BWD>
+struct Steps {
+  using S = typename Elem<T>::State;
+  using L = Lane<T, V>;
+  using K = typename L::K;
+  using R = typename L::R;
+  static constexpr int NA = BWD ? (SIG ? 4 : 3) : 2;
+  Stream<T, V, NA, NA == 2 ? 8 : NA == 3 ? 4 : 3> rows;
+  bool start;  // backward: step 0, which has no h before it, comes after the others
+  const T *g, *x, *e;
+
+  __device__ __forceinline__ void aim(const ScanArgs& p, const Place& at) {
+    start = BWD && at.t0 == 0 && at.end > 0;
+    g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
+    x = (const T*)p.x + at.b * p.xb + at.d * p.xd;
+    e = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed : nullptr;
+    rows.n = at.live ? at.end - at.t0 - start : 0;
+    if constexpr (!BWD) {
+      rows.p[0] = g + at.t0 * p.gt, rows.step[0] = p.gt;
+      rows.p[1] = x + at.t0 * p.xt, rows.step[1] = p.xt;
+    } else {
+      const int64_t t = at.end - 1;
+      rows.p[0] = g + t * p.gt, rows.step[0] = -p.gt;
+      rows.p[1] = e + t * p.et, rows.step[1] = -p.et;
+      rows.p[2] = (const T*)p.h + at.b * p.hb + at.d * p.hd + (t - 1) * p.ht, rows.step[2] = -p.ht;
+      if constexpr (SIG) rows.p[3] = x + t * p.xt, rows.step[3] = -p.xt;
+    }
+  }
+
+  __device__ __forceinline__ void take(const ScanArgs& p, const ChunkArgs& a, const Place& at, L s) {
+    L zero;
+#pragma unroll
+    for (int i = 0; i < V; ++i) zero.set(i, S(0));
+    if constexpr (!BWD) {
+      T* h = (T*)p.h + at.b * p.hb + at.d * p.hd + at.t0 * p.ht;
+      rows.run([&](const R (&r)[2]) {
+        const L f = L::of(r[0]), b = L::of(r[1]);
+#pragma unroll
+        for (int i = 0; i < L::N; ++i) {
+          K fi = f.v[i], bi = b.v[i];
+          if constexpr (SIG) {
+            K rest;
+            sigmoid_pair(fi, &fi, &rest);
+            bi = bi * rest;
+          }
+          s.v[i] = mad(fi, s.v[i], bi);
+        }
+        keep<T, V>(h, s);
+        h += p.ht;
+      });
+      for (int64_t t = at.end; t < at.t1; ++t, h += p.ht) keep<T, V>(h, zero);
+    } else {
+      T* dg = (T*)p.dgate + at.b * p.pb + at.d * p.pd + (at.t1 - 1) * p.pt;
+      T* dx = (T*)p.dx + at.b * p.qb + at.d * p.qd + (at.t1 - 1) * p.qt;
+      for (int64_t t = at.t1; t > at.end; --t, dg -= p.pt, dx -= p.qt)
+        keep<T, V>(dg, zero), keep<T, V>(dx, zero);
+      auto back = [&](R rg, R re, const L& before, R rx) {
+        const L f = L::of(rg), d = L::of(re), v = L::of(rx);
+        L og, ox;
+#pragma unroll
+        for (int i = 0; i < L::N; ++i) {
+          K fi = f.v[i];
+          const K total = d.v[i] + s.v[i];
+          if constexpr (SIG) {
+            K rest;
+            sigmoid_pair(fi, &fi, &rest);
+            ox.v[i] = total * rest;
+            og.v[i] = mad(v.v[i], K::all(S(-1)), before.v[i]) * fi * ox.v[i];
+          } else {
+            ox.v[i] = total;
+            og.v[i] = total * before.v[i];
+          }
+          s.v[i] = fi * total;
+        }
+        keep<T, V>(dg, og);
+        keep<T, V>(dx, ox);
+        dg -= p.pt;
+        dx -= p.qt;
+      };
+      rows.run([&](const R (&r)[NA]) { back(r[0], r[1], L::of(r[2]), r[NA - 1]); });
+      if (start) {
+        L before;
+#pragma unroll
+        for (int i = 0; i < V; ++i) before.set(i, p.h0 ? ((const S*)p.h0)[at.c0 + i] : S(0));
+        const R rg = fetch<T, V>(g);
+        back(rg, fetch<T, V>(e), before, SIG ? fetch<T, V>(x) : rg);
+      }
+    }
+    // the state that leaves the last chunk
+    S* last = (S*)(BWD ? p.dh0 : p.h_last);
+    if (last && at.order == a.chunks - 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) last[at.c0 + i] = s.get(i);
+    }
+  }
+};
+
+// The chunk of a lane whose joined state is not finite in some channel. Where a
+// group's product of gates overflows, its map gives infinity or NaN for states that
+// the steps themselves keep finite (and NaN for an infinite state where it
+// underflows); so such a channel's state is formed step by step from the caller's,
+// as far as it is not NaN already. Out of line and to the chunk's end, so that the
+// ordinary case keeps nothing for it (with the steps after it in the kernel, 7 x 1531
+// x 1001 f32 took 95 us and not 89). Bound by the latency of one channel's loads: an
+// infinity at the start of 65537 x 1032 bf16 takes 5.9 ms, finite inputs 0.12 ms.
+template <typename T, int V, bool SIG, bool BWD>
+__device__ __noinline__ void walk(const ScanArgs& p, const ChunkArgs& a, int col, int order,
+                                  Lane<T, V> joined) {
+  using S = typename Elem<T>::State;
+  using L = Lane<T, V>;
+  using R = typename L::R;
+  constexpr int U = 8;  // steps under way
+  const Place at = place_of<T, V, BWD>(p, a, col, order);
+  const int64_t length = p.lengths ? max((int64_t)0, min((int64_t)p.lengths[at.b], p.T)) : p.T;
+  const int64_t n = BWD ? length - at.t1 : min(length, at.t0), first = BWD ? length - 1 : 0;
+  const int64_t gt = BWD ? -p.gt : p.gt, bt = BWD ? -p.et : p.xt;
+  const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd + first * p.gt;
+  const T* b = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed + first * p.et
+                   : (const T*)p.x + at.b * p.xb + at.d * p.xd + first * p.xt;
+  L s;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s.set(i, ((const S*)a.start)[at.c0 + i]);
+  for (int64_t t = 0; t < n; t += U, g += U * gt, b += U * bt) {
+    R rg[U], rb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u < n) rg[u] = fetch<T, V>(g + u * gt), rb[u] = fetch<T, V>(b + u * bt);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= n) break;
+      const L f = L::of(rg[u]), v = L::of(rb[u]);
+#pragma unroll
+      for (int i = 0; i < L::N; ++i) {
+        typename L::K fi = f.v[i], bi = v.v[i], rest;
+        if constexpr (SIG) {
+          sigmoid_pair(fi, &fi, &rest);
+          if constexpr (!BWD) bi = bi * rest;
+        }
+        s.v[i] = BWD ? fi * (bi + s.v[i]) : mad(fi, s.v[i], bi);
+      }
+    }
+    bool gone = true;  // a NaN stays
+#pragma unroll
+    for (int i = 0; i < V; ++i) gone &= s.get(i) != s.get(i) || finite(joined.get(i));
+    if (gone) break;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (!finite(joined.get(i))) joined.set(i, s.get(i));
+  Steps<T, V, SIG, BWD> steps;
+  steps.aim(p, at);
+  steps.rows.start();
+  steps.take(p, a, at, joined);
+}
+
 template <typename T, int V, bool SIG, bool BWD>
 __global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof(T) * V)) step_kernel(const __grid_constant__ ScanArgs p,
                                                              const __grid_constant__ ChunkArgs a) {
   using S = typename Elem<T>::State;
   using L = Lane<T, V>;
-  using K = typename L::K;
-  using R = typename L::R;
   constexpr int WARPS = warps_of(sizeof(T) * V);
   __shared__ Pair<S> part[WARPS][32 * V], chunk[WARPS][32 * V];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -467,24 +627,8 @@ __global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof
   // the state that enters: the caller's, through the maps of the blocks of
   // chunks before this one (shared out over the warps) and of the chunks
   // before this warp's
-  constexpr int NA = BWD ? (SIG ? 4 : 3) : 2;
-  Stream<T, V, NA, NA == 2 ? 8 : NA == 3 ? 4 : 3> rows;
-  // (backward: step 0, which has no h before it, comes after the others)
-  const bool start = BWD && at.t0 == 0 && at.end > 0;
-  const T* g = (const T*)p.gate + at.b * p.gb + at.d * p.gd;
-  const T* x = (const T*)p.x + at.b * p.xb + at.d * p.xd;
-  const T* e = BWD ? (const T*)p.dh + at.b * p.eb + at.d * p.ed : nullptr;
-  rows.n = at.live ? at.end - at.t0 - start : 0;
-  if constexpr (!BWD) {
-    rows.p[0] = g + at.t0 * p.gt, rows.step[0] = p.gt;
-    rows.p[1] = x + at.t0 * p.xt, rows.step[1] = p.xt;
-  } else {
-    const int64_t t = at.end - 1;
-    rows.p[0] = g + t * p.gt, rows.step[0] = -p.gt;
-    rows.p[1] = e + t * p.et, rows.step[1] = -p.et;
-    rows.p[2] = (const T*)p.h + at.b * p.hb + at.d * p.hd + (t - 1) * p.ht, rows.step[2] = -p.ht;
-    if constexpr (SIG) rows.p[3] = x + t * p.xt, rows.step[3] = -p.xt;
-  }
+  Steps<T, V, SIG, BWD> steps;
+  steps.aim(p, at);
   const S* from = (const S*)(a.chunks > 1 ? a.start : BWD ? p.dh_last : p.h0);
   L s;
 #pragma unroll
@@ -501,7 +645,7 @@ __global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof
       for (int k = (int)((int64_t)block * warp / WARPS); k < k1; ++k)
         m.then(Map<T, V>::take(j + k * a.pitch));
     }
-    rows.start();
+    steps.rows.start();
     m.put(&part[warp][lane * V]);
     own.put(&chunk[warp][lane * V]);
     __syncthreads();
@@ -510,75 +654,17 @@ __global__ void __launch_bounds__(warps_of(sizeof(T) * V) * 32, blocks_of(sizeof
       for (int w = 0; w < WARPS; ++w) s = Map<T, V>::take(&part[w][lane * V]).at(s);
     }
     for (int w = 0; w < tw; ++w) s = Map<T, V>::take(&chunk[team * wt + w][lane * V]).at(s);
-  } else {
-    rows.start();
-  }
-  if (!at.live) return;
-
-  L zero;
+    bool all = true;
 #pragma unroll
-  for (int i = 0; i < V; ++i) zero.set(i, S(0));
-  if constexpr (!BWD) {
-    T* h = (T*)p.h + at.b * p.hb + at.d * p.hd + at.t0 * p.ht;
-    rows.run([&](const R (&r)[2]) {
-      const L f = L::of(r[0]), b = L::of(r[1]);
-#pragma unroll
-      for (int i = 0; i < L::N; ++i) {
-        K fi = f.v[i], bi = b.v[i];
-        if constexpr (SIG) {
-          K rest;
-          sigmoid_pair(fi, &fi, &rest);
-          bi = bi * rest;
-        }
-        s.v[i] = mad(fi, s.v[i], bi);
-      }
-      keep<T, V>(h, s);
-      h += p.ht;
-    });
-    for (int64_t t = at.end; t < at.t1; ++t, h += p.ht) keep<T, V>(h, zero);
-  } else {
-    T* dg = (T*)p.dgate + at.b * p.pb + at.d * p.pd + (at.t1 - 1) * p.pt;
-    T* dx = (T*)p.dx + at.b * p.qb + at.d * p.qd + (at.t1 - 1) * p.qt;
-    for (int64_t t = at.t1; t > at.end; --t, dg -= p.pt, dx -= p.qt)
-      keep<T, V>(dg, zero), keep<T, V>(dx, zero);
-    auto back = [&](R rg, R re, const L& before, R rx) {
-      const L f = L::of(rg), d = L::of(re), v = L::of(rx);
-      L og, ox;
-#pragma unroll
-      for (int i = 0; i < L::N; ++i) {
-        K fi = f.v[i];
-        const K total = d.v[i] + s.v[i];
-        if constexpr (SIG) {
-          K rest;
-          sigmoid_pair(fi, &fi, &rest);
-          ox.v[i] = total * rest;
-          og.v[i] = mad(v.v[i], K::all(S(-1)), before.v[i]) * fi * ox.v[i];
-        } else {
-          ox.v[i] = total;
-          og.v[i] = total * before.v[i];
-        }
-        s.v[i] = fi * total;
-      }
-      keep<T, V>(dg, og);
-      keep<T, V>(dx, ox);
-      dg -= p.pt;
-      dx -= p.qt;
-    };
-    rows.run([&](const R (&r)[NA]) { back(r[0], r[1], L::of(r[2]), r[NA - 1]); });
-    if (start) {
-      L before;
-#pragma unroll
-      for (int i = 0; i < V; ++i) before.set(i, p.h0 ? ((const S*)p.h0)[at.c0 + i] : S(0));
-      const R rg = fetch<T, V>(g);
-      back(rg, fetch<T, V>(e), before, SIG ? fetch<T, V>(x) : rg);
+    for (int i = 0; i < V; ++i) all &= finite(s.get(i));
+    if (at.live && !all) {
+      walk<T, V, SIG, BWD>(p, a, col, at.order, s);
+      return;
     }
+  } else {
+    steps.rows.start();
   }
-  // the state that leaves the last chunk
-  S* last = (S*)(BWD ? p.dh0 : p.h_last);
-  if (last && at.order == a.chunks - 1) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) last[at.c0 + i] = s.get(i);
-  }
+  if (at.live) steps.take(p, a, at, s);
 }
 
 // ---- host side ---------------------------------------------------------------------

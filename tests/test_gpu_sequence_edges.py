@@ -230,3 +230,72 @@ def test_loss_gradients_of_infinite_dloss_f32(be, seq, n):
     others = np.arange(n) != 2
     near(dx.to_numpy()[others], ax[others], ex[others])
     assert not np.isfinite(dx.to_numpy()[2]).any()
+
+
+# ---- gates whose products leave the type -----------------------------------------
+
+
+def growing_inputs(t, d, dtype):
+    """A tiny state that grows by more than the type's range of factors and
+    shrinks again, is set back by a gate of zero, and the same for the gradient
+    from the other end.  Every state and gradient is finite."""
+    up = 256.0 if dtype == "f64" else 2.0
+    tiny = 2.0 ** -1000 if dtype == "f64" else 2.0 ** -120
+    r = np.random.default_rng(t + d)
+    gate = 0.5 + 0.5 * r.random((1, t, d))
+    x, dh = r.normal(size=(1, t, d)), r.normal(size=(1, t, d))
+    gate[:, :140], gate[:, 140:240], gate[:, 240:1000] = up, 1 / up, 1
+    x[:, :1000], dh[:, :1000] = 0, 0
+    gate[:, 1000], x[:, 1000] = 0, 3
+    e = t - 500
+    gate[:, e], x[:, e:], dh[:, e:] = 0, 0, 0
+    gate[:, e + 1:t - 240], gate[:, t - 240:t - 140], gate[:, t - 140:] = 1, 1 / up, up
+    st = np.float64 if dtype == "f64" else np.float32
+    ends = [(tiny * (1 + np.arange(d) % 3)).astype(st)[None] for _ in range(2)]
+    return [ref.rounded(v, dtype) for v in (gate, x, dh)] + ends
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64", "bf16"])
+@pytest.mark.parametrize("t,d", [(1700, 9), (6000, 24), (20000, 7), (6000, 2048), (3000, 4100)])
+def test_scan_gates_that_grow_past_the_type(be, seq, t, d, dtype):
+    """A product of gates outside the state's type, over states inside it."""
+    args = growing_inputs(t, d, dtype)
+    check_scan(run_scan(be, seq, *args, None, "linear", dtype), *args, None, "linear", dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_scan_growing_gates_and_lengths(be, seq, dtype):
+    t, d = 5000, 40
+    args = growing_inputs(t, d, dtype)
+    lengths = np.array([t, 0, 200, 1001, t - 1, 3000], np.int32)
+    args = [np.repeat(a, len(lengths), 0) for a in args]
+    args[4] *= np.float32(2.0 ** 60)  # the gradient of the last state, where a sequence ends early
+    # a gradient that enters before the state has shrunk again grows out of the
+    # type as the definition has it; those sequences get none
+    args[4][[2]] = 0
+    args[4][[0, 4]] *= np.float32(2.0 ** -60)
+    check_scan(run_scan(be, seq, *args, lengths, "linear", dtype), *args, lengths, "linear", dtype)
+
+
+@pytest.mark.parametrize("kind", ["linear", "sigmoid"])
+def test_scan_infinite_state(be, seq, kind):
+    """An infinite x leaves the state infinite for as long as gates are not
+    zero, however many steps that is, and 0 * inf = NaN from a zero gate on."""
+    t, d = 9000, 12
+    r = np.random.default_rng(3)
+    gate = r.normal(size=(1, t, d)) + 1
+    if kind == "linear":
+        gate = 1 / (1 + np.exp(-gate))
+    x = r.normal(size=(1, t, d))
+    x[0, 100, 2], x[0, 4000, 5], x[0, 7, 8] = np.inf, -np.inf, np.inf
+    if kind == "linear":
+        gate[0, 6000, 8] = 0
+    gate, x = ref.rounded(gate, "f32"), ref.rounded(x, "f32")
+    h, last = seq.gated_scan(be, seq.upload(be, gate, "f32"), seq.upload(be, x, "f32"), kind=kind)
+    h = h.to_numpy()[0]
+    assert (h[100:, 2] == np.inf).all() and (h[4000:, 5] == -np.inf).all() and (h[7:6000, 8] == np.inf).all()
+    assert np.isnan(h[6000:, 8]).all() if kind == "linear" else (h[6000:, 8] == np.inf).all()
+    ok = np.setdiff1d(np.arange(d), [2, 5, 8])
+    want, wl, e, el = ref.scan(gate[:, :, ok], x[:, :, ok], None, None, kind, "f32")
+    near(h[None][:, :, ok], want, e, "f32")
+    near(last.to_numpy()[:, ok], wl, el)
