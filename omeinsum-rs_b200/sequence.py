@@ -6,7 +6,8 @@ om_b200_quantize_rows, om_b200_linear_i8).
 
 Every function takes the backend first and tensors that are either
 
-  - torch CUDA tensors on the backend's device (any strides), or
+  - torch CUDA tensors on the backend's device (any strides; a view with torch's
+    negative bit is refused), or
   - `Strided` views of this backend's `Storage` (see `upload`),
 
 and returns tensors of the kind it was given, row-major.  Shapes are in the
@@ -137,6 +138,8 @@ def _operand(be, t, name):
     try:
         if t.get_device() != be.device:  # -1: not on a device at all
             raise _invalid(f"{name}: on {t.device}, the backend on cuda:{be.device}")
+        if t.is_neg():
+            raise _invalid(f"{name}: a view whose memory holds the negated values; call its resolve_neg()")
         return t.data_ptr(), _torch_codes[t.dtype], t.shape, t.stride()
     except KeyError:
         _learn_torch(t.dtype, name)
