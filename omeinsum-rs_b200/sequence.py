@@ -11,7 +11,9 @@ Every function takes the backend first and tensors that are either
   - `Strided` views of this backend's `Storage` (see `upload`),
 
 and returns tensors of the kind it was given, row-major.  Shapes are in the
-order the text names; nothing waits for the device.
+order the text names; nothing waits for the device.  torch's autograd does not
+see these calls: results carry no graph, also where an input requires a gradient,
+and the gradients come from the *_backward functions.
 
 Torch tensors are ordered with torch's current stream: when the backend runs
 on another stream, the call waits for the work queued on torch's stream and
