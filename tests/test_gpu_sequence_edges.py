@@ -4,6 +4,7 @@ to a limit of the launch, more than one piece of the vocabulary."""
 import numpy as np
 import pytest
 
+import sequence_parts as parts
 import sequence_ref as ref
 from conftest import load_pkg
 from test_gpu_sequence import be, check_loss, check_scan, i8_inputs, loss_inputs, near, run_scan, seq, torch_backend  # noqa: F401
@@ -299,3 +300,154 @@ def test_scan_infinite_state(be, seq, kind):
     want, wl, e, el = ref.scan(gate[:, :, ok], x[:, :, ok], None, None, kind, "f32")
     near(h[None][:, :, ok], want, e, "f32")
     near(last.to_numpy()[:, ok], wl, el)
+
+
+# ---- f32 in three parts --------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [9, 12, 130, 700])
+def test_f32_logits_keep_24_bits(be, seq, n):
+    """Logits found back from lse - loss, one target after another."""
+    v = 300
+    x, w = parts.logit_inputs(n, v, 31)
+    z = x @ w.T
+    X, W = seq.upload(be, x, "f32"), seq.upload(be, w, "f32")
+    for shift in range(0, v, 37):
+        targets = (np.arange(n) + shift) % v
+        loss, lse = (a.to_numpy().astype(np.float64) for a in seq.linear_cross_entropy(be, X, W, seq.upload(be, targets, "i64")))
+        want = z[np.arange(n), targets]
+        # the loss is rounded once, of a difference below 70
+        assert (np.abs(lse - loss - want) <= parts.LOGIT * want + parts.U * 70).all()
+
+
+@pytest.mark.parametrize("n,d", [(9, 40), (200, 40), (200, 328), (700, 40)])
+def test_f32_gradients_keep_24_bits(be, seq, n, d):
+    x, w, targets, g = parts.gradient_inputs(n, d, 32)
+    X, W, T = seq.upload(be, x, "f32"), seq.upload(be, w, "f32"), seq.upload(be, targets, "i64")
+    _, lse = seq.linear_cross_entropy(be, X, W, T)
+    s = lse.to_numpy().astype(np.float64)
+    dx, _ = seq.linear_cross_entropy_backward(be, X, W, T, lse, seq.upload(be, g))
+    want, _, bound, _ = ref.loss_backward(x, w, targets, s, g, "f32")
+    near(dx.to_numpy(), want, bound)
+    for k in list(range(0, n, max(1, n // 30))):
+        only = np.zeros_like(g)
+        only[k] = g[k]
+        _, dw = seq.linear_cross_entropy_backward(be, X, W, T, lse, seq.upload(be, only))
+        _, want, _, bound = ref.loss_backward(x, w, targets, s, only, "f32")
+        near(dw.to_numpy(), want, bound)
+
+
+# ---- more than one piece of the vocabulary ---------------------------------------
+
+
+def check_in_blocks(seq, be, n, d, v, dtype):
+    """The loss and its gradients against 64 bits in blocks of the vocabulary on the
+    device, by the bounds of ref.loss and ref.loss_backward (twice those in f64,
+    where the other side rounds as much)."""
+    import torch
+    tt = dict(f32=torch.float32, f64=torch.float64, bf16=torch.bfloat16, f16=torch.float16)[dtype]
+    st = torch.float64 if dtype == "f64" else torch.float32
+    unit, half, twice = ref.state_unit(dtype), ref.HALF[dtype], 2.0 if dtype == "f64" else 1.0
+    r = torch.Generator("cuda").manual_seed(n + d + v)
+    x = torch.randn(n, d, generator=r, device="cuda").to(tt)
+    w = torch.empty(v, d, device="cuda", dtype=tt)
+    step = max(1, (1 << 25) // max(n, d))
+    for i in range(0, v, step):
+        w[i:i + step] = torch.randn(min(step, v - i), d, generator=r, device="cuda").mul_(1.5 / d ** 0.5)
+    targets = torch.randint(0, v, (n,), generator=r, device="cuda")
+    targets[::7] = -100
+    targets[1], targets[2] = v - 1, 0
+    dloss = torch.rand(n, generator=r, device="cuda", dtype=st) / n
+    loss, lse = seq.linear_cross_entropy(be, x, w, targets)
+    dx, dw = seq.linear_cross_entropy_backward(be, x, w, targets, lse, dloss)
+
+    ok = targets >= 0
+    x64 = x.double()
+    x0 = torch.where(ok[:, None], x64, 0.0)
+    g = torch.where(ok, dloss.double(), 0.0)[:, None]
+    given = lse.double()[:, None]
+    true = torch.full((n,), -torch.inf, device="cuda", dtype=torch.double)
+    for i in range(0, v, step):
+        true = torch.logaddexp(true, torch.logsumexp(x64 @ w[i:i + step].double().t(), 1))
+    hit, ehit = torch.zeros(n, device="cuda", dtype=torch.double), torch.zeros(n, device="cuda", dtype=torch.double)
+    spread = torch.zeros(n, device="cuda", dtype=torch.double)
+    rx, tx, ax = (torch.zeros(n, d, device="cuda", dtype=torch.double) for _ in range(3))
+
+    def inside(got, want, bound):
+        off = (got.double() - want).abs()
+        bad = ~(off <= bound)
+        assert not bad.any(), (int(bad.sum()), bad.nonzero()[:3].tolist(), off[bad][:3].tolist(), bound[bad][:3].tolist())
+
+    def result_bound(ref_value, terms, carried, length, wide):
+        e = carried + (terms + carried) * ref.logit_error(length, dtype) + ref_value.abs() * half * 2 + ref.TINY[dtype] + terms * 16 * unit
+        return (e if dtype == "f64" else e + 2.0 ** -126 * wide) * twice
+
+    for i in range(0, v, step):
+        wb = w[i:i + step].double()
+        z = x64 @ wb.t()
+        ez = (x64.abs() @ wb.abs().t()) * ref.logit_error(d, dtype)
+        here = (targets >= i) & (targets < i + wb.shape[0])
+        rows = here.nonzero()[:, 0]
+        at = targets[rows] - i
+        hit[rows], ehit[rows] = z[rows, at], ez[rows, at]
+        p = torch.exp(z - true[:, None])
+        spread += (p * (ez + unit * (16 + 2 * (z - true[:, None]).abs()))).sum(1)
+        p = torch.exp(z - given)
+        one = torch.zeros_like(p)
+        one[rows, at] = 1
+        dz = g * (p - one)
+        ep = g * (p * (ez + unit * (16 + 2 * (z - given).abs())) + 2 * unit * (p + one))
+        if dtype in ("bf16", "f16"):
+            ep += dz.abs() * half * (1 + half)
+            if dtype == "f16":
+                ep += torch.where(ok, g.max() * 2.0 ** -38, 0.0)[:, None]
+        rx += dz @ wb
+        tx += dz.abs() @ wb.abs()
+        ax += ep @ wb.abs()
+        want = dz.t() @ x0
+        inside(dw[i:i + step], want, result_bound(want, dz.abs().t() @ x0.abs(), ep.t() @ x0.abs(), n, (x0.abs() + 4).sum(0)[None]))
+    wide = torch.zeros(d, device="cuda", dtype=torch.double)
+    for i in range(0, v, step):
+        wide += (w[i:i + step].double().abs() + 4).sum(0)
+    inside(dx, rx, result_bound(rx, tx, ax, v, wide[None]))
+    assert not dx[~ok].any() and not loss[~ok].any()
+    elae = spread + 64 * unit + 4 * unit * true.abs()
+    inside(lse, true, elae * twice)
+    inside(loss[ok], (true - hit)[ok], ((elae + ehit + 4 * unit * (true.abs() + hit.abs())) * twice)[ok])
+
+
+# 16 bits and f32: pieces of 2^28 / tokens entries in whole 256s; f32 weights in
+# pieces of 2^30 / (6 width); f64 and exact f32: pieces of 256 MiB in whole 128s.
+# (tokens, width, vocabulary): a last piece of 40 entries beside sums in 4 splits,
+# shorter than a split; pairs of SMs with an odd vocabulary; one whole piece more
+PIECES = [(4200, 64, 2 * 63744 + 40), (8200, 264, 2 * 32512 + 3), (8200, 72, 2 * 32512 + 256)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", PIECES, ids=str)
+def test_loss_in_pieces(seq, shape, dtype):
+    be = torch_backend()
+    check_in_blocks(seq, be, *shape, dtype)
+    be.close()
+
+
+@pytest.mark.parametrize("shape", [(9, 16384, 2 * 10752 + 40), (9, 16384, 3 * 10752), (130, 20000, 8704 + 1)], ids=str)
+def test_loss_f32_weights_in_pieces(seq, shape):
+    be = torch_backend()
+    check_in_blocks(seq, be, *shape, "f32")
+    be.close()
+
+
+@pytest.mark.parametrize("shape", [(4000, 16, 2 * 8320 + 40), (4000, 33, 3 * 8320)], ids=str)
+def test_loss_f64_in_pieces(seq, shape):
+    be = torch_backend()
+    check_in_blocks(seq, be, *shape, "f64")
+    be.close()
+
+
+@pytest.mark.parametrize("shape", [(4000, 16, 2 * 16768 + 40), (4000, 33, 3 * 16768)], ids=str)
+def test_loss_exact_f32_in_pieces(seq, shape):
+    be = torch_backend()
+    be.set_f32_mode("exact")
+    check_in_blocks(seq, be, *shape, "f32")
+    be.close()
