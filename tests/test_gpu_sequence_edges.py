@@ -451,3 +451,68 @@ def test_loss_exact_f32_in_pieces(seq, shape):
     be.set_f32_mode("exact")
     check_in_blocks(seq, be, *shape, "f32")
     be.close()
+
+
+# ---- next to the engine, and on another device -------------------------------------
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f64"])
+def test_an_einsum_feeds_the_operators_and_takes_their_result(be, seq, dtype):
+    """Projections by the engine, the recurrence and the loss on its column-major
+    results, and the engine again on a gradient, all on one storage."""
+    import importlib
+    E = importlib.import_module("omeinsum_b200.einsum")
+    b, t, d, e, v = 2, 130, 24, 40, 300
+    r = np.random.default_rng(41)
+    nt = np.float32 if dtype == "f32" else np.float64
+    tol = 1e-5 if dtype == "f32" else 1e-12  # of the terms' sum: the engine's own
+    u, wg, wx = (r.normal(size=s).astype(nt) for s in ((b, t, d), (d, e), (d, e)))
+    table, targets = (r.normal(size=(v, e)) / e ** 0.5).astype(nt), r.integers(-20, v, b * t)
+    sizes = {0: b, 1: t, 2: d, 3: e}
+    col = lambda a: be.from_slice(a.reshape(-1, order="F"))  # noqa: E731
+    project = E.Einsum([[0, 1, 2], [2, 3]], [0, 1, 3], sizes)
+    U = col(u)
+    G, X = (seq.Strided(project.execute(be, "standard", [U, col(m)]), (b, t, e), (1, b, b * t)) for m in (wg, wx))
+    for got, m in ((G, wg), (X, wx)):
+        assert (np.abs(got.to_numpy() - u.astype(float) @ m) <= tol * (np.abs(u) @ np.abs(m))).all()
+    gate, x = (a.to_numpy().astype(np.float64) for a in (G, X))
+    h, last = seq.gated_scan(be, G, X, kind="sigmoid")
+    flat = seq.Strided(h.storage, (b * t, e))
+    W, T = seq.upload(be, table), seq.upload(be, targets, "i64")
+    g = (r.random(b * t) / (b * t)).astype(nt)
+    check_loss(be, seq, flat, W, T, seq.upload(be, g), flat.to_numpy().astype(np.float64), table.astype(np.float64), targets, g, dtype)
+    _, lse = seq.linear_cross_entropy(be, flat, W, T)
+    dflat, _ = seq.linear_cross_entropy_backward(be, flat, W, T, lse, seq.upload(be, g))
+    dh = seq.Strided(dflat.storage, (b, t, e))
+    grads = seq.gated_scan_backward(be, G, X, h, dh, kind="sigmoid")
+    check_scan([a.to_numpy() for a in (h, last, *grads)], gate, x, dh.to_numpy().astype(np.float64), None, None, None, "sigmoid", dtype)
+    # d loss / d wx = sum over b, t of u dx: dx is row-major, so [e, t, b] to the engine
+    back = E.Einsum([[0, 1, 2], [3, 1, 0]], [2, 3], sizes).execute(be, "standard", [U, grads[1].storage])
+    got = back.to_vec().reshape(d, e, order="F")
+    dx = grads[1].to_numpy().astype(np.float64)
+    assert (np.abs(got - np.einsum("btd,bte->de", u, dx)) <= tol * np.einsum("btd,bte->de", np.abs(u), np.abs(dx))).all()
+
+
+def test_the_current_device_is_left_as_it_was(seq):
+    """Calls on device 0's backend while another device is current."""
+    import torch
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    om = load_pkg()
+    be = om.B200(0, stream=torch.cuda.default_stream(0).cuda_stream)
+    x = torch.randn(4, 20, 64, device="cuda:0")
+    w = torch.randn(30, 64, device="cuda:0")
+    t = torch.zeros(80, device="cuda:0", dtype=torch.int64)
+    torch.cuda.synchronize(0)
+    with torch.cuda.device(1):
+        calls = [lambda: seq.gated_scan(be, x, x, kind="sigmoid"),
+                 lambda: seq.gated_scan_backward(be, x, x, x, x, kind="sigmoid"),
+                 lambda: seq.linear_cross_entropy(be, x.view(80, 64), w, t),
+                 lambda: seq.linear_cross_entropy_backward(be, x.view(80, 64), w, t, t.float(), t.float()),
+                 lambda: seq.linear_i8(be, w, *seq.quantize_rows(be, w)),
+                 lambda: seq.matmul_i8(be, *seq.quantize_rows(be, x[0]), *seq.quantize_rows(be, w))]
+        for call in calls:
+            call()
+            assert torch.cuda.current_device() == 1
+    torch.cuda.synchronize(0)
+    be.close()
