@@ -258,11 +258,11 @@ __global__ void pack_i8(const int8_t* __restrict__ src, int64_t rows, int K, int
 constexpr int TOKEN_ROWS = 8;
 constexpr int TOKEN_SMEM = 160 * 1024;
 
-// Up to eight rows: from nine on the tensor cores' product, which wastes most of
-// its rows but none of the weights, is as fast (the dot products of sixteen rows
-// would take longer than the weights). One row of 4096 through 4096 x 4096:
-// 5.6 us with the weights in L2, 9.3 us from memory (floor 2.6 us): latency of
-// the row, its maximum and the first weights.
+// Up to eight rows, whose dot products grow with them: 7.1, 8.7, 12.0 and 19.4 us
+// for 1, 2, 4 and 8 bf16 rows of 4096 through 4096 x 4096 from memory (floor 2.6
+// us), where the tensor cores' product, which wastes most of its rows but none of the
+// weights, takes 15 us for any of them with its quantiser and 11.7 without. See
+// few_rows for where they cross.
 // A block keeps the M <= MM rows of q in shared memory and walks its share of
 // the channels, a warp per channel: 16 weights per lane and step, four
 // products per instruction, one shuffle reduction per row. T: the type of y,
@@ -454,8 +454,17 @@ int launch_token_rows(om_backend* be, const I8Args& p, const T* x, int64_t xk, i
   return check_cuda(cudaGetLastError(), "matmul_i8 launch");
 }
 
-bool few_rows(int64_t M, int64_t K) {
-  return M <= TOKEN_ROWS && M * ((K + 15) / 16 * 16) <= TOKEN_SMEM;
+// Whether the token kernel takes the rows: one always does, more where the products
+// are at most 2^26, or 2^25 where the rows come quantised and the tensor cores need
+// one launch instead of two. Measured, token kernel against tensor cores: quantising,
+// 4 x 4096 x 4096 (2^26) 12.0 and 15.0 us, 4 x 2048 x 8200 11.0 and 11.9, 8 x 2048 x
+// 4096 12.0 and 10.7, 6 x 4096 x 4096 17.2 and 15.1, 4 x 4096 x 12288 22 and 17.8;
+// quantised, 2 x 4096 x 4096 (2^25) 9.3 and 11.7, 4 x 2048 x 2048 6.9 and 7.3, 4 x 2048
+// x 4096 8.5 and 8.1, 3 x 4096 x 6000 15.3 and 12.8; one row of 4096 x 12288 13.5 and
+// 14.2. (At the limit it depends on the shape: 8 x 4096 x 1024 quantised 13.6 and 11.1.)
+bool few_rows(int64_t M, int64_t K, int64_t N, bool quantising) {
+  return M <= TOKEN_ROWS && M * ((K + 15) / 16 * 16) <= TOKEN_SMEM &&
+         (M == 1 || M * K * N <= (int64_t)1 << (quantising ? 26 : 25));
 }
 
 // p.q == null: the rows are x's, quantised within the kernel
@@ -475,7 +484,7 @@ int launch_tokens(om_backend* be, I8Args p, const T* x, int64_t xk, int64_t xm) 
 
 template <typename T>
 int launch_matmul(om_backend* be, const I8Args& p) {
-  if (few_rows(p.M, p.K)) return launch_tokens<T>(be, p, nullptr, 0, 0);
+  if (few_rows(p.M, p.K, p.N, false)) return launch_tokens<T>(be, p, nullptr, 0, 0);
   Scratch qc, wc;
   mma::Matrix q, w;
   OM_TRY(readable_i8(be, p.q, p.M, p.K, p.qm, p.qk, qc, &q));
@@ -573,7 +582,7 @@ extern "C" int om_b200_linear_i8(om_backend* be, om_dtype dtype, const int64_t* 
   OM_CUDA(guard.status, "linear_i8: device");
   const int64_t none[2] = {0, 0};
   if (!K) strides_x = strides_w = none;
-  if (K && few_rows(M, K)) {
+  if (K && few_rows(M, K, N, true)) {
     const I8Args p{M, N, K, nullptr, 0, 0, (const int8_t*)w, strides_w[0], strides_w[1], nullptr,
                    w_scale, bias, y, strides_y[0], strides_y[1]};
     if (dtype == OM_BF16)

@@ -516,3 +516,17 @@ def test_the_current_device_is_left_as_it_was(seq):
             assert torch.cuda.current_device() == 1
     torch.cuda.synchronize(0)
     be.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(2, 4096, 4096), (2, 4096, 4097), (4, 4096, 4096), (4, 4096, 4100), (8, 2048, 4096), (8, 2064, 4096), (3, 1037, 11000),
+                                   (8, 1031, 4100), (1, 4096, 16500), (5, 32, 300000), (8, 20480, 300)], ids=str)
+def test_i8_few_rows_on_both_sides_of_the_rule(be, seq, shape, dtype):
+    """Where few rows change from the CUDA cores to the tensor cores."""
+    x, w, ws, bias = i8_inputs(sum(shape), *shape, dtype)
+    X, W, WS, B = seq.upload(be, x, dtype), seq.upload(be, w), seq.upload(be, ws), seq.upload(be, bias)
+    rq, rs = ref.quantize(x)
+    want = ref.matmul_i8(rq, rs, w, ws, bias, dtype)
+    assert np.array_equal(seq.linear_i8(be, X, W, WS, bias=B).to_numpy().astype(np.float64), want)
+    q, scale = seq.quantize_rows(be, X)
+    assert np.array_equal(seq.matmul_i8(be, q, scale, W, WS, bias=B, dtype=dtype).to_numpy().astype(np.float64), want)
