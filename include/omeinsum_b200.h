@@ -412,9 +412,9 @@ int om_b200_linear_cross_entropy(om_backend* be, om_dtype dtype, const int64_t* 
 /* Its gradients, from lse and the gradient dloss of each token's loss (both N
  * contiguous values): with p = exp(z - lse),
  *     dz_nv = dloss_n (p_nv - [v == targets[n]]),  dx = dz w,  dw = dz^T x
- * Tokens without a loss get dx = 0 and reach dw with nothing, whatever their
- * row of x holds.  In the 16-bit types dz is rounded to dtype before the two
- * products, whose sums are f32. */
+ * Tokens without a loss get dx = 0 and reach dw with nothing, whatever their row
+ * of x and w hold (for the others 0 * w of an infinite w is NaN).  In the 16-bit
+ * types dz is rounded to dtype before the two products, whose sums are f32. */
 int om_b200_linear_cross_entropy_backward(om_backend* be, om_dtype dtype, const int64_t* shape,
                                           const void* x, const int64_t* strides_x, const void* w,
                                           const int64_t* strides_w, om_dtype target_dtype,

@@ -8,7 +8,7 @@
 // vocabulary at a time, writes dz of the piece once and multiplies it twice:
 // 8 N D V operations, of which 6 are needed. Bound by the tensor cores, or,
 // for few tokens, by reading w. Measured: 8192 x 4096 x 128000 bf16 with
-// gradients 25.3 ms (34.4 TFLOP at 1.36 PFLOP/s, the card's power limit; writing
+// gradients 25.3 to 26.7 ms (34.4 TFLOP at 1.36 PFLOP/s, the card's power limit; writing
 // the logits once and reading them three times would save 8.6 TFLOP and cost
 // 4.2 GB held); 24 x 2048 x 32000 f16 forward 34 us, 20 of which w needs.
 #include <algorithm>

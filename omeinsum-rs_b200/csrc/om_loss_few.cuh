@@ -12,7 +12,8 @@
 // Bound by HBM: w is read once forward, twice backward, and dw written once,
 // where the tensor cores' products make and read three planes of w. Sums are
 // formed in one order. Measured with gradients: 3 x 1344 x 11307 93 us (tensor
-// cores 202), 8 x 2048 x 32000 341 us (nine tokens, on the tensor cores, 617). In
+// cores 202), 8 x 2048 x 32000 341 us (nine tokens, on the tensor cores, 617: eight is
+// what the kernels are compiled for, not where the two forms cross). In
 // 16 bits, where w needs no planes, the tensor cores win even for one token (8 x
 // 2048 x 32000 bf16: 149 us against 418 in this form).
 #pragma once

@@ -14,13 +14,21 @@
 // order whatever the timing. Where the channels alone fill the card, a sequence
 // is one chunk and map_kernel does not run.
 //
-// Bound by HBM: step_kernel moves 3 arrays (forward) or 5 to 6 (backward) per
-// element, map_kernel 2 more. Measured on 65537 x 1032 bf16: map_kernel 270 MB in
-// 45 us (6.0 TB/s), step_kernel 406 MB in 65 us (6.2 TB/s); 4 x 4096 x 2048 bf16
-// sigmoid with the backward pass 168 us, 92 of which its 604 MB need at the
-// card's copy rate. (One pass over tiles in shared memory that looked back at one
-// another read everything once, but spent its time on the tiles' bookkeeping:
-// 217 us.)
+// step_kernel moves 3 arrays (forward) or 5 to 6 (backward) per element, map_kernel 2
+// more. Long sequences are bound by HBM: 65537 x 1032 bf16 map_kernel 270 MB in 45 us
+// (6.0 TB/s), step_kernel 406 MB in 65 us (6.2 TB/s). Shorter ones are not: the four
+// launches of 4 x 4096 x 2048 bf16 sigmoid with the backward pass, 32 to 63 us each and
+// 168 together, have DRAM busy for 49 to 70 %, and its 604 MB need 92 us at the card's
+// copy rate; what is left is the ramps, the latency of the chunks' joined maps and,
+// for sigmoid gates, an exponential and a reciprocal per element and kernel (150 us
+// with linear gates). (One pass over tiles in shared memory that looked back at one
+// another read everything once, but spent its time on the tiles' bookkeeping: 217
+// us.)
+//
+// The backward pass takes h_{t-1} as the forward returned it, so in 16 bits dgate
+// carries that rounding beside its own (relative to 64 bits 2.3e-3 against 1.7e-3
+// with linear gates in bf16, 1.8e-3 with sigmoid gates): a 32-bit copy would be 4
+// more bytes written and read per element, forward and backward.
 #include <algorithm>
 
 #include "om_convert.cuh"

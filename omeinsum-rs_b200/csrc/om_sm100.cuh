@@ -25,6 +25,11 @@
 // summed from zero and added up in the epilogue warps' registers. The planes
 // of a slab are loaded once for all six.
 //
+// Without P3 an accumulator runs over all of k in f32. The tensor core cuts the
+// running sum where it adds to it instead of rounding to nearest: up to 2^-23 of the
+// sum for each 16 products (16 bits; sums of 8-bit integers are exact). Measured: lse
+// of 24 x 2048 x 32000 in f16 is 4e-7 off 64 bits, 3e-8 by sums rounded to nearest.
+//
 // Bound by the tensor cores: 4096 x 1024 by 50001 x 1024 bf16 with the cross
 // entropy's forward epilogue takes 257 us, 1.63 PFLOP/s with the tensor pipe 93 %
 // active (the library product of the same size 293 us); 8192 x 4096 by 12288 x 4096

@@ -335,7 +335,8 @@ def linear_cross_entropy(be, x, w, targets):
     """(loss, lse) of the logits x w^T, per token (om_b200_linear_cross_entropy).
 
     x [tokens, width], w [vocabulary, width], targets [tokens] (i32 or i64;
-    one outside the vocabulary carries no loss).  The logits are never kept."""
+    one outside the vocabulary carries no loss).  The logits are never kept; they
+    may be -inf (a masked vocabulary)."""
     L = _bind()
     code, n, _, _, args, st = _loss_args(be, x, w, targets, "linear_cross_entropy")
     call = _Call(be, x, w, targets)
