@@ -173,10 +173,11 @@ GemmArgs gemm(om_dtype dt, int64_t M, int64_t N, int64_t K, const void* a, int64
   return g;
 }
 
-// Vocabulary entries per piece: a piece's logits take at most 256 MiB
+// Vocabulary entries per piece: a piece's logits take at most 256 MiB, and the
+// products' grids hold 65535 tiles of 64 columns
 int64_t piece_size(int64_t N, int64_t V, size_t elem) {
   const int64_t fit = ((int64_t)256 << 20) / (int64_t)elem / std::max<int64_t>(N, 1) / 128 * 128;
-  return std::min(V, std::max<int64_t>(128, fit));
+  return std::min({V, std::max<int64_t>(128, fit), (int64_t)1 << 21});
 }
 
 // f64, and f32 in exact mode: pieces through the library's own products

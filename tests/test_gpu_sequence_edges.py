@@ -530,3 +530,11 @@ def test_i8_few_rows_on_both_sides_of_the_rule(be, seq, shape, dtype):
     assert np.array_equal(seq.linear_i8(be, X, W, WS, bias=B).to_numpy().astype(np.float64), want)
     q, scale = seq.quantize_rows(be, X)
     assert np.array_equal(seq.matmul_i8(be, q, scale, W, WS, bias=B, dtype=dtype).to_numpy().astype(np.float64), want)
+
+
+def test_loss_exact_f32_of_few_tokens_and_a_vocabulary_past_2_to_22(seq):
+    """16 tokens: a piece's columns would be more than the products' grid holds."""
+    be = torch_backend()
+    be.set_f32_mode("exact")
+    check_in_blocks(seq, be, 16, 9, (1 << 22) + 70, "f32")
+    be.close()
