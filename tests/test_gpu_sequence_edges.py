@@ -7,7 +7,7 @@ import pytest
 import sequence_parts as parts
 import sequence_ref as ref
 from conftest import load_pkg
-from test_gpu_sequence import be, check_loss, check_scan, i8_inputs, loss_inputs, near, run_scan, seq, torch_backend  # noqa: F401
+from test_gpu_sequence import be, check_loss, check_scan, i8_inputs, loss_inputs, near, run_scan, scan_inputs, seq, torch_backend  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 TYPES = ["f32", "f64", "bf16", "f16"]
@@ -538,3 +538,84 @@ def test_loss_exact_f32_of_few_tokens_and_a_vocabulary_past_2_to_22(seq):
     be.set_f32_mode("exact")
     check_in_blocks(seq, be, 16, 9, (1 << 22) + 70, "f32")
     be.close()
+
+
+# ---- strides of zero and below ---------------------------------------------------
+
+
+def strided(seq, be, m, layout, dtype):
+    """(a view with the layout's strides, the matrix that it shows)."""
+    r, c = m.shape
+    up = lambda v: seq.upload(be, np.ascontiguousarray(v), dtype).storage  # noqa: E731
+    if layout == "rows_backwards":
+        return seq.Strided(up(m[::-1]), (r, c), (-c, 1), offset=(r - 1) * c), m
+    if layout == "columns_backwards":
+        return seq.Strided(up(m[:, ::-1]), (r, c), (c, -1), offset=c - 1), m
+    if layout == "both_backwards_transposed":
+        return seq.Strided(up(m[::-1, ::-1].T), (r, c), (-1, -r), offset=r * c - 1), m
+    if layout == "one_row":
+        return seq.Strided(up(m[:1]), (r, c), (0, 1)), np.repeat(m[:1], r, 0)
+    if layout == "one_column":
+        return seq.Strided(up(m[:, :1]), (r, c), (1, 0)), np.repeat(m[:, :1], c, 1)
+    return seq.Strided(up(m[:1, :1]), (r, c), (0, 0)), np.full_like(m, m[0, 0])
+
+
+LAYOUTS = ["rows_backwards", "columns_backwards", "both_backwards_transposed", "one_row", "one_column", "one_value"]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,d,v", [(5, 72, 130), (70, 104, 333), (150, 33, 400)])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_loss_strides_of_zero_and_below(be, seq, layout, n, d, v, dtype):
+    x, w, targets, g = loss_inputs(51, n, d, v, dtype)
+    (X, xs), (W, ws) = strided(seq, be, x, layout, dtype), strided(seq, be, w, layout, dtype)
+    check_loss(be, seq, X, W, seq.upload(be, targets, "i64"), seq.upload(be, g), xs, ws, targets, g, dtype)
+
+
+def test_loss_exact_f32_strides_of_zero_and_below(seq):
+    om = load_pkg()
+    be = om.B200(0)
+    be.set_f32_mode("exact")
+    for layout in LAYOUTS:
+        for n, d, v in ((70, 104, 333), (150, 33, 400)):
+            x, w, targets, g = loss_inputs(52, n, d, v, "f32")
+            (X, xs), (W, ws) = strided(seq, be, x, layout, "f32"), strided(seq, be, w, layout, "f32")
+            check_loss(be, seq, X, W, seq.upload(be, targets, "i64"), seq.upload(be, g), xs, ws, targets, g, "f32")
+    be.close()
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 96, 70), (6, 113, 70), (30, 192, 150), (200, 65, 150)])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_i8_strides_of_zero_and_below(be, seq, layout, m, k, n):
+    x, w, ws, bias = i8_inputs(53, m, k, n, "bf16")
+    WS, B = seq.upload(be, ws), seq.upload(be, bias)
+    (X, xs), (W, shown) = strided(seq, be, x, layout, "bf16"), strided(seq, be, w, layout, None)
+    rq, rs = ref.quantize(xs)
+    want = ref.matmul_i8(rq, rs, shown, ws, bias, "bf16")
+    assert np.array_equal(seq.linear_i8(be, X, W, WS, bias=B).to_numpy().astype(np.float64), want)
+    q, scale = seq.quantize_rows(be, X)
+    assert np.array_equal(q.to_numpy(), rq) and np.array_equal(scale.to_numpy(), rs)
+    Q, shown_q = strided(seq, be, rq, layout, None)
+    S = np.linspace(0.5, 1.5, m).astype(np.float32)
+    want = ref.matmul_i8(shown_q, S, shown, ws, bias, "bf16")
+    assert np.array_equal(seq.matmul_i8(be, Q, seq.upload(be, S), W, WS, bias=B, dtype="bf16").to_numpy().astype(np.float64), want)
+
+
+@pytest.mark.parametrize("kind", ["linear", "sigmoid"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("axes", [(0,), (2,), (0, 1, 2)], ids=str)
+def test_scan_strides_below_zero(be, seq, axes, dtype, kind):
+    b, t, d = 3, 700, 40
+    gate, x, dh, h0, dl = scan_inputs(54, b, t, d, dtype, kind)
+
+    def place(v):
+        strides, at = [t * d, d, 1], 0
+        for a in axes:
+            at += (v.shape[a] - 1) * strides[a]
+            strides[a] = -strides[a]
+        return seq.Strided(seq.upload(be, np.ascontiguousarray(np.flip(v, axes)), dtype).storage, (b, t, d), strides, offset=at)
+
+    G, X, E, H0, DL = place(gate), place(x), place(dh), seq.upload(be, h0), seq.upload(be, dl)
+    h, last = seq.gated_scan(be, G, X, h0=H0, kind=kind)
+    grads = seq.gated_scan_backward(be, G, X, place(h.to_numpy()), E, h0=H0, dh_last=DL, kind=kind)
+    check_scan([v.to_numpy() for v in (h, last, *grads)], gate, x, dh, h0, dl, None, kind, dtype)
