@@ -619,3 +619,68 @@ def test_scan_strides_below_zero(be, seq, axes, dtype, kind):
     h, last = seq.gated_scan(be, G, X, h0=H0, kind=kind)
     grads = seq.gated_scan_backward(be, G, X, place(h.to_numpy()), E, h0=H0, dh_last=DL, kind=kind)
     check_scan([v.to_numpy() for v in (h, last, *grads)], gate, x, dh, h0, dl, None, kind, dtype)
+
+
+# ---- long in one extent ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1200000, 9, 600), (300, 1, 5000), (9, 70001, 300), (300000, 24, 1), (40, 16, 2200000)], ids=str)
+def test_loss_long_in_one_extent(seq, shape, dtype):
+    be = torch_backend()
+    check_in_blocks(seq, be, *shape, dtype)
+    be.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 100000, 1), (1, 60000, 3), (70000, 3, 8), (200, 2, 9001), (1, 1, 1 << 20), (3, 17, 200003)], ids=str)
+def test_scan_long_in_one_extent(be, seq, shape, dtype):
+    args = scan_inputs(61, *shape, dtype, "sigmoid")
+    check_scan(run_scan(be, seq, *args, None, "sigmoid", dtype), *args, None, "sigmoid", dtype)
+
+
+@pytest.mark.parametrize("shape", [(1000003, 5, 3), (70001, 33, 1), (1, 7, 1000001), (9, 1, 300007), (3, 131071, 50), (2000, 131071, 30)], ids=str)
+def test_i8_long_in_one_extent(be, seq, shape):
+    x, w, ws, _ = i8_inputs(62, *shape, "f32")
+    X, W, WS = seq.upload(be, x, "f32"), seq.upload(be, w), seq.upload(be, ws)
+    rq, rs = ref.quantize(x)
+    want = ref.matmul_i8(rq, rs, w, ws, None, "f32")
+    q, scale = seq.quantize_rows(be, X)
+    assert np.array_equal(q.to_numpy(), rq) and np.array_equal(scale.to_numpy(), rs)
+    assert np.array_equal(seq.linear_i8(be, X, W, WS).to_numpy().astype(np.float64), want)
+    assert np.array_equal(seq.matmul_i8(be, q, scale, W, WS).to_numpy().astype(np.float64), want)
+
+
+def test_views_recorded_and_replayed(seq):
+    """A recording whose results are views of storages that it allocates itself."""
+    om = load_pkg()
+    be = om.B200(0)
+    gate, x, dh, h0, _ = scan_inputs(71, 2, 300, 40, "bf16", "sigmoid")
+    _, w, targets, g = loss_inputs(72, 600, 40, 500, "bf16")
+    G, X, E, H0, W, T, D = (seq.upload(be, *a) for a in ((gate, "bf16"), (x, "bf16"), (dh, "bf16"), (h0,), (w, "bf16"), (targets, "i64"), (g,)))
+
+    def run():
+        h, last = seq.gated_scan(be, G, X, h0=H0, kind="sigmoid")
+        flat = seq.Strided(h.storage, (600, 40))
+        loss, lse = seq.linear_cross_entropy(be, flat, W, T)
+        grads = seq.linear_cross_entropy_backward(be, flat, W, T, lse, D)
+        back = seq.gated_scan_backward(be, G, X, h, E, h0=H0, kind="sigmoid")
+        q, scale = seq.quantize_rows(be, W)
+        return [h, last, loss, lse, *grads, *back, seq.linear_i8(be, flat, q, scale)]
+
+    want = [v.to_numpy() for v in run()]
+    be.graph_begin()
+    out = run()
+    graph = be.graph_end()
+    for _ in range(3):
+        graph.launch()
+        be.synchronize()
+        assert all(np.array_equal(a.to_numpy(), b) for a, b in zip(out, want))
+    # other inputs, in place
+    be.upload_into(X.storage, seq.upload(be, -x, "bf16").storage.to_vec())
+    want = [v.to_numpy() for v in run()]
+    graph.launch()
+    be.synchronize()
+    assert all(np.array_equal(a.to_numpy(), b) for a, b in zip(out, want))
+    del out, graph
+    be.close()
