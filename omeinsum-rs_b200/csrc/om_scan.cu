@@ -15,10 +15,10 @@
 // is one chunk and map_kernel does not run.
 //
 // step_kernel moves 3 arrays (forward) or 5 to 6 (backward) per element, map_kernel 2
-// more. Long sequences are bound by HBM: 65537 x 1032 bf16 map_kernel 270 MB in 45 us
-// (6.0 TB/s), step_kernel 406 MB in 65 us (6.2 TB/s). Shorter ones are not: the four
-// launches of 4 x 4096 x 2048 bf16 sigmoid with the backward pass, 32 to 63 us each and
-// 168 together, have DRAM busy for 49 to 70 %, and its 604 MB need 92 us at the card's
+// more. Long sequences are bound by HBM: 65537 x 1032 bf16 map_kernel 270 MB in 45 to
+// 47 us (5.8 to 6.0 TB/s), step_kernel 406 MB in 65 to 68 us (6.0 to 6.2). Shorter ones are not: the four
+// launches of 4 x 4096 x 2048 bf16 sigmoid with the backward pass, 31 to 63 us each and
+// 168 together, have DRAM busy for 50 to 70 %, and its 604 MB need 92 us at the card's
 // copy rate; what is left is the ramps, the latency of the chunks' joined maps and,
 // for sigmoid gates, an exponential and a reciprocal per element and kernel (150 us
 // with linear gates). (One pass over tiles in shared memory that looked back at one
