@@ -384,7 +384,8 @@ __global__ void gradient_scale(const float* __restrict__ dloss, const void* targ
   float m = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += blockDim.x) {
     const int64_t t = target_of(targets, t64, i);
-    if (t >= 0 && t < vocab) m = fmaxf(m, fabsf(dloss[i]));
+    const float g = fabsf(dloss[i]);
+    if (t >= 0 && t < vocab && g < INFINITY) m = fmaxf(m, g);  // one that is no number scales nothing
   }
   __shared__ float part[32];
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -394,7 +395,7 @@ __global__ void gradient_scale(const float* __restrict__ dloss, const void* targ
   for (int i = 1; i < (int)(blockDim.x >> 5); ++i) m = fmaxf(m, part[i]);
   // a scale below f32's normal numbers would lose bits, none is needed at 0
   const float f = m / top;
-  *scale = f >= FLT_MIN && f < INFINITY ? f : 1.f;
+  *scale = f >= FLT_MIN ? f : 1.f;
 }
 
 // 32 columns of a warp's rows, rounded to T, through TMA; m: this lane's row. A

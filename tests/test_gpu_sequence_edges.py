@@ -684,3 +684,22 @@ def test_views_recorded_and_replayed(seq):
     assert all(np.array_equal(a.to_numpy(), b) for a, b in zip(out, want))
     del out, graph
     be.close()
+
+
+@pytest.mark.parametrize("n", [8, 200])
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f64"])
+@pytest.mark.parametrize("value", [np.inf, -np.inf, np.nan])
+def test_loss_gradients_beside_a_dloss_that_is_no_number(be, seq, value, dtype, n):
+    """The other tokens' rows of dx keep their accuracy, however small their dloss."""
+    x, w, targets, g = loss_inputs(81, n, 40, 3000, dtype)
+    targets[:4] = 7
+    g *= 2.0 ** -20
+    g[2] = value
+    X, W, T = seq.upload(be, x, dtype), seq.upload(be, w, dtype), seq.upload(be, targets, "i64")
+    _, lse = seq.linear_cross_entropy(be, X, W, T)
+    dx, _ = seq.linear_cross_entropy_backward(be, X, W, T, lse, seq.upload(be, g))
+    g[2] = 0
+    ax, _, ex, _ = ref.loss_backward(x, w, targets, lse.to_numpy().astype(np.float64), g, dtype)
+    others = np.arange(n) != 2
+    near(dx.to_numpy()[others], ax[others], ex[others])
+    assert not np.isfinite(np.asarray(dx.to_numpy(), np.float64)[2]).any()
